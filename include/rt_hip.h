@@ -17,8 +17,9 @@
  * on the CPU; a C ABI reports instead.)  Kernels run asynchronously on the
  * given stream (NULL = the legacy default stream); a status of 0 means the
  * launch was accepted.  Calls on different streams may run concurrently,
- * except calls that use the per-device library workspace -- argmax, GEMM,
- * decode and FLUX attention, and GEMV with m > 1 (its K-slice partials and
+ * except calls that use the per-device library workspace or its arrival
+ * counters -- argmax, GEMM, decode, paged and FLUX attention, paged_plan,
+ * verify_drafts, and GEMV with m > 1 (its K-slice partials and
  * arrival counters), of any format and size: those must not overlap on one
  * device (issue them on one stream, or order the streams).
  *
@@ -65,7 +66,8 @@ typedef enum {
     RT_HIP_Q4K = 2,
     RT_HIP_Q4_0 = 3,
     RT_HIP_Q4MAT = 4,
-    RT_HIP_Q6K = 5   /* GGUF Q6_K blocks: the decode engine's Llama down projection (rt_hip_decoder_set_tensor) */
+    RT_HIP_Q6K = 5,  /* GGUF Q6_K blocks: the decode engine's Llama down projection (rt_hip_decoder_set_tensor) */
+    RT_HIP_F16 = 6   /* f16 values: the paged KV cache and its attention */
 } rt_hip_format;
 
 /* Largest activation batch the GEMV kernels take; the reference's
@@ -88,8 +90,8 @@ int rt_hip_init(int ordinal);
  * Some calls take scratch from a per-device library workspace: the GEMM (bf16
  * copies of f32 A and of a Q4_K weight shared by several M tiles, split-K
  * partials), the batched GEMV of every format (K-slice partials), decode
- * attention (split partials), FLUX attention (the states of blocks cut between
- * workgroups) and argmax (8 bytes per row).  It grows on demand (the reference
+ * attention (split partials), FLUX and paged attention (the states of blocks cut
+ * between workgroups), verify_drafts (the rows' sums) and argmax (8 bytes per row).  It grows on demand (the reference
  * likewise grows its Metal scratch on demand, src/metal_ops.mm:378-423).  A
  * replaced buffer is kept until the process ends, because a hipGraph that
  * captured a call still writes the buffer that call used on every replay.
@@ -642,6 +644,123 @@ int rt_hip_decoder_step_batch(rt_hip_decoder* dec, const int32_t* tokens, int32_
 int64_t rt_hip_decoder_vocab(const rt_hip_decoder* dec);
 const float* rt_hip_decoder_logits(const rt_hip_decoder* dec);
 int rt_hip_decoder_destroy(rt_hip_decoder* dec);
+
+/* ---- batched serving over a paged KV cache ----------------------------------
+ * No counterpart in the reference, whose engine holds one sequence in one
+ * contiguous cache (MetalDecodeContext).  Here many requests share a cache
+ * in pages, and one step of a serving loop, with any number of new tokens per
+ * request (single tokens, drafts to verify, chunks of prompts), is
+ *   rt_hip_paged_plan       the requests' pages, the new tokens' slots and positions
+ *   rt_hip_paged_append     per layer: the new keys and values into the pages
+ *   rt_hip_paged_attention  per layer: the new tokens' attention
+ *   rt_hip_verify_drafts    the drafted tokens accepted or replaced
+ * All lengths live in device memory, so a captured step serves every batch
+ * that fits its sizes (n_seq requests, n_tokens rows), and nothing is copied
+ * to the host.  Whatever the device arrays hold, no call reads or writes
+ * outside the buffers described by its arguments.
+ *
+ * The cache: k and v, each n_pages pages of page_size rows of n_kv_heads *
+ * head_dim values of type dtype (RT_HIP_F32, RT_HIP_F16 or RT_HIP_BF16),
+ * page_stride values from a page to the next (0: dense; larger where k and v
+ * share an allocation).  page_size is a power of two from 8 to 1024, head_dim
+ * 64, 128 or 256, n_pages * page_size < 2^31; pages start 16-byte aligned.
+ * Slot i is row i % page_size of page i / page_size. */
+typedef struct rt_hip_paged_kv {
+    void* k;
+    void* v;
+    int32_t dtype;
+    int32_t n_pages, page_size, n_kv_heads, head_dim;
+    int64_t page_stride;
+} rt_hip_paged_kv;
+
+/* rt_hip_paged_plan: request s (of n_seq <= 4096) has cached[s] tokens in the
+ * cache, holds held[s] pages (the first held[s] entries of its row of table
+ * [n_seq][table_cols]) and gets fresh[s] new tokens; fresh[s] < 0: it has
+ * ended and gives its pages back.  queue [n_pages] is a ring of free pages,
+ * queue_state {index of the first, count}.  Written:
+ *   q_start [n_seq + 1]  request s's new tokens are rows q_start[s] ..
+ *                        q_start[s + 1] of the step
+ *   kv_len [n_seq]       cached + fresh: the keys its last row sees; 0 where the
+ *                        request was not served or has ended
+ *   slots, positions [n_tokens]  of each row; -1 for rows of requests not served
+ *                        and behind the last row
+ *   table                the pages taken, at columns held[s] ..
+ *   held_out, queue_state_out, queue  the state after the step
+ * A request takes as many pages as cached + fresh tokens need beyond those
+ * held (held may be more: after drafts were refused, say) from the queue's
+ * front.  Requests are served in order until one wants more pages than are
+ * left; that one and those after it that need pages are not served, nor is one
+ * whose pages pass table_cols, whose rows pass n_tokens, or whose numbers are
+ * negative; their held stays.  Pages given back join the queue's end, in
+ * request order, for the next step.  cached is the caller's to advance, by
+ * fresh or by what rt_hip_verify_drafts accepted.
+ * held_out may be held and queue_state_out may be queue_state; nothing else
+ * may overlap.  n_seq * table_cols and table_cols * page_size < 2^31. */
+int rt_hip_paged_plan(const int32_t* cached, const int32_t* fresh, const int32_t* held, int32_t* held_out,
+                      int32_t* table, int64_t table_cols, int32_t* queue, const int32_t* queue_state,
+                      int32_t* queue_state_out, int32_t n_pages, int32_t page_size, int32_t n_seq, int32_t n_tokens,
+                      int32_t* q_start, int32_t* kv_len, int32_t* slots, int32_t* positions, rt_hip_stream stream);
+
+/* rt_hip_paged_append: row t of k and v (n_kv_heads * head_dim values of type
+ * dtype, F32, F16 or BF16, rows row_stride values apart, so that they may be
+ * part of a joint projection's output) to slot slots[t], rounded to the cache's
+ * type (to nearest even).  Rows whose slot is negative or outside the cache are
+ * skipped.  Of rows with the same slot one is kept, no telling which. */
+int rt_hip_paged_append(const rt_hip_paged_kv* kv, const void* k, const void* v, int32_t dtype, int64_t row_stride,
+                        const int32_t* slots, int32_t n_tokens, rt_hip_stream stream);
+
+/* rt_hip_paged_attention: rows q_start[s] .. q_start[s + 1] of q (n_q_heads *
+ * head_dim values, q_stride apart) attend to the first kv_len[s] keys of
+ * request s: the last row to all of them, each row before it to one fewer, of
+ * those only the last `window` where window > 0.  Head h reads KV head
+ * h / (n_q_heads / n_kv_heads); s_j = scale * (q . k_j), out = sum_j
+ * softmax(s)_j v_j; zeros for a row that sees no key (kv_len[s] below the
+ * request's rows: its first ones; all where it is 0) or only scores of -inf.
+ * Rows outside every request are left as they were.  Keys on a page whose
+ * table entry is no page of the cache count as zeros.
+ * dtype is q's and out's: the cache's (F16 or BF16: products of 16-bit values
+ * summed in f32, the softmax in f32 and its weights rounded to the type before
+ * they multiply v), or F32 with any cache (products and sums to f32
+ * accuracy).  n_q_heads is any multiple of n_kv_heads up to 1024, scale > 0.
+ * Results are deterministic.
+ * max_fresh is a hint, the most rows a request of this step may have (0: not
+ * known); the result does not depend on it beyond rounding.
+ * Uses the library workspace (rt_hip_paged_attention_workspace_bytes, to
+ * reserve before a graph capture; -1 for invalid sizes). */
+int rt_hip_paged_attention(const void* q, int32_t dtype, int64_t q_stride, int32_t n_q_heads, const rt_hip_paged_kv* kv,
+                           const int32_t* table, int64_t table_cols, const int32_t* q_start, const int32_t* kv_len,
+                           int32_t n_seq, int32_t n_tokens, int32_t max_fresh, float scale, int32_t window, void* out,
+                           int64_t out_stride, rt_hip_stream stream);
+int64_t rt_hip_paged_attention_workspace_bytes(const rt_hip_paged_kv* kv, int32_t dtype, int32_t n_q_heads,
+                                               int32_t n_seq, int32_t n_tokens, int32_t max_fresh);
+
+/* rt_hip_verify_drafts: speculative decoding's decision.  Request s's rows
+ * row_start[s] .. row_start[s + 1] of tokens are its last accepted token and
+ * then its drafts; row r of logits [n_rows][vocab] (logit_stride apart, F32 or
+ * BF16) is the target model's prediction of the token behind row r, and row r
+ * of draft_logits the distribution that token was drawn from (null: drafts are
+ * taken as certain; the rows of last drafts are not read).  With p and q their
+ * softmax(x / temperature[s]), drafts d are accepted in order while
+ *   accept_u[r] * q(d) < p(d)          (r the row before d's),
+ * then one token more is drawn: the first whose running sum of w exceeds
+ * sample_u[s] * sum(w), w = max(0, p - q) at the first refused draft (p where
+ * that is zero everywhere), w = p behind the last one.  Random numbers are in
+ * [0, 1).  temperature 0 (or negative, or NaN) is greedy: drafts are accepted
+ * while they are the first largest logit, as rt_hip_argmax; a null temperature
+ * is 1 for every request.  Sums are in f64.  NaN logits count as -inf, a row of
+ * nothing else as certain of token 0; +inf leaves the weight to the infinite
+ * ones.  A draft outside the vocabulary is refused.
+ * out_tokens [n_seq][max_draft + 1]: the accepted drafts, the token drawn, then
+ * -1; out_count [n_seq]: how many (0 for a request without rows).  Drafts past
+ * max_draft are not looked at.  vocab <= 2^20, max_draft <= 255, n_seq <= 4096,
+ * n_seq * (max_draft + 1) <= 65535.  Uses the library workspace. */
+int rt_hip_verify_drafts(const void* logits, int64_t logit_stride, const void* draft_logits, int64_t draft_stride,
+                         int32_t dtype, int32_t vocab, const int32_t* tokens, const int32_t* row_start,
+                         const float* accept_u, const float* sample_u, const float* temperature, int32_t n_seq,
+                         int32_t n_rows, int32_t max_draft, int32_t* out_tokens, int32_t* out_count,
+                         rt_hip_stream stream);
+int64_t rt_hip_verify_drafts_workspace_bytes(int32_t vocab, int32_t n_seq, int32_t n_rows, int32_t max_draft,
+                                             int32_t with_draft_logits);
 
 /* ---- linear dispatch ------------------------------------------------------
  * The QLinear / Linear2::fused_linear dispatch over whichever weight format

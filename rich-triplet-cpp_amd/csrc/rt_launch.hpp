@@ -270,6 +270,79 @@ hipError_t launch_gelu_mul(const float* gate, const float* up, float* out, int64
 hipError_t launch_swiglu(const float* gate, const float* up, float* out, int64_t n, hipStream_t s);
 hipError_t launch_add(const float* a, const float* b, float* out, int64_t n, hipStream_t s);
 
+// ---- paged KV cache (paged.hip, paged_attention.hip, verify.hip) -----------------
+// The cache: pages of 1 << page_shift tokens, rows of n_kv * head_dim values,
+// page_stride values from one page to the next.
+struct PagedKv {
+    void* k = nullptr;
+    void* v = nullptr;
+    int dtype = 0;  // RT_HIP_F32, RT_HIP_F16 or RT_HIP_BF16
+    int n_pages = 0, page_shift = 0, n_kv = 0, head_dim = 0;
+    int64_t page_stride = 0;
+};
+// One step's bookkeeping; the arrays are device memory.  n_seq <=
+// kPlanMaxSeq, n_seq * cols and cols << page_shift and n_pages << page_shift
+// below 2^31.  `arrivals`: one zeroed counter (left zero).
+struct PagedPlan {
+    const int32_t* cached = nullptr;
+    const int32_t* fresh = nullptr;
+    const int32_t* held = nullptr;
+    int32_t* held_out = nullptr;  // may be held
+    int32_t* table = nullptr;     // [n_seq][cols]
+    int64_t cols = 0;
+    int32_t* queue = nullptr;     // [n_pages], a ring
+    const int32_t* queue_state = nullptr;  // head, count
+    int32_t* queue_state_out = nullptr;    // may be queue_state
+    int32_t* q_start = nullptr;   // [n_seq + 1]
+    int32_t* kv_len = nullptr;    // [n_seq]
+    int32_t* slots = nullptr;     // [n_tokens]
+    int32_t* positions = nullptr;
+    int n_pages = 0, page_shift = 0, n_seq = 0, n_tokens = 0;
+};
+constexpr int kPlanMaxSeq = 4096;
+hipError_t launch_paged_plan(const PagedPlan& p, uint32_t* arrivals, hipStream_t s);
+// k and v rows (src_stride values apart) to the slots; a slot outside the
+// cache is skipped.  n_tokens * n_kv * head_dim / 8 < 2^31.
+hipError_t launch_paged_append(int src_dtype, const void* k, const void* v, int64_t src_stride, const PagedKv& kv,
+                               const int32_t* slots, int n_tokens, hipStream_t s);
+// Attention of rows q_start[s] .. q_start[s + 1] of q over request s's first
+// kv_len[s] keys; the last row sees them all, each row before one fewer, of
+// those the last `window` (0: all).  q and out: rows of n_q heads, q_stride
+// and out_stride values apart, of type dtype (the cache's, or f32).
+struct PagedAttn {
+    const void* q = nullptr;
+    void* out = nullptr;
+    int64_t q_stride = 0, out_stride = 0;
+    int dtype = 0, n_q = 0;
+    PagedKv kv;
+    const int32_t* table = nullptr;  // [n_seq][cols]
+    int64_t cols = 0;
+    const int32_t* q_start = nullptr;
+    const int32_t* kv_len = nullptr;
+    int n_seq = 0, n_tokens = 0, window = 0;
+    int max_fresh = 0;  // most rows of one request as far as the caller knows (a hint); 0: not stated
+    float scale = 0.0f;
+};
+size_t paged_attention_workspace(const PagedAttn& p);
+hipError_t launch_paged_attention(const PagedAttn& p, void* part, uint32_t* counters, hipStream_t s);
+// Drafted tokens against the target's distributions (verify.hip).
+struct VerifyDrafts {
+    const void* logits = nullptr;        // rows of vocab values, logit_stride apart
+    const void* draft_logits = nullptr;  // or null: drafts are certain
+    int dtype = 0;                       // RT_HIP_F32 or RT_HIP_BF16
+    int64_t logit_stride = 0, draft_stride = 0;
+    const int32_t* tokens = nullptr;
+    const int32_t* row_start = nullptr;  // [n_seq + 1]
+    const float* accept_u = nullptr;     // [n_rows]
+    const float* sample_u = nullptr;     // [n_seq]
+    const float* temperature = nullptr;  // [n_seq] or null: 1
+    int32_t* out_tokens = nullptr;       // [n_seq][max_draft + 1]
+    int32_t* out_count = nullptr;        // [n_seq]
+    int vocab = 0, n_seq = 0, n_rows = 0, max_draft = 0;
+};
+size_t verify_drafts_workspace(const VerifyDrafts& p);
+hipError_t launch_verify_drafts(const VerifyDrafts& p, void* work, uint32_t* counters, hipStream_t s);
+
 // scratch false (BF16 W, k % 256 != 0): no library workspace.
 hipError_t launch_gemm(int w_fmt, const void* a, bool a_bf16, const void* w, const float* bias,
                        float* c, int64_t m, int64_t n, int64_t k, hipStream_t s, bool scratch = true);

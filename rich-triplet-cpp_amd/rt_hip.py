@@ -18,10 +18,17 @@ ROOT = os.path.dirname(HERE)
 LIB_PATH = os.environ.get("RT_HIP_LIB_PATH", os.path.join(HERE, "lib", "librt_hip.so"))
 HEADER_PATH = os.path.join(ROOT, "include", "rt_hip.h")
 
-F32, BF16, Q4K, Q4_0, Q4MAT, Q6K = 0, 1, 2, 3, 4, 5
+F32, BF16, Q4K, Q4_0, Q4MAT, Q6K, F16 = 0, 1, 2, 3, 4, 5, 6
 GEMV_MAX_M = 8
 
 _vp, _i64, _i32 = C.c_void_p, C.c_int64, C.c_int32
+
+
+class PagedKvStruct(C.Structure):
+    """rt_hip_paged_kv (include/rt_hip.h)."""
+    _fields_ = [("k", _vp), ("v", _vp), ("dtype", _i32), ("n_pages", _i32), ("page_size", _i32), ("n_kv_heads", _i32),
+                ("head_dim", _i32), ("page_stride", _i64)]
+
 
 # name -> argtypes (restype is int unless noted)
 _SIGNATURES = {
@@ -73,6 +80,13 @@ _SIGNATURES = {
     "rt_hip_gemv_q4mat": [_vp, _vp, _vp, _i64, _i64, _i32, _vp],
     "rt_hip_gemm": [_i32, _vp, _i32, _vp, _vp, _vp, _i64, _i64, _i64, _vp],
     "rt_hip_dequant": [_i32, _vp, _vp, _i32, _i64, _i64, _vp],
+    "rt_hip_paged_plan": [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp,
+                          _vp],
+    "rt_hip_paged_append": [C.POINTER(PagedKvStruct), _vp, _vp, _i32, _i64, _vp, _i32, _vp],
+    "rt_hip_paged_attention": [_vp, _i32, _i64, _i32, C.POINTER(PagedKvStruct), _vp, _i64, _vp, _vp, _i32, _i32, _i32,
+                               C.c_float, _i32, _vp, _i64, _vp],
+    "rt_hip_verify_drafts": [_vp, _i64, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp,
+                             _vp],
 }
 
 # name -> argtypes of the int64-returning size queries
@@ -86,6 +100,8 @@ _SIZE_SIGNATURES = {
     "rt_hip_flux_attention_workspace_bytes": [_i64, _i32, _i32],
     "rt_hip_q4mat_bytes": [_i64, _i64],
     "rt_hip_q4mat_scales_offset": [_i64, _i64],
+    "rt_hip_paged_attention_workspace_bytes": [C.POINTER(PagedKvStruct), _i32, _i32, _i32, _i32, _i32],
+    "rt_hip_verify_drafts_workspace_bytes": [_i32, _i32, _i32, _i32, _i32],
 }
 
 
@@ -653,6 +669,203 @@ def probe_read(buf, nbytes: int, workgroups: int, out, out_bytes: int = 0, strea
 def probe_empty(workgroups: int = 1, threads: int = 64, stream=None) -> None:
     """rt_hip_probe_empty: an empty kernel launch (calibration)."""
     library().call("rt_hip_probe_empty", workgroups, threads, _stream(stream))
+
+
+# ------------------------------------------- serving over a paged KV cache --
+
+def _value_type(t) -> int:
+    torch = _torch()
+    types = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+    if t.dtype not in types:
+        raise ValueError(f"rt_hip: {t.dtype} is not float32, float16 or bfloat16")
+    return types[t.dtype]
+
+
+def _want(t, name: str, dtype, shape) -> None:
+    """t is contiguous, on the GPU and of the given dtype and shape (None: any size)."""
+    if t.dtype != dtype:
+        raise ValueError(f"rt_hip: {name} must be {dtype}, not {t.dtype}")
+    if t.dim() != len(shape) or any(n is not None and a != n for a, n in zip(t.shape, shape)):
+        raise ValueError(f"rt_hip: {name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
+    _dev_check(t)
+
+
+def _rows(t, name: str, heads: int, dim: int) -> int:
+    """Stride in values between the rows of t [n, heads, dim], whose rows are dense."""
+    if not t.is_cuda:
+        raise ValueError("rt_hip: tensors must live on the GPU")
+    if t.dim() != 3 or tuple(t.shape[1:]) != (heads, dim):
+        raise ValueError(f"rt_hip: {name} must have shape (rows, {heads}, {dim}), not {tuple(t.shape)}")
+    if t.stride(2) != 1 or (heads > 1 and t.stride(1) != dim):
+        raise ValueError(f"rt_hip: the rows of {name} must be dense")
+    return t.stride(0) if t.shape[0] > 1 else heads * dim
+
+
+class _on:
+    """The device of t is current inside, and every tensor given lives on it."""
+
+    def __init__(self, t, *others):
+        for o in others:
+            if o is not None and o.device != t.device:
+                raise ValueError("rt_hip: tensors must live on one device")
+        self._guard = None if t.device.index == _torch().cuda.current_device() else _torch().cuda.device(t.device)
+
+    def __enter__(self):
+        if self._guard is not None:
+            self._guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self._guard is not None:
+            self._guard.__exit__(*exc)
+
+
+class PagedKV:
+    """A KV cache in pages: k and v [n_pages, page_size, n_kv_heads, head_dim]
+    of float32, float16 or bfloat16; pages are dense, with any one stride
+    between them (two halves of one tensor, say)."""
+
+    def __init__(self, k, v):
+        if not (k.is_cuda and v.is_cuda and k.device == v.device):
+            raise ValueError("rt_hip: the cache must live on one GPU")
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
+            raise ValueError("rt_hip: k and v must be [n_pages, page_size, n_kv_heads, head_dim] of one dtype")
+        n_pages, page, heads, dim = k.shape
+        dense = (heads * dim, dim, 1)
+        for t in (k, v):
+            if any(n > 1 and a != b for n, a, b in zip(t.shape[1:], t.stride()[1:], dense)):
+                raise ValueError("rt_hip: the pages of the cache must be dense")
+        stride = k.stride(0) if n_pages > 1 else page * heads * dim
+        if n_pages > 1 and v.stride(0) != stride:
+            raise ValueError("rt_hip: k and v must have one page stride")
+        self.k, self.v = k, v
+        self.struct = PagedKvStruct(k.data_ptr(), v.data_ptr(), _value_type(k), n_pages, page, heads, dim, stride)
+
+    @property
+    def device(self):
+        return self.k.device
+
+    def _ref(self):
+        return C.byref(self.struct)
+
+
+class PagedPlan:
+    """What paged_plan writes (int32 tensors): q_start [n_seq + 1], kv_len
+    [n_seq], slots and positions [tokens], and the state after the step, held
+    [n_seq] and queue_state [2]."""
+
+    def __init__(self, n_seq: int, tokens: int, device, held=None, queue_state=None):
+        torch = _torch()
+        buf = torch.empty(2 * n_seq + 1 + 2 * tokens, dtype=torch.int32, device=device)
+        self.q_start, self.kv_len, self.slots, self.positions = buf.split([n_seq + 1, n_seq, tokens, tokens])
+        self.held = torch.empty(n_seq, dtype=torch.int32, device=device) if held is None else held
+        self.queue_state = torch.empty(2, dtype=torch.int32, device=device) if queue_state is None else queue_state
+
+
+def paged_plan(cached, fresh, held, table, queue, queue_state, page_size: int, tokens: int, plan=None, stream=None):
+    """Pages, slots and positions of a step's new tokens; table and queue are
+    updated in place.  tokens: rows of the step (at least the sum of fresh).
+    plan: a PagedPlan of these sizes to write into; with its held and
+    queue_state the ones passed, the state is updated in place."""
+    torch = _torch()
+    n = cached.shape[0]
+    i32 = torch.int32
+    for t, name in ((cached, "cached"), (fresh, "fresh"), (held, "held")):
+        _want(t, name, i32, (n,))
+    _want(table, "table", i32, (n, None))
+    _want(queue, "queue", i32, (None,))
+    _want(queue_state, "queue_state", i32, (2,))
+    if plan is None:
+        plan = PagedPlan(n, tokens, cached.device)
+    else:
+        for t, name, size in ((plan.q_start, "q_start", n + 1), (plan.kv_len, "kv_len", n), (plan.slots, "slots", tokens),
+                              (plan.positions, "positions", tokens), (plan.held, "plan.held", n),
+                              (plan.queue_state, "plan.queue_state", 2)):
+            _want(t, name, i32, (size,))
+    with _on(cached, fresh, held, table, queue, queue_state, plan.q_start, plan.held, plan.queue_state):
+        library().call("rt_hip_paged_plan", _ptr(cached), _ptr(fresh), _ptr(held), _ptr(plan.held), _ptr(table),
+                       table.shape[1], _ptr(queue), _ptr(queue_state), _ptr(plan.queue_state), queue.shape[0], page_size,
+                       n, tokens, _ptr(plan.q_start), _ptr(plan.kv_len), _ptr(plan.slots), _ptr(plan.positions),
+                       _stream(stream))
+    return plan
+
+
+def paged_append(kv: PagedKV, k, v, slots, stream=None) -> None:
+    """Rows of k and v [tokens, n_kv_heads, head_dim] (slices of a joint
+    projection, say) into the cache at slots, rounded to its type."""
+    c = kv.struct
+    stride = _rows(k, "k", c.n_kv_heads, c.head_dim)
+    if k.shape != v.shape or k.dtype != v.dtype or _rows(v, "v", c.n_kv_heads, c.head_dim) != stride:
+        raise ValueError("rt_hip: k and v must have one shape, dtype and stride")
+    _want(slots, "slots", _torch().int32, (k.shape[0],))
+    with _on(kv, k, v, slots):
+        library().call("rt_hip_paged_append", kv._ref(), _ptr(k), _ptr(v), _value_type(k), stride, _ptr(slots),
+                       k.shape[0], _stream(stream))
+
+
+def paged_attention(q, kv: PagedKV, table, q_start, kv_len, scale: float, window: int = 0, max_fresh: int = 0, out=None,
+                    stream=None):
+    """Attention of the step's rows q [tokens, n_q_heads, head_dim] over the
+    pages; the cache's dtype, or float32 over any cache.  max_fresh: the most
+    new tokens of one request, where known.  Rows of out outside every request
+    are left as they were (a new out starts with zeros)."""
+    torch = _torch()
+    c = kv.struct
+    if q.dim() != 3:
+        raise ValueError("rt_hip: q must have shape (rows, n_q_heads, head_dim)")
+    if out is None:
+        out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+    if out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError("rt_hip: out must have q's shape and dtype")
+    heads, n = q.shape[1], kv_len.shape[0]
+    q_stride, out_stride = _rows(q, "q", heads, c.head_dim), _rows(out, "out", heads, c.head_dim)
+    _want(table, "table", torch.int32, (n, None))
+    _want(q_start, "q_start", torch.int32, (n + 1,))
+    _want(kv_len, "kv_len", torch.int32, (n,))
+    with _on(kv, q, table, q_start, kv_len, out):
+        library().call("rt_hip_paged_attention", _ptr(q), _value_type(q), q_stride, heads, kv._ref(), _ptr(table),
+                       table.shape[1], _ptr(q_start), _ptr(kv_len), n, q.shape[0], max_fresh, C.c_float(scale), window,
+                       _ptr(out), out_stride, _stream(stream))
+    return out
+
+
+def paged_attention_workspace_bytes(kv: PagedKV, dtype: int, n_q_heads: int, n_seq: int, tokens: int,
+                                    max_fresh: int = 0) -> int:
+    return int(library().lib.rt_hip_paged_attention_workspace_bytes(kv._ref(), dtype, n_q_heads, n_seq, tokens,
+                                                                    max_fresh))
+
+
+def verify_drafts(logits, tokens, row_start, accept_u, sample_u, max_draft: int, draft_logits=None, temperature=None,
+                  out=None, stream=None):
+    """Drafted tokens accepted or replaced: (out_tokens [n_seq, max_draft + 1],
+    out_count [n_seq]), int32.  logits and draft_logits [rows, vocab], float32
+    or bfloat16, rows dense with any stride; out: a pair to write into."""
+    torch = _torch()
+    rows, vocab = logits.shape
+    n = sample_u.shape[0]
+    for t, name in ((logits, "logits"), (draft_logits, "draft_logits")):
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError("rt_hip: tensors must live on the GPU")
+        if tuple(t.shape) != (rows, vocab) or t.dtype != logits.dtype or (vocab > 1 and t.stride(1) != 1):
+            raise ValueError(f"rt_hip: {name} must be dense rows ({rows}, {vocab}) of one dtype")
+    _want(tokens, "tokens", torch.int32, (rows,))
+    _want(row_start, "row_start", torch.int32, (n + 1,))
+    _want(accept_u, "accept_u", torch.float32, (rows,))
+    _want(sample_u, "sample_u", torch.float32, (n,))
+    if temperature is not None:
+        _want(temperature, "temperature", torch.float32, (n,))
+    if out is None:
+        out = (torch.empty((n, max_draft + 1), dtype=torch.int32, device=logits.device),
+               torch.empty(n, dtype=torch.int32, device=logits.device))
+    _want(out[0], "out tokens", torch.int32, (n, max_draft + 1))
+    _want(out[1], "out count", torch.int32, (n,))
+    row = [0 if t is None else (t.stride(0) if rows > 1 else vocab) for t in (logits, draft_logits)]
+    with _on(logits, draft_logits, tokens, row_start, accept_u, sample_u, temperature, *out):
+        library().call("rt_hip_verify_drafts", _ptr(logits), row[0], _ptr(draft_logits), row[1], _value_type(logits),
+                       vocab, _ptr(tokens), _ptr(row_start), _ptr(accept_u), _ptr(sample_u), _ptr(temperature), n, rows,
+                       max_draft, _ptr(out[0]), _ptr(out[1]), _stream(stream))
+    return out
 
 
 # ---------------------------------------------------------------- decoder --

@@ -1,0 +1,311 @@
+"""rt_hip_paged_attention against its definition in float64.
+
+Tolerances, from the roundings.  With A = sum_j p_j |v_j| for an output value
+o = sum_j p_j v_j, S the largest scale * sum |q_i k_i| of the row and n keys:
+ * a score is a sum of head_dim products in f32: at most head_dim roundings of
+   2^-24 relative to a partial sum, of which a quarter may add up, an error of
+   2^-24 head_dim S / 4; scaling, exponential and its argument (at most S +
+   log2 n) add 2^-24 (S + 32).  Each weight is off by that much, twice (itself
+   and the sum it is divided by).
+ * n additions of f32 to o and to the sum of weights: independent roundings, so
+   sqrt(n / 3) standard deviations of 2^-24 A; six of them are 3.5 sqrt(n) 2^-24.
+ * 16-bit types: each weight is rounded by eps / 2 of its type before it
+   multiplies v, at most eps / 2 A in all; and o by eps / 2 |o|.
+"""
+import math
+
+import pytest
+import torch
+
+from helpers import say
+
+pytestmark = pytest.mark.gpu
+
+DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+PAIRS = [("bf16", "bf16"), ("f16", "f16"), ("f32", "f32"), ("f32", "f16"), ("f32", "bf16")]
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+class Step:
+    """Random requests (rows, keys) over a cache whose unused slots hold NaN."""
+
+    def __init__(self, q, kv, heads, kv_heads, dim, page, lens, seed=0, window=0, q_scale=1.0, joint=False, behind=0,
+                 garbage=float("nan")):
+        self.page, self.window, self.dim, self.kv_heads, self.group = page, window, dim, kv_heads, heads // kv_heads
+        self.lens = lens
+        self.scale = 1.0 / math.sqrt(dim)
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        rows = sum(n for n, _ in lens) + behind
+        self.starts = [0]
+        for n, _ in lens:
+            self.starts.append(self.starts[-1] + n)
+        x = torch.randn((rows, heads + (2 * kv_heads if joint else 0), dim), generator=g, device="cuda") * q_scale
+        self.q = x.to(DT[q])[:, :heads]
+        self.out = torch.full((rows, heads + (1 if joint else 0), dim), -77.0, dtype=DT[q], device="cuda")[:, :heads]
+        held = [-(-n // page) for _, n in lens]
+        n_pages = sum(held) + 3
+        ids = torch.randperm(n_pages, generator=g, device="cuda").tolist()
+        cols = max(held) + 2
+        table, at = [], 0
+        for h in held:
+            table.append(ids[at:at + h] + [-1, 2**31 - 1, 10**6][:1] * (cols - h))
+            at += h
+        self.table = i32(table)
+        shape = (n_pages, 2, page, kv_heads, dim) if joint else (2, n_pages, page, kv_heads, dim)
+        both = torch.randn(shape, generator=g, device="cuda").to(DT[kv])
+        self.k, self.v = (both[:, 0], both[:, 1]) if joint else (both[0], both[1])
+        used = torch.zeros((n_pages, page), dtype=torch.bool, device="cuda")
+        for row, (_, n) in zip(table, lens):
+            for c in range(-(-n // page)):
+                used[row[c], :min(page, n - c * page)] = True
+        for t in (self.k, self.v):
+            t[~used] = garbage
+        self.kv = None
+
+    def keys(self, s):
+        """Keys and values of request s in float64, zeros on pages that are none."""
+        n = self.lens[s][1]
+        ids = self.table[s, :-(-n // self.page)].long()
+        bad = (ids < 0) | (ids >= self.k.shape[0])
+        out = []
+        for t in (self.k, self.v):
+            x = t[ids.clamp(0, self.k.shape[0] - 1)].double()
+            x[bad] = 0.0
+            out.append(x.reshape(-1, self.kv_heads, self.dim)[:n])
+        return out
+
+    def run(self, rt, out=None, max_fresh=0, stream=None):
+        self.kv = self.kv or rt.PagedKV(self.k, self.v)
+        out = self.out if out is None else out
+        return rt.paged_attention(self.q, self.kv, self.table, i32(self.starts), i32([n for _, n in self.lens]), self.scale,
+                                  window=self.window, max_fresh=max_fresh, out=out, stream=stream)
+
+    def reference(self):
+        """(expected, tolerance), float64, rows of all requests."""
+        want = torch.zeros(self.q.shape, dtype=torch.float64, device="cuda")
+        tol = torch.zeros_like(want)
+        small = self.q.dtype != torch.float32
+        eps = torch.finfo(self.q.dtype).eps / 2 if small else 0.0
+        for s, (n, length) in enumerate(self.lens):
+            if n == 0:
+                continue
+            k, v = self.keys(s)
+            at = torch.arange(length - n, length, device="cuda")[:, None]
+            j = torch.arange(length, device="cuda")[None]
+            seen = j <= at
+            if self.window:
+                seen &= j > at - self.window
+            for h in range(self.kv_heads):
+                for i in range(self.group):
+                    head = h * self.group + i
+                    q = self.q[self.starts[s]:self.starts[s + 1], head].double()
+                    # rows and keys apart, so that what a row does not see cannot reach it
+                    score = torch.where(seen, (q @ k[:, h].T) * self.scale, -math.inf)
+                    size = torch.where(seen, (q.abs() @ k[:, h].abs().T) * self.scale, 0.0)
+                    rows = slice(self.starts[s], self.starts[s + 1])
+                    if length == 0:
+                        continue
+                    p = torch.softmax(score, 1)
+                    p = torch.where(seen.any(1, keepdim=True), p, 0.0)
+                    vh = v[:, h]
+                    if torch.isfinite(vh).all():
+                        o, a = p @ vh, p @ vh.abs()
+                    else:
+                        o = torch.stack([(r[m][:, None] * vh[m]).sum(0) for r, m in zip(p, seen)])
+                        a = torch.stack([(r[m][:, None] * vh[m].abs()).sum(0) for r, m in zip(p, seen)])
+                    big = size.amax(1, keepdim=True) if length else size.sum(1, keepdim=True)
+                    err = 2.0**-24 * (2 * (self.dim * big / 4 + big + 32) + 3.5 * math.sqrt(length)) + eps
+                    want[rows, head] = o
+                    tol[rows, head] = err * a + (torch.finfo(self.q.dtype).eps / 2) * o.abs() + 1e-30
+                    if self.q.dtype == torch.float16:
+                        tol[rows, head] += 2.0**-25  # below 2^-14 f16 has steps of 2^-24
+        return want, tol
+
+    def check(self, rt, max_fresh=0):
+        got = self.run(rt, max_fresh=max_fresh).double()
+        rows = self.starts[-1]
+        want, tol = self.reference()
+        bad = ~((got[:rows] - want[:rows]).abs() <= tol[:rows])
+        assert not bad.any(), (int(bad.sum()), (got[:rows] - want[:rows]).abs().max().item(), torch.nonzero(bad)[:3].tolist())
+        assert (got[rows:] == -77.0).all()
+
+
+RAGGED = [(1, 1), (1, 5), (3, 3), (7, 100), (1, 63), (1, 64), (1, 65), (2, 200), (0, 50), (33, 64), (64, 65), (1, 0), (5, 3),
+          (9, 0), (0, 0), (130, 300), (1, 1000), (16, 16)]
+
+
+@pytest.mark.parametrize("q, kv", PAIRS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("kv_heads, group, page, window", [
+    (1, 1, 16, 0), (2, 3, 8, 0), (1, 4, 64, 7), (3, 5, 32, 1), (2, 8, 128, 100), (1, 16, 16, 65), (8, 1, 1024, 0)])
+def test_ragged(rt, q, kv, dim, kv_heads, group, page, window):
+    """Single tokens, drafts and chunks in one step, requests without rows or keys, fewer keys than rows, rows behind."""
+    say("ragged", q, kv, dim, kv_heads, group, page, window)
+    Step(q, kv, kv_heads * group, kv_heads, dim, page, RAGGED, seed=dim + group, window=window, behind=3,
+         joint=page == 32).check(rt)
+
+
+@pytest.mark.parametrize("q, kv", PAIRS)
+@pytest.mark.parametrize("hint", [0, 1, 4, 1000])
+def test_hint_is_only_a_hint(rt, q, kv, hint):
+    """max_fresh right, wrong or missing: the same requests within the same tolerance."""
+    say("hint", q, kv, hint)
+    Step(q, kv, 6, 2, 128, 16, [(1, 700), (40, 333), (1, 2), (4, 90)], window=0).check(rt, max_fresh=hint)
+    Step(q, kv, 6, 2, 64, 16, [(300, 700)], window=50).check(rt, max_fresh=hint)
+    Step(q, kv, 6, 2, 64, 16, [(1, 3000)]).check(rt, max_fresh=hint)
+
+
+@pytest.mark.parametrize("q, kv", PAIRS)
+@pytest.mark.parametrize("kv_heads, group, dim, lens, window", [
+    (1, 1, 128, [(1, 40000)], 0), (8, 3, 128, [(1, 9001), (1, 17)], 0), (1, 8, 256, [(3, 20000)], 0),
+    (2, 2, 64, [(5, 30000), (1, 12000)], 5000), (2, 3, 128, [(700, 2100)], 0), (1, 2, 256, [(513, 1500), (1, 9)], 300),
+    (4, 4, 64, [(1000, 1000), (200, 5000)], 0)])
+def test_long(rt, q, kv, kv_heads, group, dim, lens, window):
+    """Long caches whose keys are cut between workgroups, chunks over long caches."""
+    say("long", q, kv, kv_heads, group, dim, lens, window)
+    Step(q, kv, kv_heads * group, kv_heads, dim, 16, lens, seed=7, window=window).check(rt)
+
+
+@pytest.mark.parametrize("q, kv", PAIRS)
+def test_many_requests(rt, q, kv):
+    """More requests than a workgroup has threads."""
+    say("many", q, kv)
+    lens = [(1 + i % 3, 3 + (i * 37) % 150) for i in range(1100)]
+    Step(q, kv, 2, 1, 64, 8, lens, seed=3).check(rt)
+
+
+@pytest.mark.parametrize("q, kv", PAIRS)
+def test_sharp_scores(rt, q, kv):
+    """Scores far apart: the maximum moves and the weights of most keys vanish."""
+    say("sharp", q, kv)
+    Step(q, kv, 4, 2, 128, 16, [(1, 3000), (90, 400), (6, 64)], seed=2, q_scale=12.0).check(rt)
+
+
+@pytest.mark.parametrize("q, kv", PAIRS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_what_a_row_does_not_see(rt, q, kv, dim, bad):
+    """Infinities and NaN in keys and values of positions that come later, or lie before the window: the rows that do
+    not see them are as without them, those that do are NaN or infinite."""
+    say("unseen", q, kv, dim, bad)
+    for lens, window, at in (([(40, 90)], 0, 70), ([(8, 70)], 0, 66), ([(90, 200)], 16, 130), ([(3, 300)], 100, 199),
+                             ([(1, 300)], 100, 199), ([(200, 400)], 33, 300)):
+        st = Step(q, kv, 3, 1, dim, 16, lens, seed=5, window=window)
+        n, length = lens[0]
+        pos = torch.arange(length - n, length, device="cuda")
+        sees = (pos >= at) & ((pos < at + window) if window else True)
+        clean = st.run(rt).clone()
+        page = st.table[0, at // 16]
+        for t, name in ((st.v, "v"), (st.k, "k")):
+            saved = t[page, at % 16].clone()
+            t[page, at % 16, 0, 3:dim:7] = bad
+            got = st.run(rt)
+            # (a sum may be split otherwise than without them, by rounding)
+            want, tol = st.reference()
+            ok = ((got.double() - want).abs() <= tol) | (got.double() == want) | (torch.isnan(got) & torch.isnan(want))
+            assert ok[~sees].all(), (name, lens)
+            assert torch.equal(torch.isfinite(got[~sees]), torch.isfinite(clean[~sees]))
+            if name == "v":
+                assert not torch.isfinite(got[sees][..., 3:dim:7]).any()
+                assert torch.isfinite(got[sees][..., 4:dim:7]).all()
+            elif math.isnan(bad):
+                assert torch.isnan(got[sees]).all()
+            t[page, at % 16] = saved
+
+
+@pytest.mark.parametrize("q, kv", PAIRS)
+def test_garbage_tables(rt, q, kv):
+    """Pages that are none of the cache's count as zeros; starts and lengths that make no sense touch nothing else."""
+    say("tables", q, kv)
+    st = Step(q, kv, 4, 2, 128, 16, [(2, 90), (50, 200), (1, 33)], seed=4)
+    st.table[0, 2], st.table[1, 0], st.table[1, 7], st.table[2, 2] = -1, st.k.shape[0], 2**31 - 1, -2**31
+    st.check(rt)
+    # lengths past the table's row are cut to it, starts to the rows there are
+    st.table.clamp_(0, st.k.shape[0] - 1)
+    st.k.nan_to_num_(0.5), st.v.nan_to_num_(0.5)
+    kvs = rt.PagedKV(st.k, st.v)
+    for starts, lens in (([0, 2, 52, 53], [90, 2**31 - 1, -5]), ([0, 1000, 20, 53], [90, 200, 33]),
+                         ([-7, 2, 2**31 - 1, -2**31], [10**9, 10**9, 10**9])):
+        out = rt.paged_attention(st.q, kvs, st.table, i32(starts), i32(lens), st.scale)
+        assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("q, kv", PAIRS)
+def test_same_bits(rt, q, kv):
+    """The same call twice, and on another stream: the same bits."""
+    say("bits", q, kv)
+    st = Step(q, kv, 6, 2, 128, 16, [(1, 9000), (300, 900), (4, 77)], seed=9)
+    a = st.run(rt, out=torch.zeros_like(st.out))
+    b = st.run(rt, out=torch.zeros_like(st.out))
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        c = st.run(rt, out=torch.zeros_like(st.out))
+    torch.cuda.synchronize()
+    assert torch.equal(a, b) and torch.equal(a, c)
+
+
+@pytest.mark.parametrize("q, kv", PAIRS)
+def test_captured(rt, q, kv):
+    """A captured call, replayed over other lengths, starts and tables between eager work: eager's bits each time."""
+    say("captured", q, kv)
+    rows, n = 64, 5
+    st = Step(q, kv, 6, 2, 128, 16, [(20, 3000), (1, 500), (3, 3), (30, 64), (0, 9)], seed=1, behind=rows - 54)
+    kvs = rt.PagedKV(st.k, st.v)
+    dt = {"f32": rt.F32, "f16": rt.F16, "bf16": rt.BF16}[q]
+    rt.reserve_workspace(rt.paged_attention_workspace_bytes(kvs, dt, 6, n, rows))
+    starts, lens = i32(st.starts), i32([x for _, x in st.lens])
+    out = torch.zeros_like(st.out)
+    call = lambda o: rt.paged_attention(st.q, kvs, st.table, starts, lens, st.scale, out=o)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(out)
+    for a, b in (([0, 20, 21, 24, 54, 54], [3000, 500, 3, 64, 9]), ([0, 1, 2, 3, 4, 5], [2900, 490, 2, 64, 9]),
+                 ([0, 0, 60, 60, 61, 61], [3000, 200, 1, 33, 0])):
+        starts.copy_(i32(a)), lens.copy_(i32(b))
+        for _ in range(3):
+            out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            eager = call(torch.zeros_like(out))
+            assert torch.equal(out, eager)
+
+
+def test_offsets_past_32_bits(rt):
+    """A cache of more than 2^32 bytes, the request's pages at its end."""
+    heads, dim, page = 8, 256, 128
+    pages = (5 << 30) // (page * heads * dim * 2)
+    k = torch.zeros((pages, page, heads, dim), dtype=torch.bfloat16, device="cuda")
+    v = torch.zeros_like(k)
+    ids = [pages - 1, 0, pages - 2]
+    for t in (k, v):
+        for i in ids:
+            t[i] = torch.randn(t[i].shape, device="cuda").bfloat16()
+    q = torch.randn((2, heads, dim), device="cuda").bfloat16()
+    args = (i32([0, 2]), i32([300]), 0.06)
+    far = rt.paged_attention(q, rt.PagedKV(k, v), i32([ids]), *args)
+    near = rt.paged_attention(q, rt.PagedKV(k[ids].clone(), v[ids].clone()), i32([[0, 1, 2]]), *args)
+    assert torch.equal(far, near) and far.abs().max() > 0
+
+
+def test_another_head_layouts_refusals(rt):
+    st = Step("bf16", "bf16", 4, 2, 64, 16, [(2, 20)])
+    kvs = rt.PagedKV(st.k, st.v)
+    args = (st.table, i32(st.starts), i32([20]), 0.1)
+    with pytest.raises(rt.RtHipError):
+        rt.paged_attention(st.q[:, :3].contiguous(), kvs, *args)
+    with pytest.raises(rt.RtHipError):
+        rt.paged_attention(st.q.half(), kvs, *args)
+    with pytest.raises(ValueError):
+        rt.paged_attention(st.q.transpose(0, 1), kvs, *args)
+    with pytest.raises(ValueError):
+        rt.paged_attention(st.q, kvs, st.table.long(), *args[1:])
+    with pytest.raises(ValueError):
+        rt.PagedKV(st.k, st.v[:, :8])
+    with pytest.raises(ValueError):
+        rt.PagedKV(st.k.transpose(1, 2), st.v.transpose(1, 2))

@@ -1,0 +1,149 @@
+"""Arguments that the calls of batched serving refuse: a status and a message,
+before anything reaches the device (no GPU needed)."""
+import ctypes as C
+
+import pytest
+
+from conftest import load_package
+
+ARG, SHAPE, ALIGN, UNSUPPORTED = 1, 2, 3, 6
+
+
+@pytest.fixture(scope="module")
+def rt():
+    return load_package().rt_hip
+
+
+@pytest.fixture(scope="module")
+def mem():
+    """Addresses of 24 separate, 16-byte aligned pieces of 4096 bytes."""
+    buf = C.create_string_buffer(24 * 4096 + 64)
+    base = (C.addressof(buf) + 63) & ~63
+    yield [base + 4096 * i for i in range(24)]
+    del buf
+
+
+def cache(rt, mem, **over):
+    args = dict(k=mem[20], v=mem[22], dtype=rt.F16, n_pages=2, page_size=8, n_kv_heads=1, head_dim=64, page_stride=0)
+    args.update(over)
+    return C.byref(rt.PagedKvStruct(**args))
+
+
+def plan(rt, m, **over):
+    a = dict(cached=m[0], fresh=m[1], held=m[2], held_out=m[3], table=m[4], cols=4, queue=m[5], state=m[6], state_out=m[7],
+             n_pages=8, page=16, n_seq=3, n_tokens=5, q_start=m[8], kv_len=m[9], slots=m[10], positions=m[11])
+    a.update(over)
+    return rt.library().status("rt_hip_paged_plan", *a.values(), None)
+
+
+def append(rt, m, **over):
+    a = dict(kv=cache(rt, m), k=m[0], v=m[1], dtype=rt.F32, stride=64, slots=m[2], n=4)
+    a.update(over)
+    return rt.library().status("rt_hip_paged_append", *a.values(), None)
+
+
+def attention(rt, m, **over):
+    a = dict(q=m[0], dtype=rt.F16, q_stride=128, heads=2, kv=cache(rt, m), table=m[1], cols=2, q_start=m[2], kv_len=m[3],
+             n_seq=2, n_tokens=4, max_fresh=0, scale=C.c_float(0.1), window=0, out=m[4], out_stride=128)
+    a.update(over)
+    return rt.library().status("rt_hip_paged_attention", *a.values(), None)
+
+
+def verify(rt, m, **over):
+    a = dict(logits=m[0], stride=50, draft=m[1], draft_stride=50, dtype=rt.F32, vocab=50, tokens=m[2], row_start=m[3],
+             accept=m[4], sample=m[5], temp=m[6], n_seq=2, n_rows=6, max_draft=2, out=m[7], count=m[8])
+    a.update(over)
+    return rt.library().status("rt_hip_verify_drafts", *a.values(), None)
+
+
+@pytest.mark.parametrize("over, code", [
+    (dict(n_seq=-1), ARG), (dict(n_tokens=-1), ARG), (dict(n_seq=4097), SHAPE), (dict(cached=None), ARG),
+    (dict(slots=None), ARG), (dict(queue=None), ARG), (dict(page=12), SHAPE), (dict(page=4), SHAPE),
+    (dict(page=2048), SHAPE), (dict(n_pages=0), ARG | SHAPE), (dict(n_pages=1 << 27), SHAPE), (dict(cols=0), ARG),
+    (dict(cols=1 << 30), SHAPE), (dict(table=None), ARG)])
+def test_plan_refuses(rt, mem, over, code):
+    assert plan(rt, mem, **over) in ((ARG, SHAPE) if code == ARG | SHAPE else (code,))
+    assert b"rt_hip_paged_plan" in rt.library().lib.rt_hip_last_error()
+
+
+@pytest.mark.parametrize("a, b", [("held_out", "cached"), ("slots", "positions"), ("table", "queue"), ("kv_len", "fresh"),
+                                  ("state_out", "held"), ("q_start", "kv_len")])
+def test_plan_refuses_overlap(rt, mem, a, b):
+    names = dict(cached=0, fresh=1, held=2, held_out=3, table=4, queue=5, state=6, state_out=7, q_start=8, kv_len=9,
+                 slots=10, positions=11)
+    assert plan(rt, mem, **{a: mem[names[b]]}) == ARG
+
+
+@pytest.mark.parametrize("over, code", [
+    (dict(dtype=2), UNSUPPORTED), (dict(n=-1), ARG), (dict(k=None), ARG), (dict(slots=None), ARG), (dict(stride=63), ARG),
+    (dict(stride=66), ALIGN), (dict(n=1 << 30), SHAPE)])
+def test_append_refuses(rt, mem, over, code):
+    assert append(rt, mem, **over) == code
+    assert append(rt, mem, k=mem[0] + 8) == ALIGN
+    assert append(rt, mem, v=mem[20]) == ARG  # rows inside the cache
+
+
+@pytest.mark.parametrize("over, code", [
+    (dict(k=None), ARG), (dict(dtype=2), UNSUPPORTED), (dict(page_size=24), SHAPE), (dict(head_dim=96), SHAPE),
+    (dict(n_kv_heads=0), SHAPE), (dict(n_pages=0), SHAPE), (dict(page_stride=511), ARG), (dict(page_stride=516), ALIGN),
+    (dict(n_pages=1 << 28), SHAPE)])
+def test_cache_refused_everywhere(rt, mem, over, code):
+    assert append(rt, mem, kv=cache(rt, mem, **over)) == code
+    assert attention(rt, mem, kv=cache(rt, mem, **over)) == code
+    assert append(rt, mem, kv=None) == ARG
+    assert attention(rt, mem, kv=cache(rt, mem, v=mem[22] + 2)) == ALIGN
+
+
+@pytest.mark.parametrize("over, code", [
+    (dict(q=None), ARG), (dict(dtype=1), UNSUPPORTED), (dict(dtype=2), UNSUPPORTED), (dict(heads=0), SHAPE),
+    (dict(heads=1025), SHAPE), (dict(n_seq=4097), SHAPE), (dict(n_seq=-1), ARG), (dict(n_tokens=-2), ARG),
+    (dict(max_fresh=-1), ARG), (dict(scale=C.c_float(0.0)), ARG), (dict(scale=C.c_float(-1.0)), ARG),
+    (dict(scale=C.c_float(float("nan"))), ARG), (dict(scale=C.c_float(float("inf"))), ARG), (dict(window=-1), ARG),
+    (dict(q_stride=127), ARG), (dict(out_stride=64), ARG), (dict(q_stride=129), ALIGN), (dict(cols=0), ARG),
+    (dict(table=None), ARG), (dict(kv_len=None), ARG), (dict(n_tokens=0x7fffffff), SHAPE)])
+def test_attention_refuses(rt, mem, over, code):
+    assert attention(rt, mem, **over) == code
+    assert b"rt_hip_paged_attention" in rt.library().lib.rt_hip_last_error()
+
+
+def test_attention_refuses_overlap_and_heads(rt, mem):
+    assert attention(rt, mem, out=mem[0] + 16) == ARG
+    assert attention(rt, mem, out=mem[22]) == ARG
+    assert attention(rt, mem, kv=cache(rt, mem, n_kv_heads=2, n_pages=1), heads=3, q_stride=192, out_stride=192) == SHAPE
+    assert attention(rt, mem, q=mem[0] + 4) == ALIGN
+    lib = rt.library().lib
+    assert lib.rt_hip_paged_attention_workspace_bytes(cache(rt, mem), rt.BF16, 2, 1, 1, 1) == -1
+    assert lib.rt_hip_paged_attention_workspace_bytes(cache(rt, mem), rt.F16, 2, 0, 0, 0) == 0
+
+
+@pytest.mark.parametrize("over, code", [
+    (dict(dtype=6), UNSUPPORTED), (dict(vocab=0), ARG), (dict(vocab=(1 << 20) + 1, stride=1 << 21), SHAPE),
+    (dict(n_seq=-1), ARG), (dict(n_rows=-1), ARG), (dict(max_draft=-1), ARG), (dict(max_draft=256), SHAPE),
+    (dict(n_seq=4000, max_draft=20), SHAPE), (dict(logits=None), ARG), (dict(tokens=None), ARG), (dict(out=None), ARG),
+    (dict(sample=None), ARG), (dict(stride=49), ARG), (dict(draft_stride=49), ARG)])
+def test_verify_refuses(rt, mem, over, code):
+    assert verify(rt, mem, **over) == code
+    assert verify(rt, mem, logits=mem[0] + 2) == ALIGN
+    assert verify(rt, mem, out=mem[2]) == ARG
+    assert verify(rt, mem, count=mem[7] + 4) == ARG
+    assert rt.library().lib.rt_hip_verify_drafts_workspace_bytes(0, 1, 1, 1, 0) == -1
+
+
+def test_nothing_to_do(rt, mem):
+    """No rows or no requests: accepted without a launch."""
+    assert append(rt, mem, n=0, k=None, v=None, slots=None) == 0
+    assert attention(rt, mem, n_tokens=0) == 0
+    assert attention(rt, mem, n_seq=0) == 0
+    assert verify(rt, mem, n_seq=0) == 0
+
+
+def test_binding_checks_before_it_calls(rt):
+    """The Python binding refuses what the C call could not see: CPU tensors, dtypes, shapes, strides."""
+    import torch
+    k = torch.zeros(2, 8, 1, 64, dtype=torch.float16)
+    with pytest.raises(ValueError, match="GPU"):
+        rt.PagedKV(k, k)
+    with pytest.raises(ValueError, match="int32"):
+        rt.paged_plan(torch.zeros(2), torch.zeros(2), torch.zeros(2), None, None, None, 16, 4)
+    with pytest.raises(ValueError, match="GPU"):
+        rt.verify_drafts(torch.zeros(3, 9), None, None, None, torch.zeros(1), 1)
