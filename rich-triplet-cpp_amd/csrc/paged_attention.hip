@@ -1,86 +1,1095 @@
 // paged_attention.hip -- attention of the new tokens of many requests over a
 // KV cache in pages.
 //
-// Row i of request s (n rows, kv_len keys) has position kv_len - n + i and
-// sees the keys (position - window, position]:
+// Row i of request s (n rows, len keys) has position len - n + i and sees the
+// keys (position - window, position]:
 //   out = sum_j softmax_j(scale q . k_j) v_j,
 // zeros where it sees none.  Key j of the request is row j % page of page
 // table[s][j / page].
 //
-// One wave per (row, head): lane l holds values l, l + 64, .. of q and of the
-// accumulator, and takes the keys one by one with an online softmax.
+// Work.  The rows of one request that share a KV head, (token, head of the
+// group) in that order, are taken in blocks; an item is (request, KV head,
+// block) and its tiles are the spans of keys the block's rows can see.  The
+// sequence of all tiles of all items is cut into equal ranges, one per
+// workgroup: the lengths are read on the device, so nothing is known of them
+// when the launch is made, and a batch of very unequal requests still ends
+// everywhere at once.  A workgroup finds its range by summing the requests'
+// tiles itself.  An item cut between workgroups leaves its states (o, m, l) in
+// the workspace; the last to arrive joins them in order, so results do not
+// depend on who that is.
+//
+// Arithmetic.  Products on the matrix cores, online softmax per row:
+//  * S^T = K Q^T, so that a lane holds one row's scores against several keys:
+//    the row's maximum and sum are the lane's own and its partners' in the
+//    other halves (32x32) or quarters (16x16) of the wave.
+//  * O^T += V^T P^T: the lane that has a row's weights supplies them as they
+//    are, for the keys its registers hold; V's fragments are read from LDS
+//    transposed (ds_read_b64_tr_b16) for the same keys.
+//  * 16-bit rows of q: products of 16-bit values, weights rounded to the type.
+//    f16 weights are kept times 2^6, so that a weight of 2^-20 of the largest
+//    still has all its bits.
+//  * f32 rows over a 16-bit cache: q and the weights as limbs of the cache's
+//    type, two of f16 (22 bits; q's row times a power of two that puts its
+//    largest value at 2^14) or three of bf16 (24 bits), each multiplied with
+//    the exact values of the cache.
+//  * an f32 cache: f32 matrix steps.
+//
+// Keys a row does not see get weight 0, but 0 times an infinity or a NaN of
+// their v would reach the row: in tiles with such pairs those values of v are
+// made 0 in LDS, and added at the end to the rows that see them.
 #include "rt_common.hpp"
 #include "rt_launch.hpp"
 
 namespace rt_hip {
 namespace {
 
-constexpr float kLog2e = 1.44269504088896341f;
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-template <class Q, class T, int HD>
-__global__ __launch_bounds__(64) void k_paged_attn(PagedAttn p) {
-    constexpr int N = HD / 64;
-    const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-    int s = 0;
-    while (s < p.n_seq && p.q_start[s + 1] <= t) ++s;
-    if (s == p.n_seq || t < p.q_start[s]) return;
-    const int cap = static_cast<int>(p.cols << p.kv.page_shift);
-    const int len = min(max(p.kv_len[s], 0), cap);
-    const int pos = len - (p.q_start[s + 1] - t);
-    const int from = p.window ? max(0, pos - p.window + 1) : 0;
-    const int kvh = h / (p.n_q / p.kv.n_kv);
-    const int64_t row = static_cast<int64_t>(p.kv.n_kv) * HD;
-    float q[N], o[N], m = -__builtin_inff(), l = 0.0f;
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-        q[e] = static_cast<float>(static_cast<const Q*>(p.q)[t * p.q_stride + h * HD + e * 64 + lane]) * (p.scale * kLog2e);
-        o[e] = 0.0f;
-    }
-    for (int j = from; j <= pos; ++j) {
-        const int page = p.table[s * p.cols + (j >> p.kv.page_shift)];
-        const bool ok = static_cast<uint32_t>(page) < static_cast<uint32_t>(p.kv.n_pages);
-        const int64_t at = (ok ? page : 0) * p.kv.page_stride + (j & ((1 << p.kv.page_shift) - 1)) * row + kvh * HD + lane;
-        float d = 0.0f, v[N];
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-            d += q[e] * (ok ? static_cast<float>(static_cast<const T*>(p.kv.k)[at + e * 64]) : 0.0f);
-            v[e] = ok ? static_cast<float>(static_cast<const T*>(p.kv.v)[at + e * 64]) : 0.0f;
-        }
-        d = segment_sum<64>(d);
-        const float mn = fmaxf(m, d), mu = mn == -__builtin_inff() ? 0.0f : mn;
-        const float a = __builtin_amdgcn_exp2f(m - mu), b = __builtin_amdgcn_exp2f(d - mu);
-        l = l * a + b;
-#pragma unroll
-        for (int e = 0; e < N; ++e) o[e] = o[e] * a + b * v[e];
-        m = mn;
-    }
-#pragma unroll
-    for (int e = 0; e < N; ++e)
-        static_cast<Q*>(p.out)[t * p.out_stride + h * HD + e * 64 + lane] = static_cast<Q>(l == 0.0f ? 0.0f : o[e] / l);
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kInf = __builtin_inff();
+
+#define LDS_AS __attribute__((address_space(3)))
+#define GLOBAL_AS __attribute__((address_space(1)))
+#define CONST_AS __attribute__((address_space(4)))
+
+// A page of the cache that is none: its keys and values (at most one row of
+// 256 f32 is read, every row from the same place).
+__device__ const __attribute__((aligned(16))) float kZeros[256] = {};
+
+template <class T> struct KindOf;
+template <> struct KindOf<float> { static constexpr bool f32 = true, f16 = false; };
+template <> struct KindOf<_Float16> { static constexpr bool f32 = false, f16 = true; };
+template <> struct KindOf<__bf16> { static constexpr bool f32 = false, f16 = false; };
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+__device__ __forceinline__ void st_dev(float* p, float v) {
+    __hip_atomic_store((GLOBAL_AS float*)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float ld_dev(const float* p) {
+    return __hip_atomic_load((const GLOBAL_AS float*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-template <class Q, class T>
-hipError_t run(const PagedAttn& p, hipStream_t s) {
-    const dim3 grid(static_cast<unsigned>(p.n_tokens), static_cast<unsigned>(p.n_q));
-    switch (p.kv.head_dim) {
-        case 64: hipLaunchKernelGGL((k_paged_attn<Q, T, 64>), grid, dim3(64), 0, s, p); break;
-        case 128: hipLaunchKernelGGL((k_paged_attn<Q, T, 128>), grid, dim3(64), 0, s, p); break;
-        default: hipLaunchKernelGGL((k_paged_attn<Q, T, 256>), grid, dim3(64), 0, s, p); break;
+// Two f32 to 16 bits each (nearest even), and back.
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (KindOf<T>::f16) return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2));
+    else return bf16_pair(a, b);
+}
+template <class T>
+__device__ __forceinline__ f32x2 unpack2(uint32_t w) {
+    if constexpr (KindOf<T>::f16) return __builtin_convertvector(__builtin_bit_cast(f16x2, w), f32x2);
+    else return f32x2{bf16_lo_to_f32(w), bf16_hi_to_f32(w)};
+}
+
+// N steps that each read a fragment from LDS and use it, B reads ahead of the
+// uses; the scheduling barriers keep the compiler from moving all the reads to
+// the front, into registers that the accumulators need.
+template <class F, int N, int B, class R, class U>
+__device__ __forceinline__ void read_ahead(R read, U use) {
+    static_assert(N % B == 0, "whole batches");
+    F f[2][B];
+#pragma unroll
+    for (int x = 0; x < B; ++x) f[0][x] = read(x);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int g = 0; g < N / B; ++g) {
+        if (g + 1 < N / B) {
+#pragma unroll
+            for (int x = 0; x < B; ++x) f[(g + 1) & 1][x] = read((g + 1) * B + x);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int x = 0; x < B; ++x) use(g * B + x, f[g & 1][x]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// A value that every lane of the wave holds, in a scalar register.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
+    const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
+    return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// 16 bytes a lane from memory to LDS at dst + 16 lane.  (In assembly, without a
+// result: after the builtin the compiler waits for all such copies before it
+// reads anything transposed from LDS.  The kernels wait themselves.  M0 needs
+// a wait state before the copy.)
+__device__ __forceinline__ void copy_to_lds(const uint8_t* src, uint32_t offset, uint32_t dst) {
+    src = reinterpret_cast<const uint8_t*>(uniform(static_cast<int64_t>(reinterpret_cast<uintptr_t>(src))));
+    dst = static_cast<uint32_t>(uniform(static_cast<int>(dst)));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(offset), "s"(src) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const LDS_AS void*)p));
+}
+
+template <class V>
+__device__ __forceinline__ V lds_read(uint32_t at) {
+    return *(const LDS_AS V*)(static_cast<uintptr_t>(at));
+}
+// A lane's number that the compiler must take as new here: what is derived from
+// it (addresses of fragments) is then derived again for every tile, instead of
+// being kept in registers that the accumulators need.
+__device__ __forceinline__ uint32_t anew(uint32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+// The core of both kernels: DB rows of queries per block, RBLK blocks a wave,
+// DB x DB matrix steps (DB = 32 or 16), tiles of BK keys.
+template <class Q, class T, int HD, int DB, int RBLK, int BK>
+struct Core {
+    static constexpr bool F32 = KindOf<T>::f32, F16 = KindOf<T>::f16;
+    static constexpr int NL = F32 || sizeof(Q) == 2 ? 1 : (F16 ? 2 : 3);  // limbs of q and of the weights
+    static constexpr int RB = HD * static_cast<int>(sizeof(T));           // bytes of a key
+    static constexpr int CPR = RB / 16, RPI = 64 / CPR;  // 16-byte chunks of a key, keys a wave's copy takes
+    static constexpr int KG = 64 / DB, EL = 16 / static_cast<int>(sizeof(T));  // lane groups of a step, values of a chunk
+    static constexpr int STEPS = CPR / KG, NC = HD / DB, KB = BK / DB, ACC = DB == 32 ? 16 : 4;
+    static constexpr int KS = DB == 32 ? 16 : 32;  // keys of a 16-bit step of P V
+    static constexpr int TB = BK * RB;             // bytes of a tile of K or V
+    // Weights are kept times 2^kBias, and the running maximum may lag by 2^kLag.
+    static constexpr int kBias = F16 ? 6 : 0;
+    static constexpr float kLag = 8.0f;
+    using Acc = typename std::conditional<DB == 32, f32x16, f32x4>::type;
+
+    u32x4 q[RBLK][NL][STEPS];
+    Acc o[RBLK][NC], s[RBLK][KB];
+    float m[RBLK], l[RBLK], c[RBLK];  // maximum of scores, sum of weights (this lane's keys), scale log2(e)
+    int last[RBLK], first[RBLK];      // the keys the row sees
+    int n, kg;                        // this lane's row of the block, its group
+
+    __device__ __forceinline__ static Acc mma(u32x4 a, u32x4 b, Acc x) {
+        if constexpr (F32) {
+            const f32x4 fa = __builtin_bit_cast(f32x4, a), fb = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x = mma1(fa[e], fb[e], x);
+            return x;
+        } else if constexpr (F16) {
+            if constexpr (DB == 32)
+                return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), x, 0, 0, 0);
+            else
+                return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), x, 0, 0, 0);
+        } else {
+            if constexpr (DB == 32)
+                return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), x, 0, 0, 0);
+            else
+                return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), x, 0, 0, 0);
+        }
+    }
+    __device__ __forceinline__ static Acc mma1(float a, float b, Acc x) {
+        if constexpr (DB == 32) return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, x, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, x, 0, 0, 0);
+    }
+
+    // Granules of 16 bytes of a key's row are exchanged by these, so that the
+    // lanes that LDS serves together read different banks.
+    __device__ __forceinline__ static int swz_k(int row) { return row & 7; }
+    __device__ __forceinline__ static int swz_v(int row) {
+        if constexpr (F32) return 4 * ((row >> 2) & 3);
+        else return (2 * row) & (CPR - 1) & 15;
+    }
+
+    // Copies of keys [8 j, 8 j + 8) of a tile, those from `off` (a multiple of
+    // RPI) on that one instruction takes, to LDS at `dst`; base: key 8 j's (and
+    // head's) bytes, or zeros with row_bytes 0; at most `most` keys further.
+    template <bool V>
+    __device__ __forceinline__ static void copy_rows(const uint8_t* base, uint32_t row_bytes, int most, int j, int off,
+                                                     uint32_t dst) {
+        const int lane = threadIdx.x & 63;
+        const int r = off + lane / CPR, row = 8 * j + r;
+        const uint32_t at = static_cast<uint32_t>(min(r, most)) * row_bytes +
+                            16u * static_cast<uint32_t>((lane % CPR) ^ (V ? swz_v(row) : swz_k(row)));
+        copy_to_lds(base, at, dst);
+    }
+
+    __device__ __forceinline__ void setup() {
+        n = threadIdx.x & (DB - 1);
+        kg = (threadIdx.x & 63) / DB;
+    }
+
+    // Queries of block b: `row` points at the row's head, null where there is none.
+    __device__ __forceinline__ void load_q(int b, const Q* row, float c1) {
+        m[b] = -kInf;
+        l[b] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) o[b][i] = Acc{};
+        c[b] = c1;
+        if constexpr (NL == 1) {
+#pragma unroll
+            for (int t = 0; t < STEPS; ++t) q[b][0][t] = row ? ld16(row + (t * KG + kg) * EL) : u32x4{0, 0, 0, 0};
+        } else {
+            f32x4 x[STEPS][2];
+#pragma unroll
+            for (int t = 0; t < STEPS; ++t)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    x[t][i] = row ? *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(row) + (t * KG + kg) * EL + 4 * i)
+                                  : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            float up = 1.0f;
+            if constexpr (F16) {
+                float big = 0.0f;
+#pragma unroll
+                for (int t = 0; t < STEPS; ++t)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) big = fmaxf(big, fabsf(x[t][i][e]));
+                big = across_max(big);
+                // 2^(14 - exponent): the largest value in [2^14, 2^15); c has the inverse.  (Exponents that
+                // leave f32's range on either side are cut: values below 2^-112 count less, above 2^126 too.)
+                int ex = static_cast<int>(__float_as_uint(big) >> 23);
+                ex = big > 0.0f && ex < 255 ? min(max(14 + 127 - ex + 127, 1), 253) : 127;
+                up = __uint_as_float(static_cast<uint32_t>(ex) << 23);
+                c[b] = c1 * __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
+            }
+#pragma unroll
+            for (int t = 0; t < STEPS; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t w[NL];
+                    limbs(x[t][i >> 1][2 * (i & 1)] * up, x[t][i >> 1][2 * (i & 1) + 1] * up, w);
+#pragma unroll
+                    for (int k = 0; k < NL; ++k) q[b][k][t][i] = w[k];
+                }
+        }
+    }
+
+    // A pair of f32 as NL limbs, packed.
+    __device__ __forceinline__ static void limbs(float a, float b, uint32_t (&w)[NL]) {
+#pragma unroll
+        for (int k = 0; k < NL; ++k) {
+            w[k] = pack2<T>(a, b);
+            if (k + 1 < NL) {
+                const f32x2 h = unpack2<T>(w[k]);
+                a -= h[0];
+                b -= h[1];
+            }
+        }
+    }
+
+    // Maximum and sum over the lanes that hold one row (a swap of a register
+    // with itself leaves a lane's own value in one half and its partner's in
+    // the other).
+    __device__ __forceinline__ static float across_max(float v) {
+        if constexpr (DB == 16) {
+            const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+            v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+        }
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    }
+    __device__ __forceinline__ static float across_sum(float v) {
+        if constexpr (DB == 16) {
+            const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+            v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+        }
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+
+    // Scores of the tile whose keys lie at `k`.
+    __device__ __forceinline__ void scores(uint32_t k) {
+#pragma unroll
+        for (int b = 0; b < RBLK; ++b)
+#pragma unroll
+            for (int j = 0; j < KB; ++j) s[b][j] = Acc{};
+        // (tiles start at multiples of a key's bytes, so the granule's exchange is an xor of the address)
+        const uint32_t at = anew(k + n * RB + ((kg ^ swz_k(n)) << 4));
+        read_ahead<u32x4, KB * STEPS, F32 ? 2 : 4>(
+            [&](int x) { return lds_read<u32x4>((at ^ (x % STEPS * KG * 16)) + x / STEPS * DB * RB); },
+            [&](int x, u32x4 a) {
+#pragma unroll
+                for (int i = NL - 1; i >= 0; --i)
+#pragma unroll
+                    for (int b = 0; b < RBLK; ++b) s[b][x / STEPS] = mma(a, q[b][i][x % STEPS], s[b][x / STEPS]);
+            });
+    }
+
+    // Weights in place of the scores; the running state moved to a new maximum
+    // where one grew by more than 2^kLag.  key: the tile's first; edge: some
+    // row does not see some of its keys.
+    __device__ __forceinline__ void softmax(int key, bool edge) {
+#pragma unroll
+        for (int b = 0; b < RBLK; ++b) {
+            float mx = -kInf;
+            if (edge) {
+#pragma unroll
+                for (int j = 0; j < KB; ++j)
+#pragma unroll
+                    for (int e = 0; e < ACC; ++e) {
+                        // (what the row sees from key + 4 kg on)
+                        const int at = j * DB + 8 * (e >> 2) + (e & 3);
+                        s[b][j][e] = at > last[b] - key - 4 * kg || at < first[b] - key - 4 * kg ? -kInf : s[b][j][e];
+                        if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                    }
+            }
+#pragma unroll
+            for (int j = 0; j < KB; ++j)
+#pragma unroll
+                for (int e = 0; e < ACC; ++e) mx = fmaxf(mx, s[b][j][e]);
+            mx = across_max(mx);
+            // (a row of nothing but -inf so far: m stays -inf, weights are 0)
+            if (__builtin_amdgcn_ballot_w64(mx * c[b] > m[b] * c[b] + kLag) != 0) {
+                const float mn = fmaxf(m[b], mx);
+                const float a = mn == -kInf ? 1.0f : exp2_fast((m[b] - mn) * c[b]);
+                m[b] = mn;
+                l[b] *= a;
+#pragma unroll
+                for (int i = 0; i < NC; ++i) o[b][i] *= a;
+            }
+            const float base = static_cast<float>(kBias) - (m[b] == -kInf ? 0.0f : m[b]) * c[b];
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < KB; ++j)
+#pragma unroll
+                for (int e = 0; e < ACC; ++e) {
+                    s[b][j][e] = exp2_fast(__builtin_fmaf(s[b][j][e], c[b], base));
+                    sum += s[b][j][e];
+                }
+            l[b] += sum;
+        }
+    }
+
+    // Weights of step t (8 registers of the blocks' sequence) as limbs.
+    __device__ __forceinline__ void weights(int b, int t, u32x4 (&p)[NL]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int e = 8 * t + 2 * i;
+            uint32_t w[NL];
+            limbs(s[b][e / ACC][e % ACC], s[b][(e + 1) / ACC][(e + 1) % ACC], w);
+#pragma unroll
+            for (int k = 0; k < NL; ++k) p[k][i] = w[k];
+        }
+    }
+    // V's fragments.  16-bit step t, dims DB c ..: keys t KS + (KS / 2) a + 4 kg
+    // + {0..3}, a = 0, 1, from the lane's first address.
+    __device__ __forceinline__ uint32_t v_first(uint32_t v) const {
+        const int lane = threadIdx.x & 63;
+        if constexpr (F32) {  // the value for a register's key and this lane's dim
+            return v + 4 * kg * RB + (((n >> 2) ^ (4 * kg)) << 4) + 4 * (n & 3);
+        } else {
+            const int row = 4 * kg + ((lane & 15) >> 2);
+            const int chunk = (DB == 32 ? 2 * ((lane >> 4) & 1) : 0) + ((lane & 3) >> 1);
+            return v + row * RB + ((chunk ^ swz_v(row)) << 4) + 8 * (lane & 1);
+        }
+    }
+    __device__ __forceinline__ static u32x4 v_frag(uint32_t at, int t, int c) {
+        u32x4 f;
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            const uint32_t x = (at ^ (c * DB * 2)) + (t * KS + a * (KS / 2)) * RB;
+            const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s16x4*)static_cast<uintptr_t>(x));
+            const u32x2 w = __builtin_bit_cast(u32x2, y);
+            f[2 * a] = w[0];
+            f[2 * a + 1] = w[1];
+        }
+        return f;
+    }
+    // f32: register e of block j, dims DB c ..
+    __device__ __forceinline__ static float v_val(uint32_t at, int j, int e, int c) {
+        return lds_read<float>((at ^ (c * DB * 4) ^ (DB == 32 && ((e >> 2) & 1) ? 128 : 0)) +
+                               (j * DB + 8 * (e >> 2) + (e & 3)) * RB);
+    }
+
+    // o += P V of the tile whose values lie at `v`.
+    __device__ __forceinline__ void pv(uint32_t v) {
+        const uint32_t at = anew(v_first(v));
+        if constexpr (F32) {
+            read_ahead<float, KB * ACC * NC, 4>(
+                [&](int x) { return v_val(at, x / NC / ACC, x / NC % ACC, x % NC); },
+                [&](int x, float a) {
+#pragma unroll
+                    for (int b = 0; b < RBLK; ++b)
+                        o[b][x % NC] = mma1(a, s[b][x / NC / ACC][x / NC % ACC], o[b][x % NC]);
+                });
+        } else {
+            u32x4 p[RBLK][NL];
+            read_ahead<u32x4, BK / KS * NC, NC < 4 ? NC : 4>([&](int x) { return v_frag(at, x / NC, x % NC); },
+                                                             [&](int x, u32x4 a) {
+                if (x % NC == 0) {
+#pragma unroll
+                    for (int b = 0; b < RBLK; ++b) weights(b, x / NC, p[b]);
+                }
+#pragma unroll
+                for (int k = NL - 1; k >= 0; --k)
+#pragma unroll
+                    for (int b = 0; b < RBLK; ++b) o[b][x % NC] = mma(a, p[b][k], o[b][x % NC]);
+            });
+        }
+    }
+
+    // Infinities and NaN in 16 bytes of v made 0; whether there were any.
+    __device__ __forceinline__ static bool clean(u32x4& x) {
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t was = x[i];
+            if constexpr (F32) {
+                if ((x[i] & 0x7f800000u) == 0x7f800000u) x[i] = 0;
+            } else {
+                constexpr uint32_t kTop = F16 ? 0x7c00u : 0x7f80u;
+                if ((x[i] & kTop) == kTop) x[i] &= 0xffff0000u;
+                if ((x[i] >> 16 & kTop) == kTop) x[i] &= 0xffffu;
+            }
+            any |= x[i] != was;
+        }
+        return any;
+    }
+    // The same for this lane's granule at LDS address `at`.
+    __device__ __forceinline__ static bool clean_at(uint32_t at) {
+        u32x4 x = lds_read<u32x4>(at);
+        const bool any = clean(x);
+        if (any) *(LDS_AS u32x4*)static_cast<uintptr_t>(at) = x;
+        return any;
+    }
+    // What was made 0 of key's values, whose head's bytes are at v, added to the
+    // rows that see the key.
+    __device__ __forceinline__ void add_special(int key, const uint8_t* v) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+#pragma unroll
+            for (int e = 0; e < ACC; e += 4) {
+                f32x4 x;
+                const T* const at = reinterpret_cast<const T*>(v) + dim_of(i, e);
+                if constexpr (F32) {
+                    x = *reinterpret_cast<const f32x4*>(at);
+                } else {
+                    const u32x2 w = *reinterpret_cast<const u32x2*>(at);
+                    const f32x2 lo = unpack2<T>(w[0]), hi = unpack2<T>(w[1]);
+                    x = f32x4{lo[0], lo[1], hi[0], hi[1]};
+                }
+#pragma unroll
+                for (int b = 0; b < RBLK; ++b)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (key <= last[b] && key >= first[b] && !(fabsf(x[r]) < kInf)) o[b][i][e + r] += x[r];
+                __builtin_amdgcn_sched_barrier(0);
+            }
+    }
+
+    // Dim of register e of block i of o.
+    __device__ __forceinline__ int dim_of(int i, int e) const { return i * DB + 8 * (e >> 2) + 4 * kg + (e & 3); }
+};
+
+// ---- the walk over the items ---------------------------------------------------
+
+// Which requests a launch takes, its blocks, and where states go.
+struct Launch {
+    float* part;         // [workgroups][2] states
+    uint32_t* counters;  // per workgroup: arrivals of the item cut at its end
+    int min_rows, max_rows;  // requests with rows (tokens x group) in (min_rows, max_rows]
+    int min_tiles;       // of a workgroup
+};
+
+template <int BM, int BN>
+struct Walk {
+    const PagedAttn& p;
+    int group, cap;
+    // the request
+    int s = 0, row0 = 0, n = 0, len = 0, blocks = 0;
+    // the item: KV head, block, its first tile (a multiple of BN keys) and number of tiles
+    int kvh = 0, blk = 0, tile0 = 0, tiles = 0;
+
+    __device__ __forceinline__ explicit Walk(const PagedAttn& p_) : p(p_) {
+        group = p.n_q / p.kv.n_kv;
+        cap = static_cast<int>(p.cols << p.kv.page_shift);
+    }
+    __device__ __forceinline__ int rows() const { return n * group; }
+    __device__ __forceinline__ void request(int s_, const Launch& la) {
+        s = s_;
+        const CONST_AS int* qs = (const CONST_AS int*)p.q_start;
+        const CONST_AS int* kl = (const CONST_AS int*)p.kv_len;
+        row0 = min(max(qs[s], 0), p.n_tokens);
+        n = min(max(qs[s + 1], row0), p.n_tokens) - row0;
+        len = min(max(kl[s], 0), cap);
+        if (rows() <= la.min_rows || rows() > la.max_rows) n = 0;
+        blocks = (rows() + BM - 1) / BM;
+    }
+    // Keys [lo, hi) that block b's rows see.
+    __device__ __forceinline__ void span(int b, int* lo, int* hi) const {
+        const int i0 = b * BM / group, i1 = min(n - 1, (b * BM + BM - 1) / group);
+        *hi = len - n + i1 + 1;
+        *lo = p.window ? max(0, len - n + i0 - p.window + 1) : 0;
+    }
+    __device__ __forceinline__ int count(int b, int* first) const {
+        int lo, hi;
+        span(b, &lo, &hi);
+        *first = hi > lo ? lo / BN : 0;
+        return hi > lo ? (hi + BN - 1) / BN - *first : 1;  // (none visible: one tile, to write zeros)
+    }
+    // Tiles of the request for one KV head.
+    __device__ __forceinline__ int64_t total() const {
+        int64_t t = 0;
+        int first;
+        for (int b = 0; b < blocks; ++b) t += count(b, &first);
+        return t;
+    }
+    __device__ __forceinline__ void block(int b) {
+        blk = b;
+        tiles = count(b, &tile0);
+    }
+    // The walk is the same in every lane: its numbers in scalar registers.
+    __device__ __forceinline__ void pin() {
+        s = uniform(s), row0 = uniform(row0), n = uniform(n), len = uniform(len), blocks = uniform(blocks);
+        kvh = uniform(kvh), blk = uniform(blk), tile0 = uniform(tile0), tiles = uniform(tiles);
+    }
+    // The item behind this one; false where there is none.
+    __device__ __forceinline__ bool next(const Launch& la) {
+        if (blk + 1 < blocks) {
+            block(blk + 1);
+            return true;
+        }
+        if (++kvh == p.kv.n_kv) {
+            kvh = 0;
+            n = 0;
+            while (n == 0 && s + 1 < p.n_seq) request(s + 1, la);
+        }
+        block(0);
+        return n > 0;
+    }
+};
+
+// Positions this walk at tile `u` of the sequence of all tiles for workgroup
+// `w` of `nw`, returns how many tiles the workgroup takes (0: none) and in
+// *skip how many tiles of the first item lie before them.  *per: tiles of
+// every workgroup's range.
+template <int NT, class W>
+__device__ __forceinline__ int64_t find_range(W& walk, const Launch& la, int w, int nw, int64_t* skip, int64_t* per) {
+    __shared__ int64_t sums[NT / 64];
+    __shared__ int found_s;
+    __shared__ int64_t found_before;
+    const int tid = threadIdx.x, n_seq = walk.p.n_seq, each = (n_seq + NT - 1) / NT;
+    int64_t mine = 0;
+    W scan(walk.p);
+    for (int i = 0; i < each; ++i) {
+        const int s = tid * each + i;
+        if (s >= n_seq) break;
+        scan.request(s, la);
+        mine += scan.total() * scan.p.kv.n_kv;
+    }
+    // inclusive sums: within waves, then the waves'
+    int64_t incl = mine;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const int64_t o = __shfl_up(incl, off, kWave);
+        if ((tid & 63) >= off) incl += o;
+    }
+    if ((tid & 63) == 63) sums[tid >> 6] = incl;
+    __syncthreads();
+    int64_t before = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) {
+        if (i == (tid >> 6)) before = all;
+        all += sums[i];
+    }
+    incl += before;
+    all = uniform(all);
+    *per = max((all + nw - 1) / nw, static_cast<int64_t>(la.min_tiles));
+    const int64_t u = w * *per;
+    if (u >= all) return 0;
+    if (u < incl && u >= incl - mine) {
+        int64_t at = incl - mine;
+        for (int i = 0; i < each; ++i) {
+            const int s = tid * each + i;
+            scan.request(s, la);
+            const int64_t t = scan.total() * scan.p.kv.n_kv;
+            if (u < at + t) {
+                found_s = s;
+                found_before = at;
+                break;
+            }
+            at += t;
+        }
+    }
+    __syncthreads();
+    walk.request(uniform(found_s), la);
+    int64_t off = u - uniform(found_before);
+    const int64_t t = walk.total();
+    walk.kvh = static_cast<int>(off / t);
+    off -= walk.kvh * t;
+    int b = 0, first, c;
+    while (off >= (c = walk.count(b, &first)) && b + 1 < walk.blocks) {
+        off -= c;
+        ++b;
+    }
+    walk.block(b);
+    *skip = off;
+    return min(*per, all - u);
+}
+
+constexpr int part_floats(int bm, int hd) { return bm * hd + 2 * bm; }
+
+// States of an item cut between workgroups first_wg .. last_wg, joined into
+// out.  Part of workgroup w: its second slot for first_wg (whose range ends
+// inside the item), the first for the others.
+template <class Q, int BM, int HD, int NT>
+__device__ __forceinline__ void join_parts(const PagedAttn& p, const Launch& la, int first_wg, int last_wg, int rows,
+                                           int row_first, int row0, int kvh, int group) {
+    constexpr int kPart = part_floats(BM, HD);
+    for (int i = threadIdx.x; i < rows * (HD / 4); i += NT) {
+        const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
+        float M = -kInf, L = 0.0f;
+        f32x4 O = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int w = first_wg; w <= last_wg; ++w) {
+            const float* const src = la.part + (static_cast<int64_t>(w) * 2 + (w == first_wg)) * kPart;
+            const float m = ld_dev(src + BM * HD + r), l = ld_dev(src + BM * HD + BM + r);
+            f32x4 o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = ld_dev(src + r * HD + d + e);
+            const float mn = fmaxf(M, m);
+            // (m in powers of two: scores times c)
+            const float a = mn == -kInf ? 0.0f : exp2_fast(M - mn), b = mn == -kInf ? 0.0f : exp2_fast(m - mn);
+            L = L * a + l * b;
+            O = O * a + o * b;
+            M = mn;
+        }
+        const int row = row_first + r, t = row0 + row / group, h = kvh * group + row % group;
+        Q* const dst = static_cast<Q*>(p.out) + t * p.out_stride + h * HD + d;
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+        if constexpr (sizeof(Q) == 4) {
+            *reinterpret_cast<f32x4*>(dst) = L == 0.0f ? f32x4{} : O * inv;
+        } else {
+            u32x2 w = {pack2<Q>(O[0] * inv, O[1] * inv), pack2<Q>(O[2] * inv, O[3] * inv)};
+            if (L == 0.0f) w = u32x2{0, 0};
+            *reinterpret_cast<u32x2*>(dst) = w;
+        }
+    }
+}
+
+// Copies of one group of 8 keys: where they are.
+struct Group {
+    const uint8_t* k;
+    const uint8_t* v;
+    uint32_t row_bytes;
+    int most;  // the last key that may be read, from the group's first
+};
+// The group with the keys from `key` (a multiple of 8) on, of those up to
+// `end` (its last key; groups behind it read that of `end` again).
+template <class T>
+__device__ __forceinline__ Group group_of(const PagedAttn& p, const CONST_AS int* table_row, int kvh, int key, int end) {
+    const int at = min(key, end & ~7);
+    const int id = table_row[at >> p.kv.page_shift];
+    const bool real = static_cast<uint32_t>(id) < static_cast<uint32_t>(p.kv.n_pages);
+    const int64_t off = ((real ? id : 0) * p.kv.page_stride +
+                         (static_cast<int64_t>(at & ((1 << p.kv.page_shift) - 1)) * p.kv.n_kv + kvh) * p.kv.head_dim) *
+                        static_cast<int64_t>(sizeof(T));
+    const uint8_t* const zeros = reinterpret_cast<const uint8_t*>(kZeros);
+    Group g;
+    g.k = real ? static_cast<const uint8_t*>(p.kv.k) + off : zeros;
+    g.v = real ? static_cast<const uint8_t*>(p.kv.v) + off : zeros;
+    g.row_bytes = real ? static_cast<uint32_t>(p.kv.n_kv * p.kv.head_dim) * static_cast<uint32_t>(sizeof(T)) : 0u;
+    g.most = end - at;
+    return g;
+}
+
+// Where the values of one key are.
+template <class T>
+__device__ __forceinline__ const uint8_t* value_of(const PagedAttn& p, const CONST_AS int* table_row, int kvh, int key) {
+    const Group g = group_of<T>(p, table_row, kvh, key & ~7, key);
+    return g.v + static_cast<uint32_t>(key & 7) * g.row_bytes;
+}
+
+// The store of four values of a row (zeros where its sum of weights is 0).
+template <class Q>
+__device__ __forceinline__ void store_out(Q* dst, f32x4 o, float l) {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    o *= inv;
+    if (l == 0.0f) o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (sizeof(Q) == 4) *reinterpret_cast<f32x4*>(dst) = o;
+    else *reinterpret_cast<u32x2*>(dst) = u32x2{pack2<Q>(o[0], o[1]), pack2<Q>(o[2], o[3])};
+}
+
+// Counts this workgroup's state of an item in; true in the one that is last.
+// Relaxed: the states went out in agent-scope stores that every wave waits for
+// here, and are read with agent-scope loads once the count is known.
+__device__ __forceinline__ bool arrive(uint32_t* counter, int parts, int* flag) {
+    wait_vmcnt<0>();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const uint32_t before = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const bool is_last = before == static_cast<uint32_t>(parts) - 1;
+        if (is_last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *flag = is_last;
+    }
+    __syncthreads();
+    return *flag != 0;
+}
+
+// Workgroup blockIdx.x's place in the sequence: neighbours share an XCD (block
+// b runs on XCD b % 8), whose L2 then serves the blocks of one KV head.
+__device__ __forceinline__ int place_of(int b, int nw) {
+    const int q = nw / 8, r = nw % 8, x = b % 8;
+    return x * q + min(x, r) + b / 8;
+}
+
+// ---- few rows: the waves split the keys ------------------------------------------
+// Single tokens and drafts, bound by the bytes of keys and values.  A wave
+// streams tiles of its own through its own LDS ring, no barrier between them,
+// and the four waves' states are joined at the item's end.
+template <class Q, class T, int HD, int RBLK>
+__global__ __launch_bounds__(256, RBLK == 1 || HD < 256 ? 2 : 1) void k_paged_narrow(PagedAttn p, Launch la) {
+    constexpr int NW = 4, DB = 16, BM = DB * RBLK, BK = KindOf<T>::f32 ? 16 : 32, BN = NW * BK;
+    using C = Core<Q, T, HD, DB, RBLK, BK>;
+    constexpr int D = 16384 / C::TB;    // tiles of K, and of V, in the ring
+    constexpr int H = BK / C::RPI;      // copies of a tile of K, or of V
+    constexpr int G = BK / 8, PER = 8 / C::RPI;
+    constexpr int kPart = part_floats(BM, HD);
+    static_assert(BM * HD * 4 <= 32768, "a wave's state fits its ring");
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    __shared__ float sm[NW][BM], sl[NW][BM];
+    __shared__ int flag;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    uint8_t* const ring = lds + wave * 32768;
+    const int nw = gridDim.x, w = place_of(blockIdx.x, nw);
+    Walk<BM, BN> walk(p);
+    int64_t skip = 0, per = 0;
+    int64_t left = find_range<256>(walk, la, w, nw, &skip, &per);
+    int64_t item_at = w * per - skip;  // of the item's first tile in the sequence
+    const uint32_t ring_at = uniform(static_cast<int>(lds_address(ring)));
+    const float c1 = p.scale * kLog2e;
+    C core;
+    core.setup();
+    while ((left = uniform(left)) > 0) {
+        walk.pin();
+        const int a = uniform(static_cast<int>(skip));
+        const int b = uniform(static_cast<int>(min(static_cast<int64_t>(walk.tiles), skip + left)));
+        skip = 0;
+        left -= b - a;
+        int lo, hi;
+        walk.span(walk.blk, &lo, &hi);
+        const int rows = min(BM, walk.rows() - walk.blk * BM), row_first = walk.blk * BM;
+        const int pos0 = walk.len - walk.n;
+        const int low_pos = pos0 + row_first / walk.group;  // position of the block's first row
+#pragma unroll
+        for (int i = 0; i < RBLK; ++i) {
+            const int r = i * DB + core.n, row = row_first + r;
+            const bool real = r < rows;
+            const int t = row / walk.group;
+            core.load_q(i, real ? static_cast<const Q*>(p.q) + (walk.row0 + t) * p.q_stride +
+                                      (walk.kvh * walk.group + row % walk.group) * HD
+                                : nullptr, c1);
+            core.last[i] = real ? pos0 + t : -1;
+            core.first[i] = p.window ? core.last[i] - p.window + 1 : 0;
+        }
+        const CONST_AS int* const table_row = (const CONST_AS int*)p.table + static_cast<int64_t>(walk.s) * p.cols;
+        const int key0 = (walk.tile0 + a) * BN + wave * BK;
+        int nt = b - a;
+        if (key0 + (nt - 1) * BN >= hi) --nt;  // (the last tile's keys may end before this wave's)
+        auto copy_k = [&](int i, const Group (&g)[G]) {
+#pragma unroll
+            for (int j = 0; j < H; ++j)
+                C::template copy_rows<false>(g[j / PER].k, g[j / PER].row_bytes, g[j / PER].most, j / PER,
+                                             j % PER * C::RPI, ring_at + (i % D) * C::TB + j * 1024);
+        };
+        auto copy_v = [&](int i, const Group (&g)[G]) {
+#pragma unroll
+            for (int j = 0; j < H; ++j)
+                C::template copy_rows<true>(g[j / PER].v, g[j / PER].row_bytes, g[j / PER].most, j / PER,
+                                            j % PER * C::RPI, ring_at + (D + i % D) * C::TB + j * 1024);
+        };
+        auto groups = [&](int i, Group (&g)[G]) {
+#pragma unroll
+            for (int j = 0; j < G; ++j) g[j] = group_of<T>(p, table_row, walk.kvh, key0 + i * BN + 8 * j, hi - 1);
+        };
+        wait_copies<0>();  // (q is here: from now on only copies are in flight)
+        for (int i = 0; i < D; ++i)
+            if (i < nt) {
+                Group g[G];
+                groups(i, g);
+                copy_k(i, g);
+                copy_v(i, g);
+            }
+        auto is_edge = [&](int key) { return key + BK - 1 > low_pos || (p.window && key <= hi - 1 - p.window); };
+        bool special = false;
+        for (int i = 0; i < nt; ++i) {
+            const int key = key0 + i * BN;
+            const bool more = i + D < nt;
+            const bool edge = is_edge(key);
+            Group g[G];
+            if (more) groups(i + D, g);
+            if (nt - i >= D) wait_copies<(2 * D - 1) * H>();
+            else wait_copies<0>();
+            core.scores(ring_at + (i % D) * C::TB);
+            wait_lds();
+            if (more) copy_k(i + D, g);
+            core.softmax(key, edge);
+            if (more) wait_copies<(2 * D - 1) * H>();
+            else wait_copies<0>();
+            const uint32_t v = ring_at + (D + i % D) * C::TB;
+            if (edge) {
+                bool any = false;
+#pragma unroll
+                for (int j = 0; j < C::TB / 1024; ++j) any |= C::clean_at(v + j * 1024 + anew((tid & 63) * 16));
+                special |= __builtin_amdgcn_ballot_w64(any) != 0;
+                wait_lds();
+            }
+            core.pv(v);
+            wait_lds();
+            if (more) copy_v(i + D, g);
+        }
+        if (special) {
+            for (int i = 0; i < nt; ++i)
+                if (const int key = key0 + i * BN; is_edge(key))
+                    for (int j = key; j < min(key + BK, hi); ++j)
+                        core.add_special(j, value_of<T>(p, table_row, walk.kvh, j));
+        }
+        // The waves' states, joined in order.
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        float* const mine = reinterpret_cast<float*>(ring);
+#pragma unroll
+        for (int i = 0; i < RBLK; ++i) {
+            const int r = i * DB + core.n;
+            const float l = C::across_sum(core.l[i]);
+            if (core.kg == 0) {
+                sm[wave][r] = core.m[i] * core.c[i];
+                sl[wave][r] = l;
+            }
+#pragma unroll
+            for (int j = 0; j < C::NC; ++j)
+                *reinterpret_cast<f32x4*>(mine + r * HD + ((j * DB + 4 * core.kg) ^ (4 * (core.n & 7)))) = core.o[i][j];
+        }
+        __syncthreads();
+        const int first_wg = static_cast<int>(item_at / per), last_wg = static_cast<int>((item_at + walk.tiles - 1) / per);
+        const bool cut = first_wg != last_wg;
+        float* const part = la.part + (static_cast<int64_t>(w) * 2 + (w == first_wg)) * kPart;
+        for (int i = tid; i < rows * (HD / 4); i += 256) {
+            const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
+            float M = -kInf, L = 0.0f;
+#pragma unroll
+            for (int x = 0; x < NW; ++x) M = fmaxf(M, sm[x][r]);
+            f32x4 O = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int x = 0; x < NW; ++x) {
+                const float f = M == -kInf ? 1.0f : exp2_fast(sm[x][r] - M);
+                L += sl[x][r] * f;
+                O += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + x * 32768) + r * HD + (d ^ (4 * (r & 7)))) * f;
+            }
+            if (!cut) {
+                const int row = row_first + r;
+                store_out(static_cast<Q*>(p.out) + (walk.row0 + row / walk.group) * p.out_stride +
+                              (walk.kvh * walk.group + row % walk.group) * HD + d, O, L);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) st_dev(part + r * HD + d + e, O[e]);
+                if (d == 0) {
+                    st_dev(part + BM * HD + r, M);
+                    st_dev(part + BM * HD + BM + r, L);
+                }
+            }
+        }
+        if (cut) {
+            if (arrive(la.counters + first_wg, last_wg - first_wg + 1, &flag))
+                join_parts<Q, BM, HD, 256>(p, la, first_wg, last_wg, rows, row_first, walk.row0, walk.kvh, walk.group);
+        }
+        __syncthreads();  // the rings are free again
+        item_at += walk.tiles;
+        if (left > 0 && !walk.next(la)) break;
+    }
+}
+
+// ---- many rows: the waves split the rows -------------------------------------------
+// Chunks of prompts, bound by the matrix cores: every wave has 32 rows of its
+// own, and K and V tiles are read from memory once for all of them.
+template <class Q, class T, int HD, int NW>
+__global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) {
+    constexpr int DB = 32, BM = DB * NW, BK = KindOf<T>::f32 ? 32 : 64, BN = BK, NT = NW * 64;
+    using C = Core<Q, T, HD, DB, 1, BK>;
+    constexpr int PER = 8 / C::RPI, COPIES = BK / C::RPI / NW;  // copies of a tile of K, or of V, by each wave
+    constexpr int kPart = part_floats(BM, HD);
+    static_assert(COPIES >= 1 && COPIES * NW * C::RPI == BK, "every wave copies alike");
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];  // two tiles of K and V
+    __shared__ int special;  // the last of this workgroup's items whose v held what was made 0
+    __shared__ int flag;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int nw = gridDim.x, w = place_of(blockIdx.x, nw);
+    Walk<BM, BN> walk(p);
+    int64_t skip = 0, per = 0;
+    int64_t left = find_range<NT>(walk, la, w, nw, &skip, &per);
+    int64_t item_at = w * per - skip;
+    const uint32_t lds_at = uniform(static_cast<int>(lds_address(lds)));
+    const float c1 = p.scale * kLog2e;
+    if (tid == 0) special = -1;
+    int step = 0, item = 0;  // tiles and items so far
+    C core;
+    core.setup();
+    while ((left = uniform(left)) > 0) {
+        walk.pin();
+        const int a = uniform(static_cast<int>(skip));
+        const int b = uniform(static_cast<int>(min(static_cast<int64_t>(walk.tiles), skip + left)));
+        skip = 0;
+        left -= b - a;
+        int lo, hi;
+        walk.span(walk.blk, &lo, &hi);
+        const int rows = min(BM, walk.rows() - walk.blk * BM), row_first = walk.blk * BM;
+        const int pos0 = walk.len - walk.n;
+        const int low_pos = pos0 + row_first / walk.group;
+        const int r = wave * DB + core.n, row = row_first + r;
+        const bool real = r < rows;
+        const int t = row / walk.group;
+        const int64_t head = (walk.kvh * walk.group + row % walk.group) * HD;
+        core.load_q(0, real ? static_cast<const Q*>(p.q) + (walk.row0 + t) * p.q_stride + head : nullptr, c1);
+        core.last[0] = real ? pos0 + t : -1;
+        core.first[0] = p.window ? core.last[0] - p.window + 1 : 0;
+        // the wave's rows see keys from wave_lo to wave_hi
+        const bool busy = wave * DB < rows;
+        const int wave_low = pos0 + (row_first + wave * DB) / walk.group;
+        const int wave_hi = pos0 + (row_first + min(wave * DB + DB, rows) - 1) / walk.group;
+        const CONST_AS int* const table_row = (const CONST_AS int*)p.table + static_cast<int64_t>(walk.s) * p.cols;
+        const int key0 = (walk.tile0 + a) * BN;
+        const int nt = hi > 0 ? b - a : 0;
+        auto copy_tile = [&](int i) {
+            const uint32_t k = lds_at + ((step + i) & 1) * 2 * C::TB;
+#pragma unroll
+            for (int x = 0; x < COPIES; ++x) {
+                const int j = wave * COPIES + x, grp = j / PER;
+                const Group g = group_of<T>(p, table_row, walk.kvh, key0 + i * BN + 8 * grp, hi - 1);
+                C::template copy_rows<false>(g.k, g.row_bytes, g.most, grp, j % PER * C::RPI, k + j * 1024);
+                C::template copy_rows<true>(g.v, g.row_bytes, g.most, grp, j % PER * C::RPI, k + C::TB + j * 1024);
+            }
+        };
+        lds_barrier();  // (every wave is done with the item before)
+        auto is_edge = [&](int key) { return key + BK - 1 > low_pos || (p.window && key <= hi - 1 - p.window); };
+        if (nt > 0) copy_tile(0);
+        for (int i = 0; i < nt; ++i) {
+            const int key = key0 + i * BN, slot = (step + i) & 1;
+            const uint32_t k = lds_at + slot * 2 * C::TB;
+            wait_copies<0>();
+            if (is_edge(key)) {
+                bool any = false;
+#pragma unroll
+                for (int x = 0; x < COPIES; ++x)
+                    any |= C::clean_at(k + C::TB + (wave * COPIES + x) * 1024 + anew((tid & 63) * 16));
+                if (__builtin_amdgcn_ballot_w64(any) != 0) special = item;
+            }
+            lds_barrier();
+            if (i + 1 < nt) copy_tile(i + 1);
+            // (tiles that none of the wave's rows sees)
+            if (!busy || key > wave_hi || (p.window && key + BK <= wave_low - p.window + 1)) continue;
+            const bool wave_edge = key + BK - 1 > wave_low || (p.window && key <= wave_hi - p.window);
+            core.scores(k);
+            core.softmax(key, wave_edge);
+            core.pv(k + C::TB);
+        }
+        step += nt;
+        lds_barrier();
+        if (uniform(special) == item++) {
+            for (int i = 0; i < nt; ++i)
+                if (const int key = key0 + i * BN; is_edge(key))
+                    for (int j = key; j < min(key + BK, hi); ++j)
+                        core.add_special(j, value_of<T>(p, table_row, walk.kvh, j));
+        }
+        const float l = C::across_sum(core.l[0]);
+        const int first_wg = static_cast<int>(item_at / per), last_wg = static_cast<int>((item_at + walk.tiles - 1) / per);
+        if (first_wg == last_wg) {
+            if (real) {
+                Q* const dst = static_cast<Q*>(p.out) + (walk.row0 + t) * p.out_stride + head;
+#pragma unroll
+                for (int i = 0; i < C::NC; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        store_out(dst + core.dim_of(i, 4 * e), f32x4{core.o[0][i][4 * e], core.o[0][i][4 * e + 1], core.o[0][i][4 * e + 2], core.o[0][i][4 * e + 3]}, l);
+            }
+        } else {
+            float* const part = la.part + (static_cast<int64_t>(w) * 2 + (w == first_wg)) * kPart;
+            if (real) {
+#pragma unroll
+                for (int i = 0; i < C::NC; ++i)
+#pragma unroll
+                    for (int e = 0; e < C::ACC; ++e) st_dev(part + r * HD + core.dim_of(i, e), core.o[0][i][e]);
+                if (core.kg == 0) {
+                    st_dev(part + BM * HD + r, core.m[0] * core.c[0]);
+                    st_dev(part + BM * HD + BM + r, l);
+                }
+            }
+            if (arrive(la.counters + first_wg, last_wg - first_wg + 1, &flag))
+                join_parts<Q, BM, HD, NT>(p, la, first_wg, last_wg, rows, row_first, walk.row0, walk.kvh, walk.group);
+        }
+        item_at += walk.tiles;
+        if (left > 0 && !walk.next(la)) break;
+    }
+}
+
+// Rows (tokens x group) of a request up to which its keys are split over the waves.
+constexpr int kNarrowRows = 32;
+// Waves of 32 rows: two to a SIMD where the accumulator and q fit 256 registers.
+template <class Q>
+constexpr int wide_waves(int hd) {
+    return sizeof(Q) == 4 || hd == 256 ? 4 : 8;
+}
+
+int slots() { return static_cast<int>(device_info().cus); }
+
+// The most rows a request can have.
+int64_t most_rows(const PagedAttn& p) {
+    const int fresh = p.max_fresh > 0 && p.max_fresh < p.n_tokens ? p.max_fresh : p.n_tokens;
+    return static_cast<int64_t>(fresh) * (p.n_q / p.kv.n_kv);
+}
+
+template <class Q, class T, int HD>
+hipError_t run(const PagedAttn& p, float* part, uint32_t* counters, hipStream_t s) {
+    constexpr int NW = wide_waves<Q>(HD);
+    Launch la;
+    la.part = part;
+    la.counters = counters;
+    const int64_t rows = most_rows(p);
+    const bool wide = rows > kNarrowRows, narrow = !wide || p.n_seq > 1;
+    const unsigned grid = static_cast<unsigned>(slots());
+    if (wide) {
+        constexpr int BK = KindOf<T>::f32 ? 32 : 64;
+        la.min_rows = narrow ? kNarrowRows : 0;
+        la.max_rows = 0x7fffffff;
+        la.min_tiles = 2;
+        hipLaunchKernelGGL((k_paged_wide<Q, T, HD, NW>), dim3(grid), dim3(NW * 64), 4 * BK * HD * sizeof(T), s, p, la);
+    }
+    if (narrow) {
+        la.min_rows = 0;
+        la.max_rows = wide ? kNarrowRows : 0x7fffffff;
+        la.min_tiles = 1;
+        if (rows <= 16) hipLaunchKernelGGL((k_paged_narrow<Q, T, HD, 1>), dim3(grid), dim3(256), 4 * 32768, s, p, la);
+        else hipLaunchKernelGGL((k_paged_narrow<Q, T, HD, 2>), dim3(grid), dim3(256), 4 * 32768, s, p, la);
     }
     return hipGetLastError();
 }
 
+template <class Q, class T>
+hipError_t run_hd(const PagedAttn& p, float* part, uint32_t* counters, hipStream_t s) {
+    switch (p.kv.head_dim) {
+        case 64: return run<Q, T, 64>(p, part, counters, s);
+        case 128: return run<Q, T, 128>(p, part, counters, s);
+        default: return run<Q, T, 256>(p, part, counters, s);
+    }
+}
+
 }  // namespace
 
-size_t paged_attention_workspace(const PagedAttn&) { return 0; }
+size_t paged_attention_workspace(const PagedAttn& p) {
+    const int64_t rows = most_rows(p);
+    const int waves = p.dtype == RT_HIP_F32 ? wide_waves<float>(p.kv.head_dim) : wide_waves<__bf16>(p.kv.head_dim);
+    const int bm = rows > kNarrowRows ? waves * 32 : (rows <= 16 ? 16 : 32);
+    return static_cast<size_t>(slots()) * 2 * part_floats(bm, p.kv.head_dim) * sizeof(float);
+}
 
-hipError_t launch_paged_attention(const PagedAttn& p, void*, uint32_t*, hipStream_t s) {
-    if (p.dtype == RT_HIP_BF16) return run<__bf16, __bf16>(p, s);
-    if (p.dtype == RT_HIP_F16) return run<_Float16, _Float16>(p, s);
+hipError_t launch_paged_attention(const PagedAttn& p, void* part, uint32_t* counters, hipStream_t s) {
+    if (static_cast<size_t>(slots()) > kArrivalCounters) return hipErrorInvalidValue;
+    float* const f = static_cast<float*>(part);
+    if (p.dtype == RT_HIP_BF16) return run_hd<__bf16, __bf16>(p, f, counters, s);
+    if (p.dtype == RT_HIP_F16) return run_hd<_Float16, _Float16>(p, f, counters, s);
     switch (p.kv.dtype) {
-        case RT_HIP_F32: return run<float, float>(p, s);
-        case RT_HIP_F16: return run<float, _Float16>(p, s);
-        default: return run<float, __bf16>(p, s);
+        case RT_HIP_F32: return run_hd<float, float>(p, f, counters, s);
+        case RT_HIP_F16: return run_hd<float, _Float16>(p, f, counters, s);
+        default: return run_hd<float, __bf16>(p, f, counters, s);
     }
 }
 
