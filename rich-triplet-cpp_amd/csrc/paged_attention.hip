@@ -489,6 +489,9 @@ struct Core {
 struct Launch {
     float* part;         // [workgroups][2] states
     uint32_t* counters;  // per workgroup: arrivals of the item cut at its end
+    int group;               // query heads of a KV head
+    uint32_t group_mul;      // x / group = x * group_mul >> group_shift for x < 2^31
+    int group_shift;
     int min_rows, max_rows;  // requests with rows (tokens x group) in (min_rows, max_rows]
     int min_tiles;       // of a workgroup
 };
@@ -496,18 +499,24 @@ struct Launch {
 template <int BM, int BN>
 struct Walk {
     const PagedAttn& p;
+    const Launch& la;
     int group, cap;
     // the request
     int s = 0, row0 = 0, n = 0, len = 0, blocks = 0;
     // the item: KV head, block, its first tile (a multiple of BN keys) and number of tiles
     int kvh = 0, blk = 0, tile0 = 0, tiles = 0;
 
-    __device__ __forceinline__ explicit Walk(const PagedAttn& p_) : p(p_) {
-        group = p.n_q / p.kv.n_kv;
+    __device__ __forceinline__ Walk(const PagedAttn& p_, const Launch& la_) : p(p_), la(la_) {
+        group = la.group;
         cap = static_cast<int>(p.cols << p.kv.page_shift);
     }
     __device__ __forceinline__ int rows() const { return n * group; }
-    __device__ __forceinline__ void request(int s_, const Launch& la) {
+    // Row's token; its head in the group.
+    __device__ __forceinline__ int token(int row) const {
+        return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(row)) * la.group_mul >> la.group_shift);
+    }
+    __device__ __forceinline__ int head(int row, int token) const { return row - token * group; }
+    __device__ __forceinline__ void request(int s_) {
         s = s_;
         const CONST_AS int* qs = (const CONST_AS int*)p.q_start;
         const CONST_AS int* kl = (const CONST_AS int*)p.kv_len;
@@ -519,7 +528,7 @@ struct Walk {
     }
     // Keys [lo, hi) that block b's rows see.
     __device__ __forceinline__ void span(int b, int* lo, int* hi) const {
-        const int i0 = b * BM / group, i1 = min(n - 1, (b * BM + BM - 1) / group);
+        const int i0 = token(b * BM), i1 = min(n - 1, token(b * BM + BM - 1));
         *hi = len - n + i1 + 1;
         *lo = p.window ? max(0, len - n + i0 - p.window + 1) : 0;
     }
@@ -546,7 +555,7 @@ struct Walk {
         kvh = uniform(kvh), blk = uniform(blk), tile0 = uniform(tile0), tiles = uniform(tiles);
     }
     // The item behind this one; false where there is none.
-    __device__ __forceinline__ bool next(const Launch& la) {
+    __device__ __forceinline__ bool next() {
         if (blk + 1 < blocks) {
             block(blk + 1);
             return true;
@@ -554,70 +563,89 @@ struct Walk {
         if (++kvh == p.kv.n_kv) {
             kvh = 0;
             n = 0;
-            while (n == 0 && s + 1 < p.n_seq) request(s + 1, la);
+            while (n == 0 && s + 1 < p.n_seq) request(s + 1);
         }
         block(0);
         return n > 0;
     }
 };
 
-// Positions this walk at tile `u` of the sequence of all tiles for workgroup
-// `w` of `nw`, returns how many tiles the workgroup takes (0: none) and in
-// *skip how many tiles of the first item lie before them.  *per: tiles of
-// every workgroup's range.
+// a / b, of numbers that rarely need 64 bits.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
+}
+
+// Positions the walk at workgroup w's range of the sequence of all tiles (of
+// nw equal ones) and returns how many tiles it takes (0: none); *skip: how many
+// of the first item's lie before them; *per: tiles of a range.  Up to 64
+// requests every wave sums for itself, one to a lane; otherwise the workgroup's
+// threads do, several to a thread.
 template <int NT, class W>
-__device__ __forceinline__ int64_t find_range(W& walk, const Launch& la, int w, int nw, int64_t* skip, int64_t* per) {
+__device__ __forceinline__ int64_t find_range(W& walk, int w, int nw, int64_t* skip, int64_t* per) {
+    const int tid = threadIdx.x, lane = tid & 63, n_seq = walk.p.n_seq, n_kv = walk.p.kv.n_kv;
     __shared__ int64_t sums[NT / 64];
     __shared__ int found_s;
     __shared__ int64_t found_before;
-    const int tid = threadIdx.x, n_seq = walk.p.n_seq, each = (n_seq + NT - 1) / NT;
+    const bool small = n_seq <= 64;
+    const int each = small ? 1 : (n_seq + NT - 1) / NT, base = small ? lane : tid * each;
     int64_t mine = 0;
-    W scan(walk.p);
+    W scan(walk.p, walk.la);
     for (int i = 0; i < each; ++i) {
-        const int s = tid * each + i;
-        if (s >= n_seq) break;
-        scan.request(s, la);
-        mine += scan.total() * scan.p.kv.n_kv;
+        if (base + i >= n_seq) break;
+        scan.request(base + i);
+        mine += scan.total() * n_kv;
     }
-    // inclusive sums: within waves, then the waves'
     int64_t incl = mine;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
         const int64_t o = __shfl_up(incl, off, kWave);
-        if ((tid & 63) >= off) incl += o;
+        if (lane >= off) incl += o;
     }
-    if ((tid & 63) == 63) sums[tid >> 6] = incl;
-    __syncthreads();
-    int64_t before = 0, all = 0;
+    int64_t all = __shfl(incl, 63, kWave);
+    if (!small) {
+        if (lane == 63) sums[tid >> 6] = incl;
+        __syncthreads();
+        int64_t before = 0;
+        all = 0;
 #pragma unroll
-    for (int i = 0; i < NT / 64; ++i) {
-        if (i == (tid >> 6)) before = all;
-        all += sums[i];
+        for (int i = 0; i < NT / 64; ++i) {
+            if (i == (tid >> 6)) before = all;
+            all += sums[i];
+        }
+        incl += before;
     }
-    incl += before;
     all = uniform(all);
-    *per = max((all + nw - 1) / nw, static_cast<int64_t>(la.min_tiles));
+    *per = max(quotient(all + nw - 1, nw), static_cast<int64_t>(walk.la.min_tiles));
     const int64_t u = w * *per;
     if (u >= all) return 0;
-    if (u < incl && u >= incl - mine) {
-        int64_t at = incl - mine;
-        for (int i = 0; i < each; ++i) {
-            const int s = tid * each + i;
-            scan.request(s, la);
-            const int64_t t = scan.total() * scan.p.kv.n_kv;
-            if (u < at + t) {
-                found_s = s;
-                found_before = at;
-                break;
+    const bool here = u < incl && u >= incl - mine;
+    int s;
+    int64_t at = incl - mine;  // tiles before the request
+    if (small) {
+        s = __builtin_ctzll(__builtin_amdgcn_ballot_w64(here));
+        at = __shfl(at, s, kWave);
+    } else {
+        if (here) {
+            for (int i = 0; i < each; ++i) {
+                scan.request(base + i);
+                const int64_t t = scan.total() * n_kv;
+                if (u < at + t) {
+                    found_s = base + i;
+                    found_before = at;
+                    break;
+                }
+                at += t;
             }
-            at += t;
         }
+        __syncthreads();
+        s = found_s;
+        at = found_before;
     }
-    __syncthreads();
-    walk.request(uniform(found_s), la);
-    int64_t off = u - uniform(found_before);
+    walk.request(uniform(s));
+    int64_t off = u - uniform(at);
     const int64_t t = walk.total();
-    walk.kvh = static_cast<int>(off / t);
+    walk.kvh = static_cast<int>(quotient(off, t));
     off -= walk.kvh * t;
     int b = 0, first, c;
     while (off >= (c = walk.count(b, &first)) && b + 1 < walk.blocks) {
@@ -631,39 +659,73 @@ __device__ __forceinline__ int64_t find_range(W& walk, const Launch& la, int w, 
 
 constexpr int part_floats(int bm, int hd) { return bm * hd + 2 * bm; }
 
+// The store of four values of a row (zeros where its sum of weights is 0).
+template <class Q>
+__device__ __forceinline__ void store_out(Q* dst, f32x4 o, float l) {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    o *= inv;
+    if (l == 0.0f) o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (sizeof(Q) == 4) *reinterpret_cast<f32x4*>(dst) = o;
+    else *reinterpret_cast<u32x2*>(dst) = u32x2{pack2<Q>(o[0], o[1]), pack2<Q>(o[2], o[3])};
+}
+
+// Four values of a row with the row's maximum (in powers of two) and sum.
+struct State {
+    float m, l;
+    f32x4 o;
+};
+__device__ __forceinline__ void join_state(State& a, const State& b) {
+    const float m = fmaxf(a.m, b.m);
+    const float fa = m == -kInf ? 0.0f : exp2_fast(a.m - m), fb = m == -kInf ? 0.0f : exp2_fast(b.m - m);
+    a.l = a.l * fa + b.l * fb;
+    a.o = a.o * fa + b.o * fb;
+    a.m = m;
+}
+
 // States of an item cut between workgroups first_wg .. last_wg, joined into
 // out.  Part of workgroup w: its second slot for first_wg (whose range ends
-// inside the item), the first for the others.
-template <class Q, int BM, int HD, int NT>
-__device__ __forceinline__ void join_parts(const PagedAttn& p, const Launch& la, int first_wg, int last_wg, int rows,
-                                           int row_first, int row0, int kvh, int group) {
-    constexpr int kPart = part_floats(BM, HD);
-    for (int i = threadIdx.x; i < rows * (HD / 4); i += NT) {
-        const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
-        float M = -kInf, L = 0.0f;
-        f32x4 O = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int w = first_wg; w <= last_wg; ++w) {
-            const float* const src = la.part + (static_cast<int64_t>(w) * 2 + (w == first_wg)) * kPart;
-            const float m = ld_dev(src + BM * HD + r), l = ld_dev(src + BM * HD + BM + r);
-            f32x4 o;
+// inside the item), the first for the others.  A thread takes four values of a
+// row; where there are fewer of those than threads, several share the parts,
+// each in order, and their results are joined through LDS (`tmp`, NT states).
+template <class Q, int BM, int HD, int NT, class W>
+__device__ __forceinline__ void join_parts(const W& walk, int first_wg, int last_wg, int rows, State* tmp) {
+    const PagedAttn& p = walk.p;
+    const Launch& la = walk.la;
+    constexpr int kPart = part_floats(BM, HD), kAhead = 8;
+    const int quads = rows * (HD / 4), share = quads >= NT ? 1 : NT / quads;
+    for (int i0 = 0; i0 < quads; i0 += NT) {
+        const int i = share == 1 ? i0 + static_cast<int>(threadIdx.x) : static_cast<int>(threadIdx.x) % quads;
+        const int g = share == 1 ? 0 : static_cast<int>(threadIdx.x) / quads;
+        const bool in = i < quads && g < share;
+        const int r = in ? i / (HD / 4) : 0, d = in ? (i % (HD / 4)) * 4 : 0;
+        State s = {-kInf, 0.0f, {0.0f, 0.0f, 0.0f, 0.0f}};
+        for (int w = first_wg + g; in && w <= last_wg; w += share * kAhead) {
+            State x[kAhead];  // all loads in flight together
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = ld_dev(src + r * HD + d + e);
-            const float mn = fmaxf(M, m);
-            // (m in powers of two: scores times c)
-            const float a = mn == -kInf ? 0.0f : exp2_fast(M - mn), b = mn == -kInf ? 0.0f : exp2_fast(m - mn);
-            L = L * a + l * b;
-            O = O * a + o * b;
-            M = mn;
+            for (int k = 0; k < kAhead; ++k) {
+                const int at = w + k * share;
+                if (at > last_wg) continue;
+                const float* const src = la.part + (static_cast<int64_t>(at) * 2 + (at == first_wg)) * kPart;
+                x[k].m = ld_dev(src + BM * HD + r);
+                x[k].l = ld_dev(src + BM * HD + BM + r);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[k].o[e] = ld_dev(src + r * HD + d + e);
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k)
+                if (w + k * share <= last_wg) join_state(s, x[k]);
         }
-        const int row = row_first + r, t = row0 + row / group, h = kvh * group + row % group;
-        Q* const dst = static_cast<Q*>(p.out) + t * p.out_stride + h * HD + d;
-        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-        if constexpr (sizeof(Q) == 4) {
-            *reinterpret_cast<f32x4*>(dst) = L == 0.0f ? f32x4{} : O * inv;
-        } else {
-            u32x2 w = {pack2<Q>(O[0] * inv, O[1] * inv), pack2<Q>(O[2] * inv, O[3] * inv)};
-            if (L == 0.0f) w = u32x2{0, 0};
-            *reinterpret_cast<u32x2*>(dst) = w;
+        if (share > 1) {
+            __syncthreads();
+            tmp[threadIdx.x] = s;
+            __syncthreads();
+            if (in && g == 0)
+                for (int k = 1; k < share; ++k) join_state(s, tmp[threadIdx.x + k * quads]);
+        }
+        if (in && g == 0) {
+            const int row = walk.blk * BM + r, t = walk.token(row);
+            store_out(static_cast<Q*>(p.out) + (walk.row0 + t) * p.out_stride +
+                          (walk.kvh * walk.group + walk.head(row, t)) * HD + d, s.o, s.l);
         }
     }
 }
@@ -701,16 +763,6 @@ __device__ __forceinline__ const uint8_t* value_of(const PagedAttn& p, const CON
     return g.v + static_cast<uint32_t>(key & 7) * g.row_bytes;
 }
 
-// The store of four values of a row (zeros where its sum of weights is 0).
-template <class Q>
-__device__ __forceinline__ void store_out(Q* dst, f32x4 o, float l) {
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    o *= inv;
-    if (l == 0.0f) o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    if constexpr (sizeof(Q) == 4) *reinterpret_cast<f32x4*>(dst) = o;
-    else *reinterpret_cast<u32x2*>(dst) = u32x2{pack2<Q>(o[0], o[1]), pack2<Q>(o[2], o[3])};
-}
-
 // Counts this workgroup's state of an item in; true in the one that is last.
 // Relaxed: the states went out in agent-scope stores that every wave waits for
 // here, and are read with agent-scope loads once the count is known.
@@ -734,6 +786,8 @@ __device__ __forceinline__ int place_of(int b, int nw) {
     return x * q + min(x, r) + b / 8;
 }
 
+constexpr int narrow_ring(int hd) { return hd == 256 ? 32768 : 16384; }
+
 // ---- few rows: the waves split the keys ------------------------------------------
 // Single tokens and drafts, bound by the bytes of keys and values.  A wave
 // streams tiles of its own through its own LDS ring, no barrier between them,
@@ -742,20 +796,21 @@ template <class Q, class T, int HD, int RBLK>
 __global__ __launch_bounds__(256, RBLK == 1 || HD < 256 ? 2 : 1) void k_paged_narrow(PagedAttn p, Launch la) {
     constexpr int NW = 4, DB = 16, BM = DB * RBLK, BK = KindOf<T>::f32 ? 16 : 32, BN = NW * BK;
     using C = Core<Q, T, HD, DB, RBLK, BK>;
-    constexpr int D = 16384 / C::TB;    // tiles of K, and of V, in the ring
+    constexpr int kRing = narrow_ring(HD);  // bytes of a wave's ring
+    constexpr int D = kRing / 2 / C::TB;    // tiles of K, and of V, in the ring
     constexpr int H = BK / C::RPI;      // copies of a tile of K, or of V
     constexpr int G = BK / 8, PER = 8 / C::RPI;
     constexpr int kPart = part_floats(BM, HD);
-    static_assert(BM * HD * 4 <= 32768, "a wave's state fits its ring");
+    static_assert(BM * HD * 4 <= kRing && D >= 1, "a tile and a wave's state fit its ring");
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     __shared__ float sm[NW][BM], sl[NW][BM];
     __shared__ int flag;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    uint8_t* const ring = lds + wave * 32768;
+    uint8_t* const ring = lds + wave * kRing;
     const int nw = gridDim.x, w = place_of(blockIdx.x, nw);
-    Walk<BM, BN> walk(p);
+    Walk<BM, BN> walk(p, la);
     int64_t skip = 0, per = 0;
-    int64_t left = find_range<256>(walk, la, w, nw, &skip, &per);
+    int64_t left = find_range<256>(walk, w, nw, &skip, &per);
     int64_t item_at = w * per - skip;  // of the item's first tile in the sequence
     const uint32_t ring_at = uniform(static_cast<int>(lds_address(ring)));
     const float c1 = p.scale * kLog2e;
@@ -771,18 +826,7 @@ __global__ __launch_bounds__(256, RBLK == 1 || HD < 256 ? 2 : 1) void k_paged_na
         walk.span(walk.blk, &lo, &hi);
         const int rows = min(BM, walk.rows() - walk.blk * BM), row_first = walk.blk * BM;
         const int pos0 = walk.len - walk.n;
-        const int low_pos = pos0 + row_first / walk.group;  // position of the block's first row
-#pragma unroll
-        for (int i = 0; i < RBLK; ++i) {
-            const int r = i * DB + core.n, row = row_first + r;
-            const bool real = r < rows;
-            const int t = row / walk.group;
-            core.load_q(i, real ? static_cast<const Q*>(p.q) + (walk.row0 + t) * p.q_stride +
-                                      (walk.kvh * walk.group + row % walk.group) * HD
-                                : nullptr, c1);
-            core.last[i] = real ? pos0 + t : -1;
-            core.first[i] = p.window ? core.last[i] - p.window + 1 : 0;
-        }
+        const int low_pos = pos0 + walk.token(row_first);  // position of the block's first row
         const CONST_AS int* const table_row = (const CONST_AS int*)p.table + static_cast<int64_t>(walk.s) * p.cols;
         const int key0 = (walk.tile0 + a) * BN + wave * BK;
         int nt = b - a;
@@ -803,7 +847,6 @@ __global__ __launch_bounds__(256, RBLK == 1 || HD < 256 ? 2 : 1) void k_paged_na
 #pragma unroll
             for (int j = 0; j < G; ++j) g[j] = group_of<T>(p, table_row, walk.kvh, key0 + i * BN + 8 * j, hi - 1);
         };
-        wait_copies<0>();  // (q is here: from now on only copies are in flight)
         for (int i = 0; i < D; ++i)
             if (i < nt) {
                 Group g[G];
@@ -811,6 +854,18 @@ __global__ __launch_bounds__(256, RBLK == 1 || HD < 256 ? 2 : 1) void k_paged_na
                 copy_k(i, g);
                 copy_v(i, g);
             }
+#pragma unroll
+        for (int i = 0; i < RBLK; ++i) {
+            const int r = i * DB + core.n, row = row_first + r;
+            const bool real = r < rows;
+            const int t = walk.token(row);
+            core.load_q(i, real ? static_cast<const Q*>(p.q) + (walk.row0 + t) * p.q_stride +
+                                      (walk.kvh * walk.group + walk.head(row, t)) * HD
+                                : nullptr, c1);
+            core.last[i] = real ? pos0 + t : -1;
+            core.first[i] = p.window ? core.last[i] - p.window + 1 : 0;
+        }
+        wait_copies<0>();  // (q is here: from now on only copies are in flight)
         auto is_edge = [&](int key) { return key + BK - 1 > low_pos || (p.window && key <= hi - 1 - p.window); };
         bool special = false;
         for (int i = 0; i < nt; ++i) {
@@ -819,6 +874,7 @@ __global__ __launch_bounds__(256, RBLK == 1 || HD < 256 ? 2 : 1) void k_paged_na
             const bool edge = is_edge(key);
             Group g[G];
             if (more) groups(i + D, g);
+            // (what is in flight behind this tile's K: its V, and the later tiles in the ring)
             if (nt - i >= D) wait_copies<(2 * D - 1) * H>();
             else wait_copies<0>();
             core.scores(ring_at + (i % D) * C::TB);
@@ -874,12 +930,12 @@ __global__ __launch_bounds__(256, RBLK == 1 || HD < 256 ? 2 : 1) void k_paged_na
             for (int x = 0; x < NW; ++x) {
                 const float f = M == -kInf ? 1.0f : exp2_fast(sm[x][r] - M);
                 L += sl[x][r] * f;
-                O += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + x * 32768) + r * HD + (d ^ (4 * (r & 7)))) * f;
+                O += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + x * kRing) + r * HD + (d ^ (4 * (r & 7)))) * f;
             }
             if (!cut) {
-                const int row = row_first + r;
-                store_out(static_cast<Q*>(p.out) + (walk.row0 + row / walk.group) * p.out_stride +
-                              (walk.kvh * walk.group + row % walk.group) * HD + d, O, L);
+                const int row = row_first + r, t = walk.token(row);
+                store_out(static_cast<Q*>(p.out) + (walk.row0 + t) * p.out_stride +
+                              (walk.kvh * walk.group + walk.head(row, t)) * HD + d, O, L);
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) st_dev(part + r * HD + d + e, O[e]);
@@ -891,11 +947,11 @@ __global__ __launch_bounds__(256, RBLK == 1 || HD < 256 ? 2 : 1) void k_paged_na
         }
         if (cut) {
             if (arrive(la.counters + first_wg, last_wg - first_wg + 1, &flag))
-                join_parts<Q, BM, HD, 256>(p, la, first_wg, last_wg, rows, row_first, walk.row0, walk.kvh, walk.group);
+                join_parts<Q, BM, HD, 256>(walk, first_wg, last_wg, rows, reinterpret_cast<State*>(lds));
         }
         __syncthreads();  // the rings are free again
         item_at += walk.tiles;
-        if (left > 0 && !walk.next(la)) break;
+        if (left > 0 && !walk.next()) break;
     }
 }
 
@@ -914,9 +970,9 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
     __shared__ int flag;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int nw = gridDim.x, w = place_of(blockIdx.x, nw);
-    Walk<BM, BN> walk(p);
+    Walk<BM, BN> walk(p, la);
     int64_t skip = 0, per = 0;
-    int64_t left = find_range<NT>(walk, la, w, nw, &skip, &per);
+    int64_t left = find_range<NT>(walk, w, nw, &skip, &per);
     int64_t item_at = w * per - skip;
     const uint32_t lds_at = uniform(static_cast<int>(lds_address(lds)));
     const float c1 = p.scale * kLog2e;
@@ -934,18 +990,18 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
         walk.span(walk.blk, &lo, &hi);
         const int rows = min(BM, walk.rows() - walk.blk * BM), row_first = walk.blk * BM;
         const int pos0 = walk.len - walk.n;
-        const int low_pos = pos0 + row_first / walk.group;
+        const int low_pos = pos0 + walk.token(row_first);
         const int r = wave * DB + core.n, row = row_first + r;
         const bool real = r < rows;
-        const int t = row / walk.group;
-        const int64_t head = (walk.kvh * walk.group + row % walk.group) * HD;
+        const int t = walk.token(row);
+        const int64_t head = (walk.kvh * walk.group + walk.head(row, t)) * HD;
         core.load_q(0, real ? static_cast<const Q*>(p.q) + (walk.row0 + t) * p.q_stride + head : nullptr, c1);
         core.last[0] = real ? pos0 + t : -1;
         core.first[0] = p.window ? core.last[0] - p.window + 1 : 0;
         // the wave's rows see keys from wave_lo to wave_hi
         const bool busy = wave * DB < rows;
-        const int wave_low = pos0 + (row_first + wave * DB) / walk.group;
-        const int wave_hi = pos0 + (row_first + min(wave * DB + DB, rows) - 1) / walk.group;
+        const int wave_low = pos0 + walk.token(row_first + wave * DB);
+        const int wave_hi = pos0 + walk.token(row_first + min(wave * DB + DB, rows) - 1);
         const CONST_AS int* const table_row = (const CONST_AS int*)p.table + static_cast<int64_t>(walk.s) * p.cols;
         const int key0 = (walk.tile0 + a) * BN;
         const int nt = hi > 0 ? b - a : 0;
@@ -1014,10 +1070,10 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
                 }
             }
             if (arrive(la.counters + first_wg, last_wg - first_wg + 1, &flag))
-                join_parts<Q, BM, HD, NT>(p, la, first_wg, last_wg, rows, row_first, walk.row0, walk.kvh, walk.group);
+                join_parts<Q, BM, HD, NT>(walk, first_wg, last_wg, rows, reinterpret_cast<State*>(lds));
         }
         item_at += walk.tiles;
-        if (left > 0 && !walk.next(la)) break;
+        if (left > 0 && !walk.next()) break;
     }
 }
 
@@ -1031,6 +1087,9 @@ constexpr int wide_waves(int hd) {
 
 int slots() { return static_cast<int>(device_info().cus); }
 
+// Workgroups of the narrow form: those the CUs hold at once.
+int narrow_slots(int hd) { return slots() * (hd == 256 ? 1 : 2); }
+
 // The most rows a request can have.
 int64_t most_rows(const PagedAttn& p) {
     const int fresh = p.max_fresh > 0 && p.max_fresh < p.n_tokens ? p.max_fresh : p.n_tokens;
@@ -1043,6 +1102,11 @@ hipError_t run(const PagedAttn& p, float* part, uint32_t* counters, hipStream_t 
     Launch la;
     la.part = part;
     la.counters = counters;
+    la.group = p.n_q / p.kv.n_kv;
+    int log = 0;
+    while (1 << log < la.group) ++log;
+    la.group_shift = 31 + log;  // (group_mul <= 2^31, over the quotient by less than x / 2^31)
+    la.group_mul = static_cast<uint32_t>(((uint64_t{1} << la.group_shift) + la.group - 1) / la.group);
     const int64_t rows = most_rows(p);
     const bool wide = rows > kNarrowRows, narrow = !wide || p.n_seq > 1;
     const unsigned grid = static_cast<unsigned>(slots());
@@ -1057,8 +1121,9 @@ hipError_t run(const PagedAttn& p, float* part, uint32_t* counters, hipStream_t 
         la.min_rows = 0;
         la.max_rows = wide ? kNarrowRows : 0x7fffffff;
         la.min_tiles = 1;
-        if (rows <= 16) hipLaunchKernelGGL((k_paged_narrow<Q, T, HD, 1>), dim3(grid), dim3(256), 4 * 32768, s, p, la);
-        else hipLaunchKernelGGL((k_paged_narrow<Q, T, HD, 2>), dim3(grid), dim3(256), 4 * 32768, s, p, la);
+        const unsigned many = static_cast<unsigned>(narrow_slots(HD));
+        if (rows <= 16) hipLaunchKernelGGL((k_paged_narrow<Q, T, HD, 1>), dim3(many), dim3(256), 4 * narrow_ring(HD), s, p, la);
+        else hipLaunchKernelGGL((k_paged_narrow<Q, T, HD, 2>), dim3(many), dim3(256), 4 * narrow_ring(HD), s, p, la);
     }
     return hipGetLastError();
 }
@@ -1077,12 +1142,14 @@ hipError_t run_hd(const PagedAttn& p, float* part, uint32_t* counters, hipStream
 size_t paged_attention_workspace(const PagedAttn& p) {
     const int64_t rows = most_rows(p);
     const int waves = p.dtype == RT_HIP_F32 ? wide_waves<float>(p.kv.head_dim) : wide_waves<__bf16>(p.kv.head_dim);
-    const int bm = rows > kNarrowRows ? waves * 32 : (rows <= 16 ? 16 : 32);
-    return static_cast<size_t>(slots()) * 2 * part_floats(bm, p.kv.head_dim) * sizeof(float);
+    const int hd = p.kv.head_dim;
+    const size_t narrow = static_cast<size_t>(narrow_slots(hd)) * 2 * part_floats(rows <= 16 ? 16 : 32, hd);
+    const size_t wide = rows > kNarrowRows ? static_cast<size_t>(slots()) * 2 * part_floats(waves * 32, hd) : 0;
+    return (narrow > wide ? narrow : wide) * sizeof(float);
 }
 
 hipError_t launch_paged_attention(const PagedAttn& p, void* part, uint32_t* counters, hipStream_t s) {
-    if (static_cast<size_t>(slots()) > kArrivalCounters) return hipErrorInvalidValue;
+    if (static_cast<size_t>(narrow_slots(64)) > kArrivalCounters) return hipErrorInvalidValue;
     float* const f = static_cast<float*>(part);
     if (p.dtype == RT_HIP_BF16) return run_hd<__bf16, __bf16>(p, f, counters, s);
     if (p.dtype == RT_HIP_F16) return run_hd<_Float16, _Float16>(p, f, counters, s);
