@@ -663,7 +663,8 @@ int rt_hip_decoder_destroy(rt_hip_decoder* dec);
  * head_dim values of type dtype (RT_HIP_F32, RT_HIP_F16 or RT_HIP_BF16),
  * page_stride values from a page to the next (0: dense; larger where k and v
  * share an allocation).  page_size is a power of two from 8 to 1024, head_dim
- * 64, 128 or 256, n_pages * page_size < 2^31; pages start 16-byte aligned.
+ * 64, 128 or 256, n_pages * page_size < 2^31, page_stride < 2^32 bytes; pages
+ * start 16-byte aligned.
  * Slot i is row i % page_size of page i / page_size. */
 typedef struct rt_hip_paged_kv {
     void* k;

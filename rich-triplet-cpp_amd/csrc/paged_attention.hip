@@ -37,6 +37,8 @@
 // Keys a row does not see get weight 0, but 0 times an infinity or a NaN of
 // their v would reach the row: in tiles with such pairs those values of v are
 // made 0 in LDS, and added at the end to the rows that see them.
+#include <utility>
+
 #include "rt_common.hpp"
 #include "rt_launch.hpp"
 
@@ -89,24 +91,26 @@ __device__ __forceinline__ f32x2 unpack2(uint32_t w) {
 // N steps that each read a fragment from LDS and use it, B reads ahead of the
 // uses; the scheduling barriers keep the compiler from moving all the reads to
 // the front, into registers that the accumulators need.
+// (A fold instead of a loop, which the compiler leaves rolled past some length.)
+template <class F, int N, int B, class R, class U, int... X>
+__device__ __forceinline__ void read_ahead_steps(R read, U use, std::integer_sequence<int, X...>) {
+    F f[B];
+    auto first = [&](int x) {
+        if (x < B) f[x] = read(x);
+    };
+    auto step = [&](int x) {
+        use(x, f[x % B]);
+        if (x + B < N) f[x % B] = read(x + B);
+        if (x % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+    };
+    (first(X), ...);
+    __builtin_amdgcn_sched_barrier(0);
+    (step(X), ...);
+    __builtin_amdgcn_sched_barrier(0);
+}
 template <class F, int N, int B, class R, class U>
 __device__ __forceinline__ void read_ahead(R read, U use) {
-    static_assert(N % B == 0, "whole batches");
-    F f[2][B];
-#pragma unroll
-    for (int x = 0; x < B; ++x) f[0][x] = read(x);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int g = 0; g < N / B; ++g) {
-        if (g + 1 < N / B) {
-#pragma unroll
-            for (int x = 0; x < B; ++x) f[(g + 1) & 1][x] = read((g + 1) * B + x);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int x = 0; x < B; ++x) use(g * B + x, f[g & 1][x]);
-        __builtin_amdgcn_sched_barrier(0);
-    }
+    read_ahead_steps<F, N, B>(read, use, std::make_integer_sequence<int, N>());
 }
 
 // A value that every lane of the wave holds, in a scalar register.
@@ -125,6 +129,12 @@ __device__ __forceinline__ void copy_to_lds(const uint8_t* src, uint32_t offset,
     src = reinterpret_cast<const uint8_t*>(uniform(static_cast<int64_t>(reinterpret_cast<uintptr_t>(src))));
     dst = static_cast<uint32_t>(uniform(static_cast<int>(dst)));
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(offset), "s"(src) : "memory");
+}
+// 4 bytes a lane to LDS at dst + 4 lane.
+__device__ __forceinline__ void copy_words_to_lds(const void* src, uint32_t offset, uint32_t dst) {
+    src = reinterpret_cast<const void*>(uniform(static_cast<int64_t>(reinterpret_cast<uintptr_t>(src))));
+    dst = static_cast<uint32_t>(uniform(static_cast<int>(dst)));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(dst), "v"(offset), "s"(src) : "memory");
 }
 template <int N>
 __device__ __forceinline__ void wait_copies() {
@@ -159,6 +169,7 @@ struct Core {
     static constexpr int STEPS = CPR / KG, NC = HD / DB, KB = BK / DB, ACC = DB == 32 ? 16 : 4;
     static constexpr int KS = DB == 32 ? 16 : 32;  // keys of a 16-bit step of P V
     static constexpr int TB = BK * RB;             // bytes of a tile of K or V
+    static constexpr int kAhead = 8;  // fragments read ahead of the matrix steps
     // Weights are kept times 2^kBias, and the running maximum may lag by 2^kLag.
     static constexpr int kBias = F16 ? 6 : 0;
     static constexpr float kLag = 8.0f;
@@ -166,6 +177,7 @@ struct Core {
 
     u32x4 q[RBLK][NL][STEPS];
     Acc o[RBLK][NC], s[RBLK][KB];
+    u32x4 w[RBLK][F32 ? 1 : BK / KS][NL];  // weights as matrix operands (an f32 cache's stay in s)
     float m[RBLK], l[RBLK], c[RBLK];  // maximum of scores, sum of weights (this lane's keys), scale log2(e)
     int last[RBLK], first[RBLK];      // the keys the row sees
     int n, kg;                        // this lane's row of the block, its group
@@ -193,12 +205,16 @@ struct Core {
         else return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, x, 0, 0, 0);
     }
 
-    // Granules of 16 bytes of a key's row are exchanged by these, so that the
-    // lanes that LDS serves together read different banks.
-    __device__ __forceinline__ static int swz_k(int row) { return row & 7; }
+    // Granules of 16 bytes of a key's row are exchanged by these (xor), so that
+    // the lanes that LDS serves together, 256 bytes' worth of them, read
+    // different banks: 16 keys' granules of K, 4 keys' 64 bytes (DB = 32) or 8
+    // keys' 32 bytes (16) of V, for f32 the keys 4 apart of the lane groups.
+    // (Rows of 128 bytes lie two to 256.)  swz_v is the same 8 keys on.
+    __device__ __forceinline__ static int swz_k(int row) { return CPR >= 16 ? row & 15 : (row >> 1) & 7; }
     __device__ __forceinline__ static int swz_v(int row) {
-        if constexpr (F32) return 4 * ((row >> 2) & 3);
-        else return (2 * row) & (CPR - 1) & 15;
+        if constexpr (F32) return DB == 32 ? 8 * ((row >> 2) & 1) : 4 * ((row >> 2) & 3);
+        else if constexpr (DB == 32) return CPR >= 16 ? 4 * (row & 3) : 4 * ((row >> 1) & 1);
+        else return CPR >= 16 ? 2 * (row & 7) : 2 * ((row >> 1) & 3);
     }
 
     // Copies of keys [8 j, 8 j + 8) of a tile, those from `off` (a multiple of
@@ -215,6 +231,12 @@ struct Core {
     }
 
     __device__ __forceinline__ void setup() {
+#pragma unroll
+        for (int b = 0; b < RBLK; ++b)
+#pragma unroll
+            for (int t = 0; t < (F32 ? 1 : BK / KS); ++t)
+#pragma unroll
+                for (int k = 0; k < NL; ++k) w[b][t][k] = u32x4{0, 0, 0, 0};
         n = threadIdx.x & (DB - 1);
         kg = (threadIdx.x & 63) / DB;
     }
@@ -299,31 +321,46 @@ struct Core {
         return __uint_as_float(r[0]) + __uint_as_float(r[1]);
     }
 
-    // Scores of the tile whose keys lie at `k`.
-    __device__ __forceinline__ void scores(uint32_t k) {
+    // K's fragments, from the lane's first address.  (Tiles start at multiples of
+    // a key's bytes, so the granule's exchange is an xor of the address.)
+    __device__ __forceinline__ uint32_t k_first(uint32_t k) const { return k + n * RB + ((kg ^ swz_k(n)) << 4); }
+    __device__ __forceinline__ static u32x4 k_frag(uint32_t at, int x) {
+        return lds_read<u32x4>((at ^ (x / KB * KG * 16)) + x % KB * DB * RB);
+    }
+    __device__ __forceinline__ void score(int x, u32x4 a) {
+#pragma unroll
+        for (int i = NL - 1; i >= 0; --i)
+#pragma unroll
+            for (int b = 0; b < RBLK; ++b) s[b][x % KB] = mma(a, q[b][i][x / KB], s[b][x % KB]);
+    }
+    __device__ __forceinline__ void no_values() {
+#pragma unroll
+        for (int b = 0; b < RBLK; ++b)
+#pragma unroll
+            for (int i = 0; i < NC; ++i) o[b][i] = Acc{};
+    }
+    __device__ __forceinline__ void no_scores() {
 #pragma unroll
         for (int b = 0; b < RBLK; ++b)
 #pragma unroll
             for (int j = 0; j < KB; ++j) s[b][j] = Acc{};
-        // (tiles start at multiples of a key's bytes, so the granule's exchange is an xor of the address)
-        const uint32_t at = anew(k + n * RB + ((kg ^ swz_k(n)) << 4));
-        read_ahead<u32x4, KB * STEPS, F32 ? 2 : 4>(
-            [&](int x) { return lds_read<u32x4>((at ^ (x % STEPS * KG * 16)) + x / STEPS * DB * RB); },
-            [&](int x, u32x4 a) {
-#pragma unroll
-                for (int i = NL - 1; i >= 0; --i)
-#pragma unroll
-                    for (int b = 0; b < RBLK; ++b) s[b][x / STEPS] = mma(a, q[b][i][x % STEPS], s[b][x / STEPS]);
-            });
+    }
+    // Scores of the tile whose keys lie at `k`.
+    __device__ __forceinline__ void scores(uint32_t k) {
+        no_scores();
+        const uint32_t at = anew(k_first(k));
+        read_ahead<u32x4, KB * STEPS, F32 ? 2 : kAhead>([&](int x) { return k_frag(at, x); },
+                                                   [&](int x, u32x4 a) { score(x, a); });
     }
 
     // Weights in place of the scores; the running state moved to a new maximum
     // where one grew by more than 2^kLag.  key: the tile's first; edge: some
     // row does not see some of its keys.
-    __device__ __forceinline__ void softmax(int key, bool edge) {
+    // halfway(): called between the maximum and the weights.
+    template <class F>
+    __device__ __forceinline__ void softmax(int key, bool edge, F halfway) {
 #pragma unroll
         for (int b = 0; b < RBLK; ++b) {
-            float mx = -kInf;
             if (edge) {
 #pragma unroll
                 for (int j = 0; j < KB; ++j)
@@ -335,11 +372,13 @@ struct Core {
                         if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
                     }
             }
+            // (four chains: one would wait for each of its steps)
+            float top[4] = {-kInf, -kInf, -kInf, -kInf};
 #pragma unroll
             for (int j = 0; j < KB; ++j)
 #pragma unroll
-                for (int e = 0; e < ACC; ++e) mx = fmaxf(mx, s[b][j][e]);
-            mx = across_max(mx);
+                for (int e = 0; e < ACC; ++e) top[e & 3] = fmaxf(top[e & 3], s[b][j][e]);
+            const float mx = across_max(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
             // (a row of nothing but -inf so far: m stays -inf, weights are 0)
             if (__builtin_amdgcn_ballot_w64(mx * c[b] > m[b] * c[b] + kLag) != 0) {
                 const float mn = fmaxf(m[b], mx);
@@ -350,35 +389,58 @@ struct Core {
                 for (int i = 0; i < NC; ++i) o[b][i] *= a;
             }
             const float base = static_cast<float>(kBias) - (m[b] == -kInf ? 0.0f : m[b]) * c[b];
-            float sum = 0.0f;
+            if (b == 0) halfway();
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int j = 0; j < KB; ++j)
 #pragma unroll
                 for (int e = 0; e < ACC; ++e) {
                     s[b][j][e] = exp2_fast(__builtin_fmaf(s[b][j][e], c[b], base));
-                    sum += s[b][j][e];
+                    if constexpr (F32 || NL > 1) sum[e & 3] += s[b][j][e];
                 }
-            l[b] += sum;
+            if constexpr (!F32) {
+#pragma unroll
+                for (int t = 0; t < BK / KS; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int e = 8 * t + 2 * i;
+                        uint32_t x[NL];
+                        limbs(s[b][e / ACC][e % ACC], s[b][(e + 1) / ACC][(e + 1) % ACC], x);
+#pragma unroll
+                        for (int k = 0; k < NL; ++k) w[b][t][k][i] = x[k];
+                        // (the sum of the weights as they multiply v, two to an instruction)
+                        if constexpr (NL == 1) sum[i] = sum2(x[0], sum[i]);
+                    }
+            }
+            l[b] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            // (opaque: the compiler would compute them where they are used, among the products)
+            if constexpr (F32) {
+#pragma unroll
+                for (int j = 0; j < KB; ++j) asm volatile("" : "+v"(s[b][j]));
+            } else {
+#pragma unroll
+                for (int t = 0; t < BK / KS; ++t)
+#pragma unroll
+                    for (int k = 0; k < NL; ++k) asm volatile("" : "+v"(w[b][t][k]));
+            }
+        }
+    }
+    __device__ __forceinline__ static float sum2(uint32_t x, float sum) {
+        if constexpr (F16) {
+            typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+            return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, x), h2{1.0f, 1.0f}, sum, false);
+        } else {
+            const uint32_t one = 0x3f803f80u;
+            return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, x), __builtin_bit_cast(bf16x2, one), sum, false);
         }
     }
 
-    // Weights of step t (8 registers of the blocks' sequence) as limbs.
-    __device__ __forceinline__ void weights(int b, int t, u32x4 (&p)[NL]) const {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int e = 8 * t + 2 * i;
-            uint32_t w[NL];
-            limbs(s[b][e / ACC][e % ACC], s[b][(e + 1) / ACC][(e + 1) % ACC], w);
-#pragma unroll
-            for (int k = 0; k < NL; ++k) p[k][i] = w[k];
-        }
-    }
     // V's fragments.  16-bit step t, dims DB c ..: keys t KS + (KS / 2) a + 4 kg
     // + {0..3}, a = 0, 1, from the lane's first address.
     __device__ __forceinline__ uint32_t v_first(uint32_t v) const {
         const int lane = threadIdx.x & 63;
         if constexpr (F32) {  // the value for a register's key and this lane's dim
-            return v + 4 * kg * RB + (((n >> 2) ^ (4 * kg)) << 4) + 4 * (n & 3);
+            return v + 4 * kg * RB + (((n >> 2) ^ swz_v(4 * kg)) << 4) + 4 * (n & 3);
         } else {
             const int row = 4 * kg + ((lane & 15) >> 2);
             const int chunk = (DB == 32 ? 2 * ((lane >> 4) & 1) : 0) + ((lane & 3) >> 1);
@@ -399,15 +461,14 @@ struct Core {
     }
     // f32: register e of block j, dims DB c ..
     __device__ __forceinline__ static float v_val(uint32_t at, int j, int e, int c) {
-        return lds_read<float>((at ^ (c * DB * 4) ^ (DB == 32 && ((e >> 2) & 1) ? 128 : 0)) +
-                               (j * DB + 8 * (e >> 2) + (e & 3)) * RB);
+        return lds_read<float>((at ^ (c * DB * 4)) + (j * DB + 8 * (e >> 2) + (e & 3)) * RB);
     }
 
     // o += P V of the tile whose values lie at `v`.
     __device__ __forceinline__ void pv(uint32_t v) {
         const uint32_t at = anew(v_first(v));
         if constexpr (F32) {
-            read_ahead<float, KB * ACC * NC, 4>(
+            read_ahead<float, KB * ACC * NC, 8>(
                 [&](int x) { return v_val(at, x / NC / ACC, x / NC % ACC, x % NC); },
                 [&](int x, float a) {
 #pragma unroll
@@ -415,18 +476,37 @@ struct Core {
                         o[b][x % NC] = mma1(a, s[b][x / NC / ACC][x / NC % ACC], o[b][x % NC]);
                 });
         } else {
-            u32x4 p[RBLK][NL];
-            read_ahead<u32x4, BK / KS * NC, NC < 4 ? NC : 4>([&](int x) { return v_frag(at, x / NC, x % NC); },
-                                                             [&](int x, u32x4 a) {
-                if (x % NC == 0) {
+            read_ahead<u32x4, BK / KS * NC, kAhead>([&](int x) { return v_frag(at, x / NC, x % NC); },
+                                                             [&](int x, u32x4 a) { add_value(x, a); });
+        }
+    }
+    __device__ __forceinline__ void add_value(int x, u32x4 a) {
 #pragma unroll
-                    for (int b = 0; b < RBLK; ++b) weights(b, x / NC, p[b]);
-                }
+        for (int k = NL - 1; k >= 0; --k)
 #pragma unroll
-                for (int k = NL - 1; k >= 0; --k)
+            for (int b = 0; b < RBLK; ++b) o[b][x % NC] = mma(a, w[b][x / NC][k], o[b][x % NC]);
+    }
+    // pv(v), then scores(k), the reads of the second running ahead into the
+    // first; between(i), i < N, at even distances.
+    template <int N, class F>
+    __device__ __forceinline__ void products(uint32_t k, uint32_t v, F between) {
+        if constexpr (F32) {
 #pragma unroll
-                    for (int b = 0; b < RBLK; ++b) o[b][x % NC] = mma(a, p[b][k], o[b][x % NC]);
-            });
+            for (int i = 0; i < N; ++i) between(i);
+            pv(v);
+            scores(k);
+        } else {
+            constexpr int NV = BK / KS * NC, NK = KB * STEPS;
+            const uint32_t at_v = anew(v_first(v)), at_k = anew(k_first(k));
+            no_scores();
+            read_ahead<u32x4, NV + NK, kAhead>([&](int x) { return x < NV ? v_frag(at_v, x / NC, x % NC) : k_frag(at_k, x - NV); },
+                                          [&](int x, u32x4 a) {
+#pragma unroll
+                                              for (int i = 0; i < N; ++i)
+                                                  if (x == (i + 1) * ((NV + NK) / (N + 1))) between(i);
+                                              if (x < NV) add_value(x, a);
+                                              else score(x - NV, a);
+                                          });
         }
     }
 
@@ -576,11 +656,32 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
     return a / b;
 }
 
+// Inclusive sum over the wave's lanes.
+__device__ __forceinline__ int64_t wave_scan(int64_t v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const int64_t o = __shfl_up(v, off, kWave);
+        if (lane >= off) v += o;
+    }
+    return v;
+}
+// Tiles of the walk's request for one KV head, its blocks counted by the wave's
+// lanes (the walk is the same in all of them).
+template <class W>
+__device__ __forceinline__ int64_t wave_total(const W& walk) {
+    int64_t t = 0;
+    int first;
+    for (int b = threadIdx.x & 63; b < walk.blocks; b += 64) t += walk.count(b, &first);
+    return uniform(__shfl(wave_scan(t), 63, kWave));
+}
+
 // Positions the walk at workgroup w's range of the sequence of all tiles (of
 // nw equal ones) and returns how many tiles it takes (0: none); *skip: how many
 // of the first item's lie before them; *per: tiles of a range.  Up to 64
 // requests every wave sums for itself, one to a lane; otherwise the workgroup's
-// threads do, several to a thread.
+// threads do, several to a thread.  A request of many blocks is counted by its
+// wave's lanes together.
 template <int NT, class W>
 __device__ __forceinline__ int64_t find_range(W& walk, int w, int nw, int64_t* skip, int64_t* per) {
     const int tid = threadIdx.x, lane = tid & 63, n_seq = walk.p.n_seq, n_kv = walk.p.kv.n_kv;
@@ -589,19 +690,25 @@ __device__ __forceinline__ int64_t find_range(W& walk, int w, int nw, int64_t* s
     __shared__ int64_t found_before;
     const bool small = n_seq <= 64;
     const int each = small ? 1 : (n_seq + NT - 1) / NT, base = small ? lane : tid * each;
+    // tiles of this lane's i-th request
+    auto tiles_of = [&](int i) -> int64_t {
+        W scan(walk.p, walk.la);
+        if (base + i < n_seq) scan.request(base + i);
+        int64_t t = scan.blocks <= 2 ? scan.total() : 0;
+        for (uint64_t many = __builtin_amdgcn_ballot_w64(scan.blocks > 2); many; many &= many - 1) {
+            const int src = __builtin_ctzll(many);
+            W one(walk.p, walk.la);
+            one.n = __builtin_amdgcn_readlane(scan.n, src);
+            one.len = __builtin_amdgcn_readlane(scan.len, src);
+            one.blocks = __builtin_amdgcn_readlane(scan.blocks, src);
+            const int64_t sum = wave_total(one);
+            if (lane == src) t = sum;
+        }
+        return t * n_kv;
+    };
     int64_t mine = 0;
-    W scan(walk.p, walk.la);
-    for (int i = 0; i < each; ++i) {
-        if (base + i >= n_seq) break;
-        scan.request(base + i);
-        mine += scan.total() * n_kv;
-    }
-    int64_t incl = mine;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const int64_t o = __shfl_up(incl, off, kWave);
-        if (lane >= off) incl += o;
-    }
+    for (int i = 0; i < each; ++i) mine += tiles_of(i);
+    int64_t incl = wave_scan(mine);
     int64_t all = __shfl(incl, 63, kWave);
     if (!small) {
         if (lane == 63) sums[tid >> 6] = incl;
@@ -626,14 +733,12 @@ __device__ __forceinline__ int64_t find_range(W& walk, int w, int nw, int64_t* s
         s = __builtin_ctzll(__builtin_amdgcn_ballot_w64(here));
         at = __shfl(at, s, kWave);
     } else {
-        if (here) {
+        if (__builtin_amdgcn_ballot_w64(here) != 0) {  // (whole waves, as tiles_of counts)
             for (int i = 0; i < each; ++i) {
-                scan.request(base + i);
-                const int64_t t = scan.total() * n_kv;
-                if (u < at + t) {
+                const int64_t t = tiles_of(i);
+                if (here && u >= at && u < at + t) {
                     found_s = base + i;
                     found_before = at;
-                    break;
                 }
                 at += t;
             }
@@ -644,20 +749,32 @@ __device__ __forceinline__ int64_t find_range(W& walk, int w, int nw, int64_t* s
     }
     walk.request(uniform(s));
     int64_t off = u - uniform(at);
-    const int64_t t = walk.total();
+    const int64_t t = wave_total(walk);
     walk.kvh = static_cast<int>(quotient(off, t));
     off -= walk.kvh * t;
-    int b = 0, first, c;
-    while (off >= (c = walk.count(b, &first)) && b + 1 < walk.blocks) {
-        off -= c;
-        ++b;
+    for (int b0 = 0;; b0 += 64) {
+        int first;
+        const int c = b0 + lane < walk.blocks ? walk.count(b0 + lane, &first) : 0;
+        const int64_t sum = wave_scan(c);
+        const uint64_t behind = __builtin_amdgcn_ballot_w64(off < sum);
+        if (behind || b0 + 64 >= walk.blocks) {
+            const int l = behind ? __builtin_ctzll(behind) : 0;
+            walk.block(b0 + l);
+            off -= uniform(__shfl(sum - c, l, kWave));
+            break;
+        }
+        off -= uniform(__shfl(sum, 63, kWave));
     }
-    walk.block(b);
     *skip = off;
     return min(*per, all - u);
 }
 
+// A state of the few-row form: o [bm][hd], maxima [bm], sums [bm]; of the
+// many-row form: a lane's values, maximum and sum, two lanes to a row.
 constexpr int part_floats(int bm, int hd) { return bm * hd + 2 * bm; }
+constexpr int wide_part_floats(int bm, int hd) { return bm * hd + 4 * bm; }
+// Tiles of K, and of V, that the many-row form keeps in LDS.
+constexpr int wide_slots(int tile_bytes) { return 6 * tile_bytes <= 147456 ? 3 : 2; }
 
 // The store of four values of a row (zeros where its sum of weights is 0).
 template <class Q>
@@ -730,38 +847,85 @@ __device__ __forceinline__ void join_parts(const W& walk, int first_wg, int last
     }
 }
 
-// Copies of one group of 8 keys: where they are.
-struct Group {
-    const uint8_t* k;
-    const uint8_t* v;
-    uint32_t row_bytes;
-    int most;  // the last key that may be read, from the group's first
+// A request's pages, for one KV head.
+struct Pages {
+    const CONST_AS int* table;  // its row
+    const uint8_t* k;           // the head's first key in page 0
+    int64_t v;                  // from keys to values
+    uint32_t page_bytes, row_bytes;
+    int shift, n_pages, end;    // end: the last key that is read
 };
-// The group with the keys from `key` (a multiple of 8) on, of those up to
-// `end` (its last key; groups behind it read that of `end` again).
 template <class T>
-__device__ __forceinline__ Group group_of(const PagedAttn& p, const CONST_AS int* table_row, int kvh, int key, int end) {
-    const int at = min(key, end & ~7);
-    const int id = table_row[at >> p.kv.page_shift];
-    const bool real = static_cast<uint32_t>(id) < static_cast<uint32_t>(p.kv.n_pages);
-    const int64_t off = ((real ? id : 0) * p.kv.page_stride +
-                         (static_cast<int64_t>(at & ((1 << p.kv.page_shift) - 1)) * p.kv.n_kv + kvh) * p.kv.head_dim) *
-                        static_cast<int64_t>(sizeof(T));
-    const uint8_t* const zeros = reinterpret_cast<const uint8_t*>(kZeros);
-    Group g;
-    g.k = real ? static_cast<const uint8_t*>(p.kv.k) + off : zeros;
-    g.v = real ? static_cast<const uint8_t*>(p.kv.v) + off : zeros;
-    g.row_bytes = real ? static_cast<uint32_t>(p.kv.n_kv * p.kv.head_dim) * static_cast<uint32_t>(sizeof(T)) : 0u;
-    g.most = end - at;
+__device__ __forceinline__ Pages pages_of(const PagedAttn& p, int s, int kvh, int end) {
+    constexpr int64_t B = sizeof(T);
+    Pages g;
+    g.table = (const CONST_AS int*)p.table + static_cast<int64_t>(s) * p.cols;
+    g.k = static_cast<const uint8_t*>(p.kv.k) + kvh * p.kv.head_dim * B;
+    g.v = static_cast<const uint8_t*>(p.kv.v) - static_cast<const uint8_t*>(p.kv.k);
+    g.page_bytes = static_cast<uint32_t>(p.kv.page_stride * B);  // (the host keeps it below 2^32)
+    g.row_bytes = static_cast<uint32_t>(p.kv.n_kv * p.kv.head_dim * B);
+    g.shift = p.kv.page_shift;
+    g.n_pages = p.kv.n_pages;
+    g.end = end;
     return g;
 }
-
-// Where the values of one key are.
-template <class T>
-__device__ __forceinline__ const uint8_t* value_of(const PagedAttn& p, const CONST_AS int* table_row, int kvh, int key) {
-    const Group g = group_of<T>(p, table_row, kvh, key & ~7, key);
-    return g.v + static_cast<uint32_t>(key & 7) * g.row_bytes;
+// A group of 8 keys: where they are.
+struct Group {
+    const uint8_t* k;
+    int64_t v;           // from keys to values
+    uint32_t row_bytes;
+    int most;            // the last key that may be read, from the group's first
+};
+// The group's place in the request: that of `key` (a multiple of 8), behind the
+// last key the one that holds it.
+__device__ __forceinline__ int group_at(const Pages& g, int key) { return min(key, g.end & ~7); }
+// The group at `at` on page `id`.
+__device__ __forceinline__ Group group_on(const Pages& g, int at, int id) {
+    const bool real = static_cast<uint32_t>(id) < static_cast<uint32_t>(g.n_pages);
+    const uint8_t* const k = g.k + static_cast<uint64_t>(static_cast<uint32_t>(id)) * g.page_bytes +
+                             static_cast<uint32_t>(at & ((1 << g.shift) - 1)) * g.row_bytes;
+    Group x;
+    x.k = real ? k : reinterpret_cast<const uint8_t*>(kZeros);
+    x.v = real ? g.v : 0;
+    x.row_bytes = real ? g.row_bytes : 0u;
+    x.most = g.end - at;
+    return x;
 }
+__device__ __forceinline__ Group group_of(const Pages& g, int key) {
+    const int at = group_at(g, key);
+    return group_on(g, at, g.table[at >> g.shift]);
+}
+// Where the values of one key are (key <= end).
+__device__ __forceinline__ const uint8_t* value_of(const Pages& g, int key) {
+    const Group x = group_of(g, key & ~7);
+    return x.k + x.v + static_cast<uint32_t>(key & 7) * x.row_bytes;
+}
+
+// Page numbers of a walk along a request's keys: a wave's ring of 128 table
+// entries in LDS, filled 64 at a time by copies that its waits for keys and
+// values cover.  Entry `col` is word col % 128.
+struct PageWindow {
+    uint32_t ring;
+    int base;  // entries base .. base + 127 are there or on their way
+    __device__ __forceinline__ void fill(const Pages& g, int col) const {
+        const int at = min(col + (static_cast<int>(threadIdx.x) & 63), g.end >> g.shift);
+        copy_words_to_lds((const void*)g.table, static_cast<uint32_t>(at) * 4u, ring + (col & 127) * 4);
+    }
+    __device__ __forceinline__ void start(const Pages& g, int col) {
+        base = col & ~63;
+        fill(g, base);
+        fill(g, base + 64);
+    }
+    // Entry `col`, no smaller than those asked for before and at most 64 from
+    // the last of them; the copies that were on their way at that one are there.
+    __device__ __forceinline__ int at(const Pages& g, int col) {
+        if (col - base >= 64) {
+            base += 64;
+            fill(g, base + 64);
+        }
+        return uniform(lds_read<int>(ring + (col & 127) * 4));
+    }
+};
 
 // Counts this workgroup's state of an item in; true in the one that is last.
 // Relaxed: the states went out in agent-scope stores that every wave waits for
@@ -827,7 +991,7 @@ __global__ __launch_bounds__(256, RBLK == 1 || HD < 256 ? 2 : 1) void k_paged_na
         const int rows = min(BM, walk.rows() - walk.blk * BM), row_first = walk.blk * BM;
         const int pos0 = walk.len - walk.n;
         const int low_pos = pos0 + walk.token(row_first);  // position of the block's first row
-        const CONST_AS int* const table_row = (const CONST_AS int*)p.table + static_cast<int64_t>(walk.s) * p.cols;
+        const Pages pages = pages_of<T>(p, walk.s, walk.kvh, hi - 1);
         const int key0 = (walk.tile0 + a) * BN + wave * BK;
         int nt = b - a;
         if (key0 + (nt - 1) * BN >= hi) --nt;  // (the last tile's keys may end before this wave's)
@@ -840,12 +1004,12 @@ __global__ __launch_bounds__(256, RBLK == 1 || HD < 256 ? 2 : 1) void k_paged_na
         auto copy_v = [&](int i, const Group (&g)[G]) {
 #pragma unroll
             for (int j = 0; j < H; ++j)
-                C::template copy_rows<true>(g[j / PER].v, g[j / PER].row_bytes, g[j / PER].most, j / PER,
+                C::template copy_rows<true>(g[j / PER].k + g[j / PER].v, g[j / PER].row_bytes, g[j / PER].most, j / PER,
                                             j % PER * C::RPI, ring_at + (D + i % D) * C::TB + j * 1024);
         };
         auto groups = [&](int i, Group (&g)[G]) {
 #pragma unroll
-            for (int j = 0; j < G; ++j) g[j] = group_of<T>(p, table_row, walk.kvh, key0 + i * BN + 8 * j, hi - 1);
+            for (int j = 0; j < G; ++j) g[j] = group_of(pages, key0 + i * BN + 8 * j);
         };
         for (int i = 0; i < D; ++i)
             if (i < nt) {
@@ -865,7 +1029,10 @@ __global__ __launch_bounds__(256, RBLK == 1 || HD < 256 ? 2 : 1) void k_paged_na
             core.last[i] = real ? pos0 + t : -1;
             core.first[i] = p.window ? core.last[i] - p.window + 1 : 0;
         }
-        wait_copies<0>();  // (q is here: from now on only copies are in flight)
+        // q is here: from now on only copies are in flight.  (The builtin, which the
+        // compiler understands: it would wait for q's loads in every tile otherwise,
+        // and with them for the copies.)
+        wait_vmcnt<0>();
         auto is_edge = [&](int key) { return key + BK - 1 > low_pos || (p.window && key <= hi - 1 - p.window); };
         bool special = false;
         for (int i = 0; i < nt; ++i) {
@@ -880,7 +1047,7 @@ __global__ __launch_bounds__(256, RBLK == 1 || HD < 256 ? 2 : 1) void k_paged_na
             core.scores(ring_at + (i % D) * C::TB);
             wait_lds();
             if (more) copy_k(i + D, g);
-            core.softmax(key, edge);
+            core.softmax(key, edge, [] {});
             if (more) wait_copies<(2 * D - 1) * H>();
             else wait_copies<0>();
             const uint32_t v = ring_at + (D + i % D) * C::TB;
@@ -899,7 +1066,7 @@ __global__ __launch_bounds__(256, RBLK == 1 || HD < 256 ? 2 : 1) void k_paged_na
             for (int i = 0; i < nt; ++i)
                 if (const int key = key0 + i * BN; is_edge(key))
                     for (int j = key; j < min(key + BK, hi); ++j)
-                        core.add_special(j, value_of<T>(p, table_row, walk.kvh, j));
+                        core.add_special(j, value_of(pages, j));
         }
         // The waves' states, joined in order.
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -962,10 +1129,15 @@ template <class Q, class T, int HD, int NW>
 __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) {
     constexpr int DB = 32, BM = DB * NW, BK = KindOf<T>::f32 ? 32 : 64, BN = BK, NT = NW * 64;
     using C = Core<Q, T, HD, DB, 1, BK>;
-    constexpr int PER = 8 / C::RPI, COPIES = BK / C::RPI / NW;  // copies of a tile of K, or of V, by each wave
-    constexpr int kPart = part_floats(BM, HD);
-    static_assert(COPIES >= 1 && COPIES * NW * C::RPI == BK, "every wave copies alike");
-    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];  // two tiles of K and V
+    constexpr int PER = 8 / C::RPI;               // copies of a group of 8 keys
+    constexpr int COPIES = BK / C::RPI / NW;      // copies of a tile of K, or of V, by each wave
+    constexpr int GROUPS = COPIES < PER ? 1 : COPIES / PER;  // groups they are of
+    constexpr int SLOTS = wide_slots(C::TB), L = SLOTS - 2;  // tiles of K, and of V, in LDS; copies run L steps further ahead
+    constexpr int kPart = wide_part_floats(BM, HD);
+    static_assert(COPIES >= 1 && COPIES * NW * C::RPI == BK && (COPIES < PER ? PER % COPIES : COPIES % PER) == 0,
+                  "every wave copies alike, whole groups or part of one");
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];  // SLOTS tiles of K, SLOTS of V
+    __shared__ int page_ring[NW][128];
     __shared__ int special;  // the last of this workgroup's items whose v held what was made 0
     __shared__ int flag;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -977,7 +1149,7 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
     const uint32_t lds_at = uniform(static_cast<int>(lds_address(lds)));
     const float c1 = p.scale * kLog2e;
     if (tid == 0) special = -1;
-    int step = 0, item = 0;  // tiles and items so far
+    int item = 0;
     C core;
     core.setup();
     while ((left = uniform(left)) > 0) {
@@ -995,82 +1167,164 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
         const bool real = r < rows;
         const int t = walk.token(row);
         const int64_t head = (walk.kvh * walk.group + walk.head(row, t)) * HD;
+        // the wave's rows see keys from wave_lo to wave_hi
+        const int wave_low = pos0 + walk.token(row_first + wave * DB);
+        const int wave_hi = pos0 + walk.token(row_first + min(wave * DB + DB, rows) - 1);
+        const Pages pages = pages_of<T>(p, walk.s, walk.kvh, hi - 1);
+        const int key0 = (walk.tile0 + a) * BN;
+        const int nt = hi > 0 ? b - a : 0;
+        // This wave's groups of the tiles whose K and whose V are copied next.
+        PageWindow window;
+        window.ring = uniform(static_cast<int>(lds_address(page_ring[wave])));
+        Group grp_k[GROUPS], grp_v[GROUPS];
+        const int group0 = wave * COPIES / PER;  // (the wave's copies start in it, at part0)
+        const int part0 = COPIES < PER ? wave * COPIES % PER : 0;
+        auto find_groups = [&](int i) {
+#pragma unroll
+            for (int x = 0; x < GROUPS; ++x) {
+                const int at = group_at(pages, key0 + i * BN + 8 * (group0 + x));
+                grp_k[x] = group_on(pages, at, window.at(pages, at >> pages.shift));
+            }
+        };
+        // Copy x of this wave's of a tile of K, or V, into a slot.
+        auto copy_k = [&](int slot, int x) {
+            const Group& g = grp_k[x / PER];
+            C::template copy_rows<false>(g.k, g.row_bytes, g.most, group0 + x / PER, (part0 + x % PER) * C::RPI,
+                                         lds_at + slot * C::TB + (wave * COPIES + x) * 1024);
+        };
+        auto copy_v = [&](int slot, int x) {
+            const Group& g = grp_v[x / PER];
+            C::template copy_rows<true>(g.k + g.v, g.row_bytes, g.most, group0 + x / PER, (part0 + x % PER) * C::RPI,
+                                        lds_at + (SLOTS + slot) * C::TB + (wave * COPIES + x) * 1024);
+        };
+        auto is_edge = [&](int key) { return key + BK - 1 > low_pos || (p.window && key <= hi - 1 - p.window); };
+        int ahead = 0;  // the tile grp_k is of
+        auto advance = [&] {
+#pragma unroll
+            for (int x = 0; x < GROUPS; ++x) grp_v[x] = grp_k[x];
+            find_groups(++ahead);
+        };
+        lds_barrier();  // (every wave is done with the item before)
+        if (nt > 0) {
+            window.start(pages, group_at(pages, key0 + 8 * group0) >> pages.shift);
+            wait_copies<0>();
+            find_groups(0);
+#pragma unroll
+            for (int x = 0; x < COPIES; ++x) copy_k(0, x);
+            advance();
+            if constexpr (L == 1) {
+#pragma unroll
+                for (int x = 0; x < COPIES; ++x) copy_v(0, x);
+#pragma unroll
+                for (int x = 0; x < COPIES; ++x) copy_k(1, x);
+                advance();
+            }
+        }
         core.load_q(0, real ? static_cast<const Q*>(p.q) + (walk.row0 + t) * p.q_stride + head : nullptr, c1);
         core.last[0] = real ? pos0 + t : -1;
         core.first[0] = p.window ? core.last[0] - p.window + 1 : 0;
-        // the wave's rows see keys from wave_lo to wave_hi
-        const bool busy = wave * DB < rows;
-        const int wave_low = pos0 + walk.token(row_first + wave * DB);
-        const int wave_hi = pos0 + walk.token(row_first + min(wave * DB + DB, rows) - 1);
-        const CONST_AS int* const table_row = (const CONST_AS int*)p.table + static_cast<int64_t>(walk.s) * p.cols;
-        const int key0 = (walk.tile0 + a) * BN;
-        const int nt = hi > 0 ? b - a : 0;
-        auto copy_tile = [&](int i) {
-            const uint32_t k = lds_at + ((step + i) & 1) * 2 * C::TB;
-#pragma unroll
-            for (int x = 0; x < COPIES; ++x) {
-                const int j = wave * COPIES + x, grp = j / PER;
-                const Group g = group_of<T>(p, table_row, walk.kvh, key0 + i * BN + 8 * grp, hi - 1);
-                C::template copy_rows<false>(g.k, g.row_bytes, g.most, grp, j % PER * C::RPI, k + j * 1024);
-                C::template copy_rows<true>(g.v, g.row_bytes, g.most, grp, j % PER * C::RPI, k + C::TB + j * 1024);
-            }
-        };
-        lds_barrier();  // (every wave is done with the item before)
-        auto is_edge = [&](int key) { return key + BK - 1 > low_pos || (p.window && key <= hi - 1 - p.window); };
-        if (nt > 0) copy_tile(0);
-        for (int i = 0; i < nt; ++i) {
-            const int key = key0 + i * BN, slot = (step + i) & 1;
-            const uint32_t k = lds_at + slot * 2 * C::TB;
-            wait_copies<0>();
-            if (is_edge(key)) {
+        wait_vmcnt<0>();  // (the builtin: so that the compiler, too, knows that q is there)
+        lds_barrier();
+        // Step i in two halves: the products, O += P V of tile i - 1 and the
+        // scores of tile i, and the weighing of tile i.  With eight waves, w and
+        // w + 4 share a SIMD: the second four run a half behind the first, so
+        // that one wave of a SIMD has the matrix cores while the other has the
+        // VALU, a barrier between the halves.
+        // Among its products a wave sends the copies of V of tile i + L and K of
+        // tile i + 1 + L, into the slots of V of tile i - 2 and K of tile i - 1,
+        // which every wave has read by then; it waits for them in step i + L,
+        // before the barrier that step i + L + 1 lies behind.  (Past the last
+        // tile they bring its last keys again, for no one.)
+        constexpr bool kTwo = NW == 8;
+        static_assert(!kTwo || L == 1, "the second four send their copies a half late");
+        const bool second = kTwo && wave >= 4;
+        // This wave's copies of V of tile i are there; of an edge tile's, cleaned.
+        auto settle = [&](int i, int slot) {
+            wait_copies<2 * COPIES * L>();
+            if (is_edge(key0 + i * BN)) {
                 bool any = false;
 #pragma unroll
                 for (int x = 0; x < COPIES; ++x)
-                    any |= C::clean_at(k + C::TB + (wave * COPIES + x) * 1024 + anew((tid & 63) * 16));
+                    any |= C::clean_at(lds_at + (SLOTS + slot) * C::TB + (wave * COPIES + x) * 1024 + anew((tid & 63) * 16));
                 if (__builtin_amdgcn_ballot_w64(any) != 0) special = item;
             }
-            lds_barrier();
-            if (i + 1 < nt) copy_tile(i + 1);
-            // (tiles that none of the wave's rows sees)
-            if (!busy || key > wave_hi || (p.window && key + BK <= wave_low - p.window + 1)) continue;
-            const bool wave_edge = key + BK - 1 > wave_low || (p.window && key <= wave_hi - p.window);
-            core.scores(k);
-            core.softmax(key, wave_edge);
-            core.pv(k + C::TB);
+        };
+        if (nt > 0) {
+            if (second) lds_barrier();
+            int now = 0;  // slot of tile i
+            for (int i = 0; i <= nt; ++i) {
+                const int before = now == 0 ? SLOTS - 1 : now - 1, behind = now + 1 == SLOTS ? 0 : now + 1;
+                // (no branch around the products of what is not there or not seen: the
+                // weights of a tile that no row of the wave sees are 0 and its V is
+                // clean, being an edge tile; in step 0 the accumulator is cleared
+                // after; scores of no tile are not used)
+                __builtin_amdgcn_s_setprio(1);
+                core.template products<2 * COPIES>(lds_at + now * C::TB, lds_at + (SLOTS + before) * C::TB, [&](int x) {
+                    if (x < COPIES) copy_v(L ? behind : now, x);
+                    else copy_k(before, x - COPIES);
+                });
+                __builtin_amdgcn_s_setprio(0);
+                if (i == 0) core.no_values();
+                if (second && i < nt) settle(i, now);
+                if (kTwo) lds_barrier();
+                // (behind the last tile: keys that no row sees, which change nothing)
+                const int key = i < nt ? key0 + i * BN : 0x40000000;
+                core.softmax(key, key + BK - 1 > wave_low || (p.window && key <= wave_hi - p.window), [] {});
+                advance();
+                if (!second && i < nt) settle(i, now);
+                lds_barrier();
+                now = behind;
+            }
+            if (kTwo && !second) lds_barrier();
+            wait_copies<0>();
         }
-        step += nt;
-        lds_barrier();
         if (uniform(special) == item++) {
             for (int i = 0; i < nt; ++i)
                 if (const int key = key0 + i * BN; is_edge(key))
                     for (int j = key; j < min(key + BK, hi); ++j)
-                        core.add_special(j, value_of<T>(p, table_row, walk.kvh, j));
+                        core.add_special(j, value_of(pages, j));
         }
-        const float l = C::across_sum(core.l[0]);
+        float l = C::across_sum(core.l[0]);
         const int first_wg = static_cast<int>(item_at / per), last_wg = static_cast<int>((item_at + walk.tiles - 1) / per);
-        if (first_wg == last_wg) {
-            if (real) {
-                Q* const dst = static_cast<Q*>(p.out) + (walk.row0 + t) * p.out_stride + head;
+        bool whole = first_wg == last_wg;
+        if (!whole) {
+            // States as the registers are, a lane's values NT apart.
+            auto part = [&](int wg) { return la.part + (static_cast<int64_t>(wg) * 2 + (wg == first_wg)) * kPart + tid; };
+            float* const mine = part(w);
 #pragma unroll
-                for (int i = 0; i < C::NC; ++i)
+            for (int i = 0; i < C::NC; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        store_out(dst + core.dim_of(i, 4 * e), f32x4{core.o[0][i][4 * e], core.o[0][i][4 * e + 1], core.o[0][i][4 * e + 2], core.o[0][i][4 * e + 3]}, l);
-            }
-        } else {
-            float* const part = la.part + (static_cast<int64_t>(w) * 2 + (w == first_wg)) * kPart;
-            if (real) {
+                for (int e = 0; e < C::ACC; ++e) st_dev(mine + (i * C::ACC + e) * NT, core.o[0][i][e]);
+            st_dev(mine + BM * HD, core.m[0] * core.c[0]);
+            st_dev(mine + BM * HD + NT, l);
+            whole = arrive(la.counters + first_wg, last_wg - first_wg + 1, &flag);
+            if (whole) {
+                float M = -kInf;
+                l = 0.0f;
+                core.no_values();
+                for (int x = first_wg; x <= last_wg; ++x) {
+                    const float* const src = part(x);
+                    const float m = ld_dev(src + BM * HD), sum = ld_dev(src + BM * HD + NT);
+                    const float top = fmaxf(M, m);
+                    const float fa = top == -kInf ? 0.0f : exp2_fast(M - top), fb = top == -kInf ? 0.0f : exp2_fast(m - top);
+                    l = l * fa + sum * fb;
 #pragma unroll
-                for (int i = 0; i < C::NC; ++i)
+                    for (int i = 0; i < C::NC; ++i)
 #pragma unroll
-                    for (int e = 0; e < C::ACC; ++e) st_dev(part + r * HD + core.dim_of(i, e), core.o[0][i][e]);
-                if (core.kg == 0) {
-                    st_dev(part + BM * HD + r, core.m[0] * core.c[0]);
-                    st_dev(part + BM * HD + BM + r, l);
+                        for (int e = 0; e < C::ACC; ++e)
+                            core.o[0][i][e] = core.o[0][i][e] * fa + ld_dev(src + (i * C::ACC + e) * NT) * fb;
+                    M = top;
                 }
             }
-            if (arrive(la.counters + first_wg, last_wg - first_wg + 1, &flag))
-                join_parts<Q, BM, HD, NT>(walk, first_wg, last_wg, rows, reinterpret_cast<State*>(lds));
+        }
+        if (whole && real) {
+            Q* const dst = static_cast<Q*>(p.out) + (walk.row0 + t) * p.out_stride + head;
+#pragma unroll
+            for (int i = 0; i < C::NC; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    store_out(dst + core.dim_of(i, 4 * e),
+                              f32x4{core.o[0][i][4 * e], core.o[0][i][4 * e + 1], core.o[0][i][4 * e + 2], core.o[0][i][4 * e + 3]}, l);
         }
         item_at += walk.tiles;
         if (left > 0 && !walk.next()) break;
@@ -1115,7 +1369,7 @@ hipError_t run(const PagedAttn& p, float* part, uint32_t* counters, hipStream_t 
         la.min_rows = narrow ? kNarrowRows : 0;
         la.max_rows = 0x7fffffff;
         la.min_tiles = 2;
-        hipLaunchKernelGGL((k_paged_wide<Q, T, HD, NW>), dim3(grid), dim3(NW * 64), 4 * BK * HD * sizeof(T), s, p, la);
+        hipLaunchKernelGGL((k_paged_wide<Q, T, HD, NW>), dim3(grid), dim3(NW * 64), 2 * wide_slots(BK * HD * sizeof(T)) * BK * HD * sizeof(T), s, p, la);
     }
     if (narrow) {
         la.min_rows = 0;
@@ -1144,7 +1398,7 @@ size_t paged_attention_workspace(const PagedAttn& p) {
     const int waves = p.dtype == RT_HIP_F32 ? wide_waves<float>(p.kv.head_dim) : wide_waves<__bf16>(p.kv.head_dim);
     const int hd = p.kv.head_dim;
     const size_t narrow = static_cast<size_t>(narrow_slots(hd)) * 2 * part_floats(rows <= 16 ? 16 : 32, hd);
-    const size_t wide = rows > kNarrowRows ? static_cast<size_t>(slots()) * 2 * part_floats(waves * 32, hd) : 0;
+    const size_t wide = rows > kNarrowRows ? static_cast<size_t>(slots()) * 2 * wide_part_floats(waves * 32, hd) : 0;
     return (narrow > wide ? narrow : wide) * sizeof(float);
 }
 

@@ -56,6 +56,7 @@ int cache_args(const char* fn, const rt_hip_paged_kv* kv, PagedKv* out) {
     const int64_t dense = (static_cast<int64_t>(kv->n_kv_heads) * kv->head_dim) << shift;
     const int64_t stride = kv->page_stride ? kv->page_stride : dense;
     if (stride < dense) return fail(fn, RT_HIP_E_ARG, "page_stride below a page's values");
+    if (stride > 0xffffffffLL / value_bytes(kv->dtype)) return fail(fn, RT_HIP_E_SHAPE, "page_stride must be below 2^32 bytes");
     if (!aligned(kv->k, 16) || !aligned(kv->v, 16) || stride * value_bytes(kv->dtype) % 16)
         return fail(fn, RT_HIP_E_ALIGN, "pages must be 16-byte aligned");
     out->k = kv->k;
