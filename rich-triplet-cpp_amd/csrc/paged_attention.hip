@@ -573,10 +573,12 @@ struct Launch {
     uint32_t group_mul;      // x / group = x * group_mul >> group_shift for x < 2^31
     int group_shift;
     int min_rows, max_rows;  // requests with rows (tokens x group) in (min_rows, max_rows]
-    int min_tiles;       // of a workgroup
+    int min_units;       // of a workgroup's range
 };
 
-template <int BM, int BN>
+// An item is EXTRA units, what its start and end cost, and then a unit for each
+// of its tiles.
+template <int BM, int BN, int EXTRA>
 struct Walk {
     const PagedAttn& p;
     const Launch& la;
@@ -618,11 +620,14 @@ struct Walk {
         *first = hi > lo ? lo / BN : 0;
         return hi > lo ? (hi + BN - 1) / BN - *first : 1;  // (none visible: one tile, to write zeros)
     }
-    // Tiles of the request for one KV head.
+    // Units of block b, and of the request for one KV head.
+    __device__ __forceinline__ int units(int b) const {
+        int first;
+        return count(b, &first) + EXTRA;
+    }
     __device__ __forceinline__ int64_t total() const {
         int64_t t = 0;
-        int first;
-        for (int b = 0; b < blocks; ++b) t += count(b, &first);
+        for (int b = 0; b < blocks; ++b) t += units(b);
         return t;
     }
     __device__ __forceinline__ void block(int b) {
@@ -666,19 +671,18 @@ __device__ __forceinline__ int64_t wave_scan(int64_t v) {
     }
     return v;
 }
-// Tiles of the walk's request for one KV head, its blocks counted by the wave's
+// Units of the walk's request for one KV head, its blocks counted by the wave's
 // lanes (the walk is the same in all of them).
 template <class W>
 __device__ __forceinline__ int64_t wave_total(const W& walk) {
     int64_t t = 0;
-    int first;
-    for (int b = threadIdx.x & 63; b < walk.blocks; b += 64) t += walk.count(b, &first);
+    for (int b = threadIdx.x & 63; b < walk.blocks; b += 64) t += walk.units(b);
     return uniform(__shfl(wave_scan(t), 63, kWave));
 }
 
-// Positions the walk at workgroup w's range of the sequence of all tiles (of
-// nw equal ones) and returns how many tiles it takes (0: none); *skip: how many
-// of the first item's lie before them; *per: tiles of a range.  Up to 64
+// Positions the walk at workgroup w's range of the sequence of all units (of
+// nw equal ones) and returns how many units it takes (0: none); *skip: how many
+// of the first item's lie before them; *per: units of a range.  Up to 64
 // requests every wave sums for itself, one to a lane; otherwise the workgroup's
 // threads do, several to a thread.  A request of many blocks is counted by its
 // wave's lanes together.
@@ -690,8 +694,8 @@ __device__ __forceinline__ int64_t find_range(W& walk, int w, int nw, int64_t* s
     __shared__ int64_t found_before;
     const bool small = n_seq <= 64;
     const int each = small ? 1 : (n_seq + NT - 1) / NT, base = small ? lane : tid * each;
-    // tiles of this lane's i-th request
-    auto tiles_of = [&](int i) -> int64_t {
+    // units of this lane's i-th request
+    auto units_of = [&](int i) -> int64_t {
         W scan(walk.p, walk.la);
         if (base + i < n_seq) scan.request(base + i);
         int64_t t = scan.blocks <= 2 ? scan.total() : 0;
@@ -707,7 +711,7 @@ __device__ __forceinline__ int64_t find_range(W& walk, int w, int nw, int64_t* s
         return t * n_kv;
     };
     int64_t mine = 0;
-    for (int i = 0; i < each; ++i) mine += tiles_of(i);
+    for (int i = 0; i < each; ++i) mine += units_of(i);
     int64_t incl = wave_scan(mine);
     int64_t all = __shfl(incl, 63, kWave);
     if (!small) {
@@ -723,19 +727,19 @@ __device__ __forceinline__ int64_t find_range(W& walk, int w, int nw, int64_t* s
         incl += before;
     }
     all = uniform(all);
-    *per = max(quotient(all + nw - 1, nw), static_cast<int64_t>(walk.la.min_tiles));
+    *per = max(quotient(all + nw - 1, nw), static_cast<int64_t>(walk.la.min_units));
     const int64_t u = w * *per;
     if (u >= all) return 0;
     const bool here = u < incl && u >= incl - mine;
     int s;
-    int64_t at = incl - mine;  // tiles before the request
+    int64_t at = incl - mine;  // units before the request
     if (small) {
         s = __builtin_ctzll(__builtin_amdgcn_ballot_w64(here));
         at = __shfl(at, s, kWave);
     } else {
-        if (__builtin_amdgcn_ballot_w64(here) != 0) {  // (whole waves, as tiles_of counts)
+        if (__builtin_amdgcn_ballot_w64(here) != 0) {  // (whole waves, as units_of counts)
             for (int i = 0; i < each; ++i) {
-                const int64_t t = tiles_of(i);
+                const int64_t t = units_of(i);
                 if (here && u >= at && u < at + t) {
                     found_s = base + i;
                     found_before = at;
@@ -753,8 +757,7 @@ __device__ __forceinline__ int64_t find_range(W& walk, int w, int nw, int64_t* s
     walk.kvh = static_cast<int>(quotient(off, t));
     off -= walk.kvh * t;
     for (int b0 = 0;; b0 += 64) {
-        int first;
-        const int c = b0 + lane < walk.blocks ? walk.count(b0 + lane, &first) : 0;
+        const int c = b0 + lane < walk.blocks ? walk.units(b0 + lane) : 0;
         const int64_t sum = wave_scan(c);
         const uint64_t behind = __builtin_amdgcn_ballot_w64(off < sum);
         if (behind || b0 + 64 >= walk.blocks) {
@@ -972,7 +975,7 @@ __global__ __launch_bounds__(256, RBLK == 1 || HD < 256 ? 2 : 1) void k_paged_na
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     uint8_t* const ring = lds + wave * kRing;
     const int nw = gridDim.x, w = place_of(blockIdx.x, nw);
-    Walk<BM, BN> walk(p, la);
+    Walk<BM, BN, 0> walk(p, la);
     int64_t skip = 0, per = 0;
     int64_t left = find_range<256>(walk, w, nw, &skip, &per);
     int64_t item_at = w * per - skip;  // of the item's first tile in the sequence
@@ -1142,10 +1145,12 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
     __shared__ int flag;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int nw = gridDim.x, w = place_of(blockIdx.x, nw);
-    Walk<BM, BN> walk(p, la);
+    // tiles that take as long as an item's start and end (5 us)
+    constexpr int EXTRA = KindOf<T>::f32 ? 1 : (sizeof(Q) == 4 || HD == 256 ? 3 : 6);
+    Walk<BM, BN, EXTRA> walk(p, la);
     int64_t skip = 0, per = 0;
     int64_t left = find_range<NT>(walk, w, nw, &skip, &per);
-    int64_t item_at = w * per - skip;
+    int64_t item_at = w * per - skip + EXTRA;  // of the item's first tile in the sequence
     const uint32_t lds_at = uniform(static_cast<int>(lds_address(lds)));
     const float c1 = p.scale * kLog2e;
     if (tid == 0) special = -1;
@@ -1154,10 +1159,12 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
     core.setup();
     while ((left = uniform(left)) > 0) {
         walk.pin();
-        const int a = uniform(static_cast<int>(skip));
-        const int b = uniform(static_cast<int>(min(static_cast<int64_t>(walk.tiles), skip + left)));
+        const int from = uniform(static_cast<int>(skip));
+        const int to = uniform(static_cast<int>(min(static_cast<int64_t>(walk.tiles + EXTRA), skip + left)));
         skip = 0;
-        left -= b - a;
+        left -= to - from;
+        const int a = max(from - EXTRA, 0), b = max(to - EXTRA, 0);  // tiles
+        if (a >= b) break;  // (the range ends before the item's first tile)
         int lo, hi;
         walk.span(walk.blk, &lo, &hi);
         const int rows = min(BM, walk.rows() - walk.blk * BM), row_first = walk.blk * BM;
@@ -1303,8 +1310,14 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
                 l = 0.0f;
                 core.no_values();
                 for (int x = first_wg; x <= last_wg; ++x) {
+                    // (all loads before the first use: they are served one latency after
+                    // the other otherwise)
                     const float* const src = part(x);
                     const float m = ld_dev(src + BM * HD), sum = ld_dev(src + BM * HD + NT);
+                    float o[C::NC * C::ACC];
+#pragma unroll
+                    for (int i = 0; i < C::NC * C::ACC; ++i) o[i] = ld_dev(src + i * NT);
+                    __builtin_amdgcn_sched_barrier(0);
                     const float top = fmaxf(M, m);
                     const float fa = top == -kInf ? 0.0f : exp2_fast(M - top), fb = top == -kInf ? 0.0f : exp2_fast(m - top);
                     l = l * fa + sum * fb;
@@ -1312,7 +1325,7 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
                     for (int i = 0; i < C::NC; ++i)
 #pragma unroll
                         for (int e = 0; e < C::ACC; ++e)
-                            core.o[0][i][e] = core.o[0][i][e] * fa + ld_dev(src + (i * C::ACC + e) * NT) * fb;
+                            core.o[0][i][e] = core.o[0][i][e] * fa + o[i * C::ACC + e] * fb;
                     M = top;
                 }
             }
@@ -1326,7 +1339,7 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
                     store_out(dst + core.dim_of(i, 4 * e),
                               f32x4{core.o[0][i][4 * e], core.o[0][i][4 * e + 1], core.o[0][i][4 * e + 2], core.o[0][i][4 * e + 3]}, l);
         }
-        item_at += walk.tiles;
+        item_at += walk.tiles + EXTRA;
         if (left > 0 && !walk.next()) break;
     }
 }
@@ -1368,13 +1381,13 @@ hipError_t run(const PagedAttn& p, float* part, uint32_t* counters, hipStream_t 
         constexpr int BK = KindOf<T>::f32 ? 32 : 64;
         la.min_rows = narrow ? kNarrowRows : 0;
         la.max_rows = 0x7fffffff;
-        la.min_tiles = 2;
+        la.min_units = 8;
         hipLaunchKernelGGL((k_paged_wide<Q, T, HD, NW>), dim3(grid), dim3(NW * 64), 2 * wide_slots(BK * HD * sizeof(T)) * BK * HD * sizeof(T), s, p, la);
     }
     if (narrow) {
         la.min_rows = 0;
         la.max_rows = wide ? kNarrowRows : 0x7fffffff;
-        la.min_tiles = 1;
+        la.min_units = 1;
         const unsigned many = static_cast<unsigned>(narrow_slots(HD));
         if (rows <= 16) hipLaunchKernelGGL((k_paged_narrow<Q, T, HD, 1>), dim3(many), dim3(256), 4 * narrow_ring(HD), s, p, la);
         else hipLaunchKernelGGL((k_paged_narrow<Q, T, HD, 2>), dim3(many), dim3(256), 4 * narrow_ring(HD), s, p, la);
