@@ -673,50 +673,58 @@ def probe_empty(workgroups: int = 1, threads: int = 64, stream=None) -> None:
 
 # ------------------------------------------- serving over a paged KV cache --
 
+_VALUE_TYPES: dict = {}
+
+
 def _value_type(t) -> int:
-    torch = _torch()
-    types = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
-    if t.dtype not in types:
+    if not _VALUE_TYPES:
+        torch = _torch()
+        _VALUE_TYPES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    if t.dtype not in _VALUE_TYPES:
         raise ValueError(f"rt_hip: {t.dtype} is not float32, float16 or bfloat16")
-    return types[t.dtype]
+    return _VALUE_TYPES[t.dtype]
 
 
-def _want(t, name: str, dtype, shape) -> None:
-    """t is contiguous, on the GPU and of the given dtype and shape (None: any size)."""
-    if t.dtype != dtype:
-        raise ValueError(f"rt_hip: {name} must be {dtype}, not {t.dtype}")
-    if t.dim() != len(shape) or any(n is not None and a != n for a, n in zip(t.shape, shape)):
-        raise ValueError(f"rt_hip: {name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
-    _dev_check(t)
+def _want(device: int, *args) -> None:
+    """Each (tensor, name, dtype, shape) is contiguous, on GPU `device` and of that
+    dtype and shape (a None in it: any size)."""
+    for t, name, dtype, shape in args:
+        if t.dtype is not dtype:
+            raise ValueError(f"rt_hip: {name} must be {dtype}, not {t.dtype}")
+        have = t.shape
+        if have != shape and (len(have) != len(shape) or any(n is not None and a != n for a, n in zip(have, shape))):
+            raise ValueError(f"rt_hip: {name} must have shape {tuple(shape)}, not {tuple(have)}")
+        if t.get_device() != device:
+            raise ValueError(f"rt_hip: {name} must live on the GPU of the others" if t.is_cuda else
+                             "rt_hip: tensors must live on the GPU")
+        if not t.is_contiguous():
+            raise ValueError("rt_hip: tensors must be contiguous")
 
 
-def _rows(t, name: str, heads: int, dim: int) -> int:
+def _rows(device: int, t, name: str, heads: int, dim: int) -> int:
     """Stride in values between the rows of t [n, heads, dim], whose rows are dense."""
-    if not t.is_cuda:
-        raise ValueError("rt_hip: tensors must live on the GPU")
-    if t.dim() != 3 or tuple(t.shape[1:]) != (heads, dim):
-        raise ValueError(f"rt_hip: {name} must have shape (rows, {heads}, {dim}), not {tuple(t.shape)}")
-    if t.stride(2) != 1 or (heads > 1 and t.stride(1) != dim):
+    have = t.shape
+    if len(have) != 3 or have[1] != heads or have[2] != dim:
+        raise ValueError(f"rt_hip: {name} must have shape (rows, {heads}, {dim}), not {tuple(have)}")
+    if t.get_device() != device:
+        raise ValueError(f"rt_hip: {name} must live on the GPU of the others" if t.is_cuda else
+                         "rt_hip: tensors must live on the GPU")
+    stride = t.stride()
+    if stride[2] != 1 or (heads > 1 and stride[1] != dim):
         raise ValueError(f"rt_hip: the rows of {name} must be dense")
-    return t.stride(0) if t.shape[0] > 1 else heads * dim
+    return stride[0] if have[0] > 1 else heads * dim
 
 
-class _on:
-    """The device of t is current inside, and every tensor given lives on it."""
-
-    def __init__(self, t, *others):
-        for o in others:
-            if o is not None and o.device != t.device:
-                raise ValueError("rt_hip: tensors must live on one device")
-        self._guard = None if t.device.index == _torch().cuda.current_device() else _torch().cuda.device(t.device)
-
-    def __enter__(self):
-        if self._guard is not None:
-            self._guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self._guard is not None:
-            self._guard.__exit__(*exc)
+def _call_on(device: int, name: str, stream, *args) -> None:
+    """A library call with GPU `device` current and on its current stream, or
+    the one given."""
+    torch = _torch()
+    if device != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            library().call(name, *args, _stream(stream))
+        return
+    library().call(name, *args, stream.cuda_stream if stream is not None else
+                   torch._C._cuda_getCurrentRawStream(device))
 
 
 class PagedKV:
@@ -737,15 +745,9 @@ class PagedKV:
         stride = k.stride(0) if n_pages > 1 else page * heads * dim
         if n_pages > 1 and v.stride(0) != stride:
             raise ValueError("rt_hip: k and v must have one page stride")
-        self.k, self.v = k, v
+        self.k, self.v, self.device = k, v, k.get_device()
         self.struct = PagedKvStruct(k.data_ptr(), v.data_ptr(), _value_type(k), n_pages, page, heads, dim, stride)
-
-    @property
-    def device(self):
-        return self.k.device
-
-    def _ref(self):
-        return C.byref(self.struct)
+        self.ref = C.byref(self.struct)
 
 
 class PagedPlan:
@@ -755,10 +757,13 @@ class PagedPlan:
 
     def __init__(self, n_seq: int, tokens: int, device, held=None, queue_state=None):
         torch = _torch()
-        buf = torch.empty(2 * n_seq + 1 + 2 * tokens, dtype=torch.int32, device=device)
-        self.q_start, self.kv_len, self.slots, self.positions = buf.split([n_seq + 1, n_seq, tokens, tokens])
-        self.held = torch.empty(n_seq, dtype=torch.int32, device=device) if held is None else held
-        self.queue_state = torch.empty(2, dtype=torch.int32, device=device) if queue_state is None else queue_state
+        buf = torch.empty(3 * n_seq + 3 + 2 * tokens, dtype=torch.int32, device=device)
+        (self.q_start, self.kv_len, self.slots, self.positions, self.held,
+         self.queue_state) = buf.split_with_sizes((n_seq + 1, n_seq, tokens, tokens, n_seq, 2))
+        if held is not None:
+            self.held = held
+        if queue_state is not None:
+            self.queue_state = queue_state
 
 
 def paged_plan(cached, fresh, held, table, queue, queue_state, page_size: int, tokens: int, plan=None, stream=None):
@@ -766,40 +771,36 @@ def paged_plan(cached, fresh, held, table, queue, queue_state, page_size: int, t
     updated in place.  tokens: rows of the step (at least the sum of fresh).
     plan: a PagedPlan of these sizes to write into; with its held and
     queue_state the ones passed, the state is updated in place."""
-    torch = _torch()
-    n = cached.shape[0]
-    i32 = torch.int32
-    for t, name in ((cached, "cached"), (fresh, "fresh"), (held, "held")):
-        _want(t, name, i32, (n,))
-    _want(table, "table", i32, (n, None))
-    _want(queue, "queue", i32, (None,))
-    _want(queue_state, "queue_state", i32, (2,))
+    i32 = _torch().int32
+    n, device = cached.shape[0], cached.get_device()
+    per_request = (n,)
+    _want(device, (cached, "cached", i32, per_request), (fresh, "fresh", i32, per_request),
+          (held, "held", i32, per_request), (table, "table", i32, (n, None)), (queue, "queue", i32, (None,)),
+          (queue_state, "queue_state", i32, (2,)))
     if plan is None:
         plan = PagedPlan(n, tokens, cached.device)
     else:
-        for t, name, size in ((plan.q_start, "q_start", n + 1), (plan.kv_len, "kv_len", n), (plan.slots, "slots", tokens),
-                              (plan.positions, "positions", tokens), (plan.held, "plan.held", n),
-                              (plan.queue_state, "plan.queue_state", 2)):
-            _want(t, name, i32, (size,))
-    with _on(cached, fresh, held, table, queue, queue_state, plan.q_start, plan.held, plan.queue_state):
-        library().call("rt_hip_paged_plan", _ptr(cached), _ptr(fresh), _ptr(held), _ptr(plan.held), _ptr(table),
-                       table.shape[1], _ptr(queue), _ptr(queue_state), _ptr(plan.queue_state), queue.shape[0], page_size,
-                       n, tokens, _ptr(plan.q_start), _ptr(plan.kv_len), _ptr(plan.slots), _ptr(plan.positions),
-                       _stream(stream))
+        _want(device, (plan.q_start, "q_start", i32, (n + 1,)), (plan.kv_len, "kv_len", i32, per_request),
+              (plan.slots, "slots", i32, (tokens,)), (plan.positions, "positions", i32, (tokens,)),
+              (plan.held, "plan.held", i32, per_request), (plan.queue_state, "plan.queue_state", i32, (2,)))
+    _call_on(device, "rt_hip_paged_plan", stream, cached.data_ptr(), fresh.data_ptr(), held.data_ptr(),
+             plan.held.data_ptr(), table.data_ptr(), table.shape[1], queue.data_ptr(), queue_state.data_ptr(),
+             plan.queue_state.data_ptr(), queue.shape[0], page_size, n, tokens, plan.q_start.data_ptr(),
+             plan.kv_len.data_ptr(), plan.slots.data_ptr(), plan.positions.data_ptr())
     return plan
 
 
 def paged_append(kv: PagedKV, k, v, slots, stream=None) -> None:
     """Rows of k and v [tokens, n_kv_heads, head_dim] (slices of a joint
     projection, say) into the cache at slots, rounded to its type."""
-    c = kv.struct
-    stride = _rows(k, "k", c.n_kv_heads, c.head_dim)
-    if k.shape != v.shape or k.dtype != v.dtype or _rows(v, "v", c.n_kv_heads, c.head_dim) != stride:
+    c, device = kv.struct, kv.device
+    stride = _rows(device, k, "k", c.n_kv_heads, c.head_dim)
+    if k.shape != v.shape or k.dtype is not v.dtype or _rows(device, v, "v", c.n_kv_heads, c.head_dim) != stride:
         raise ValueError("rt_hip: k and v must have one shape, dtype and stride")
-    _want(slots, "slots", _torch().int32, (k.shape[0],))
-    with _on(kv, k, v, slots):
-        library().call("rt_hip_paged_append", kv._ref(), _ptr(k), _ptr(v), _value_type(k), stride, _ptr(slots),
-                       k.shape[0], _stream(stream))
+    n = k.shape[0]
+    _want(device, (slots, "slots", _torch().int32, (n,)))
+    _call_on(device, "rt_hip_paged_append", stream, kv.ref, k.data_ptr(), v.data_ptr(), _value_type(k), stride,
+             slots.data_ptr(), n)
 
 
 def paged_attention(q, kv: PagedKV, table, q_start, kv_len, scale: float, window: int = 0, max_fresh: int = 0, out=None,
@@ -809,29 +810,27 @@ def paged_attention(q, kv: PagedKV, table, q_start, kv_len, scale: float, window
     new tokens of one request, where known.  Rows of out outside every request
     are left as they were (a new out starts with zeros)."""
     torch = _torch()
-    c = kv.struct
+    c, device = kv.struct, kv.device
     if q.dim() != 3:
         raise ValueError("rt_hip: q must have shape (rows, n_q_heads, head_dim)")
     if out is None:
         out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
-    if out.shape != q.shape or out.dtype != q.dtype:
+    if out.shape != q.shape or out.dtype is not q.dtype:
         raise ValueError("rt_hip: out must have q's shape and dtype")
-    heads, n = q.shape[1], kv_len.shape[0]
-    q_stride, out_stride = _rows(q, "q", heads, c.head_dim), _rows(out, "out", heads, c.head_dim)
-    _want(table, "table", torch.int32, (n, None))
-    _want(q_start, "q_start", torch.int32, (n + 1,))
-    _want(kv_len, "kv_len", torch.int32, (n,))
-    with _on(kv, q, table, q_start, kv_len, out):
-        library().call("rt_hip_paged_attention", _ptr(q), _value_type(q), q_stride, heads, kv._ref(), _ptr(table),
-                       table.shape[1], _ptr(q_start), _ptr(kv_len), n, q.shape[0], max_fresh, C.c_float(scale), window,
-                       _ptr(out), out_stride, _stream(stream))
+    rows, heads, _ = q.shape
+    n, i32 = kv_len.shape[0], torch.int32
+    q_stride = _rows(device, q, "q", heads, c.head_dim)
+    out_stride = _rows(device, out, "out", heads, c.head_dim)
+    _want(device, (table, "table", i32, (n, None)), (q_start, "q_start", i32, (n + 1,)), (kv_len, "kv_len", i32, (n,)))
+    _call_on(device, "rt_hip_paged_attention", stream, q.data_ptr(), _value_type(q), q_stride, heads, kv.ref,
+             table.data_ptr(), table.shape[1], q_start.data_ptr(), kv_len.data_ptr(), n, rows, max_fresh, scale, window,
+             out.data_ptr(), out_stride)
     return out
 
 
 def paged_attention_workspace_bytes(kv: PagedKV, dtype: int, n_q_heads: int, n_seq: int, tokens: int,
                                     max_fresh: int = 0) -> int:
-    return int(library().lib.rt_hip_paged_attention_workspace_bytes(kv._ref(), dtype, n_q_heads, n_seq, tokens,
-                                                                    max_fresh))
+    return int(library().lib.rt_hip_paged_attention_workspace_bytes(kv.ref, dtype, n_q_heads, n_seq, tokens, max_fresh))
 
 
 def verify_drafts(logits, tokens, row_start, accept_u, sample_u, max_draft: int, draft_logits=None, temperature=None,
@@ -841,30 +840,30 @@ def verify_drafts(logits, tokens, row_start, accept_u, sample_u, max_draft: int,
     or bfloat16, rows dense with any stride; out: a pair to write into."""
     torch = _torch()
     rows, vocab = logits.shape
-    n = sample_u.shape[0]
+    n, device = sample_u.shape[0], logits.get_device()
+    i32, f32 = torch.int32, torch.float32
+    strides = []
     for t, name in ((logits, "logits"), (draft_logits, "draft_logits")):
         if t is None:
+            strides.append(0)
             continue
-        if not t.is_cuda:
-            raise ValueError("rt_hip: tensors must live on the GPU")
-        if tuple(t.shape) != (rows, vocab) or t.dtype != logits.dtype or (vocab > 1 and t.stride(1) != 1):
+        if device < 0 or t.get_device() != device:
+            raise ValueError("rt_hip: tensors must live on the GPU, on one")
+        if tuple(t.shape) != (rows, vocab) or t.dtype is not logits.dtype or (vocab > 1 and t.stride(1) != 1):
             raise ValueError(f"rt_hip: {name} must be dense rows ({rows}, {vocab}) of one dtype")
-    _want(tokens, "tokens", torch.int32, (rows,))
-    _want(row_start, "row_start", torch.int32, (n + 1,))
-    _want(accept_u, "accept_u", torch.float32, (rows,))
-    _want(sample_u, "sample_u", torch.float32, (n,))
+        strides.append(t.stride(0) if rows > 1 else vocab)
+    _want(device, (tokens, "tokens", i32, (rows,)), (row_start, "row_start", i32, (n + 1,)),
+          (accept_u, "accept_u", f32, (rows,)), (sample_u, "sample_u", f32, (n,)))
     if temperature is not None:
-        _want(temperature, "temperature", torch.float32, (n,))
+        _want(device, (temperature, "temperature", f32, (n,)))
     if out is None:
-        out = (torch.empty((n, max_draft + 1), dtype=torch.int32, device=logits.device),
-               torch.empty(n, dtype=torch.int32, device=logits.device))
-    _want(out[0], "out tokens", torch.int32, (n, max_draft + 1))
-    _want(out[1], "out count", torch.int32, (n,))
-    row = [0 if t is None else (t.stride(0) if rows > 1 else vocab) for t in (logits, draft_logits)]
-    with _on(logits, draft_logits, tokens, row_start, accept_u, sample_u, temperature, *out):
-        library().call("rt_hip_verify_drafts", _ptr(logits), row[0], _ptr(draft_logits), row[1], _value_type(logits),
-                       vocab, _ptr(tokens), _ptr(row_start), _ptr(accept_u), _ptr(sample_u), _ptr(temperature), n, rows,
-                       max_draft, _ptr(out[0]), _ptr(out[1]), _stream(stream))
+        out = (torch.empty((n, max_draft + 1), dtype=i32, device=logits.device),
+               torch.empty(n, dtype=i32, device=logits.device))
+    else:
+        _want(device, (out[0], "out tokens", i32, (n, max_draft + 1)), (out[1], "out count", i32, (n,)))
+    _call_on(device, "rt_hip_verify_drafts", stream, logits.data_ptr(), strides[0], _ptr(draft_logits), strides[1],
+             _value_type(logits), vocab, tokens.data_ptr(), row_start.data_ptr(), accept_u.data_ptr(),
+             sample_u.data_ptr(), _ptr(temperature), n, rows, max_draft, out[0].data_ptr(), out[1].data_ptr())
     return out
 
 
