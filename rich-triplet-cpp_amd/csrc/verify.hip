@@ -15,16 +15,16 @@
 // so weights and sums are in 64 bits: a token of probability 1e-5 then changes
 // hands with odds below 1e-10, with 32-bit sums 1e-3.
 //
-// Two launches: k_verify_stats reads every row once, in chunks, and leaves
+// Two launches.  k_verify_stats reads every row once, in chunks, and leaves
 // each chunk's maximum and sum of exp((x - maximum) / T); k_verify_pick joins
 // them (every workgroup of a request for itself), decides on the drafts, sums
 // w of the deciding row by chunks and, in the request's last workgroup to
-// arrive, finds the chunk that holds the border and the token in it.  Rows of
-// a request whose T is 0 need no sums.
+// arrive, finds the chunk that holds the border and the token in it (behind the
+// last draft the chunks' sums are there already).  Rows of a request whose T is
+// 0 need no sums.
 //
-// Bound: the bytes of the logits.  A 64-bit exponential is about 20
-// instructions at the rate of 32-bit ones, 21 us of the card for 320 rows of
-// 128256 values, which take 30 us to read.
+// Bound: the bytes of the logits, and as much the exponentials, 18 64-bit
+// instructions each at the rate of 32-bit ones.
 #include "rt_common.hpp"
 #include "rt_launch.hpp"
 
@@ -39,39 +39,41 @@ constexpr float kInf = __builtin_inff();
 struct Stat {
     double sum;   // of exp((x - top) / T) over the chunk
     float top;    // its maximum, NaN aside (-inf: nothing above)
-    int32_t idx;  // where that first stands
+    int32_t idx;  // where that first stands (T = 0)
 };
 
-// exp(x) for x <= 0 (zero below -745): 2^n times the Taylor polynomial of
-// degree 12 in |r| <= ln(2) / 2, whose remainder is below 2e-16.
-__device__ __forceinline__ double exp64(double x) {
-    x = fmax(x, -800.0);
-    const double n = __builtin_rint(x * 1.4426950408889634074);
-    double r = __builtin_fma(n, -6.93147180369123816490e-01, x);
-    r = __builtin_fma(n, -1.90821492927058770002e-10, r);
-    double y = 1.0 / 479001600.0;
-    y = __builtin_fma(y, r, 1.0 / 39916800.0);
-    y = __builtin_fma(y, r, 1.0 / 3628800.0);
-    y = __builtin_fma(y, r, 1.0 / 362880.0);
-    y = __builtin_fma(y, r, 1.0 / 40320.0);
-    y = __builtin_fma(y, r, 1.0 / 5040.0);
-    y = __builtin_fma(y, r, 1.0 / 720.0);
-    y = __builtin_fma(y, r, 1.0 / 120.0);
-    y = __builtin_fma(y, r, 1.0 / 24.0);
-    y = __builtin_fma(y, r, 1.0 / 6.0);
-    y = __builtin_fma(y, r, 0.5);
+// 2^x for x <= 0, exactly 1 for 0, and 0 for -inf and NaN.  Adding 1.5 2^52
+// leaves the whole part of x in the low bits; 2^r of the rest, |r| <= 1/2, is
+// 1 + r P(r), where P takes the values of (2^r - 1) / r at the nine Chebyshev
+// nodes (relative error below 4e-14).
+__device__ __forceinline__ double exp2_64(double x) {
+    constexpr double kMagic = 6755399441055744.0;
+    x = __builtin_fmax(x, -2000.0);
+    const double t = x + kMagic;
+    const double r = x - (t - kMagic);
+    double y = 1.0203121063391729e-07;
+    y = __builtin_fma(y, r, 1.3255224878668817e-06);
+    y = __builtin_fma(y, r, 1.525268684626772e-05);
+    y = __builtin_fma(y, r, 0.00015403455852453838);
+    y = __builtin_fma(y, r, 0.0013333558179043112);
+    y = __builtin_fma(y, r, 0.009618129159402558);
+    y = __builtin_fma(y, r, 0.055504108664760424);
+    y = __builtin_fma(y, r, 0.2402265069581299);
+    y = __builtin_fma(y, r, 0.6931471805599453);
     y = __builtin_fma(y, r, 1.0);
-    y = __builtin_fma(y, r, 1.0);
-    return __builtin_ldexp(y, static_cast<int>(n));
+    return __builtin_ldexp(y, static_cast<int>(__builtin_bit_cast(uint64_t, t)));
 }
 
-// Weight of x in a row whose maximum is top > -inf (the rule for infinities:
-// what equals the maximum weighs 1).
-__device__ __forceinline__ double weight(float x, float top, double inv_t) {
-    if (x == top) return 1.0;
-    if (!(x > -kInf)) return 0.0;
-    return exp64((static_cast<double>(x) - static_cast<double>(top)) * inv_t);
-}
+// Weights of a row's values against its maximum, top > -inf: exp((x - top) / T),
+// 1 for what equals the maximum (infinities share the weight), 0 for -inf and NaN.
+struct Weigh {
+    double scale;  // log2(e) / T
+    float top;
+    __device__ __forceinline__ double finite(float x) const {  // top < inf
+        return exp2_64((static_cast<double>(x) - static_cast<double>(top)) * scale);
+    }
+    __device__ __forceinline__ double operator()(float x) const { return x == top ? 1.0 : finite(x); }
+};
 
 typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint16_t u16x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
@@ -114,19 +116,51 @@ __device__ __forceinline__ int rows_of(const VerifyDrafts& p, int s, int* first)
     return min(b - a, p.max_draft + 1);  // rows; drafts are one fewer
 }
 
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, kWave);
-    return v;
+// Lane i's value in a lane ahead of it, `old` in lanes without one: rows of 16
+// shifted by 1, 2, 4, 8, then the last lane of a row or half to the rows behind
+// it.  Running an operation over these six leaves lane i with lanes 0 .. i.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int from_before(int old, int v) {
+    return __builtin_amdgcn_update_dpp(old, v, CTRL, ROWS, 0xf, false);
 }
-__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) {
-        const uint64_t o = __shfl_xor(v, off, kWave);
-        v = o > v ? o : v;
-    }
-    return v;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float from_before(float old, float v) {
+    return __int_as_float(from_before<CTRL, ROWS>(__float_as_int(old), __float_as_int(v)));
 }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double from_before(double old, double v) {
+    const uint64_t o = __builtin_bit_cast(uint64_t, old), b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = from_before<CTRL, ROWS>(static_cast<int>(o), static_cast<int>(b));
+    const uint32_t hi = from_before<CTRL, ROWS>(static_cast<int>(o >> 32), static_cast<int>(b >> 32));
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+template <class V, class F>
+__device__ __forceinline__ V running(V v, V none, F op) {
+    v = op(v, from_before<0x111, 0xf>(none, v));
+    v = op(v, from_before<0x112, 0xf>(none, v));
+    v = op(v, from_before<0x114, 0xf>(none, v));
+    v = op(v, from_before<0x118, 0xf>(none, v));
+    v = op(v, from_before<0x142, 0xa>(none, v));
+    return op(v, from_before<0x143, 0xc>(none, v));
+}
+__device__ __forceinline__ int of_lane(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ float of_lane(float v, int lane) { return __int_as_float(of_lane(__float_as_int(v), lane)); }
+__device__ __forceinline__ double of_lane(double v, int lane) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = of_lane(static_cast<int>(b), lane), hi = of_lane(static_cast<int>(b >> 32), lane);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ double running_sum(double v) {
+    return running(v, 0.0, [](double a, double b) { return a + b; });
+}
+__device__ __forceinline__ double wave_sum(double v) { return of_lane(running_sum(v), 63); }
+__device__ __forceinline__ float wave_max(float v) {
+    return of_lane(running(v, -kInf, [](float a, float b) { return fmaxf(a, b); }), 63);
+}
+__device__ __forceinline__ int wave_min(int v) {
+    return of_lane(running(v, 0x7fffffff, [](int a, int b) { return min(a, b); }), 63);
+}
+
 // Sum over the workgroup, the same bits in every thread.
 __device__ __forceinline__ double block_sum(double v, double* tmp) {
     v = wave_sum(v);
@@ -138,14 +172,8 @@ __device__ __forceinline__ double block_sum(double v, double* tmp) {
 // Sum over the threads before this one; *total: over all of them.
 __device__ __forceinline__ double block_before(double v, double* tmp, double* total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    double sum = v;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const double o = __shfl_up(sum, off, kWave);
-        if (lane >= off) sum += o;
-    }
-    double before = __shfl_up(sum, 1, kWave);
-    if (lane == 0) before = 0.0;
+    const double sum = running_sum(v);
+    const double before = from_before<0x138, 0xf>(0.0, sum);  // (one lane on)
     __syncthreads();
     if (lane == 63) tmp[wave] = sum;
     __syncthreads();
@@ -163,31 +191,86 @@ __device__ __forceinline__ double block_before(double v, double* tmp, double* to
 // the last weight above 0, else -1.  place(e): where weight e stands, below 2^31.
 template <int N, class F>
 __device__ __forceinline__ int find_border(const double (&w)[N], double before, double target, F place, int* tmp2) {
-    if (threadIdx.x == 0) {
-        tmp2[0] = 0x7fffffff;
-        tmp2[1] = -1;
-    }
-    __syncthreads();
-    int hit = 0x7fffffff, heavy = -1;
+    const int wave = threadIdx.x >> 6;
+    int hit = -1, heavy = -1;
 #pragma unroll
     for (int e = 0; e < N; ++e) {
         before += w[e];
         if (w[e] > 0.0) {
             heavy = place(e);
-            if (before > target && hit == 0x7fffffff) hit = heavy;
+            if (before > target && hit < 0) hit = heavy;
         }
     }
-    if (hit != 0x7fffffff) atomicMin(tmp2, hit);
-    if (heavy >= 0) atomicMax(tmp2 + 1, heavy);
+    const uint64_t hits = __ballot(hit >= 0), heavies = __ballot(heavy >= 0);
+    hit = hits ? of_lane(hit, __builtin_ctzll(hits)) : -1;  // (by all lanes, which hold them)
+    heavy = heavies ? of_lane(heavy, 63 - __builtin_clzll(heavies)) : -1;
     __syncthreads();
-    return tmp2[0] != 0x7fffffff ? tmp2[0] : tmp2[1];
+    if ((threadIdx.x & 63) == 0) {
+        tmp2[wave] = hit;
+        tmp2[kT / 64 + wave] = heavy;
+    }
+    __syncthreads();
+    int first = -1, last = -1;
+#pragma unroll
+    for (int i = 0; i < kT / 64; ++i) {
+        if (first < 0) first = tmp2[i];
+        last = max(last, tmp2[kT / 64 + i]);
+    }
+    return first >= 0 ? first : last;
+}
+
+__device__ __forceinline__ void st_dev(double* p, double v) {
+    __hip_atomic_store((__attribute__((address_space(1))) double*)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ double ld_dev(const double* p) {
+    return __hip_atomic_load((const __attribute__((address_space(1))) double*)p, __ATOMIC_RELAXED,
+                             __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// A row's maximum (-inf: nothing above), its first place, and the inverse of its
+// sum, from its chunks (up to 256, four to a lane); one wave, all lanes end with
+// them.
+struct RowStat {
+    double inv_sum;
+    float top;
+    int idx;
+};
+__device__ __forceinline__ RowStat join_row(const Stat* st, int chunks, double scale) {
+    const int lane = threadIdx.x & 63;
+    Stat x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[i] = st[min(lane + 64 * i, chunks - 1)];
+        if (lane + 64 * i >= chunks) x[i] = Stat{0.0, -kInf, 0};
+    }
+    RowStat r;
+    r.top = wave_max(fmaxf(fmaxf(x[0].top, x[1].top), fmaxf(x[2].top, x[3].top)));
+    int idx = 0x7fffffff;
+    double sum = 0.0;
+    const Weigh weigh{scale, r.top};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        idx = x[i].top == r.top ? min(idx, x[i].idx) : idx;
+        sum += x[i].sum * weigh(x[i].top);
+    }
+    idx = wave_min(idx);
+    r.idx = r.top > -kInf ? idx : 0;
+    r.inv_sum = 1.0 / wave_sum(sum);
+    return r;
+}
+
+// Probability from a row's joined statistics (nothing above -inf: certain of token 0).
+__device__ __forceinline__ double prob(float x, int at, const RowStat& r, double scale) {
+    if (r.top == -kInf) return at == 0 ? 1.0 : 0.0;
+    return Weigh{scale, r.top}(x) * r.inv_sum;
 }
 
 // Statistics [which][row][chunk]; grid (chunks, n_seq * (max_draft + 1), 1 or 2).
 template <class X>
 __global__ __launch_bounds__(kT) void k_verify_stats(VerifyDrafts p, Stat* __restrict__ stats) {
     __shared__ double tmp[4];
-    __shared__ uint64_t tmp_key[4];
+    __shared__ float tmp_top[4];
+    __shared__ int tmp_idx[4];
     const int s = blockIdx.y / (p.max_draft + 1), j = blockIdx.y % (p.max_draft + 1);
     const bool draft = blockIdx.z != 0;
     int first;
@@ -202,77 +285,44 @@ __global__ __launch_bounds__(kT) void k_verify_stats(VerifyDrafts p, Stat* __res
     float v[kQuads][4];
 #pragma unroll
     for (int i = 0; i < kQuads; ++i) load4(x, c0 + (i * kT + tid) * 4, p.vocab, v[i]);
-    // first place of the maximum: larger values, then lower indices, have larger keys
-    uint64_t key = 0;
+    float top = -kInf;  // (the maximum passes NaN over)
 #pragma unroll
     for (int i = 0; i < kQuads; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int at = c0 + (i * kT + tid) * 4 + e;
-            const uint64_t k = v[i][e] == v[i][e] && at < p.vocab ? argmax_key(v[i][e], at) : 0;
-            key = k > key ? k : key;
-        }
-    key = wave_max(key);
-    if ((tid & 63) == 0) tmp_key[tid >> 6] = key;
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, v[i][e]);
+    top = wave_max(top);
+    if ((tid & 63) == 0) tmp_top[tid >> 6] = top;
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kT / 64; ++w) key = tmp_key[w] > key ? tmp_key[w] : key;
-    const uint32_t u = static_cast<uint32_t>(key >> 32);
-    const float top = key == 0 ? -kInf : __uint_as_float((u & 0x80000000u) ? u & 0x7fffffffu : ~u);
-    double sum = 0.0;
-    if (temp > 0.0f && top > -kInf) {
-        const double inv_t = 1.0 / static_cast<double>(temp);
+    top = fmaxf(fmaxf(tmp_top[0], tmp_top[1]), fmaxf(tmp_top[2], tmp_top[3]));
+    Stat o{0.0, top, 0};
+    if (temp == 0.0f) {
+        int idx = 0x7fffffff;
 #pragma unroll
         for (int i = 0; i < kQuads; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum += weight(v[i][e], top, inv_t);
-        sum = block_sum(sum, tmp);
+            for (int e = 0; e < 4; ++e)
+                if (v[i][e] == top) idx = min(idx, c0 + (i * kT + tid) * 4 + e);
+        idx = wave_min(idx);
+        if ((tid & 63) == 0) tmp_idx[tid >> 6] = idx;
+        __syncthreads();
+        o.idx = min(min(tmp_idx[0], tmp_idx[1]), min(tmp_idx[2], tmp_idx[3]));
+    } else if (top > -kInf) {
+        const Weigh weigh{1.4426950408889634074 / static_cast<double>(temp), top};
+        double sum[4] = {0.0, 0.0, 0.0, 0.0};
+        if (top < kInf) {
+#pragma unroll
+            for (int i = 0; i < kQuads; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[e] += weigh.finite(v[i][e]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kQuads; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[e] += v[i][e] == top ? 1.0 : 0.0;
+        }
+        o.sum = block_sum((sum[0] + sum[1]) + (sum[2] + sum[3]), tmp);
     }
-    if (tid == 0) {
-        Stat& o = stats[(static_cast<int64_t>(draft ? p.n_rows : 0) + row) * gridDim.x + blockIdx.x];
-        o.sum = sum;
-        o.top = top;
-        o.idx = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(key));
-    }
-}
-
-// The row's maximum (-inf: nothing above), its first place and the sum, from
-// its chunks; one wave, every lane ends with them.
-struct RowStat {
-    double inv_sum;
-    float top;
-    int idx;
-};
-__device__ __forceinline__ RowStat join_row(const Stat* st, int chunks, double inv_t) {
-    const int lane = threadIdx.x & 63;
-    uint64_t key = 0;
-    for (int c = lane; c < chunks; c += 64) {
-        const uint64_t k = st[c].top > -kInf ? argmax_key(st[c].top, static_cast<uint32_t>(st[c].idx)) : 0;
-        key = k > key ? k : key;
-    }
-    key = wave_max(key);
-    RowStat r;
-    const uint32_t u = static_cast<uint32_t>(key >> 32);
-    r.top = key == 0 ? -kInf : __uint_as_float((u & 0x80000000u) ? u & 0x7fffffffu : ~u);
-    r.idx = key == 0 ? 0 : static_cast<int>(0xffffffffu - static_cast<uint32_t>(key));
-    double sum = 0.0;
-    for (int c = lane; c < chunks; c += 64) sum += st[c].sum * (key == 0 ? 0.0 : weight(st[c].top, r.top, inv_t));
-    r.inv_sum = 1.0 / wave_sum(sum);
-    return r;
-}
-
-// Probability from a row's joined statistics (nothing above -inf: certain of token 0).
-__device__ __forceinline__ double prob(float x, int at, const RowStat& r, double inv_t) {
-    if (r.top == -kInf) return at == 0 ? 1.0 : 0.0;
-    return weight(x, r.top, inv_t) * r.inv_sum;
-}
-
-__device__ __forceinline__ void st_dev(double* p, double v) {
-    __hip_atomic_store((__attribute__((address_space(1))) double*)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ double ld_dev(const double* p) {
-    return __hip_atomic_load((const __attribute__((address_space(1))) double*)p, __ATOMIC_RELAXED,
-                             __HIP_MEMORY_SCOPE_AGENT);
+    if (tid == 0) stats[(static_cast<int64_t>(draft ? p.n_rows : 0) + row) * gridDim.x + blockIdx.x] = o;
 }
 
 // grid (chunks, n_seq); sums [n_seq][chunks].
@@ -282,8 +332,8 @@ __global__ __launch_bounds__(kT) void k_verify_pick(VerifyDrafts p, const Stat* 
     constexpr int kWaves = kT / 64;
     __shared__ RowStat best[kWaves][2];   // statistics of the row each wave saw first refused
     __shared__ int stop[kWaves];
-    __shared__ double tmp[kWaves];
-    __shared__ int last, tmp2[2];
+    __shared__ double tmp[kWaves], left;
+    __shared__ int last, tmp2[2 * kWaves];
     const int s = blockIdx.y, chunks = gridDim.x, tid = threadIdx.x, wave = tid >> 6;
     int first;
     const int rows = rows_of(p, s, &first);
@@ -296,7 +346,7 @@ __global__ __launch_bounds__(kT) void k_verify_pick(VerifyDrafts p, const Stat* 
         return;
     }
     const float temp = temperature_of(p, s);
-    const double inv_t = temp > 0.0f ? 1.0 / static_cast<double>(temp) : 1.0;
+    const double scale = temp > 0.0f ? 1.4426950408889634074 / static_cast<double>(temp) : 1.0;
     const Stat* const draft_stats = stats + static_cast<int64_t>(p.n_rows) * chunks;
 
     // Wave w takes rows w, w + 4, ..: the first that stops the request (a
@@ -304,23 +354,26 @@ __global__ __launch_bounds__(kT) void k_verify_pick(VerifyDrafts p, const Stat* 
     if ((tid & 63) == 0) stop[wave] = rows;
     for (int j = wave; j < rows; j += kWaves) {
         const int row = first + j;
-        const RowStat rp = join_row(stats + static_cast<int64_t>(row) * chunks, chunks, inv_t);
+        const bool behind = j + 1 == rows;
+        // (loads that depend on each other first)
+        const int d = behind ? -1 : p.tokens[row + 1];
+        const float u = behind ? 0.0f : p.accept_u[row];
+        const bool real = static_cast<uint32_t>(d) < static_cast<uint32_t>(p.vocab);
+        const float xd = real ? load1(static_cast<const X*>(p.logits) + row * p.logit_stride, d) : 0.0f;
+        const float yd = real && p.draft_logits
+                             ? load1(static_cast<const X*>(p.draft_logits) + row * p.draft_stride, d) : 0.0f;
+        const RowStat rp = join_row(stats + static_cast<int64_t>(row) * chunks, chunks, scale);
         RowStat rq = rp;
-        bool stops = j + 1 == rows;
-        if (!stops) {
-            const int d = p.tokens[row + 1];
-            const bool real = static_cast<uint32_t>(d) < static_cast<uint32_t>(p.vocab);
-            if (temp == 0.0f) {
-                stops = d != rp.idx;
-            } else {
-                double pd = 0.0, qd = real ? 1.0 : 0.0;
-                if (real) pd = prob(load1(static_cast<const X*>(p.logits) + row * p.logit_stride, d), d, rp, inv_t);
-                if (p.draft_logits) {
-                    rq = join_row(draft_stats + static_cast<int64_t>(row) * chunks, chunks, inv_t);
-                    if (real) qd = prob(load1(static_cast<const X*>(p.draft_logits) + row * p.draft_stride, d), d, rq, inv_t);
-                }
-                stops = !(static_cast<double>(p.accept_u[row]) * qd < pd);
+        bool stops = behind;
+        if (!behind && temp == 0.0f) {
+            stops = d != rp.idx;
+        } else if (!behind) {
+            double qd = real ? 1.0 : 0.0;
+            if (p.draft_logits) {
+                rq = join_row(draft_stats + static_cast<int64_t>(row) * chunks, chunks, scale);
+                if (real) qd = prob(yd, d, rq, scale);
             }
+            stops = !(static_cast<double>(u) * qd < (real ? prob(xd, d, rp, scale) : 0.0));
         }
         if (stops) {
             if ((tid & 63) == 0) {
@@ -341,20 +394,18 @@ __global__ __launch_bounds__(kT) void k_verify_pick(VerifyDrafts p, const Stat* 
         }
     const RowStat rp = best[who][0], rq = best[who][1];
     const int row = first + j;
-    const bool refused = j + 1 < rows;
+    const bool refused = j + 1 < rows, certain = temp == 0.0f || rp.top == -kInf;
     const int d = refused ? p.tokens[row + 1] : -1;
     if (blockIdx.x == 0) {
         for (int i = tid; i <= p.max_draft; i += kT)
-            if (i != j) out[i] = i < j ? p.tokens[first + 1 + i] : -1;
+            if (i != j || certain) out[i] = i < j ? p.tokens[first + 1 + i] : (i == j ? rp.idx : -1);
         if (tid == 0) p.out_count[s] = j + 1;
     }
-    if (temp == 0.0f || rp.top == -kInf) {  // a certain row
-        if (blockIdx.x == 0 && tid == 0) out[j] = rp.idx;
-        return;
-    }
+    if (certain || (!refused && blockIdx.x != 0)) return;  // (the chunks' sums of p are there: one workgroup is enough)
     const X* const x = static_cast<const X*>(p.logits) + row * p.logit_stride;
     const X* const y = p.draft_logits ? static_cast<const X*>(p.draft_logits) + row * p.draft_stride : nullptr;
     const Stat* const st = stats + static_cast<int64_t>(row) * chunks;
+    const Weigh weigh_p{scale, rp.top};
 
     // Weights of four values from `at` on.
     auto weights4 = [&](int at, bool rest, double (&w)[4]) {
@@ -363,18 +414,19 @@ __global__ __launch_bounds__(kT) void k_verify_pick(VerifyDrafts p, const Stat* 
         if (rest && y) load4(y, at, p.vocab, yv);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            w[e] = at + e < p.vocab ? weight(xv[e], rp.top, inv_t) * rp.inv_sum : 0.0;
+            w[e] = at + e < p.vocab ? weigh_p(xv[e]) * rp.inv_sum : 0.0;
             if (rest) {
-                const double q = y ? (at + e < p.vocab ? prob(yv[e], at + e, rq, inv_t) : 0.0) : (at + e == d ? 1.0 : 0.0);
+                const double q = y ? (at + e < p.vocab ? prob(yv[e], at + e, rq, scale) : 0.0)
+                                   : (at + e == d ? 1.0 : 0.0);
                 w[e] = fmax(w[e] - q, 0.0);
             }
         }
     };
+    auto of_p = [&](int chunk) { return st[chunk].top > -kInf ? st[chunk].sum * weigh_p(st[chunk].top) * rp.inv_sum : 0.0; };
 
-    __shared__ double left;
     bool rest = refused;
     double* const mine = sums + static_cast<int64_t>(s) * chunks;
-    if (refused) {
+    if (rest) {
         double sum = 0.0;
 #pragma unroll
         for (int i = 0; i < kQuads; ++i) {
@@ -383,6 +435,7 @@ __global__ __launch_bounds__(kT) void k_verify_pick(VerifyDrafts p, const Stat* 
             sum += (w[0] + w[1]) + (w[2] + w[3]);
         }
         sum = block_sum(sum, tmp);
+        // Relaxed: the sum goes out in an agent-scope store that is waited for.
         if (tid == 0) {
             st_dev(mine + blockIdx.x, sum);
             wait_vmcnt<0>();
@@ -392,18 +445,15 @@ __global__ __launch_bounds__(kT) void k_verify_pick(VerifyDrafts p, const Stat* 
         __syncthreads();
         if (!last) return;
         if (tid == 0) __hip_atomic_store(arrivals + s, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    } else if (blockIdx.x != 0) {
-        return;  // (the chunk sums of p are there: one workgroup finds the token)
     }
 
-    // The chunk with the border: thread c holds chunk c's sum.
+    // The chunk with the border: thread i holds chunk i's sum.
     double w1[1] = {0.0}, total;
-    if (tid < chunks)
-        w1[0] = rest ? ld_dev(mine + tid) : (st[tid].top > -kInf ? st[tid].sum * weight(st[tid].top, rp.top, inv_t) * rp.inv_sum : 0.0);
+    if (tid < chunks) w1[0] = rest ? ld_dev(mine + tid) : of_p(tid);
     double before = block_before(w1[0], tmp, &total);
     if (rest && !(total > 0.0)) {  // (p is nowhere above q: from p after all)
         rest = false;
-        if (tid < chunks) w1[0] = st[tid].top > -kInf ? st[tid].sum * weight(st[tid].top, rp.top, inv_t) * rp.inv_sum : 0.0;
+        if (tid < chunks) w1[0] = of_p(tid);
         before = block_before(w1[0], tmp, &total);
     }
     const double target = static_cast<double>(p.sample_u[s]) * total;
