@@ -15,16 +15,21 @@
 // so weights and sums are in 64 bits: a token of probability 1e-5 then changes
 // hands with odds below 1e-10, with 32-bit sums 1e-3.
 //
-// Two launches.  k_verify_stats reads every row once, in chunks, and leaves
-// each chunk's maximum and sum of exp((x - maximum) / T); k_verify_pick joins
-// them (every workgroup of a request for itself), decides on the drafts, sums
-// w of the deciding row by chunks and, in the request's last workgroup to
+// Three launches.  k_verify_stats reads every row once, in chunks, and leaves
+// each chunk's maximum and sum of exp((x - maximum) / T); k_verify_decide joins
+// a request's rows and decides on its drafts; k_verify_pick sums w of the row
+// behind a refused draft by chunks and, in the request's last workgroup to
 // arrive, finds the chunk that holds the border and the token in it (behind the
 // last draft the chunks' sums are there already).  Rows of a request whose T is
 // 0 need no sums.
 //
 // Bound: the bytes of the logits, and as much the exponentials, 18 64-bit
-// instructions each at the rate of 32-bit ones.
+// instructions each at the rate of 32-bit ones.  64 requests of up to 4 drafts,
+// 128256 values in f32, 173 MB: 33 us for the sums (5.2 TB/s), 5 to decide, 22
+// to pick, for which the rows behind refused drafts are read once more.  One
+// request of 7 drafts: 4.6 + 4.4 + 11, chains of dependent loads.  (Decisions
+// in every workgroup of the pick: 66 us and 25; in the sums' last workgroup to
+// arrive: 125 and 40, an arrival costs each of 10000 workgroups 2 us.)
 #include "rt_common.hpp"
 #include "rt_launch.hpp"
 
@@ -34,6 +39,8 @@ namespace {
 constexpr int kT = 256;
 constexpr int kQuads = 4;                  // groups of 4 values a thread holds
 constexpr int kChunk = kT * 4 * kQuads;    // values of a row per workgroup
+constexpr int kPickT = 512;                // (k_verify_pick, 64 requests: 22 us; 1024 threads 31, 256 25)
+constexpr int kPickQuads = kChunk / 4 / kPickT;
 constexpr float kInf = __builtin_inff();
 
 struct Stat {
@@ -72,7 +79,10 @@ struct Weigh {
     __device__ __forceinline__ double finite(float x) const {  // top < inf
         return exp2_64((static_cast<double>(x) - static_cast<double>(top)) * scale);
     }
-    __device__ __forceinline__ double operator()(float x) const { return x == top ? 1.0 : finite(x); }
+    __device__ __forceinline__ double operator()(float x) const {
+        const double w = finite(x);  // (a select, no branch)
+        return x == top ? 1.0 : w;
+    }
 };
 
 typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
@@ -109,6 +119,7 @@ __device__ __forceinline__ float temperature_of(const VerifyDrafts& p, int s) {
     const float t = p.temperature ? p.temperature[s] : 1.0f;
     return t > 0.0f ? t : 0.0f;
 }
+__device__ __forceinline__ double scale_of(float t) { return t > 0.0f ? 1.4426950408889634074 / static_cast<double>(t) : 1.0; }
 // First row and number of drafts of request s, inside the arrays.
 __device__ __forceinline__ int rows_of(const VerifyDrafts& p, int s, int* first) {
     const int a = min(max(p.row_start[s], 0), p.n_rows), b = min(max(p.row_start[s + 1], a), p.n_rows);
@@ -161,15 +172,20 @@ __device__ __forceinline__ int wave_min(int v) {
     return of_lane(running(v, 0x7fffffff, [](int a, int b) { return min(a, b); }), 63);
 }
 
-// Sum over the workgroup, the same bits in every thread.
+// Sum over a workgroup of W waves, the same bits in every thread.
+template <int W>
 __device__ __forceinline__ double block_sum(double v, double* tmp) {
     v = wave_sum(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = v;
     __syncthreads();
-    return (tmp[0] + tmp[1]) + (tmp[2] + tmp[3]);
+    double sum = tmp[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) sum += tmp[w];
+    return sum;
 }
 // Sum over the threads before this one; *total: over all of them.
+template <int W>
 __device__ __forceinline__ double block_before(double v, double* tmp, double* total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const double sum = running_sum(v);
@@ -179,8 +195,8 @@ __device__ __forceinline__ double block_before(double v, double* tmp, double* to
     __syncthreads();
     double all = 0.0, base = 0.0;
 #pragma unroll
-    for (int w = 0; w < kT / 64; ++w) {
-        if (w == wave) base = all;
+    for (int w = 0; w < W; ++w) {
+        base = w == wave ? all : base;
         all += tmp[w];
     }
     *total = all;
@@ -189,7 +205,7 @@ __device__ __forceinline__ double block_before(double v, double* tmp, double* to
 // Of the weights in thread order (thread t's first[0 .. N) lie `before` it):
 // the place of the first with which the running sum exceeds target, else of
 // the last weight above 0, else -1.  place(e): where weight e stands, below 2^31.
-template <int N, class F>
+template <int W, int N, class F>
 __device__ __forceinline__ int find_border(const double (&w)[N], double before, double target, F place, int* tmp2) {
     const int wave = threadIdx.x >> 6;
     int hit = -1, heavy = -1;
@@ -207,14 +223,14 @@ __device__ __forceinline__ int find_border(const double (&w)[N], double before, 
     __syncthreads();
     if ((threadIdx.x & 63) == 0) {
         tmp2[wave] = hit;
-        tmp2[kT / 64 + wave] = heavy;
+        tmp2[W + wave] = heavy;
     }
     __syncthreads();
     int first = -1, last = -1;
 #pragma unroll
-    for (int i = 0; i < kT / 64; ++i) {
+    for (int i = 0; i < W; ++i) {
         if (first < 0) first = tmp2[i];
-        last = max(last, tmp2[kT / 64 + i]);
+        last = max(last, tmp2[W + i]);
     }
     return first >= 0 ? first : last;
 }
@@ -261,8 +277,8 @@ __device__ __forceinline__ RowStat join_row(const Stat* st, int chunks, double s
 
 // Probability from a row's joined statistics (nothing above -inf: certain of token 0).
 __device__ __forceinline__ double prob(float x, int at, const RowStat& r, double scale) {
-    if (r.top == -kInf) return at == 0 ? 1.0 : 0.0;
-    return Weigh{scale, r.top}(x) * r.inv_sum;
+    const double w = Weigh{scale, r.top}(x) * r.inv_sum;
+    return r.top == -kInf ? (at == 0 ? 1.0 : 0.0) : w;
 }
 
 // Statistics [which][row][chunk]; grid (chunks, n_seq * (max_draft + 1), 1 or 2).
@@ -307,7 +323,7 @@ __global__ __launch_bounds__(kT) void k_verify_stats(VerifyDrafts p, Stat* __res
         __syncthreads();
         o.idx = min(min(tmp_idx[0], tmp_idx[1]), min(tmp_idx[2], tmp_idx[3]));
     } else if (top > -kInf) {
-        const Weigh weigh{1.4426950408889634074 / static_cast<double>(temp), top};
+        const Weigh weigh{scale_of(temp), top};
         double sum[4] = {0.0, 0.0, 0.0, 0.0};
         if (top < kInf) {
 #pragma unroll
@@ -320,37 +336,42 @@ __global__ __launch_bounds__(kT) void k_verify_stats(VerifyDrafts p, Stat* __res
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sum[e] += v[i][e] == top ? 1.0 : 0.0;
         }
-        o.sum = block_sum((sum[0] + sum[1]) + (sum[2] + sum[3]), tmp);
+        o.sum = block_sum<kT / 64>((sum[0] + sum[1]) + (sum[2] + sum[3]), tmp);
     }
     if (tid == 0) stats[(static_cast<int64_t>(draft ? p.n_rows : 0) + row) * gridDim.x + blockIdx.x] = o;
 }
 
-// grid (chunks, n_seq); sums [n_seq][chunks].
+// What is left to do for a request: w of `row` chooses the token out[at].
+struct Choice {
+    RowStat p, q;
+    int32_t row, at, draft;
+    int32_t kind;  // 0: nothing is; 1: w = max(0, p - q), q certain of `draft` where no logits are given; 2: w = p
+};
+
+// Accepted drafts, their count, and the choice that is left; grid n_seq.  Wave w
+// takes rows w, w + 16, ..: the first that stops the request, a refused draft or
+// the row behind the last one.
 template <class X>
-__global__ __launch_bounds__(kT) void k_verify_pick(VerifyDrafts p, const Stat* __restrict__ stats,
-                                                    double* __restrict__ sums, uint32_t* __restrict__ arrivals) {
-    constexpr int kWaves = kT / 64;
-    __shared__ RowStat best[kWaves][2];   // statistics of the row each wave saw first refused
+__global__ __launch_bounds__(kPickT) void k_verify_decide(VerifyDrafts p, const Stat* __restrict__ stats, int chunks,
+                                                          Choice* __restrict__ choices) {
+    constexpr int kWaves = kPickT / 64;
+    __shared__ RowStat best[kWaves][2];
     __shared__ int stop[kWaves];
-    __shared__ double tmp[kWaves], left;
-    __shared__ int last, tmp2[2 * kWaves];
-    const int s = blockIdx.y, chunks = gridDim.x, tid = threadIdx.x, wave = tid >> 6;
+    const int s = blockIdx.x, tid = threadIdx.x, wave = tid >> 6;
     int first;
     const int rows = rows_of(p, s, &first);
     int32_t* const out = p.out_tokens + static_cast<int64_t>(s) * (p.max_draft + 1);
     if (rows == 0) {  // no rows, no tokens
-        if (blockIdx.x == 0) {
-            for (int i = tid; i <= p.max_draft; i += kT) out[i] = -1;
-            if (tid == 0) p.out_count[s] = 0;
+        for (int i = tid; i <= p.max_draft; i += kPickT) out[i] = -1;
+        if (tid == 0) {
+            p.out_count[s] = 0;
+            choices[s].kind = 0;
         }
         return;
     }
     const float temp = temperature_of(p, s);
-    const double scale = temp > 0.0f ? 1.4426950408889634074 / static_cast<double>(temp) : 1.0;
+    const double scale = scale_of(temp);
     const Stat* const draft_stats = stats + static_cast<int64_t>(p.n_rows) * chunks;
-
-    // Wave w takes rows w, w + 4, ..: the first that stops the request (a
-    // refused draft, or the row behind the last draft).
     if ((tid & 63) == 0) stop[wave] = rows;
     for (int j = wave; j < rows; j += kWaves) {
         const int row = first + j;
@@ -392,49 +413,65 @@ __global__ __launch_bounds__(kT) void k_verify_pick(VerifyDrafts p, const Stat* 
             j = stop[w];
             who = w;
         }
-    const RowStat rp = best[who][0], rq = best[who][1];
-    const int row = first + j;
+    const RowStat rp = best[who][0];
     const bool refused = j + 1 < rows, certain = temp == 0.0f || rp.top == -kInf;
-    const int d = refused ? p.tokens[row + 1] : -1;
-    if (blockIdx.x == 0) {
-        for (int i = tid; i <= p.max_draft; i += kT)
-            if (i != j || certain) out[i] = i < j ? p.tokens[first + 1 + i] : (i == j ? rp.idx : -1);
-        if (tid == 0) p.out_count[s] = j + 1;
+    for (int i = tid; i <= p.max_draft; i += kPickT)
+        if (i != j || certain) out[i] = i < j ? p.tokens[first + 1 + i] : (i == j ? rp.idx : -1);
+    if (tid == 0) {
+        p.out_count[s] = j + 1;
+        choices[s] = Choice{rp, best[who][1], first + j, j, refused ? p.tokens[first + j + 1] : -1,
+                            certain ? 0 : (refused ? 1 : 2)};
     }
-    if (certain || (!refused && blockIdx.x != 0)) return;  // (the chunks' sums of p are there: one workgroup is enough)
-    const X* const x = static_cast<const X*>(p.logits) + row * p.logit_stride;
-    const X* const y = p.draft_logits ? static_cast<const X*>(p.draft_logits) + row * p.draft_stride : nullptr;
-    const Stat* const st = stats + static_cast<int64_t>(row) * chunks;
-    const Weigh weigh_p{scale, rp.top};
+}
+
+// grid (chunks, n_seq); sums [n_seq][chunks].
+template <class X>
+__global__ __launch_bounds__(kPickT) void k_verify_pick(VerifyDrafts p, const Stat* __restrict__ stats,
+                                                        const Choice* __restrict__ choices, double* __restrict__ sums,
+                                                        uint32_t* __restrict__ arrivals) {
+    constexpr int kWaves = kPickT / 64;
+    __shared__ double tmp[kWaves], left;
+    __shared__ int last, tmp2[2 * kWaves];
+    const int s = blockIdx.y, chunks = gridDim.x, tid = threadIdx.x;
+    const Choice c = choices[s];
+    if (c.kind == 0 || (c.kind == 2 && blockIdx.x != 0)) return;  // (sums of p are there: one workgroup is enough)
+    const double scale = scale_of(temperature_of(p, s));
+    const X* const x = static_cast<const X*>(p.logits) + c.row * p.logit_stride;
+    const X* const y = p.draft_logits ? static_cast<const X*>(p.draft_logits) + c.row * p.draft_stride : nullptr;
+    const Weigh weigh_p{scale, c.p.top};
 
     // Weights of four values from `at` on.
-    auto weights4 = [&](int at, bool rest, double (&w)[4]) {
+    auto weights4 = [&](int at, bool rest, double* w) {
         float xv[4], yv[4];
         load4(x, at, p.vocab, xv);
         if (rest && y) load4(y, at, p.vocab, yv);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            w[e] = at + e < p.vocab ? weigh_p(xv[e]) * rp.inv_sum : 0.0;
-            if (rest) {
-                const double q = y ? (at + e < p.vocab ? prob(yv[e], at + e, rq, scale) : 0.0)
-                                   : (at + e == d ? 1.0 : 0.0);
+        for (int e = 0; e < 4; ++e) w[e] = at + e < p.vocab ? weigh_p(xv[e]) * c.p.inv_sum : 0.0;
+        if (rest) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const double q = y ? (at + e < p.vocab ? prob(yv[e], at + e, c.q, scale) : 0.0)
+                                   : (at + e == c.draft ? 1.0 : 0.0);
                 w[e] = fmax(w[e] - q, 0.0);
             }
         }
     };
-    auto of_p = [&](int chunk) { return st[chunk].top > -kInf ? st[chunk].sum * weigh_p(st[chunk].top) * rp.inv_sum : 0.0; };
+    auto of_p = [&](int chunk) {
+        const Stat st = stats[static_cast<int64_t>(c.row) * chunks + chunk];
+        return st.top > -kInf ? st.sum * weigh_p(st.top) * c.p.inv_sum : 0.0;
+    };
 
-    bool rest = refused;
+    bool rest = c.kind == 1;
     double* const mine = sums + static_cast<int64_t>(s) * chunks;
     if (rest) {
         double sum = 0.0;
 #pragma unroll
-        for (int i = 0; i < kQuads; ++i) {
+        for (int i = 0; i < kPickQuads; ++i) {
             double w[4];
-            weights4(blockIdx.x * kChunk + (i * kT + tid) * 4, true, w);
+            weights4(blockIdx.x * kChunk + (i * kPickT + tid) * 4, true, w);
             sum += (w[0] + w[1]) + (w[2] + w[3]);
         }
-        sum = block_sum(sum, tmp);
+        sum = block_sum<kWaves>(sum, tmp);
         // Relaxed: the sum goes out in an agent-scope store that is waited for.
         if (tid == 0) {
             st_dev(mine + blockIdx.x, sum);
@@ -450,34 +487,27 @@ __global__ __launch_bounds__(kT) void k_verify_pick(VerifyDrafts p, const Stat* 
     // The chunk with the border: thread i holds chunk i's sum.
     double w1[1] = {0.0}, total;
     if (tid < chunks) w1[0] = rest ? ld_dev(mine + tid) : of_p(tid);
-    double before = block_before(w1[0], tmp, &total);
+    double before = block_before<kWaves>(w1[0], tmp, &total);
     if (rest && !(total > 0.0)) {  // (p is nowhere above q: from p after all)
         rest = false;
         if (tid < chunks) w1[0] = of_p(tid);
-        before = block_before(w1[0], tmp, &total);
+        before = block_before<kWaves>(w1[0], tmp, &total);
     }
     const double target = static_cast<double>(p.sample_u[s]) * total;
-    const int border = find_border(w1, before, target, [&](int) { return tid; }, tmp2);
+    const int border = find_border<kWaves>(w1, before, target, [&](int) { return tid; }, tmp2);
     if (tid == border) left = target - before;
     __syncthreads();
-    // The token in it: thread t takes values [16 t, 16 t + 16) of the chunk,
-    // the vocabulary's order.
-    constexpr int kOwn = kChunk / kT;
-    const int c0 = border * kChunk + tid * kOwn;
-    double own = 0.0, w[kOwn];
+    // The token in it: a thread's values lie next to each other, the vocabulary's order.
+    const int c0 = border * kChunk + tid * (4 * kPickQuads);
+    double w[4 * kPickQuads], own = 0.0;
 #pragma unroll
-    for (int i = 0; i < kOwn / 4; ++i) {
-        double q[4];
-        weights4(c0 + 4 * i, rest, q);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            w[4 * i + e] = q[e];
-            own += q[e];
-        }
+    for (int i = 0; i < kPickQuads; ++i) {
+        weights4(c0 + 4 * i, rest, w + 4 * i);
+        own += (w[4 * i] + w[4 * i + 1]) + (w[4 * i + 2] + w[4 * i + 3]);
     }
-    before = block_before(own, tmp, &total);
-    const int token = find_border(w, before, left, [&](int e) { return c0 + e; }, tmp2);
-    if (tid == 0) out[j] = token;
+    before = block_before<kWaves>(own, tmp, &total);
+    const int token = find_border<kWaves>(w, before, left, [&](int e) { return c0 + e; }, tmp2);
+    if (tid == 0) p.out_tokens[static_cast<int64_t>(s) * (p.max_draft + 1) + c.at] = token;
 }
 
 int chunks_of(int vocab) { return (vocab + kChunk - 1) / kChunk; }
@@ -489,19 +519,22 @@ size_t stats_bytes(const VerifyDrafts& p) {
 template <class X>
 hipError_t run(const VerifyDrafts& p, void* work, uint32_t* counters, hipStream_t s) {
     Stat* const stats = static_cast<Stat*>(work);
-    double* const sums = reinterpret_cast<double*>(static_cast<uint8_t*>(work) + stats_bytes(p));
+    Choice* const choices = reinterpret_cast<Choice*>(static_cast<uint8_t*>(work) + stats_bytes(p));
+    double* const sums = reinterpret_cast<double*>(choices + p.n_seq);
     const unsigned chunks = static_cast<unsigned>(chunks_of(p.vocab));
     const unsigned rows = static_cast<unsigned>(p.n_seq) * static_cast<unsigned>(p.max_draft + 1);
     hipLaunchKernelGGL(k_verify_stats<X>, dim3(chunks, rows, p.draft_logits ? 2 : 1), dim3(kT), 0, s, p, stats);
-    hipLaunchKernelGGL(k_verify_pick<X>, dim3(chunks, static_cast<unsigned>(p.n_seq)), dim3(kT), 0, s, p, stats, sums,
-                       counters);
+    hipLaunchKernelGGL(k_verify_decide<X>, dim3(static_cast<unsigned>(p.n_seq)), dim3(kPickT), 0, s, p, stats,
+                       static_cast<int>(chunks), choices);
+    hipLaunchKernelGGL(k_verify_pick<X>, dim3(chunks, static_cast<unsigned>(p.n_seq)), dim3(kPickT), 0, s, p, stats, choices,
+                       sums, counters);
     return hipGetLastError();
 }
 
 }  // namespace
 
 size_t verify_drafts_workspace(const VerifyDrafts& p) {
-    return stats_bytes(p) + static_cast<size_t>(p.n_seq) * chunks_of(p.vocab) * sizeof(double);
+    return stats_bytes(p) + static_cast<size_t>(p.n_seq) * (sizeof(Choice) + chunks_of(p.vocab) * sizeof(double));
 }
 
 hipError_t launch_verify_drafts(const VerifyDrafts& p, void* work, uint32_t* counters, hipStream_t s) {
