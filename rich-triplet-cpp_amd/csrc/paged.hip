@@ -22,6 +22,7 @@
 // bytes read and written.
 #include "rt_common.hpp"
 #include "rt_launch.hpp"
+#include "wave_scan.hpp"
 
 namespace rt_hip {
 namespace {
@@ -32,11 +33,7 @@ constexpr int kPlanTokens = 4;  // consecutive tokens a thread takes at a time
 template <int NT, class T>
 __device__ __forceinline__ T block_scan(T v, T* tmp, T* total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const T o = __shfl_up(v, off, kWave);
-        if (lane >= off) v += o;
-    }
+    v = running_sum(v);
     __syncthreads();  // (tmp's readers of the call before)
     if (lane == 63) tmp[wave] = v;
     __syncthreads();

@@ -41,6 +41,7 @@
 
 #include "rt_common.hpp"
 #include "rt_launch.hpp"
+#include "wave_scan.hpp"
 
 namespace rt_hip {
 namespace {
@@ -661,23 +662,13 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
     return a / b;
 }
 
-// Inclusive sum over the wave's lanes.
-__device__ __forceinline__ int64_t wave_scan(int64_t v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const int64_t o = __shfl_up(v, off, kWave);
-        if (lane >= off) v += o;
-    }
-    return v;
-}
 // Units of the walk's request for one KV head, its blocks counted by the wave's
 // lanes (the walk is the same in all of them).
 template <class W>
 __device__ __forceinline__ int64_t wave_total(const W& walk) {
     int64_t t = 0;
     for (int b = threadIdx.x & 63; b < walk.blocks; b += 64) t += walk.units(b);
-    return uniform(__shfl(wave_scan(t), 63, kWave));
+    return of_lane(running_sum(t), 63);
 }
 
 // Positions the walk at workgroup w's range of the sequence of all units (of
@@ -712,8 +703,8 @@ __device__ __forceinline__ int64_t find_range(W& walk, int w, int nw, int64_t* s
     };
     int64_t mine = 0;
     for (int i = 0; i < each; ++i) mine += units_of(i);
-    int64_t incl = wave_scan(mine);
-    int64_t all = __shfl(incl, 63, kWave);
+    int64_t incl = running_sum(mine);
+    int64_t all = of_lane(incl, 63);
     if (!small) {
         if (lane == 63) sums[tid >> 6] = incl;
         __syncthreads();
@@ -735,7 +726,7 @@ __device__ __forceinline__ int64_t find_range(W& walk, int w, int nw, int64_t* s
     int64_t at = incl - mine;  // units before the request
     if (small) {
         s = __builtin_ctzll(__builtin_amdgcn_ballot_w64(here));
-        at = __shfl(at, s, kWave);
+        at = of_lane(at, s);
     } else {
         if (__builtin_amdgcn_ballot_w64(here) != 0) {  // (whole waves, as units_of counts)
             for (int i = 0; i < each; ++i) {
@@ -758,15 +749,15 @@ __device__ __forceinline__ int64_t find_range(W& walk, int w, int nw, int64_t* s
     off -= walk.kvh * t;
     for (int b0 = 0;; b0 += 64) {
         const int c = b0 + lane < walk.blocks ? walk.units(b0 + lane) : 0;
-        const int64_t sum = wave_scan(c);
+        const int64_t sum = running_sum(static_cast<int64_t>(c));
         const uint64_t behind = __builtin_amdgcn_ballot_w64(off < sum);
         if (behind || b0 + 64 >= walk.blocks) {
             const int l = behind ? __builtin_ctzll(behind) : 0;
             walk.block(b0 + l);
-            off -= uniform(__shfl(sum - c, l, kWave));
+            off -= of_lane(sum - c, l);
             break;
         }
-        off -= uniform(__shfl(sum, 63, kWave));
+        off -= of_lane(sum, 63);
     }
     *skip = off;
     return min(*per, all - u);

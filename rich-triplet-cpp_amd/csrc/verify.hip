@@ -32,6 +32,7 @@
 // arrive: 125 and 40, an arrival costs each of 10000 workgroups 2 us.)
 #include "rt_common.hpp"
 #include "rt_launch.hpp"
+#include "wave_scan.hpp"
 
 namespace rt_hip {
 namespace {
@@ -127,43 +128,6 @@ __device__ __forceinline__ int rows_of(const VerifyDrafts& p, int s, int* first)
     return min(b - a, p.max_draft + 1);  // rows; drafts are one fewer
 }
 
-// Lane i's value in a lane ahead of it, `old` in lanes without one: rows of 16
-// shifted by 1, 2, 4, 8, then the last lane of a row or half to the rows behind
-// it.  Running an operation over these six leaves lane i with lanes 0 .. i.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int from_before(int old, int v) {
-    return __builtin_amdgcn_update_dpp(old, v, CTRL, ROWS, 0xf, false);
-}
-template <int CTRL, int ROWS>
-__device__ __forceinline__ float from_before(float old, float v) {
-    return __int_as_float(from_before<CTRL, ROWS>(__float_as_int(old), __float_as_int(v)));
-}
-template <int CTRL, int ROWS>
-__device__ __forceinline__ double from_before(double old, double v) {
-    const uint64_t o = __builtin_bit_cast(uint64_t, old), b = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = from_before<CTRL, ROWS>(static_cast<int>(o), static_cast<int>(b));
-    const uint32_t hi = from_before<CTRL, ROWS>(static_cast<int>(o >> 32), static_cast<int>(b >> 32));
-    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
-}
-template <class V, class F>
-__device__ __forceinline__ V running(V v, V none, F op) {
-    v = op(v, from_before<0x111, 0xf>(none, v));
-    v = op(v, from_before<0x112, 0xf>(none, v));
-    v = op(v, from_before<0x114, 0xf>(none, v));
-    v = op(v, from_before<0x118, 0xf>(none, v));
-    v = op(v, from_before<0x142, 0xa>(none, v));
-    return op(v, from_before<0x143, 0xc>(none, v));
-}
-__device__ __forceinline__ int of_lane(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
-__device__ __forceinline__ float of_lane(float v, int lane) { return __int_as_float(of_lane(__float_as_int(v), lane)); }
-__device__ __forceinline__ double of_lane(double v, int lane) {
-    const uint64_t b = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = of_lane(static_cast<int>(b), lane), hi = of_lane(static_cast<int>(b >> 32), lane);
-    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
-}
-__device__ __forceinline__ double running_sum(double v) {
-    return running(v, 0.0, [](double a, double b) { return a + b; });
-}
 __device__ __forceinline__ double wave_sum(double v) { return of_lane(running_sum(v), 63); }
 __device__ __forceinline__ float wave_max(float v) {
     return of_lane(running(v, -kInf, [](float a, float b) { return fmaxf(a, b); }), 63);
