@@ -91,8 +91,9 @@ int rt_hip_init(int ordinal);
  * copies of f32 A and of a Q4_K weight shared by several M tiles, split-K
  * partials), the batched GEMV of every format (K-slice partials), decode
  * attention (split partials), FLUX and paged attention (the states of blocks cut
- * between workgroups), verify_drafts (the rows' sums) and argmax (8 bytes per row).  It grows on demand (the reference
- * likewise grows its Metal scratch on demand, src/metal_ops.mm:378-423).  A
+ * between workgroups), verify_drafts (the rows' sums) and argmax (8 bytes per
+ * row).  It grows on demand (the reference likewise grows its Metal scratch on
+ * demand, src/metal_ops.mm:378-423).  A
  * replaced buffer is kept until the process ends, because a hipGraph that
  * captured a call still writes the buffer that call used on every replay.
  * Growth allocates, so it does not happen while the stream is being captured:
@@ -722,8 +723,10 @@ int rt_hip_paged_append(const rt_hip_paged_kv* kv, const void* k, const void* v,
  * dtype is q's and out's: the cache's (F16 or BF16: products of 16-bit values
  * summed in f32, the softmax in f32 and its weights rounded to the type before
  * they multiply v), or F32 with any cache (products and sums to f32
- * accuracy).  n_q_heads is any multiple of n_kv_heads up to 1024, scale > 0.
- * Results are deterministic.
+ * accuracy).  An infinity or a NaN in a row's q, or in a key that it sees,
+ * leaves that row's head undefined, and no other; in values, what is not finite
+ * reaches the rows that see it as a sum would have it.  n_q_heads is any
+ * multiple of n_kv_heads up to 1024, scale > 0.  Results are deterministic.
  * max_fresh is a hint, the most rows a request of this step may have (0: not
  * known); the result does not depend on it beyond rounding.
  * Uses the library workspace (rt_hip_paged_attention_workspace_bytes, to

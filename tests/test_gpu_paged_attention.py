@@ -170,6 +170,16 @@ def test_long(rt, q, kv, kv_heads, group, dim, lens, window):
 
 
 @pytest.mark.parametrize("q, kv", PAIRS)
+@pytest.mark.parametrize("window", [0, 90])
+def test_chunks_among_many_requests(rt, q, kv, window):
+    """Chunks of several blocks at either end and inside of a batch that a wave has not lanes enough for."""
+    say("chunks", q, kv, window)
+    lens = [(1, 1 + 13 * s % 400) for s in range(131)]
+    lens[0], lens[63], lens[64], lens[77], lens[130] = (700, 900), (300, 300), (0, 10), (513, 2000), (1030, 1030)
+    Step(q, kv, 3, 1, 64, 32, lens, seed=3, window=window).check(rt)
+
+
+@pytest.mark.parametrize("q, kv", PAIRS)
 def test_many_requests(rt, q, kv):
     """More requests than a workgroup has threads."""
     say("many", q, kv)
@@ -247,6 +257,24 @@ def test_same_bits(rt, q, kv):
         c = st.run(rt, out=torch.zeros_like(st.out))
     torch.cuda.synchronize()
     assert torch.equal(a, b) and torch.equal(a, c)
+
+
+@pytest.mark.parametrize("q, kv", PAIRS)
+def test_on_another_stream(rt, q, kv):
+    """Calls in turn on two streams that wait for each other: the workspace is shared, the results are the same."""
+    say("streams", q, kv)
+    step = Step(q, kv, 8, 2, 128, 16, [(1, 5000), (200, 900), (4, 77)])
+    want = step.run(rt).clone()
+    side, out = torch.cuda.Stream(), torch.empty_like(step.out)
+    for _ in range(3):
+        step.out.fill_(-77.0)
+        out.fill_(-77.0)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step.run(rt, out=out)
+        torch.cuda.current_stream().wait_stream(side)
+        step.run(rt)
+        assert torch.equal(out, want) and torch.equal(step.out, want)
 
 
 @pytest.mark.parametrize("q, kv", PAIRS)

@@ -106,6 +106,19 @@ def test_verify_a_vocabulary_of_a_million(rt):
     assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
 
 
+@pytest.mark.parametrize("n, lo, hi, vocab", [(3, 20, 70, 257), (600, 0, 3, 40), (2, 255, 255, 33), (2, 2, 4, 300001)])
+@pytest.mark.parametrize("with_draft", [True, False])
+def test_verify_many(rt, n, lo, hi, vocab, with_draft):
+    """More drafts than a workgroup has waves, many requests, more chunks of a row than a wave has lanes."""
+    say("verify many", n, lo, hi, vocab, with_draft)
+    logits, draft, tokens, starts, ua, us, temp = make(n, n, vocab, lo, hi)
+    ua = (ua * 0.05).astype(np.float32)  # (most drafts accepted)
+    draft = draft if with_draft else None
+    want = rules(logits, draft, tokens, starts, ua, us, temp, hi + 1)
+    got = call(rt, logits, draft, tokens, starts, ua, us, temp, hi)
+    assert np.array_equal(got[1], want[1]) and np.array_equal(got[0], want[0])
+
+
 def test_verify_special_rows(rt):
     """Masked vocabularies, rows of nothing, infinities, NaN, equal distributions, ties, random numbers at 0 and next
     to 1, drafts without probability and outside the vocabulary."""
