@@ -574,7 +574,6 @@ struct Launch {
     uint32_t group_mul;      // x / group = x * group_mul >> group_shift for x < 2^31
     int group_shift;
     int min_rows, max_rows;  // requests with rows (tokens x group) in (min_rows, max_rows]
-    int min_units;       // of a workgroup's range
 };
 
 // An item is EXTRA units, what its start and end cost, and then a unit for each
@@ -718,7 +717,7 @@ __device__ __forceinline__ int64_t find_range(W& walk, int w, int nw, int64_t* s
         incl += before;
     }
     all = uniform(all);
-    *per = max(quotient(all + nw - 1, nw), static_cast<int64_t>(walk.la.min_units));
+    *per = max(quotient(all + nw - 1, nw), int64_t{1});
     const int64_t u = w * *per;
     if (u >= all) return 0;
     const bool here = u < incl && u >= incl - mine;
@@ -767,7 +766,8 @@ __device__ __forceinline__ int64_t find_range(W& walk, int w, int nw, int64_t* s
 // many-row form: a lane's values, maximum and sum, two lanes to a row.
 constexpr int part_floats(int bm, int hd) { return bm * hd + 2 * bm; }
 constexpr int wide_part_floats(int bm, int hd) { return bm * hd + 4 * bm; }
-// Tiles of K, and of V, that the many-row form keeps in LDS.
+// Tiles of K, and of V, that the many-row form keeps in LDS: three where they
+// fit, so that copies run a step further ahead.
 constexpr int wide_slots(int tile_bytes) { return 6 * tile_bytes <= 147456 ? 3 : 2; }
 
 // The store of four values of a row (zeros where its sum of weights is 0).
@@ -966,20 +966,26 @@ __global__ __launch_bounds__(256, RBLK == 1 || HD < 256 ? 2 : 1) void k_paged_na
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     uint8_t* const ring = lds + wave * kRing;
     const int nw = gridDim.x, w = place_of(blockIdx.x, nw);
-    Walk<BM, BN, 0> walk(p, la);
+    // Tiles that take as long as an item's start and end, 6 us.  (0: 47 us where 2
+    // takes 36 for 128 requests of 50 to 2000 keys, 380 where it takes 331 for 200
+    // of up to 4000 at head_dim 256, 12 where it takes 14 for 16 of up to 900.)
+    constexpr int EXTRA = 2;
+    Walk<BM, BN, EXTRA> walk(p, la);
     int64_t skip = 0, per = 0;
     int64_t left = find_range<256>(walk, w, nw, &skip, &per);
-    int64_t item_at = w * per - skip;  // of the item's first tile in the sequence
+    int64_t item_at = w * per - skip + EXTRA;  // of the item's first tile in the sequence
     const uint32_t ring_at = uniform(static_cast<int>(lds_address(ring)));
     const float c1 = p.scale * kLog2e;
     C core;
     core.setup();
     while ((left = uniform(left)) > 0) {
         walk.pin();
-        const int a = uniform(static_cast<int>(skip));
-        const int b = uniform(static_cast<int>(min(static_cast<int64_t>(walk.tiles), skip + left)));
+        const int from = uniform(static_cast<int>(skip));
+        const int to = uniform(static_cast<int>(min(static_cast<int64_t>(walk.tiles + EXTRA), skip + left)));
         skip = 0;
-        left -= b - a;
+        left -= to - from;
+        const int a = max(from - EXTRA, 0), b = max(to - EXTRA, 0);  // tiles
+        if (a >= b) break;  // (the range ends before the item's first tile)
         int lo, hi;
         walk.span(walk.blk, &lo, &hi);
         const int rows = min(BM, walk.rows() - walk.blk * BM), row_first = walk.blk * BM;
@@ -1111,7 +1117,7 @@ __global__ __launch_bounds__(256, RBLK == 1 || HD < 256 ? 2 : 1) void k_paged_na
                 join_parts<Q, BM, HD, 256>(walk, first_wg, last_wg, rows, reinterpret_cast<State*>(lds));
         }
         __syncthreads();  // the rings are free again
-        item_at += walk.tiles;
+        item_at += walk.tiles + EXTRA;
         if (left > 0 && !walk.next()) break;
     }
 }
@@ -1136,7 +1142,9 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
     __shared__ int flag;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int nw = gridDim.x, w = place_of(blockIdx.x, nw);
-    // tiles that take as long as an item's start and end (5 us)
+    // Tiles that take as long as an item's start and end, 5 us.  (35 requests, a
+    // few of them chunks of 900, head_dim 64 in bf16: 157 us with 0, 118 with 6,
+    // 126 with 12; one chunk of 517 in f32: 120 with 1, 129 with 12.)
     constexpr int EXTRA = KindOf<T>::f32 ? 1 : (sizeof(Q) == 4 || HD == 256 ? 3 : 6);
     Walk<BM, BN, EXTRA> walk(p, la);
     int64_t skip = 0, per = 0;
@@ -1335,7 +1343,11 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
     }
 }
 
-// Rows (tokens x group) of a request up to which its keys are split over the waves.
+// Rows (tokens x group) of a request up to which its keys are split over the
+// waves.  24 requests of 1500 to 5000 keys at head_dim 128, bf16, few-row form
+// against many-row form: 16 rows 64 us; 32 rows 75 and 100; 48 rows 114 and 97;
+// 64 rows 118 and 99.  (At head_dim 64 the two meet at 64 rows, with f32 rows
+// over a bf16 cache at 40.)
 constexpr int kNarrowRows = 32;
 // Waves of 32 rows: two to a SIMD where the accumulator and q fit 256 registers.
 template <class Q>
@@ -1345,7 +1357,8 @@ constexpr int wide_waves(int hd) {
 
 int slots() { return static_cast<int>(device_info().cus); }
 
-// Workgroups of the narrow form: those the CUs hold at once.
+// Workgroups of the narrow form: those the CUs hold at once.  (With one to a CU
+// 64 decoding requests take 166 us instead of 157, a mixed step 127 instead of 118.)
 int narrow_slots(int hd) { return slots() * (hd == 256 ? 1 : 2); }
 
 // The most rows a request can have.
@@ -1367,18 +1380,18 @@ hipError_t run(const PagedAttn& p, float* part, uint32_t* counters, hipStream_t 
     la.group_mul = static_cast<uint32_t>(((uint64_t{1} << la.group_shift) + la.group - 1) / la.group);
     const int64_t rows = most_rows(p);
     const bool wide = rows > kNarrowRows, narrow = !wide || p.n_seq > 1;
+    // (one workgroup to a CU, LDS holds no more; ranges of a single tile are worth
+    // it: with 8 at least, 64 tokens over 500 keys took 65 us in f32 instead of 37)
     const unsigned grid = static_cast<unsigned>(slots());
     if (wide) {
         constexpr int BK = KindOf<T>::f32 ? 32 : 64;
         la.min_rows = narrow ? kNarrowRows : 0;
         la.max_rows = 0x7fffffff;
-        la.min_units = 8;
         hipLaunchKernelGGL((k_paged_wide<Q, T, HD, NW>), dim3(grid), dim3(NW * 64), 2 * wide_slots(BK * HD * sizeof(T)) * BK * HD * sizeof(T), s, p, la);
     }
     if (narrow) {
         la.min_rows = 0;
         la.max_rows = wide ? kNarrowRows : 0x7fffffff;
-        la.min_units = 1;
         const unsigned many = static_cast<unsigned>(narrow_slots(HD));
         if (rows <= 16) hipLaunchKernelGGL((k_paged_narrow<Q, T, HD, 1>), dim3(many), dim3(256), 4 * narrow_ring(HD), s, p, la);
         else hipLaunchKernelGGL((k_paged_narrow<Q, T, HD, 2>), dim3(many), dim3(256), 4 * narrow_ring(HD), s, p, la);
