@@ -951,7 +951,7 @@ constexpr int narrow_ring(int hd) { return hd == 256 ? 32768 : 16384; }
 // streams tiles of its own through its own LDS ring, no barrier between them,
 // and the four waves' states are joined at the item's end.
 template <class Q, class T, int HD, int RBLK>
-__global__ __launch_bounds__(256, RBLK == 1 || HD < 256 ? 2 : 1) void k_paged_narrow(PagedAttn p, Launch la) {
+__global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_narrow(PagedAttn p, Launch la) {
     constexpr int NW = 4, DB = 16, BM = DB * RBLK, BK = KindOf<T>::f32 ? 16 : 32, BN = NW * BK;
     using C = Core<Q, T, HD, DB, RBLK, BK>;
     constexpr int kRing = narrow_ring(HD);  // bytes of a wave's ring
@@ -1355,6 +1355,15 @@ constexpr int wide_waves(int hd) {
     return sizeof(Q) == 4 || hd == 256 ? 4 : 8;
 }
 
+// Blocks of 16 rows that a wave of the few-row form takes together where there
+// are more than one: two, but for f32 rows over bf16, whose three limbs of two
+// blocks do not fit the registers (24 requests of 32 rows, head_dim 128: 116 us
+// with two, 102 with one, keys and values read twice; 294 and 205 at 256).
+template <class Q, class T>
+constexpr int narrow_blocks(int hd) {
+    return hd > 64 && sizeof(Q) == 4 && !KindOf<T>::f32 && !KindOf<T>::f16 ? 1 : 2;
+}
+
 int slots() { return static_cast<int>(device_info().cus); }
 
 // Workgroups of the narrow form: those the CUs hold at once.  (With one to a CU
@@ -1393,8 +1402,8 @@ hipError_t run(const PagedAttn& p, float* part, uint32_t* counters, hipStream_t 
         la.min_rows = 0;
         la.max_rows = wide ? kNarrowRows : 0x7fffffff;
         const unsigned many = static_cast<unsigned>(narrow_slots(HD));
-        if (rows <= 16) hipLaunchKernelGGL((k_paged_narrow<Q, T, HD, 1>), dim3(many), dim3(256), 4 * narrow_ring(HD), s, p, la);
-        else hipLaunchKernelGGL((k_paged_narrow<Q, T, HD, 2>), dim3(many), dim3(256), 4 * narrow_ring(HD), s, p, la);
+        const auto kernel = rows <= 16 ? k_paged_narrow<Q, T, HD, 1> : k_paged_narrow<Q, T, HD, narrow_blocks<Q, T>(HD)>;
+        hipLaunchKernelGGL(kernel, dim3(many), dim3(256), 4 * narrow_ring(HD), s, p, la);
     }
     return hipGetLastError();
 }
