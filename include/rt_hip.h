@@ -723,10 +723,11 @@ int rt_hip_paged_append(const rt_hip_paged_kv* kv, const void* k, const void* v,
  * dtype is q's and out's: the cache's (F16 or BF16: products of 16-bit values
  * summed in f32, the softmax in f32 and its weights rounded to the type before
  * they multiply v), or F32 with any cache (products and sums to f32
- * accuracy).  An infinity or a NaN in a row's q, or in a key that it sees,
- * leaves that row's head undefined, and no other; in values, what is not finite
- * reaches the rows that see it as a sum would have it.  n_q_heads is any
- * multiple of n_kv_heads up to 1024, scale > 0.  Results are deterministic.
+ * accuracy).  An infinity or a NaN (or 2^127 and more) in a row's q, or in a
+ * key that it sees, leaves that row's head undefined, and no other; in values,
+ * what is not finite reaches the rows that see it as a sum would have it.
+ * n_q_heads is any multiple of n_kv_heads up to 1024, scale > 0.  Results are
+ * deterministic.
  * max_fresh is a hint, the most rows a request of this step may have (0: not
  * known); the result does not depend on it beyond rounding.
  * Uses the library workspace (rt_hip_paged_attention_workspace_bytes, to
