@@ -686,9 +686,10 @@ __device__ __forceinline__ int64_t find_range(W& walk, int w, int nw, int64_t* s
     __shared__ int64_t found_before;
     const bool small = n_seq <= 64;
     const int each = small ? 1 : (n_seq + NT - 1) / NT, base = small ? lane : tid * each;
-    // units of this lane's i-th request
+    W scan(walk.p, walk.la);  // at the lane's request
+    // units of this lane's i-th request, for one KV head
     auto units_of = [&](int i) -> int64_t {
-        W scan(walk.p, walk.la);
+        scan.n = scan.blocks = 0;
         if (base + i < n_seq) scan.request(base + i);
         int64_t t = scan.blocks <= 2 ? scan.total() : 0;
         for (uint64_t many = __builtin_amdgcn_ballot_w64(scan.blocks > 2); many; many &= many - 1) {
@@ -700,10 +701,13 @@ __device__ __forceinline__ int64_t find_range(W& walk, int w, int nw, int64_t* s
             const int64_t sum = wave_total(one);
             if (lane == src) t = sum;
         }
-        return t * n_kv;
+        return t;
     };
-    int64_t mine = 0;
-    for (int i = 0; i < each; ++i) mine += units_of(i);
+    int64_t mine = 0, last = 0;
+    for (int i = 0; i < each; ++i) {
+        last = units_of(i);
+        mine += last * n_kv;
+    }
     int64_t incl = running_sum(mine);
     int64_t all = of_lane(incl, 63);
     if (!small) {
@@ -723,15 +727,19 @@ __device__ __forceinline__ int64_t find_range(W& walk, int w, int nw, int64_t* s
     const int64_t u = w * *per;
     if (u >= all) return 0;
     const bool here = u < incl && u >= incl - mine;
-    int s;
-    int64_t at = incl - mine;  // units before the request
+    int64_t at = incl - mine, t;  // units before the request, and of it for one KV head
     if (small) {
-        s = __builtin_ctzll(__builtin_amdgcn_ballot_w64(here));
+        // (the lane has the request: it is not read again)
+        const int s = __builtin_ctzll(__builtin_amdgcn_ballot_w64(here));
         at = of_lane(at, s);
+        t = of_lane(last, s);
+        walk.s = s;
+        walk.row0 = of_lane(scan.row0, s), walk.n = of_lane(scan.n, s);
+        walk.len = of_lane(scan.len, s), walk.blocks = of_lane(scan.blocks, s);
     } else {
         if (__builtin_amdgcn_ballot_w64(here) != 0) {  // (whole waves, as units_of counts)
             for (int i = 0; i < each; ++i) {
-                const int64_t t = units_of(i);
+                const int64_t t = units_of(i) * n_kv;
                 if (here && u >= at && u < at + t) {
                     found_s = base + i;
                     found_before = at;
@@ -740,15 +748,15 @@ __device__ __forceinline__ int64_t find_range(W& walk, int w, int nw, int64_t* s
             }
         }
         __syncthreads();
-        s = found_s;
-        at = found_before;
+        walk.request(uniform(found_s));
+        at = uniform(found_before);
+        t = wave_total(walk);
     }
-    walk.request(uniform(s));
-    int64_t off = u - uniform(at);
-    const int64_t t = wave_total(walk);
+    int64_t off = u - at;
     walk.kvh = static_cast<int>(quotient(off, t));
     off -= walk.kvh * t;
-    for (int b0 = 0;; b0 += 64) {
+    if (walk.blocks == 1) walk.block(0);
+    else for (int b0 = 0;; b0 += 64) {
         const int c = b0 + lane < walk.blocks ? walk.units(b0 + lane) : 0;
         const int64_t sum = running_sum(static_cast<int64_t>(c));
         const uint64_t behind = __builtin_amdgcn_ballot_w64(off < sum);
