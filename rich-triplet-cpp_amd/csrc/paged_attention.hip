@@ -1163,10 +1163,11 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
     __shared__ int flag;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int nw = gridDim.x, w = place_of(blockIdx.x, nw);
-    // Tiles that take as long as an item's start and end, 5 us.  (35 requests, a
-    // few of them chunks of 900, head_dim 64 in bf16: 157 us with 0, 118 with 6,
-    // 126 with 12; one chunk of 517 in f32: 120 with 1, 129 with 12.)
-    constexpr int EXTRA = KindOf<T>::f32 ? 1 : (sizeof(Q) == 4 || HD == 256 ? 3 : 6);
+    // Tiles that take as long as an item's start and end, 5 us.  (35 requests, three
+    // of them chunks of 800 to 900, head_dim 64 in bf16: 157 us with 0, 118 with
+    // 6, 126 with 12; in f32 over f16, eight waves, 182 with 1, 144 with 6; one
+    // chunk of 517 in f32, four waves: 120 with 1, 129 with 12.)
+    constexpr int EXTRA = KindOf<T>::f32 ? (NW == 8 ? 3 : 1) : (NW == 8 ? 6 : 3);
     Walk<BM, BN, EXTRA> walk(p, la);
     int64_t skip = 0, per = 0;
     int64_t left = find_range<NT>(walk, w, nw, &skip, &per);
@@ -1370,10 +1371,12 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
 // 64 rows 118 and 99.  (At head_dim 64 the two meet at 64 rows, with f32 rows
 // over a bf16 cache at 40.)
 constexpr int kNarrowRows = 32;
-// Waves of 32 rows: two to a SIMD where the accumulator and q fit 256 registers.
-template <class Q>
-constexpr int wide_waves(int hd) {
-    return sizeof(Q) == 4 || hd == 256 ? 4 : 8;
+// Whether eight waves of 32 rows, two to a SIMD, have registers enough.  (Three
+// limbs of q at head_dim 128 have not: 2048 tokens over 4000 keys take 367 us with
+// eight, 372 with four, 64 over 500 45 and 28.)
+template <class Q, class T>
+constexpr bool eight_fit(int hd) {
+    return hd == 64 || (hd == 128 && !(sizeof(Q) == 4 && !KindOf<T>::f32 && !KindOf<T>::f16));
 }
 
 // Blocks of 16 rows that a wave of the few-row form takes together where there
@@ -1397,9 +1400,26 @@ int64_t most_rows(const PagedAttn& p) {
     return static_cast<int64_t>(fresh) * (p.n_q / p.kv.n_kv);
 }
 
+// Whether the many-row form takes blocks of 256 rows, eight waves, or of 128,
+// four: where a request's rows fill more than one of the smaller, and all rows
+// together are 40 to a CU (80 with an f32 cache), so that keys are read fewer
+// times and one wave of a SIMD can work while the other waits.  Four and eight
+// waves, us, head_dim 128, 24 heads, 3 to a KV head:
+//   tokens over keys      bf16        f32 over f16   f32
+//   64 over 500           25    31    27    36       36    56
+//   256 over 1000         27    37    32    42       63    72
+//   512 over 9000        108    86   150   131      509   478
+//   1024 over 3000        88    70   119   108      397   374
+//   2048 over 4000       209   148   296   241     1080   999
+// 40 requests, 32 heads, 4 to a KV head: of 30 tokens (120 rows) 47 and 53, of
+// 100 (400 rows) 164 and 115.
+bool enough_rows(const PagedAttn& p, int64_t rows) {
+    const int64_t each = p.kv.dtype == RT_HIP_F32 ? 80 : 40;
+    return rows > 128 && static_cast<int64_t>(p.n_tokens) * p.n_q >= slots() * each;
+}
+
 template <class Q, class T, int HD>
 hipError_t run(const PagedAttn& p, float* part, uint32_t* counters, hipStream_t s) {
-    constexpr int NW = wide_waves<Q>(HD);
     Launch la;
     la.part = part;
     la.counters = counters;
@@ -1414,10 +1434,13 @@ hipError_t run(const PagedAttn& p, float* part, uint32_t* counters, hipStream_t 
     // it: with 8 at least, 64 tokens over 500 keys took 65 us in f32 instead of 37)
     const unsigned grid = static_cast<unsigned>(slots());
     if (wide) {
-        constexpr int BK = KindOf<T>::f32 ? 32 : 64;
+        constexpr int BK = KindOf<T>::f32 ? 32 : 64, LDS = 2 * wide_slots(BK * HD * sizeof(T)) * BK * HD * sizeof(T);
+        constexpr int MOST = eight_fit<Q, T>(HD) ? 8 : 4;
         la.min_rows = narrow ? kNarrowRows : 0;
         la.max_rows = 0x7fffffff;
-        hipLaunchKernelGGL((k_paged_wide<Q, T, HD, NW>), dim3(grid), dim3(NW * 64), 2 * wide_slots(BK * HD * sizeof(T)) * BK * HD * sizeof(T), s, p, la);
+        const bool eight = MOST == 8 && enough_rows(p, rows);
+        hipLaunchKernelGGL((eight ? k_paged_wide<Q, T, HD, MOST> : k_paged_wide<Q, T, HD, 4>), dim3(grid),
+                           dim3(eight ? 512 : 256), LDS, s, p, la);
     }
     if (narrow) {
         la.min_rows = 0;
@@ -1442,8 +1465,7 @@ hipError_t run_hd(const PagedAttn& p, float* part, uint32_t* counters, hipStream
 
 size_t paged_attention_workspace(const PagedAttn& p) {
     const int64_t rows = most_rows(p);
-    const int waves = p.dtype == RT_HIP_F32 ? wide_waves<float>(p.kv.head_dim) : wide_waves<__bf16>(p.kv.head_dim);
-    const int hd = p.kv.head_dim;
+    const int hd = p.kv.head_dim, waves = hd < 256 ? 8 : 4;
     const size_t narrow = static_cast<size_t>(narrow_slots(hd)) * 2 * part_floats(rows <= 16 ? 16 : 32, hd);
     const size_t wide = rows > kNarrowRows ? static_cast<size_t>(slots()) * 2 * wide_part_floats(waves * 32, hd) : 0;
     return (narrow > wide ? narrow : wide) * sizeof(float);
