@@ -180,6 +180,46 @@ def test_chunks_among_many_requests(rt, q, kv, window):
 
 
 @pytest.mark.parametrize("q, kv", PAIRS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("window", [0, 300])
+def test_rows_that_fill_the_card(rt, q, kv, dim, window):
+    """Rows enough for the largest blocks, beside requests that have few."""
+    say("full", q, kv, dim, window)
+    Step(q, kv, 24, 8, dim, 16, [(900, 1500), (60, 700), (1, 500), (0, 4), (3, 2)], seed=dim, window=window).check(rt)
+
+
+@pytest.mark.parametrize("q, kv", PAIRS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_what_rows_of_full_blocks_do_not_see(rt, q, kv, dim, bad):
+    """As below, with rows enough for the largest blocks; the same bits in every run, captured ones among them."""
+    say("unseen full", q, kv, dim, bad)
+    for n, length, window, at in ((450, 900, 0, 611), (440, 440, 120, 130)):
+        st = Step(q, kv, 48, 2, dim, 16, [(n, length)], seed=5, window=window)
+        pos = torch.arange(length - n, length, device="cuda")
+        sees = (pos >= at) & ((pos < at + window) if window else True)
+        page = st.table[0, at // 16]
+        st.check(rt)
+        clean = st.run(rt).clone()
+        st.v[page, at % 16, 0, 3:dim:7] = bad
+        got = st.run(rt).clone()
+        # (the key's weight is 0 in those rows, so its products are zeros both times)
+        assert torch.equal(got[~sees], clean[~sees])
+        assert not torch.isfinite(got[sees][:, :24, 3:dim:7]).any() and torch.isfinite(got[sees][:, :24, 4:dim:7]).all()
+        assert torch.isfinite(got[:, 24:]).all()
+        starts, lens, out = i32(st.starts), i32([length]), torch.zeros_like(st.out)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            rt.paged_attention(st.q, st.kv, st.table, starts, lens, st.scale, window=window, out=out)
+        for _ in range(3):
+            out.zero_()
+            graph.replay()
+            assert torch.equal(st.run(rt).nan_to_num(7.0), got.nan_to_num(7.0))
+            assert torch.equal(out.nan_to_num(7.0), got.nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("q, kv", PAIRS)
 def test_many_requests(rt, q, kv):
     """More requests than a workgroup has threads."""
     say("many", q, kv)
