@@ -962,8 +962,8 @@ constexpr int narrow_ring(int hd) { return hd == 256 ? 32768 : 16384; }
 // and the four waves' states are joined at the item's end.
 // 64 requests of 100 to 16000 keys, 8 KV heads of 128 in bf16: 152 us for 782 MB
 // (5.1 TB/s; a plain read of as much reaches 5.9).  16 requests of 5 tokens, a
-// window of 1024, head_dim 256: 24 us for 48 MB.  One token over 777 keys: 11.8
-// us, of which the range takes 2.5, pages, keys and q 2, the products 1.4, the
+// window of 1024, head_dim 256: 24 us for 48 MB.  One token over 777 keys: 11.3
+// us, of which the range takes 2, pages, keys and q 2, the products 1.4, the
 // states and their join 2.
 template <class Q, class T, int HD, int RBLK>
 __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_narrow(PagedAttn p, Launch la) {
@@ -1139,12 +1139,13 @@ __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_narrow(PagedAtt
 
 // ---- many rows: the waves split the rows -------------------------------------------
 // Chunks of prompts, bound by the matrix cores: every wave has 32 rows of its
-// own, and K and V tiles are read from memory once for all of them.
+// own, and K and V tiles are read from memory once for all of them.  Four waves
+// or eight: enough_rows.
 // 4096 tokens over 8192 keys before them, 24 heads of 128 in bf16: 500 to 540 us,
 // 960 to 1030 TFLOP/s, at the clock that the power limit leaves (a library
 // product of 8192^3: 1212).  900-token chunks of head_dim 64: 99 us for 43 GFLOP,
 // there the exponentials and conversions take as long as the products.  517
-// tokens over 1100 keys in f32: 122 us, 72 TFLOP/s, the matrix cores busy for two
+// tokens over 1100 keys in f32: 121 us, 71 TFLOP/s, the matrix cores busy for two
 // thirds of it.
 template <class Q, class T, int HD, int NW>
 __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) {
