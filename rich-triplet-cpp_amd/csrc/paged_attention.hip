@@ -359,9 +359,7 @@ struct Core {
     // Weights in place of the scores; the running state moved to a new maximum
     // where one grew by more than 2^kLag.  key: the tile's first; edge: some
     // row does not see some of its keys.
-    // halfway(): called between the maximum and the weights.
-    template <class F>
-    __device__ __forceinline__ void softmax(int key, bool edge, F halfway) {
+    __device__ __forceinline__ void softmax(int key, bool edge) {
 #pragma unroll
         for (int b = 0; b < RBLK; ++b) {
             if (edge) {
@@ -392,7 +390,6 @@ struct Core {
                 for (int i = 0; i < NC; ++i) o[b][i] *= a;
             }
             const float base = static_cast<float>(kBias) - (m[b] == -kInf ? 0.0f : m[b]) * c[b];
-            if (b == 0) halfway();
             float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int j = 0; j < KB; ++j)
@@ -1062,7 +1059,7 @@ __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_narrow(PagedAtt
             core.scores(ring_at + (i % D) * C::TB);
             wait_lds();
             if (more) copy_k(i + D, g);
-            core.softmax(key, edge, [] {});
+            core.softmax(key, edge);
             if (more) wait_copies<(2 * D - 1) * H>();
             else wait_copies<0>();
             const uint32_t v = ring_at + (D + i % D) * C::TB;
@@ -1298,7 +1295,7 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
                 if (kTwo) lds_barrier();
                 // (behind the last tile: keys that no row sees, which change nothing)
                 const int key = i < nt ? key0 + i * BN : 0x40000000;
-                core.softmax(key, key + BK - 1 > wave_low || (p.window && key <= wave_hi - p.window), [] {});
+                core.softmax(key, key + BK - 1 > wave_low || (p.window && key <= wave_hi - p.window));
                 advance();
                 if (!second && i < nt) settle(i, now);
                 lds_barrier();
