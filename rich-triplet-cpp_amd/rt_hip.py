@@ -694,7 +694,7 @@ def _want(device: int, *args) -> None:
         have = t.shape
         if have != shape and (len(have) != len(shape) or any(n is not None and a != n for a, n in zip(have, shape))):
             raise ValueError(f"rt_hip: {name} must have shape {tuple(shape)}, not {tuple(have)}")
-        if t.get_device() != device:
+        if device < 0 or t.get_device() != device:  # (a device below 0: that of CPU tensors)
             raise ValueError(f"rt_hip: {name} must live on the GPU of the others" if t.is_cuda else
                              "rt_hip: tensors must live on the GPU")
         if not t.is_contiguous():

@@ -147,3 +147,25 @@ def test_binding_checks_before_it_calls(rt):
         rt.paged_plan(torch.zeros(2), torch.zeros(2), torch.zeros(2), None, None, None, 16, 4)
     with pytest.raises(ValueError, match="GPU"):
         rt.verify_drafts(torch.zeros(3, 9), None, None, None, torch.zeros(1), 1)
+
+
+@pytest.fixture
+def no_library(rt, monkeypatch):
+    """The binding with a library that is never to be called."""
+    class Never:
+        def call(self, name, *args):
+            raise AssertionError(f"{name} was called")
+    monkeypatch.setattr(rt, "library", lambda: Never())
+    return rt
+
+
+@pytest.mark.parametrize("n, tokens", [(2, 4), (0, 3), (1, 0)])
+@pytest.mark.parametrize("given", [False, True])
+def test_plan_refuses_cpu_tensors(no_library, n, tokens, given):
+    """Tensors of the right types and shapes, all of them on the CPU: none of their addresses reaches the kernel."""
+    import torch
+    rt = no_library
+    z = lambda *shape: torch.zeros(shape, dtype=torch.int32)
+    plan = rt.PagedPlan(n, tokens, "cpu") if given else None
+    with pytest.raises(ValueError, match="GPU"):
+        rt.paged_plan(z(n), z(n), z(n), z(n, 3), z(8), z(2), 16, tokens, plan=plan)
