@@ -729,8 +729,8 @@ def _call_on(device: int, name: str, stream, *args) -> None:
 
 class PagedKV:
     """A KV cache in pages: k and v [n_pages, page_size, n_kv_heads, head_dim]
-    of float32, float16 or bfloat16; pages are dense, with any one stride
-    between them (two halves of one tensor, say)."""
+    of float32, float16 or bfloat16; pages are dense and do not overlap, with
+    any one stride between them (two halves of one tensor, say)."""
 
     def __init__(self, k, v):
         if not (k.is_cuda and v.is_cuda and k.device == v.device):
@@ -745,6 +745,8 @@ class PagedKV:
         stride = k.stride(0) if n_pages > 1 else page * heads * dim
         if n_pages > 1 and v.stride(0) != stride:
             raise ValueError("rt_hip: k and v must have one page stride")
+        if stride < page * heads * dim:  # (0 among them, which the call would take as dense)
+            raise ValueError("rt_hip: the pages of the cache overlap")
         self.k, self.v, self.device = k, v, k.get_device()
         self.struct = PagedKvStruct(k.data_ptr(), v.data_ptr(), _value_type(k), n_pages, page, heads, dim, stride)
         self.ref = C.byref(self.struct)

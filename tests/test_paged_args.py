@@ -169,3 +169,33 @@ def test_plan_refuses_cpu_tensors(no_library, n, tokens, given):
     plan = rt.PagedPlan(n, tokens, "cpu") if given else None
     with pytest.raises(ValueError, match="GPU"):
         rt.paged_plan(z(n), z(n), z(n), z(n, 3), z(8), z(2), 16, tokens, plan=plan)
+
+
+class OnGpu:
+    """A CPU tensor that says it lives on GPU 0."""
+    is_cuda = True
+
+    def __init__(self, t):
+        self.t = t
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+    def get_device(self):
+        return 0
+
+
+@pytest.mark.parametrize("pages", [2, 8])
+@pytest.mark.parametrize("stride", [0, 64, 1016])
+def test_cache_whose_pages_overlap(rt, pages, stride):
+    """Pages that share memory: one page expanded (a stride of 0, which is the C call's word for dense), or pages that
+    start inside the one before."""
+    import torch
+    k = OnGpu(torch.zeros(pages * 1024).as_strided((pages, 16, 1, 64), (stride, 64, 64, 1)))
+    with pytest.raises(ValueError, match="overlap"):
+        rt.PagedKV(k, k)
+    # one page has no next one, and pages further apart than dense are a layout like any other
+    one = OnGpu(torch.zeros(1024).as_strided((1, 16, 1, 64), (stride, 64, 64, 1)))
+    assert rt.PagedKV(one, one).struct.page_stride == 1024
+    far = OnGpu(torch.zeros(pages * 2048).as_strided((pages, 16, 1, 64), (2048, 64, 64, 1)))
+    assert rt.PagedKV(far, far).struct.page_stride == 2048
