@@ -7,6 +7,7 @@ a call fails, an exception is raised.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 import re
@@ -727,6 +728,16 @@ def _call_on(device: int, name: str, stream, *args) -> None:
                    torch._C._cuda_getCurrentRawStream(device))
 
 
+_HERE = contextlib.nullcontext()
+
+
+def _made_on(stream):
+    """Where a call's results are allocated, and filled: on the stream it runs on.
+    (On the current one a fill could come after the kernel, and memory that was
+    just given back there could still be in use.)"""
+    return _HERE if stream is None else _torch().cuda.stream(stream)
+
+
 class PagedKV:
     """A KV cache in pages: k and v [n_pages, page_size, n_kv_heads, head_dim]
     of float32, float16 or bfloat16; pages are dense and do not overlap, with
@@ -780,7 +791,8 @@ def paged_plan(cached, fresh, held, table, queue, queue_state, page_size: int, t
           (held, "held", i32, per_request), (table, "table", i32, (n, None)), (queue, "queue", i32, (None,)),
           (queue_state, "queue_state", i32, (2,)))
     if plan is None:
-        plan = PagedPlan(n, tokens, cached.device)
+        with _made_on(stream):
+            plan = PagedPlan(n, tokens, cached.device)
     else:
         _want(device, (plan.q_start, "q_start", i32, (n + 1,)), (plan.kv_len, "kv_len", i32, per_request),
               (plan.slots, "slots", i32, (tokens,)), (plan.positions, "positions", i32, (tokens,)),
@@ -816,7 +828,8 @@ def paged_attention(q, kv: PagedKV, table, q_start, kv_len, scale: float, window
     if q.dim() != 3:
         raise ValueError("rt_hip: q must have shape (rows, n_q_heads, head_dim)")
     if out is None:
-        out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+        with _made_on(stream):
+            out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
     if out.shape != q.shape or out.dtype is not q.dtype:
         raise ValueError("rt_hip: out must have q's shape and dtype")
     rows, heads, _ = q.shape
@@ -859,8 +872,9 @@ def verify_drafts(logits, tokens, row_start, accept_u, sample_u, max_draft: int,
     if temperature is not None:
         _want(device, (temperature, "temperature", f32, (n,)))
     if out is None:
-        out = (torch.empty((n, max_draft + 1), dtype=i32, device=logits.device),
-               torch.empty(n, dtype=i32, device=logits.device))
+        with _made_on(stream):
+            out = (torch.empty((n, max_draft + 1), dtype=i32, device=logits.device),
+                   torch.empty(n, dtype=i32, device=logits.device))
     else:
         _want(device, (out[0], "out tokens", i32, (n, max_draft + 1)), (out[1], "out count", i32, (n,)))
     _call_on(device, "rt_hip_verify_drafts", stream, logits.data_ptr(), strides[0], _ptr(draft_logits), strides[1],

@@ -318,6 +318,23 @@ def test_on_another_stream(rt, q, kv):
 
 
 @pytest.mark.parametrize("q, kv", PAIRS)
+@pytest.mark.parametrize("lens", [[(1, 900)], [(200, 900), (1, 70)]])
+def test_result_of_a_call_on_another_stream(rt, q, kv, lens):
+    """No out, another stream's call, the current stream busy: nothing of that stream touches the result."""
+    say("result on a stream", q, kv, lens)
+    st = Step(q, kv, 6, 2, 128, 16, lens, behind=2)
+    kvs, starts, keys = rt.PagedKV(st.k, st.v), i32(st.starts), i32([n for _, n in lens])
+    want = rt.paged_attention(st.q, kvs, st.table, starts, keys, st.scale)
+    busy, side = torch.zeros((64, 1 << 20), device="cuda"), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(40):
+        busy.add_(1.0)
+    got = rt.paged_attention(st.q, kvs, st.table, starts, keys, st.scale, stream=side)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and (got[-2:] == 0).all() and got.abs().max() > 0
+
+
+@pytest.mark.parametrize("q, kv", PAIRS)
 def test_captured(rt, q, kv):
     """A captured call, replayed over other lengths, starts and tables between eager work: eager's bits each time."""
     say("captured", q, kv)

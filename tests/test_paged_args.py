@@ -199,3 +199,68 @@ def test_cache_whose_pages_overlap(rt, pages, stride):
     assert rt.PagedKV(one, one).struct.page_stride == 1024
     far = OnGpu(torch.zeros(pages * 2048).as_strided((pages, 16, 1, 64), (2048, 64, 64, 1)))
     assert rt.PagedKV(far, far).struct.page_stride == 2048
+
+
+@pytest.fixture
+def streams(rt, monkeypatch):
+    """The binding over CPU tensors that say they live on GPU 0, with a torch that keeps a current stream; what was
+    allocated and what was called on which stream, in order, by name."""
+    import contextlib
+    import torch
+    seen, now = [], ["current"]
+
+    class Stream:
+        cuda_stream = "side"
+
+    class Cuda:
+        @staticmethod
+        @contextlib.contextmanager
+        def stream(s):
+            before, now[0] = now[0], s.cuda_stream
+            yield
+            now[0] = before
+
+    class Torch:
+        cuda = Cuda
+
+        class _C:
+            _cuda_getDevice = staticmethod(lambda: 0)
+            _cuda_getCurrentRawStream = staticmethod(lambda device: now[0])
+
+        def __getattr__(self, name):
+            return getattr(torch, name)
+
+        def _made(name):
+            def make(self, *args, **kw):
+                seen.append((name, now[0]))
+                return OnGpu(getattr(torch, name)(*args, **kw))
+            return make
+        empty, zeros, full = _made("empty"), _made("zeros"), _made("full")
+
+    class Lib:
+        def call(self, name, *args):
+            seen.append((name, args[-1]))
+
+    monkeypatch.setattr(rt, "_torch", lambda: Torch())
+    monkeypatch.setattr(rt, "library", lambda: Lib())
+    return Stream(), seen
+
+
+@pytest.mark.parametrize("side", [False, True])
+@pytest.mark.parametrize("what", ["plan", "attention", "verify"])
+def test_results_are_made_on_the_stream_of_the_call(rt, streams, side, what):
+    """What a call allocates, and fills, belongs to the stream it runs on: a fill of the current stream's could come
+    after the kernel, and memory that stream has just given back could still be in use there."""
+    import torch
+    stream, seen = streams
+    i32 = lambda *shape: OnGpu(torch.zeros(shape, dtype=torch.int32))
+    f32 = lambda *shape: OnGpu(torch.zeros(shape))
+    kw = dict(stream=stream) if side else {}
+    if what == "plan":
+        rt.paged_plan(i32(2), i32(2), i32(2), i32(2, 3), i32(8), i32(2), 16, 5, **kw)
+    elif what == "attention":
+        rt.paged_attention(f32(5, 2, 64), rt.PagedKV(f32(8, 16, 1, 64), f32(8, 16, 1, 64)), i32(2, 3), i32(3), i32(2), 0.1, **kw)
+    else:
+        rt.verify_drafts(f32(5, 9), i32(5), i32(3), f32(5), f32(2), 3, **kw)
+    assert len(seen) >= 2 and seen[-1][0].startswith("rt_hip_")
+    assert {on for _, on in seen} == {"side" if side else "current"}, seen
