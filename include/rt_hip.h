@@ -724,8 +724,9 @@ int rt_hip_paged_append(const rt_hip_paged_kv* kv, const void* k, const void* v,
  * summed in f32, the softmax in f32 and its weights rounded to the type before
  * they multiply v), or F32 with any cache (products and sums to f32
  * accuracy).  An infinity or a NaN (or 2^127 and more) in a row's q, or in a
- * key that it sees, leaves that row's head undefined, and no other; in values,
- * what is not finite reaches the rows that see it as a sum would have it.
+ * key that it sees, leaves that row's head undefined, and no other.  In values,
+ * what is not finite reaches every row that sees it, however small its weight:
+ * infinities of one sign as that infinity, others and NaN as NaN.
  * n_q_heads is any multiple of n_kv_heads up to 1024, scale > 0.  Results are
  * deterministic.
  * max_fresh is a hint, the most rows a request of this step may have (0: not

@@ -36,9 +36,16 @@
 //
 // Bounds and times: at each of the two kernels.
 //
-// Keys a row does not see get weight 0, but 0 times an infinity or a NaN of
-// their v would reach the row: in tiles with such pairs those values of v are
-// made 0 in LDS, and added at the end to the rows that see them.
+// Infinities and NaN in v.  Keys a row does not see get weight 0, but 0 times an
+// infinity or a NaN of their v would reach the row: in tiles with such pairs
+// those values of v are made 0 in LDS, and added at the end to the rows that see
+// them.  In the other tiles every row sees every key, but a product with a
+// weight that has vanished, or with a limb that is 0 or negative, would turn an
+// infinity into a NaN: a workgroup whose o has come out as something not finite
+// walks its tiles again and does the same in all of them.  So whatever the tile,
+// the limbs and the weight, such a value reaches the rows that see it as it is.
+// (To look costs 0.1 to 0.3 us an item; to clean every tile from the start would
+// cost each of them the reads and compares of all its values.)
 #include <utility>
 
 #include "rt_common.hpp"
@@ -559,6 +566,19 @@ struct Core {
             }
     }
 
+    // Whether some o of the wave's is an infinity or a NaN (0 times it is a NaN).
+    __device__ __forceinline__ bool not_finite() const {
+        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int b = 0; b < RBLK; ++b)
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+#pragma unroll
+                for (int e = 0; e < ACC; ++e) x[e & 3] = __builtin_fmaf(o[b][i][e], 0.0f, x[e & 3]);
+        const float any = (x[0] + x[1]) + (x[2] + x[3]);
+        return __builtin_amdgcn_ballot_w64(any != any) != 0;
+    }
+
     // Dim of register e of block i of o.
     __device__ __forceinline__ int dim_of(int i, int e) const { return i * DB + 8 * (e >> 2) + 4 * kg + (e & 3); }
 };
@@ -787,6 +807,11 @@ __device__ __forceinline__ void store_out(Q* dst, f32x4 o, float l) {
     else *reinterpret_cast<u32x2*>(dst) = u32x2{pack2<Q>(o[0], o[1]), pack2<Q>(o[2], o[3])};
 }
 
+// The weight of a state whose maximum lies x below the one it is joined under.
+// Never 0, so that an infinity in the state's o stays one; the 2^-126 that the
+// exponential would round to 0 change a sum by no more than that of its values.
+__device__ __forceinline__ float state_weight(float x) { return fmaxf(exp2_fast(x), 0x1p-126f); }
+
 // Four values of a row with the row's maximum (in powers of two) and sum.
 struct State {
     float m, l;
@@ -794,7 +819,7 @@ struct State {
 };
 __device__ __forceinline__ void join_state(State& a, const State& b) {
     const float m = fmaxf(a.m, b.m);
-    const float fa = m == -kInf ? 0.0f : exp2_fast(a.m - m), fb = m == -kInf ? 0.0f : exp2_fast(b.m - m);
+    const float fa = m == -kInf ? 0.0f : state_weight(a.m - m), fb = m == -kInf ? 0.0f : state_weight(b.m - m);
     a.l = a.l * fa + b.l * fb;
     a.o = a.o * fa + b.o * fb;
     a.m = m;
@@ -975,6 +1000,9 @@ __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_narrow(PagedAtt
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     __shared__ float sm[NW][BM], sl[NW][BM];
     __shared__ int flag;
+    __shared__ int dirty;  // the last of this workgroup's items whose o came out as something not finite
+    if (threadIdx.x == 0) dirty = -1;
+    int item = 0;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     uint8_t* const ring = lds + wave * kRing;
     const int nw = gridDim.x, w = place_of(blockIdx.x, nw);
@@ -990,6 +1018,7 @@ __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_narrow(PagedAtt
     const float c1 = p.scale * kLog2e;
     C core;
     core.setup();
+    bool all = false;  // the item once more, every tile of it as an edge tile
     while ((left = uniform(left)) > 0) {
         walk.pin();
         const int from = uniform(static_cast<int>(skip));
@@ -1002,7 +1031,8 @@ __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_narrow(PagedAtt
         walk.span(walk.blk, &lo, &hi);
         const int rows = min(BM, walk.rows() - walk.blk * BM), row_first = walk.blk * BM;
         const int pos0 = walk.len - walk.n;
-        const int low_pos = pos0 + walk.token(row_first);  // position of the block's first row
+        // position of the block's first row (below every key: all tiles are edge tiles)
+        const int low_pos = all ? -1 : pos0 + walk.token(row_first);
         const Pages pages = pages_of<T>(p, walk.s, walk.kvh, hi - 1);
         const int key0 = (walk.tile0 + a) * BN + wave * BK;
         int nt = b - a;
@@ -1107,10 +1137,11 @@ __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_narrow(PagedAtt
             f32x4 O = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int x = 0; x < NW; ++x) {
-                const float f = M == -kInf ? 1.0f : exp2_fast(sm[x][r] - M);
+                const float f = M == -kInf ? 1.0f : state_weight(sm[x][r] - M);
                 L += sl[x][r] * f;
                 O += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + x * kRing) + r * HD + (d ^ (4 * (r & 7)))) * f;
             }
+            if (const f32x4 z = O * 0.0f; (z[0] + z[1]) + (z[2] + z[3]) != 0.0f) dirty = item;
             if (!cut) {
                 const int row = row_first + r, t = walk.token(row);
                 store_out(static_cast<Q*>(p.out) + (walk.row0 + t) * p.out_stride +
@@ -1124,11 +1155,21 @@ __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_narrow(PagedAtt
                 }
             }
         }
+        if (!all) {
+            lds_barrier();
+            if (uniform(dirty) == item) {
+                all = true;
+                skip = from, left += to - from;
+                continue;
+            }
+        }
+        ++item;
         if (cut) {
             if (arrive(la.counters + first_wg, last_wg - first_wg + 1, &flag))
                 join_parts<Q, BM, HD, 256>(walk, first_wg, last_wg, rows, reinterpret_cast<State*>(lds));
         }
         __syncthreads();  // the rings are free again
+        all = false;
         item_at += walk.tiles + EXTRA;
         if (left > 0 && !walk.next()) break;
     }
@@ -1158,6 +1199,7 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];  // SLOTS tiles of K, SLOTS of V
     __shared__ int page_ring[NW][128];
     __shared__ int special;  // the last of this workgroup's items whose v held what was made 0
+    __shared__ int dirty;    // the last whose o came out as something not finite
     __shared__ int flag;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int nw = gridDim.x, w = place_of(blockIdx.x, nw);
@@ -1172,10 +1214,11 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
     int64_t item_at = w * per - skip + EXTRA;  // of the item's first tile in the sequence
     const uint32_t lds_at = uniform(static_cast<int>(lds_address(lds)));
     const float c1 = p.scale * kLog2e;
-    if (tid == 0) special = -1;
+    if (tid == 0) special = dirty = -1;
     int item = 0;
     C core;
     core.setup();
+    bool all = false;  // the item once more, every tile of it as an edge tile
     while ((left = uniform(left)) > 0) {
         walk.pin();
         const int from = uniform(static_cast<int>(skip));
@@ -1188,7 +1231,7 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
         walk.span(walk.blk, &lo, &hi);
         const int rows = min(BM, walk.rows() - walk.blk * BM), row_first = walk.blk * BM;
         const int pos0 = walk.len - walk.n;
-        const int low_pos = pos0 + walk.token(row_first);
+        const int low_pos = all ? -1 : pos0 + walk.token(row_first);  // (as above)
         const int r = wave * DB + core.n, row = row_first + r;
         const bool real = r < rows;
         const int t = walk.token(row);
@@ -1304,7 +1347,7 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
             if (kTwo && !second) lds_barrier();
             wait_copies<0>();
         }
-        if (uniform(special) == item++) {
+        if (uniform(special) == item) {
             for (int i = 0; i < nt; ++i)
                 if (const int key = key0 + i * BN; is_edge(key))
                     for (int j = key; j < min(key + BK, hi); ++j)
@@ -1313,9 +1356,9 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
         float l = C::across_sum(core.l[0]);
         const int first_wg = static_cast<int>(item_at / per), last_wg = static_cast<int>((item_at + walk.tiles - 1) / per);
         bool whole = first_wg == last_wg;
+        auto part = [&](int wg) { return la.part + (static_cast<int64_t>(wg) * 2 + (wg == first_wg)) * kPart + tid; };
         if (!whole) {
             // States as the registers are, a lane's values NT apart.
-            auto part = [&](int wg) { return la.part + (static_cast<int64_t>(wg) * 2 + (wg == first_wg)) * kPart + tid; };
             float* const mine = part(w);
 #pragma unroll
             for (int i = 0; i < C::NC; ++i)
@@ -1323,6 +1366,18 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
                 for (int e = 0; e < C::ACC; ++e) st_dev(mine + (i * C::ACC + e) * NT, core.o[0][i][e]);
             st_dev(mine + BM * HD, core.m[0] * core.c[0]);
             st_dev(mine + BM * HD + NT, l);
+        }
+        if (!all) {
+            if (core.not_finite()) dirty = item;
+            lds_barrier();
+            if (uniform(dirty) == item) {
+                all = true;
+                skip = from, left += to - from;
+                continue;
+            }
+        }
+        ++item;
+        if (!whole) {
             whole = arrive(la.counters + first_wg, last_wg - first_wg + 1, &flag);
             if (whole) {
                 float M = -kInf;
@@ -1338,7 +1393,7 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
                     for (int i = 0; i < C::NC * C::ACC; ++i) o[i] = ld_dev(src + i * NT);
                     __builtin_amdgcn_sched_barrier(0);
                     const float top = fmaxf(M, m);
-                    const float fa = top == -kInf ? 0.0f : exp2_fast(M - top), fb = top == -kInf ? 0.0f : exp2_fast(m - top);
+                    const float fa = top == -kInf ? 0.0f : state_weight(M - top), fb = top == -kInf ? 0.0f : state_weight(m - top);
                     l = l * fa + sum * fb;
 #pragma unroll
                     for (int i = 0; i < C::NC; ++i)
@@ -1358,6 +1413,7 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
                     store_out(dst + core.dim_of(i, 4 * e),
                               f32x4{core.o[0][i][4 * e], core.o[0][i][4 * e + 1], core.o[0][i][4 * e + 2], core.o[0][i][4 * e + 3]}, l);
         }
+        all = false;
         item_at += walk.tiles + EXTRA;
         if (left > 0 && !walk.next()) break;
     }

@@ -267,6 +267,41 @@ def test_what_a_row_does_not_see(rt, q, kv, dim, bad):
 
 
 @pytest.mark.parametrize("q, kv", PAIRS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("heads, lens, window, q_scale", [
+    (2, [(1, 3000)], 0, 1.0), (2, [(1, 3000)], 0, 12.0), (3, [(5, 700), (1, 90)], 0, 1.0), (1, [(2, 5000)], 3000, 1.0),
+    (2, [(60, 3000)], 0, 1.0), (2, [(60, 3000), (1, 17)], 0, 12.0), (48, [(440, 900)], 0, 1.0), (48, [(440, 900)], 300, 1.0)])
+def test_values_that_are_not_finite(rt, q, kv, dim, heads, lens, window, q_scale):
+    """Infinities of one sign, of both, and NaN in values, in keys that all rows of a request see, that some see, far
+    from the last and next to it, with weights of every size down to those that vanish in 32 bits: what reaches a row
+    is what the sum over the keys it sees has in 64 bits, to the sign."""
+    say("not finite", q, kv, dim, heads, lens, window, q_scale)
+    inf, nan = float("inf"), float("nan")
+    st = Step(q, kv, heads, 1, dim, 16, lens, seed=11, window=window, q_scale=q_scale)
+    n, length = lens[0]
+    places = [3, length // 3, length // 2, length - n - 70, length - n - 1, length - 1 - n // 2, length - 1]
+    pos = torch.arange(length - n, length, device="cuda")
+    special = torch.zeros((n, dim), dtype=torch.float64, device="cuda")
+    for i, at in enumerate(places):
+        v = st.v[st.table[0, at // 16], at % 16, 0]
+        v[2 * i + 1] = inf if i % 2 else -inf
+        v[20] = inf
+        v[22 + i % 2] = -inf if i % 4 < 2 else inf
+        if i == 2:
+            v[25] = nan
+        # (every key that a row sees has a weight above 0)
+        sees = (pos >= at) & ((pos < at + window) if window else True)
+        special[sees] += torch.where(torch.isfinite(v), 0.0, v.double())
+    got = st.run(rt).double()[:st.starts[-1]]
+    st.v.nan_to_num_(0.0, 0.0, 0.0)  # (what is left of the sum where none of those is seen)
+    want, tol = (x[:st.starts[-1]] for x in st.reference())
+    special = torch.cat([special, special.new_zeros((st.starts[-1] - n, dim))])[:, None].expand(want.shape)
+    assert torch.isnan(special).any() and (special == inf).any() and (special == -inf).any()
+    right = torch.where(special == 0, (got - want).abs() <= tol, (got == special) | (torch.isnan(got) & torch.isnan(special)))
+    assert right.all(), (int((~right).sum()), torch.nonzero(~right)[:4].tolist(), got[~right][:4].tolist(), special[~right][:4].tolist())
+
+
+@pytest.mark.parametrize("q, kv", PAIRS)
 def test_garbage_tables(rt, q, kv):
     """Pages that are none of the cache's count as zeros; starts and lengths that make no sense touch nothing else."""
     say("tables", q, kv)
