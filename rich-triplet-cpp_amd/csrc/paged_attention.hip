@@ -631,8 +631,11 @@ struct Walk {
     __device__ __forceinline__ void span(int b, int* lo, int* hi) const {
         const int i0 = token(b * BM), i1 = min(n - 1, token(b * BM + BM - 1));
         *hi = len - n + i1 + 1;
-        *lo = p.window ? max(0, len - n + i0 - p.window + 1) : 0;
+        *lo = first_seen(len - n + i0);
     }
+    // The first key that a row at position `at` (below 0: it sees none) sees.  (The
+    // longest windows reach further back than 32 bits from a position below 0.)
+    __device__ __forceinline__ int first_seen(int at) const { return p.window && at >= p.window ? at - p.window + 1 : 0; }
     __device__ __forceinline__ int count(int b, int* first) const {
         int lo, hi;
         span(b, &lo, &hi);
@@ -1069,13 +1072,13 @@ __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_narrow(PagedAtt
                                       (walk.kvh * walk.group + walk.head(row, t)) * HD
                                 : nullptr, c1);
             core.last[i] = real ? pos0 + t : -1;
-            core.first[i] = p.window ? core.last[i] - p.window + 1 : 0;
+            core.first[i] = walk.first_seen(core.last[i]);
         }
         // q is here: from now on only copies are in flight.  (The builtin, which the
         // compiler understands: it would wait for q's loads in every tile otherwise,
         // and with them for the copies.)
         wait_vmcnt<0>();
-        auto is_edge = [&](int key) { return key + BK - 1 > low_pos || (p.window && key <= hi - 1 - p.window); };
+        auto is_edge = [&](int key) { return key + BK - 1 > low_pos || (p.window && hi - 1 - key >= p.window); };
         bool special = false;
         for (int i = 0; i < nt; ++i) {
             const int key = key0 + i * BN;
@@ -1266,7 +1269,7 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
             C::template copy_rows<true>(g.k + g.v, g.row_bytes, g.most, group0 + x / PER, (part0 + x % PER) * C::RPI,
                                         lds_at + (SLOTS + slot) * C::TB + (wave * COPIES + x) * 1024);
         };
-        auto is_edge = [&](int key) { return key + BK - 1 > low_pos || (p.window && key <= hi - 1 - p.window); };
+        auto is_edge = [&](int key) { return key + BK - 1 > low_pos || (p.window && hi - 1 - key >= p.window); };
         int ahead = 0;  // the tile grp_k is of
         auto advance = [&] {
 #pragma unroll
@@ -1291,7 +1294,7 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
         }
         core.load_q(0, real ? static_cast<const Q*>(p.q) + (walk.row0 + t) * p.q_stride + head : nullptr, c1);
         core.last[0] = real ? pos0 + t : -1;
-        core.first[0] = p.window ? core.last[0] - p.window + 1 : 0;
+        core.first[0] = walk.first_seen(core.last[0]);
         wait_vmcnt<0>();  // (the builtin: so that the compiler, too, knows that q is there)
         lds_barrier();
         // Step i in two halves: the products, O += P V of tile i - 1 and the
@@ -1338,7 +1341,7 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
                 if (kTwo) lds_barrier();
                 // (behind the last tile: keys that no row sees, which change nothing)
                 const int key = i < nt ? key0 + i * BN : 0x40000000;
-                core.softmax(key, key + BK - 1 > wave_low || (p.window && key <= wave_hi - p.window));
+                core.softmax(key, key + BK - 1 > wave_low || (p.window && wave_hi - key >= p.window));
                 advance();
                 if (!second && i < nt) settle(i, now);
                 lds_barrier();

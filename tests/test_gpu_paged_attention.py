@@ -302,6 +302,21 @@ def test_values_that_are_not_finite(rt, q, kv, dim, heads, lens, window, q_scale
 
 
 @pytest.mark.parametrize("q, kv", PAIRS)
+@pytest.mark.parametrize("heads, dim, lens", [(1, 128, [(400, 395)]), (1, 64, [(9, 4), (120, 1), (300, 211)]),
+                                              (48, 128, [(440, 300)]), (4, 256, [(4, 3), (1, 0), (1, 7)]), (16, 64, [(2, 1)])])
+def test_windows_longer_than_any_request(rt, q, kv, heads, dim, lens):
+    """The longest windows there are hide nothing, also from the rows of requests that have fewer keys than rows."""
+    say("no window", q, kv, heads, dim, lens)
+    st = Step(q, kv, heads, 1, dim, 16, lens, seed=8, behind=1)
+    st.check(rt)
+    want = st.run(rt).clone()
+    for window in (2**31 - 1, 2**31 - 2, 2**31 - 200, 2**30, 1000):
+        st.window = window
+        st.out.fill_(-77.0)
+        assert torch.equal(st.run(rt), want), window
+
+
+@pytest.mark.parametrize("q, kv", PAIRS)
 def test_garbage_tables(rt, q, kv):
     """Pages that are none of the cache's count as zeros; starts and lengths that make no sense touch nothing else."""
     say("tables", q, kv)
