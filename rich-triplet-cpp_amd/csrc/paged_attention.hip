@@ -1339,9 +1339,9 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
                 if (i == 0) core.no_values();
                 if (second && i < nt) settle(i, now);
                 if (kTwo) lds_barrier();
-                // (behind the last tile: keys that no row sees, which change nothing)
-                const int key = i < nt ? key0 + i * BN : 0x40000000;
-                core.softmax(key, key + BK - 1 > wave_low || (p.window && wave_hi - key >= p.window));
+                // (behind the last tile: from hi on, keys that no row sees, which change nothing)
+                const int key = i < nt ? key0 + i * BN : hi;
+                core.softmax(key, i == nt || key + BK - 1 > wave_low || (p.window && wave_hi - key >= p.window));
                 advance();
                 if (!second && i < nt) settle(i, now);
                 lds_barrier();

@@ -411,6 +411,40 @@ def test_captured(rt, q, kv):
             assert torch.equal(out, eager)
 
 
+@pytest.mark.parametrize("q, kv", PAIRS)
+@pytest.mark.parametrize("rows", [40, 130])
+def test_positions_past_30_bits(rt, q, kv, rows):
+    """Chunks over 2^30 keys, all on one page but the last ones, whose weight is all there is: each row's result is the
+    value of its own last key, which counts once.  (Scores of 0 for a billion keys, 60 for those: exp(-60) 2^30 < 1e-16.)"""
+    say("far", q, kv, rows)
+    page, dim, length = 1024, 64, 2**30 + 1500
+    cols = -(-length // page)
+    k, v = (torch.zeros((4, page, 1, dim), device="cuda", dtype=DT[kv]) for _ in range(2))
+    v[0] = 100.0
+    at = torch.arange(length - rows, length, device="cuda")
+    table = torch.zeros((1, cols), dtype=torch.int32, device="cuda")
+    table[0, -3:] = i32([1, 2, 3])
+    place = (at - (cols - 3) * page)
+    own, last = 1 + place // page, place % page
+    # row i's key has its own two dims, and the row asks for them alone
+    values = torch.randn((rows, dim), device="cuda").to(DT[kv])
+    keys = torch.zeros((rows, dim), device="cuda")
+    asks = torch.zeros((rows, 1, dim), device="cuda")
+    for i in range(rows):
+        a, b = i % dim, (i // dim + i + 1) % dim
+        keys[i, a], keys[i, b] = 8.0, 8.0
+        asks[i, 0, a], asks[i, 0, b] = 60.0, 60.0
+    k[own, last, 0], v[own, last, 0] = keys.to(DT[kv]), values
+    out = rt.paged_attention(asks.to(DT[q]), rt.PagedKV(k, v), table, i32([0, rows]), i32([length]), 1 / 16)
+    # of the keys that a row sees, its own has the score 60, those that share a dim with it 30, the others 0
+    score = asks[:, 0].double() @ keys.double().T / 16
+    p = torch.exp(score.masked_fill_(at[None] > at[:, None], -math.inf) - 60)
+    want = (p @ values.double()) / p.sum(1, keepdim=True)
+    eps = torch.finfo(DT[q]).eps / 2 if q != "f32" else 2.0**-20
+    tol = 2 * eps * (p @ values.double().abs()) / p.sum(1, keepdim=True) + 2**30 * math.exp(-60) * 100
+    assert ((out[:, 0].double() - want).abs() <= tol).all(), (out[:, 0].double() - want).abs().max()
+
+
 def test_offsets_past_32_bits(rt):
     """A cache of more than 2^32 bytes, the request's pages at its end."""
     heads, dim, page = 8, 256, 128
