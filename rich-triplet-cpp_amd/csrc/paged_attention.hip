@@ -640,7 +640,7 @@ struct Walk {
         int lo, hi;
         span(b, &lo, &hi);
         *first = hi > lo ? lo / BN : 0;
-        return hi > lo ? (hi + BN - 1) / BN - *first : 1;  // (none visible: one tile, to write zeros)
+        return hi > lo ? (hi - 1) / BN + 1 - *first : 1;  // (none visible: one tile, to write zeros)
     }
     // Units of block b, and of the request for one KV head.
     __device__ __forceinline__ int units(int b) const {
@@ -906,8 +906,10 @@ struct Group {
     int most;            // the last key that may be read, from the group's first
 };
 // The group's place in the request: that of `key` (a multiple of 8), behind the
-// last key the one that holds it.
-__device__ __forceinline__ int group_at(const Pages& g, int key) { return min(key, g.end & ~7); }
+// last key the one that holds it.  (Tiles copied ahead may start past 2^31.)
+__device__ __forceinline__ int group_at(const Pages& g, uint32_t key) {
+    return static_cast<int>(min(key, static_cast<uint32_t>(g.end & ~7)));
+}
 // The group at `at` on page `id`.
 __device__ __forceinline__ Group group_on(const Pages& g, int at, int id) {
     const bool real = static_cast<uint32_t>(id) < static_cast<uint32_t>(g.n_pages);
@@ -920,7 +922,7 @@ __device__ __forceinline__ Group group_on(const Pages& g, int at, int id) {
     x.most = g.end - at;
     return x;
 }
-__device__ __forceinline__ Group group_of(const Pages& g, int key) {
+__device__ __forceinline__ Group group_of(const Pages& g, uint32_t key) {
     const int at = group_at(g, key);
     return group_on(g, at, g.table[at >> g.shift]);
 }
@@ -1110,8 +1112,8 @@ __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_narrow(PagedAtt
         if (special) {
             for (int i = 0; i < nt; ++i)
                 if (const int key = key0 + i * BN; is_edge(key))
-                    for (int j = key; j < min(key + BK, hi); ++j)
-                        core.add_special(j, value_of(pages, j));
+                    for (int j = 0; j < min(BK, hi - key); ++j)
+                        core.add_special(key + j, value_of(pages, key + j));
         }
         // The waves' states, joined in order.
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -1240,7 +1242,7 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
         const int t = walk.token(row);
         const int64_t head = (walk.kvh * walk.group + walk.head(row, t)) * HD;
         // the wave's rows see keys from wave_lo to wave_hi
-        const int wave_low = pos0 + walk.token(row_first + wave * DB);
+        const int wave_low = pos0 + walk.token(row_first + min(wave * DB, rows - 1));
         const int wave_hi = pos0 + walk.token(row_first + min(wave * DB + DB, rows) - 1);
         const Pages pages = pages_of<T>(p, walk.s, walk.kvh, hi - 1);
         const int key0 = (walk.tile0 + a) * BN;
@@ -1254,7 +1256,7 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
         auto find_groups = [&](int i) {
 #pragma unroll
             for (int x = 0; x < GROUPS; ++x) {
-                const int at = group_at(pages, key0 + i * BN + 8 * (group0 + x));
+                const int at = group_at(pages, static_cast<uint32_t>(key0) + i * BN + 8 * (group0 + x));
                 grp_k[x] = group_on(pages, at, window.at(pages, at >> pages.shift));
             }
         };
@@ -1353,8 +1355,8 @@ __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) 
         if (uniform(special) == item) {
             for (int i = 0; i < nt; ++i)
                 if (const int key = key0 + i * BN; is_edge(key))
-                    for (int j = key; j < min(key + BK, hi); ++j)
-                        core.add_special(j, value_of(pages, j));
+                    for (int j = 0; j < min(BK, hi - key); ++j)
+                        core.add_special(key + j, value_of(pages, key + j));
         }
         float l = C::across_sum(core.l[0]);
         const int first_wg = static_cast<int>(item_at / per), last_wg = static_cast<int>((item_at + walk.tiles - 1) / per);

@@ -445,6 +445,27 @@ def test_positions_past_30_bits(rt, q, kv, rows):
     assert ((out[:, 0].double() - want).abs() <= tol).all(), (out[:, 0].double() - want).abs().max()
 
 
+@pytest.mark.parametrize("q, kv", PAIRS)
+@pytest.mark.parametrize("rows, dim", [(1, 128), (5, 64), (30, 256), (40, 64), (130, 128), (70, 256)])
+def test_lengths_up_to_31_bits(rt, q, kv, rows, dim):
+    """The longest request that a table can hold, 2^31 - 8 keys: the bits of one whose keys are the last 632 of it (as
+    far into a tile), also where the length given is longer still."""
+    say("longest", q, kv, rows, dim)
+    page, near = 8, 632
+    cols = 2**28 - 1
+    k, v = torch.randn((2, near // page, page, 2, dim), device="cuda").to(DT[kv])
+    x = torch.randn((rows, 4, dim), device="cuda").to(DT[q])
+    ids = torch.randperm(near // page, device="cuda").to(torch.int32)
+    table = torch.full((1, cols), -1, dtype=torch.int32, device="cuda")
+    table[0, -(near // page):] = ids
+    kvs, starts = rt.PagedKV(k, v), i32([0, rows])
+    for window in (1, 300):
+        want = rt.paged_attention(x, kvs, ids[None].contiguous(), starts, i32([near]), 0.1, window=window)
+        assert want.abs().max() > 0
+        for length in (page * cols, 2**31 - 1):
+            assert torch.equal(rt.paged_attention(x, kvs, table, starts, i32([length]), 0.1, window=window), want)
+
+
 def test_offsets_past_32_bits(rt):
     """A cache of more than 2^32 bytes, the request's pages at its end."""
     heads, dim, page = 8, 256, 128
