@@ -133,18 +133,19 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
 
 // 16 bytes a lane from memory to LDS at dst + 16 lane.  (In assembly, without a
 // result: after the builtin the compiler waits for all such copies before it
-// reads anything transposed from LDS.  The kernels wait themselves.  M0 needs
+// reads anything transposed from LDS.  The kernels wait themselves.  M0 holds the
+// place in LDS, as an operand, so that the compiler knows who writes it; it needs
 // a wait state before the copy.)
 __device__ __forceinline__ void copy_to_lds(const uint8_t* src, uint32_t offset, uint32_t dst) {
     src = reinterpret_cast<const uint8_t*>(uniform(static_cast<int64_t>(reinterpret_cast<uintptr_t>(src))));
     dst = static_cast<uint32_t>(uniform(static_cast<int>(dst)));
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(offset), "s"(src) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(dst), "v"(offset), "s"(src) : "memory");
 }
 // 4 bytes a lane to LDS at dst + 4 lane.
 __device__ __forceinline__ void copy_words_to_lds(const void* src, uint32_t offset, uint32_t dst) {
     src = reinterpret_cast<const void*>(uniform(static_cast<int64_t>(reinterpret_cast<uintptr_t>(src))));
     dst = static_cast<uint32_t>(uniform(static_cast<int>(dst)));
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(dst), "v"(offset), "s"(src) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dword %1, %2" ::"{m0}"(dst), "v"(offset), "s"(src) : "memory");
 }
 template <int N>
 __device__ __forceinline__ void wait_copies() {
