@@ -180,7 +180,13 @@ struct Core {
     static constexpr int STEPS = CPR / KG, NC = HD / DB, KB = BK / DB, ACC = DB == 32 ? 16 : 4;
     static constexpr int KS = DB == 32 ? 16 : 32;  // keys of a 16-bit step of P V
     static constexpr int TB = BK * RB;             // bytes of a tile of K or V
-    static constexpr int kAhead = 8;  // fragments read ahead of the matrix steps
+    // The forms whose limbs of q leave few registers: f32 rows over f16 in two blocks
+    // of 16, over bf16 in blocks of 32 at head_dim 256.  They derive the places of
+    // their copies anew for every tile, and the first reads less ahead: without that
+    // 20 registers went to memory at head_dim 256 (24 requests of 27 rows 150 us,
+    // now 142), 3 at 128 (73.4, now 72.1).
+    static constexpr bool kTight = NL == 2 ? RBLK == 2 && HD >= 128 : NL == 3 && DB == 32 && HD == 256;
+    static constexpr int kAhead = kTight && NL == 2 ? 6 : 8;  // fragments read ahead of the matrix steps
     // Weights are kept times 2^kBias, and the running maximum may lag by 2^kLag.
     static constexpr int kBias = F16 ? 6 : 0;
     static constexpr float kLag = 8.0f;
@@ -234,7 +240,7 @@ struct Core {
     template <bool V>
     __device__ __forceinline__ static void copy_rows(const uint8_t* base, uint32_t row_bytes, int most, int j, int off,
                                                      uint32_t dst) {
-        const int lane = threadIdx.x & 63;
+        const int lane = kTight ? static_cast<int>(anew(threadIdx.x & 63)) : threadIdx.x & 63;
         const int r = off + lane / CPR, row = 8 * j + r;
         const uint32_t at = static_cast<uint32_t>(min(r, most)) * row_bytes +
                             16u * static_cast<uint32_t>((lane % CPR) ^ (V ? swz_v(row) : swz_k(row)));
@@ -797,6 +803,13 @@ __device__ __forceinline__ int64_t find_range(W& walk, int w, int nw, int64_t* s
 // many-row form: a lane's values, maximum and sum, two lanes to a row.
 constexpr int part_floats(int bm, int hd) { return bm * hd + 2 * bm; }
 constexpr int wide_part_floats(int bm, int hd) { return bm * hd + 4 * bm; }
+// Keys of a tile of the many-row form.  (Three limbs at head_dim 256 leave no room
+// for the scores and weights of 64: 2048 tokens over 4000 keys 920 us, with 32 761;
+// 64 over 500 57 and 49.  12 registers of q still go to memory there.)
+template <class Q, class T>
+constexpr int wide_keys(int hd) {
+    return KindOf<T>::f32 || (hd == 256 && sizeof(Q) == 4 && !KindOf<T>::f16) ? 32 : 64;
+}
 // Tiles of K, and of V, that the many-row form keeps in LDS: three where they
 // fit, so that copies run a step further ahead.
 constexpr int wide_slots(int tile_bytes) { return 6 * tile_bytes <= 147456 ? 3 : 2; }
@@ -1193,7 +1206,7 @@ __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_narrow(PagedAtt
 // thirds of it.
 template <class Q, class T, int HD, int NW>
 __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) {
-    constexpr int DB = 32, BM = DB * NW, BK = KindOf<T>::f32 ? 32 : 64, BN = BK, NT = NW * 64;
+    constexpr int DB = 32, BM = DB * NW, BK = wide_keys<Q, T>(HD), BN = BK, NT = NW * 64;
     using C = Core<Q, T, HD, DB, 1, BK>;
     constexpr int PER = 8 / C::RPI;               // copies of a group of 8 keys
     constexpr int COPIES = BK / C::RPI / NW;      // copies of a tile of K, or of V, by each wave
@@ -1494,7 +1507,7 @@ hipError_t run(const PagedAttn& p, float* part, uint32_t* counters, hipStream_t 
     // it: with 8 at least, 64 tokens over 500 keys took 65 us in f32 instead of 37)
     const unsigned grid = static_cast<unsigned>(slots());
     if (wide) {
-        constexpr int BK = KindOf<T>::f32 ? 32 : 64, LDS = 2 * wide_slots(BK * HD * sizeof(T)) * BK * HD * sizeof(T);
+        constexpr int BK = wide_keys<Q, T>(HD), LDS = 2 * wide_slots(BK * HD * sizeof(T)) * BK * HD * sizeof(T);
         constexpr int MOST = eight_fit<Q, T>(HD) ? 8 : 4;
         la.min_rows = narrow ? kNarrowRows : 0;
         la.max_rows = 0x7fffffff;
