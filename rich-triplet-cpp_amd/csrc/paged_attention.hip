@@ -291,7 +291,8 @@ struct Core {
                 int ex = static_cast<int>(__float_as_uint(big) >> 23);
                 ex = big > 0.0f && ex < 255 ? min(max(14 + 127 - ex + 127, 1), 253) : 127;
                 up = __uint_as_float(static_cast<uint32_t>(ex) << 23);
-                c[b] = c1 * __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
+                // (Not 0, which would make a NaN of the maximum of no scores; times 2^-126 all scores vanish.)
+                c[b] = fmaxf(c1 * __uint_as_float(static_cast<uint32_t>(254 - ex) << 23), 0x1p-126f);
             }
 #pragma unroll
             for (int t = 0; t < STEPS; ++t)

@@ -317,6 +317,26 @@ def test_windows_longer_than_any_request(rt, q, kv, heads, dim, lens):
 
 
 @pytest.mark.parametrize("q, kv", PAIRS)
+@pytest.mark.parametrize("rows", [1, 50])
+@pytest.mark.parametrize("size, scale", [(1e-36, 1e-10), (1e-30, 1e-30), (1.0, 1e-38), (0.0, 1.0)])
+def test_scores_that_vanish(rt, q, kv, rows, size, scale):
+    """Scores so small that every key has the same weight: the mean of the values, whose keys are cut between many
+    workgroups.  (Errors: of n additions, and of the weights' rounding, which all share one value.)"""
+    say("vanish", q, kv, rows, size, scale)
+    n, dim, page = 20000, 128, 16
+    k, v = torch.randn((2, n // page, page, 1, dim), device="cuda").to(DT[kv])
+    x = (torch.ones((rows, 2, dim), device="cuda") * size).to(DT[q])
+    table = torch.arange(n // page, dtype=torch.int32, device="cuda")[None]
+    got = rt.paged_attention(x, rt.PagedKV(k, v), table, i32([0, rows]), i32([n]), scale)
+    seen = torch.arange(n - rows + 1, n + 1, device="cuda")
+    flat = v.double().reshape(n, dim)
+    want = (flat.cumsum(0)[seen - 1] / seen[:, None])[:, None]
+    size_ = (flat.abs().cumsum(0)[seen - 1] / seen[:, None])[:, None]
+    eps = torch.finfo(DT[q]).eps / 2 if q != "f32" else 2.0**-24
+    assert ((got.double() - want).abs() <= 2.0**-24 * (64 + 3.5 * math.sqrt(n)) * size_ + eps * want.abs() + 2.0**-25).all()
+
+
+@pytest.mark.parametrize("q, kv", PAIRS)
 def test_garbage_tables(rt, q, kv):
     """Pages that are none of the cache's count as zeros; starts and lengths that make no sense touch nothing else."""
     say("tables", q, kv)
