@@ -727,8 +727,8 @@ int rt_hip_paged_append(const rt_hip_paged_kv* kv, const void* k, const void* v,
  * key that it sees, leaves that row's head undefined, and no other.  In values,
  * what is not finite reaches every row that sees it, however small its weight:
  * infinities of one sign as that infinity, others and NaN as NaN.
- * n_q_heads is any multiple of n_kv_heads up to 1024, scale > 0.  Results are
- * deterministic.
+ * n_q_heads is any multiple of n_kv_heads up to 1024, 0 < scale <= 2^127.
+ * Results are deterministic.
  * max_fresh is a hint, the most rows a request of this step may have (0: not
  * known); the result does not depend on it beyond rounding.
  * Uses the library workspace (rt_hip_paged_attention_workspace_bytes, to

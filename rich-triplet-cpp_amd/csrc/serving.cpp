@@ -2,7 +2,6 @@
 // (include/rt_hip.h): argument checks, workspace and dispatch.
 #include <hip/hip_runtime.h>
 
-#include <cmath>
 #include <string>
 
 #include "rt_hip.h"
@@ -196,7 +195,8 @@ int rt_hip_paged_attention(const void* q, int32_t dtype, int64_t q_stride, int32
     const char* fn = "rt_hip_paged_attention";
     PagedAttn p;
     if (const int rc = attention_args(fn, kv, dtype, n_q_heads, n_seq, n_tokens, max_fresh, &p)) return rc;
-    if (!(scale > 0.0f) || std::isinf(scale)) return fail(fn, RT_HIP_E_ARG, "scale must be positive and finite");
+    if (!(scale > 0.0f) || scale > 0x1p127f)  // (scores are weighed as powers of two: times log2(e))
+        return fail(fn, RT_HIP_E_ARG, "scale must be positive and at most 2^127");
     if (window < 0) return fail(fn, RT_HIP_E_ARG, "window must be >= 0");
     if (n_seq == 0 || n_tokens == 0) return RT_HIP_OK;
     if (!q || !out || !q_start || !kv_len) return fail(fn, RT_HIP_E_ARG, "null pointer");

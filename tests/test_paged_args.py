@@ -264,3 +264,11 @@ def test_results_are_made_on_the_stream_of_the_call(rt, streams, side, what):
         rt.verify_drafts(f32(5, 9), i32(5), i32(3), f32(5), f32(2), 3, **kw)
     assert len(seen) >= 2 and seen[-1][0].startswith("rt_hip_")
     assert {on for _, on in seen} == {"side" if side else "current"}, seen
+
+
+@pytest.mark.parametrize("scale", [1.7014121e38, 2.4e38, 3.4028234e38])
+def test_attention_refuses_scales_whose_exponents_overflow(rt, mem, scale):
+    """Scores are weighed as powers of two, so scale * log2(e) has to be finite too: no more than 2^127."""
+    assert attention(rt, mem, scale=C.c_float(scale)) == ARG
+    assert attention(rt, mem, scale=C.c_float(scale), n_tokens=0) == ARG
+    assert attention(rt, mem, scale=C.c_float(2.0**127), n_tokens=0) == 0
