@@ -728,6 +728,13 @@ def _call_on(device: int, name: str, stream, *args) -> None:
                    torch._C._cuda_getCurrentRawStream(device))
 
 
+def _fits(**numbers) -> None:
+    """Each number is one that the C call's 32 bits hold (ctypes drops what is above)."""
+    for name, n in numbers.items():
+        if not -2**31 <= n < 2**31:
+            raise ValueError(f"rt_hip: {name} = {n} does not fit 32 bits")
+
+
 _HERE = contextlib.nullcontext()
 
 
@@ -784,6 +791,8 @@ def paged_plan(cached, fresh, held, table, queue, queue_state, page_size: int, t
     updated in place.  tokens: rows of the step (at least the sum of fresh).
     plan: a PagedPlan of these sizes to write into; with its held and
     queue_state the ones passed, the state is updated in place."""
+    if page_size >> 31:  # (below 0: the call says so)
+        _fits(page_size=page_size)
     i32 = _torch().int32
     n, device = cached.shape[0], cached.get_device()
     per_request = (n,)
@@ -825,6 +834,8 @@ def paged_attention(q, kv: PagedKV, table, q_start, kv_len, scale: float, window
     are left as they were (a new out starts with zeros)."""
     torch = _torch()
     c, device = kv.struct, kv.device
+    if (window | max_fresh) >> 31:
+        _fits(window=window, max_fresh=max_fresh)
     if q.dim() != 3:
         raise ValueError("rt_hip: q must have shape (rows, n_q_heads, head_dim)")
     if out is None:
@@ -845,6 +856,7 @@ def paged_attention(q, kv: PagedKV, table, q_start, kv_len, scale: float, window
 
 def paged_attention_workspace_bytes(kv: PagedKV, dtype: int, n_q_heads: int, n_seq: int, tokens: int,
                                     max_fresh: int = 0) -> int:
+    _fits(n_q_heads=n_q_heads, n_seq=n_seq, tokens=tokens, max_fresh=max_fresh)
     return int(library().lib.rt_hip_paged_attention_workspace_bytes(kv.ref, dtype, n_q_heads, n_seq, tokens, max_fresh))
 
 

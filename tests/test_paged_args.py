@@ -272,3 +272,21 @@ def test_attention_refuses_scales_whose_exponents_overflow(rt, mem, scale):
     assert attention(rt, mem, scale=C.c_float(scale)) == ARG
     assert attention(rt, mem, scale=C.c_float(scale), n_tokens=0) == ARG
     assert attention(rt, mem, scale=C.c_float(2.0**127), n_tokens=0) == 0
+
+
+@pytest.mark.parametrize("far", [2**31, 2**32, 2**32 + 16, 2**63, -2**31 - 1, -2**32 + 16])
+def test_numbers_that_do_not_fit(no_library, far):
+    """Numbers that the C call takes in 32 bits: larger ones would arrive as others."""
+    import torch
+    rt = no_library
+    i32 = lambda *shape: OnGpu(torch.zeros(shape, dtype=torch.int32))
+    f32 = lambda *shape: OnGpu(torch.zeros(shape))
+    kv = rt.PagedKV(f32(8, 16, 1, 64), f32(8, 16, 1, 64))
+    for name in ("window", "max_fresh"):
+        with pytest.raises(ValueError, match=name):
+            rt.paged_attention(f32(5, 2, 64), kv, i32(2, 3), i32(3), i32(2), 0.1, out=f32(5, 2, 64), **{name: far})
+    for at, name in enumerate(("n_q_heads", "n_seq", "tokens", "max_fresh")):
+        with pytest.raises(ValueError, match=name):
+            rt.paged_attention_workspace_bytes(kv, rt.F32, *[far if i == at else 2 for i in range(4)])
+    with pytest.raises(ValueError, match="page_size"):
+        rt.paged_plan(i32(2), i32(2), i32(2), i32(2, 3), i32(8), i32(2), far, 5, plan=rt.PagedPlan(2, 5, "cpu"))
