@@ -722,11 +722,14 @@ int rt_hip_paged_append(const rt_hip_paged_kv* kv, const void* k, const void* v,
  * table entry is no page of the cache count as zeros.
  * dtype is q's and out's: the cache's (F16 or BF16: products of 16-bit values
  * summed in f32, the softmax in f32 and its weights rounded to the type before
- * they multiply v), or F32 with any cache (products and sums to f32
- * accuracy).  An infinity or a NaN (or 2^127 and more) in a row's q, or in a
- * key that it sees, leaves that row's head undefined, and no other.  In values,
- * what is not finite reaches every row that sees it, however small its weight:
- * infinities of one sign as that infinity, others and NaN as NaN.
+ * they multiply v), or F32 with any cache (sums in f32; q and the weights enter
+ * their products with 24 bits over an F32 or BF16 cache, with 22 over F16).  An
+ * infinity or a NaN (or 2^127 and more) in a row's q, or in a key that it sees,
+ * or a product of the two past f32's range, leaves that row's head undefined, and
+ * no other.  In values, what is not finite reaches every row that sees it, however
+ * small its weight: infinities of one sign as that infinity, others and NaN as
+ * NaN.  Values are summed in f32 times weights of up to 2^8 before the sum is
+ * divided: where that passes 2^128 (values of 1e30 and more) it is infinite.
  * n_q_heads is any multiple of n_kv_heads up to 1024, 0 < scale <= 2^127.
  * Results are deterministic.
  * max_fresh is a hint, the most rows a request of this step may have (0: not
@@ -753,9 +756,10 @@ int64_t rt_hip_paged_attention_workspace_bytes(const rt_hip_paged_kv* kv, int32_
  * that is zero everywhere), w = p behind the last one.  Random numbers are in
  * [0, 1).  temperature 0 (or negative, or NaN) is greedy: drafts are accepted
  * while they are the first largest logit, as rt_hip_argmax; a null temperature
- * is 1 for every request.  Sums are in f64.  NaN logits count as -inf, a row of
- * nothing else as certain of token 0; +inf leaves the weight to the infinite
- * ones.  A draft outside the vocabulary is refused.
+ * is 1 for every request.  Weights and sums are in f64 (the exponentials to 4e-14
+ * of their value).  NaN logits count as -inf, a row of nothing else as certain of
+ * token 0; +inf leaves the weight to the infinite ones.  A draft outside the
+ * vocabulary is refused.
  * out_tokens [n_seq][max_draft + 1]: the accepted drafts, the token drawn, then
  * -1; out_count [n_seq]: how many (0 for a request without rows).  Drafts past
  * max_draft are not looked at.  vocab <= 2^20, max_draft <= 255, n_seq <= 4096,

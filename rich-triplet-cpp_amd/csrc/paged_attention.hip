@@ -1002,11 +1002,11 @@ constexpr int narrow_ring(int hd) { return hd == 256 ? 32768 : 16384; }
 // Single tokens and drafts, bound by the bytes of keys and values.  A wave
 // streams tiles of its own through its own LDS ring, no barrier between them,
 // and the four waves' states are joined at the item's end.
-// 64 requests of 100 to 16000 keys, 8 KV heads of 128 in bf16: 152 us for 782 MB
-// (5.1 TB/s; a plain read of as much reaches 5.9).  16 requests of 5 tokens, a
-// window of 1024, head_dim 256: 24 us for 48 MB.  One token over 777 keys: 11.3
-// us, of which the range takes 2, pages, keys and q 2, the products 1.4, the
-// states and their join 2.
+// 64 requests of 100 to 16000 keys, 8 KV heads of 128 in bf16: 151 us for 782 MB
+// (5.2 TB/s; a plain read of as much reaches 5.9).  16 requests of 5 tokens, a
+// window of 1024, head_dim 256: 23 us for 48 MB.  One token over 777 keys: 11.2
+// us, a chain of latencies: lengths, pages, keys, the waves' states, the join of
+// the workgroups'.
 template <class Q, class T, int HD, int RBLK>
 __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_narrow(PagedAttn p, Launch la) {
     constexpr int NW = 4, DB = 16, BM = DB * RBLK, BK = KindOf<T>::f32 ? 16 : 32, BN = NW * BK;
@@ -1199,12 +1199,12 @@ __global__ __launch_bounds__(256, HD < 256 ? 2 : 1) void k_paged_narrow(PagedAtt
 // Chunks of prompts, bound by the matrix cores: every wave has 32 rows of its
 // own, and K and V tiles are read from memory once for all of them.  Four waves
 // or eight: enough_rows.
-// 4096 tokens over 8192 keys before them, 24 heads of 128 in bf16: 500 to 540 us,
-// 960 to 1030 TFLOP/s, at the clock that the power limit leaves (a library
-// product of 8192^3: 1212).  900-token chunks of head_dim 64: 99 us for 43 GFLOP,
-// there the exponentials and conversions take as long as the products.  517
-// tokens over 1100 keys in f32: 121 us, 71 TFLOP/s, the matrix cores busy for two
-// thirds of it.
+// 4096 tokens over 8192 keys before them, 24 heads of 128 in bf16: 490 to 535 us,
+// 960 to 1050 TFLOP/s, by the clock that the card's power limit leaves (a library
+// product of 8192^3: 1212); the matrix cores are busy half of the time, the VALU
+// the other half.  900-token chunks of head_dim 64: 88 us for 43 GFLOP, the VALU
+// busy 40% of it, the matrix cores 20%.  517 tokens over 1100 keys in f32: 106
+// us, 81 TFLOP/s, the matrix cores busy 54% of it.
 template <class Q, class T, int HD, int NW>
 __global__ __launch_bounds__(NW * 64) void k_paged_wide(PagedAttn p, Launch la) {
     constexpr int DB = 32, BM = DB * NW, BK = wide_keys<Q, T>(HD), BN = BK, NT = NW * 64;
@@ -1486,7 +1486,9 @@ int64_t most_rows(const PagedAttn& p) {
 //   1024 over 3000        88    70   119   108      397   374
 //   2048 over 4000       209   148   296   241     1080   999
 // 40 requests, 32 heads, 4 to a KV head: of 30 tokens (120 rows) 47 and 53, of
-// 100 (400 rows) 164 and 115.
+// 100 (400 rows) 164 and 115.  (The rule does not know the keys, so that 512 over
+// 9000 in f32, 48 rows to a CU, takes four waves and loses 6%; and it counts the
+// rows there is room for.)
 bool enough_rows(const PagedAttn& p, int64_t rows) {
     const int64_t each = p.kv.dtype == RT_HIP_F32 ? 80 : 40;
     return rows > 128 && static_cast<int64_t>(p.n_tokens) * p.n_q >= slots() * each;

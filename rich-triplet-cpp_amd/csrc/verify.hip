@@ -25,9 +25,9 @@
 //
 // Bound: the bytes of the logits, and as much the exponentials, 18 64-bit
 // instructions each at the rate of 32-bit ones.  64 requests of up to 4 drafts,
-// 128256 values in f32, 173 MB: 33 us for the sums (5.2 TB/s), 5 to decide, 22
-// to pick, for which the rows behind refused drafts are read once more.  One
-// request of 7 drafts: 4.6 + 4.4 + 11, chains of dependent loads.  (Decisions
+// 128256 values in f32, 173 MB: 30 to 34 us for the sums (5.1 to 5.8 TB/s), 5 to
+// decide, 21 to pick, for which the rows behind refused drafts are read once more.
+// One request of 7 drafts: 4.7 + 4.5 + 11, chains of dependent loads.  (Decisions
 // in every workgroup of the pick: 66 us and 25; in the sums' last workgroup to
 // arrive: 125 and 40, an arrival costs each of 10000 workgroups 2 us.)
 #include "rt_common.hpp"
@@ -313,7 +313,7 @@ struct Choice {
 };
 
 // Accepted drafts, their count, and the choice that is left; grid n_seq.  Wave w
-// takes rows w, w + 16, ..: the first that stops the request, a refused draft or
+// takes rows w, w + 8, ..: the first that stops the request, a refused draft or
 // the row behind the last one.
 template <class X>
 __global__ __launch_bounds__(kPickT) void k_verify_decide(VerifyDrafts p, const Stat* __restrict__ stats, int chunks,
