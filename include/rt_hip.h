@@ -707,7 +707,8 @@ int rt_hip_paged_plan(const int32_t* cached, const int32_t* fresh, const int32_t
  * dtype, F32, F16 or BF16, rows row_stride values apart, so that they may be
  * part of a joint projection's output) to slot slots[t], rounded to the cache's
  * type (to nearest even).  Rows whose slot is negative or outside the cache are
- * skipped.  Of rows with the same slot one is kept, no telling which. */
+ * skipped.  Of rows with the same slot one is kept, no telling which.  Keys and
+ * values must not share memory (the pages of the two may lie in turn). */
 int rt_hip_paged_append(const rt_hip_paged_kv* kv, const void* k, const void* v, int32_t dtype, int64_t row_stride,
                         const int32_t* slots, int32_t n_tokens, rt_hip_stream stream);
 

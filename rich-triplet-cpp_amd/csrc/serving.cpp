@@ -74,6 +74,16 @@ Range pages_of(const PagedKv& c, const void* p) {
     return {p, ((c.n_pages - 1) * c.page_stride + page) * value_bytes(c.dtype)};
 }
 
+// Whether a page of keys and one of values share memory (pages of the two may lie in turn).
+bool keys_over_values(const PagedKv& c) {
+    const uintptr_t k = reinterpret_cast<uintptr_t>(c.k), v = reinterpret_cast<uintptr_t>(c.v), apart = k < v ? v - k : k - v;
+    const uintptr_t stride = c.page_stride * value_bytes(c.dtype);
+    const uintptr_t page = ((static_cast<uintptr_t>(c.n_kv) * c.head_dim) << c.page_shift) * value_bytes(c.dtype);
+    if (apart >= (c.n_pages - 1) * stride + page) return false;
+    // (a page's nearest of the other kind starts apart % stride before it, or what is left of a stride behind it)
+    return apart % stride < page || stride - apart % stride < page;
+}
+
 int table_args(const char* fn, const int32_t* table, int64_t cols, int n_seq, int shift) {
     if (!table && n_seq > 0) return fail(fn, RT_HIP_E_ARG, "null block table");
     if (cols < 1) return fail(fn, RT_HIP_E_ARG, "table_cols must be >= 1");
@@ -144,6 +154,7 @@ int rt_hip_paged_append(const rt_hip_paged_kv* kv, const void* k, const void* v,
     const char* fn = "rt_hip_paged_append";
     PagedKv c;
     if (const int rc = cache_args(fn, kv, &c)) return rc;
+    if (keys_over_values(c)) return fail(fn, RT_HIP_E_ARG, "the cache's keys and values overlap");
     if (n_tokens < 0) return fail(fn, RT_HIP_E_ARG, "n_tokens must be >= 0");
     if (!value_bytes(dtype)) return fail(fn, RT_HIP_E_UNSUPPORTED, "k and v must be F32, F16 or BF16");
     if (n_tokens == 0) return RT_HIP_OK;

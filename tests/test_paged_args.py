@@ -290,3 +290,17 @@ def test_numbers_that_do_not_fit(no_library, far):
             rt.paged_attention_workspace_bytes(kv, rt.F32, *[far if i == at else 2 for i in range(4)])
     with pytest.raises(ValueError, match="page_size"):
         rt.paged_plan(i32(2), i32(2), i32(2), i32(2, 3), i32(8), i32(2), far, 5, plan=rt.PagedPlan(2, 5, "cpu"))
+
+
+@pytest.mark.parametrize("apart, stride, pages, one", [
+    (0, 0, 2, True), (512, 0, 2, True), (512, 0, 1, False), (1024, 0, 2, False), (512, 1024, 4, False), (512, 1024, 1, False),
+    (1024, 1024, 4, True), (256, 1024, 4, True), (768, 1024, 4, True), (1536, 1024, 2, False), (1536, 1024, 4, False),
+    (2048, 1024, 2, False)])
+def test_append_refuses_keys_over_values(rt, mem, apart, stride, pages, one):
+    """Keys and values of one memory (values apart, of 512 to a page): both would be written there.  Either order; pages
+    of the two in turn are no such case, nor is it one to read."""
+    base = mem[12]
+    for k, v in ((base, base + 2 * apart), (base + 2 * apart, base)):
+        kv = cache(rt, mem, k=k, v=v, page_stride=stride, n_pages=pages)
+        assert append(rt, mem, kv=kv, n=0, k=None, v=None, slots=None) == (ARG if one else 0)
+        assert attention(rt, mem, kv=kv, n_tokens=0) == 0
