@@ -67,7 +67,8 @@ typedef enum {
     RT_HIP_Q4_0 = 3,
     RT_HIP_Q4MAT = 4,
     RT_HIP_Q6K = 5,  /* GGUF Q6_K blocks: the decode engine's Llama down projection (rt_hip_decoder_set_tensor) */
-    RT_HIP_F16 = 6   /* f16 values: the paged KV cache and its attention */
+    RT_HIP_F16 = 6,  /* f16 values: the paged KV cache and its attention */
+    RT_HIP_Q4KV = 7  /* a paged KV cache in 4 bits (rt_hip_paged_kv) */
 } rt_hip_format;
 
 /* Largest activation batch the GEMV kernels take; the reference's
@@ -666,7 +667,19 @@ int rt_hip_decoder_destroy(rt_hip_decoder* dec);
  * share an allocation).  page_size is a power of two from 8 to 1024, head_dim
  * 64, 128 or 256, n_pages * page_size < 2^31, page_stride < 2^32 bytes; pages
  * start 16-byte aligned.
- * Slot i is row i % page_size of page i / page_size. */
+ * Slot i is row i % page_size of page i / page_size.
+ *
+ * A cache in 4 bits (RT_HIP_Q4KV) has pages of rt_hip_paged_page_bytes bytes, 5
+ * bits a value, and its page_stride counts bytes.  32 neighbouring values of a
+ * head are a group with two f16 numbers a and b and a code c of 0 .. 15 each, which
+ * stands for the f16 number nearest a * (1 + c / 16) + b.  Append makes them, lo and
+ * hi being the group's least and greatest value and every step rounded to f32:
+ *   a = f16((hi - lo) * (16 / 15)), b = f16(lo - a),
+ *   c = rint((x - b) * (16 / a)) - 16, within 0 .. 15; 0 where a is 0:
+ * a value is off by half a step, (hi - lo) / 30, and by two roundings to f16.  A
+ * group with a value that is not finite, or past 16384, stands for 32 NaN.  Pages
+ * are for these calls to write and read; their bytes are laid out as the attention's
+ * loads want them, and bytes that append did not write stand for nothing. */
 typedef struct rt_hip_paged_kv {
     void* k;
     void* v;
@@ -674,6 +687,10 @@ typedef struct rt_hip_paged_kv {
     int32_t n_pages, page_size, n_kv_heads, head_dim;
     int64_t page_stride;
 } rt_hip_paged_kv;
+
+/* Bytes of a dense page of keys, or of values, of a cache of these sizes; -1 for
+ * sizes that no cache has. */
+int64_t rt_hip_paged_page_bytes(int32_t dtype, int32_t page_size, int32_t n_kv_heads, int32_t head_dim);
 
 /* rt_hip_paged_plan: request s (of n_seq <= 4096) has cached[s] tokens in the
  * cache, holds held[s] pages (the first held[s] entries of its row of table
@@ -707,10 +724,19 @@ int rt_hip_paged_plan(const int32_t* cached, const int32_t* fresh, const int32_t
  * dtype, F32, F16 or BF16, rows row_stride values apart, so that they may be
  * part of a joint projection's output) to slot slots[t], rounded to the cache's
  * type (to nearest even).  Rows whose slot is negative or outside the cache are
- * skipped.  Of rows with the same slot one is kept, no telling which.  Keys and
- * values must not share memory (the pages of the two may lie in turn). */
+ * skipped.  Of rows with the same slot one is kept, no telling which (in 4 bits,
+ * parts of several, and the slot's values are undefined until it is written again).
+ * Keys and values must not share memory (the pages of the two may lie in turn). */
 int rt_hip_paged_append(const rt_hip_paged_kv* kv, const void* k, const void* v, int32_t dtype, int64_t row_stride,
                         const int32_t* slots, int32_t n_tokens, rt_hip_stream stream);
+
+/* rt_hip_paged_read: the keys and values at slots[t], as the cache has them, to row
+ * t of k and v (n_kv_heads * head_dim values of type dtype, F32, F16 or BF16, rows
+ * row_stride values apart), rounded to dtype (to nearest even; a 4-bit cache's are
+ * f16 numbers).  Zeros for a slot that is negative or outside the cache.  k and v
+ * must not overlap each other (their rows may lie in turn), the cache or slots. */
+int rt_hip_paged_read(const rt_hip_paged_kv* kv, const int32_t* slots, int32_t n_tokens, void* k, void* v, int32_t dtype,
+                      int64_t row_stride, rt_hip_stream stream);
 
 /* rt_hip_paged_attention: rows q_start[s] .. q_start[s + 1] of q (n_q_heads *
  * head_dim values, q_stride apart) attend to the first kv_len[s] keys of
@@ -731,6 +757,10 @@ int rt_hip_paged_append(const rt_hip_paged_kv* kv, const void* k, const void* v,
  * small its weight: infinities of one sign as that infinity, others and NaN as
  * NaN.  Values are summed in f32 times weights of up to 2^8 before the sum is
  * divided: where that passes 2^128 (values of 1e30 and more) it is infinite.
+ * A cache in 4 bits takes q and out of any of the three types, and is computed with
+ * as the f16 numbers that it stands for (BF16 rows enter their products whole, F32
+ * ones with 22 bits; weights of 16-bit rows are rounded to f16); NaN in values
+ * reaches the rows that see it, and no others.
  * n_q_heads is any multiple of n_kv_heads up to 1024, 0 < scale <= 2^127.
  * Results are deterministic.
  * max_fresh is a hint, the most rows a request of this step may have (0: not

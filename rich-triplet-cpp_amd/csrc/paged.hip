@@ -22,6 +22,7 @@
 // Append.  One thread converts and stores 8 values of a row; bound by the
 // bytes read and written: 8192 rows of 1024 bf16 keys and values, 67 MB, in 11 us
 // (6 TB/s, part of them in the last-level cache), 40 rows of f32 in 2.4.
+#include "paged_rows.hpp"
 #include "rt_common.hpp"
 #include "rt_launch.hpp"
 #include "wave_scan.hpp"
@@ -184,46 +185,6 @@ __global__ __launch_bounds__(NT) void k_paged_plan(PagedPlan p, uint32_t* __rest
         p.queue_state_out[0] = static_cast<int>((static_cast<int64_t>(head) + take0) % cap);
         p.queue_state_out[1] = min(free_pages - take0 + gone0, cap);
     }
-}
-
-__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
-    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        v[e] = a[e];
-        v[4 + e] = b[e];
-    }
-}
-__device__ __forceinline__ void load8(const __bf16* p, float (&v)[8]) {
-    const u32x4 a = ld16(p);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        v[2 * e] = bf16_lo_to_f32(a[e]);
-        v[2 * e + 1] = bf16_hi_to_f32(a[e]);
-    }
-}
-__device__ __forceinline__ void load8(const _Float16* p, float (&v)[8]) {
-    const u32x4 a = ld16(p);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        v[2 * e] = f16_bits_to_f32(a[e] & 0xffffu);
-        v[2 * e + 1] = f16_bits_to_f32(a[e] >> 16);
-    }
-}
-__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
-    *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
-    *reinterpret_cast<f32x4*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
-}
-__device__ __forceinline__ void store8(__bf16* p, const float (&v)[8]) {
-    *reinterpret_cast<u32x4*>(p) = u32x4{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]), bf16_pair(v[4], v[5]),
-                                         bf16_pair(v[6], v[7])};
-}
-__device__ __forceinline__ void store8(_Float16* p, const float (&v)[8]) {
-    typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-    f16x8 o;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = static_cast<_Float16>(v[e]);  // round to nearest even; past the range: infinity
-    *reinterpret_cast<f16x8*>(p) = o;
 }
 
 // Units of 8 values: (token, unit of the row), keys in blockIdx.y 0, values in 1.

@@ -276,9 +276,9 @@ hipError_t launch_add(const float* a, const float* b, float* out, int64_t n, hip
 struct PagedKv {
     void* k = nullptr;
     void* v = nullptr;
-    int dtype = 0;  // RT_HIP_F32, RT_HIP_F16 or RT_HIP_BF16
+    int dtype = 0;  // RT_HIP_F32, RT_HIP_F16, RT_HIP_BF16 or RT_HIP_Q4KV
     int n_pages = 0, page_shift = 0, n_kv = 0, head_dim = 0;
-    int64_t page_stride = 0;
+    int64_t page_stride = 0;  // (RT_HIP_Q4KV: in bytes)
 };
 // One step's bookkeeping; the arrays are device memory.  n_seq <=
 // kPlanMaxSeq, n_seq * cols and cols << page_shift and n_pages << page_shift
@@ -305,6 +305,12 @@ hipError_t launch_paged_plan(const PagedPlan& p, uint32_t* arrivals, hipStream_t
 // cache is skipped.  n_tokens * n_kv * head_dim / 8 < 2^31.
 hipError_t launch_paged_append(int src_dtype, const void* k, const void* v, int64_t src_stride, const PagedKv& kv,
                                const int32_t* slots, int n_tokens, hipStream_t s);
+// The same into a cache of 4 bits (paged4.hip), and rows of any cache at slots
+// to dense ones, dst_stride values apart (zeros for a slot outside the cache).
+hipError_t launch_paged4_append(int src_dtype, const void* k, const void* v, int64_t src_stride, const PagedKv& kv,
+                                const int32_t* slots, int n_tokens, hipStream_t s);
+hipError_t launch_paged_read(const PagedKv& kv, const int32_t* slots, int n_tokens, int dst_dtype, void* k, void* v,
+                             int64_t dst_stride, hipStream_t s);
 // Attention of rows q_start[s] .. q_start[s + 1] of q over request s's first
 // kv_len[s] keys; the last row sees them all, each row before one fewer, of
 // those the last `window` (0: all).  q and out: rows of n_q heads, q_stride
@@ -325,6 +331,9 @@ struct PagedAttn {
 };
 size_t paged_attention_workspace(const PagedAttn& p);
 hipError_t launch_paged_attention(const PagedAttn& p, void* part, uint32_t* counters, hipStream_t s);
+// Over a cache of 4 bits (paged4_attention.hip).
+size_t paged4_attention_workspace(const PagedAttn& p);
+hipError_t launch_paged4_attention(const PagedAttn& p, void* part, uint32_t* counters, hipStream_t s);
 // Drafted tokens against the target's distributions (verify.hip).
 struct VerifyDrafts {
     const void* logits = nullptr;        // rows of vocab values, logit_stride apart

@@ -34,6 +34,14 @@ bool overlap(const Range& a, const Range& b) {
 
 int value_bytes(int32_t dtype) { return dtype == RT_HIP_F32 ? 4 : (dtype == RT_HIP_F16 || dtype == RT_HIP_BF16 ? 2 : 0); }
 
+bool cache_type(int32_t dtype) { return value_bytes(dtype) != 0 || dtype == RT_HIP_Q4KV; }
+// Bytes of `values` of a cache's; of its page_stride.
+int64_t cache_bytes(int32_t dtype, int64_t values) { return dtype == RT_HIP_Q4KV ? values / 8 * 5 : values * value_bytes(dtype); }
+int64_t stride_bytes(const PagedKv& c) { return c.dtype == RT_HIP_Q4KV ? c.page_stride : c.page_stride * value_bytes(c.dtype); }
+int64_t page_bytes(const PagedKv& c) {
+    return cache_bytes(c.dtype, (static_cast<int64_t>(c.n_kv) * c.head_dim) << c.page_shift);
+}
+
 // log2 of a page size the kernels take, -1 otherwise.
 int page_shift(int32_t page_size) {
     for (int s = 3; s <= 10; ++s)
@@ -44,7 +52,7 @@ int page_shift(int32_t page_size) {
 // The caller's description of a cache, checked, as the kernels take it.
 int cache_args(const char* fn, const rt_hip_paged_kv* kv, PagedKv* out) {
     if (!kv || !kv->k || !kv->v) return fail(fn, RT_HIP_E_ARG, "null cache");
-    if (!value_bytes(kv->dtype)) return fail(fn, RT_HIP_E_UNSUPPORTED, "the cache must be F32, F16 or BF16");
+    if (!cache_type(kv->dtype)) return fail(fn, RT_HIP_E_UNSUPPORTED, "the cache must be F32, F16, BF16 or Q4KV");
     const int shift = page_shift(kv->page_size);
     if (shift < 0) return fail(fn, RT_HIP_E_SHAPE, "page_size must be a power of two from 8 to 1024");
     if (kv->head_dim != 64 && kv->head_dim != 128 && kv->head_dim != 256)
@@ -52,11 +60,13 @@ int cache_args(const char* fn, const rt_hip_paged_kv* kv, PagedKv* out) {
     if (kv->n_kv_heads < 1 || kv->n_kv_heads > 256) return fail(fn, RT_HIP_E_SHAPE, "n_kv_heads must be in [1, 256]");
     if (kv->n_pages < 1 || (static_cast<int64_t>(kv->n_pages) << shift) > 0x7fffffffLL)
         return fail(fn, RT_HIP_E_SHAPE, "n_pages must be >= 1 and n_pages * page_size below 2^31");
-    const int64_t dense = (static_cast<int64_t>(kv->n_kv_heads) * kv->head_dim) << shift;
+    const bool four = kv->dtype == RT_HIP_Q4KV;  // (its page_stride counts bytes)
+    const int64_t values = (static_cast<int64_t>(kv->n_kv_heads) * kv->head_dim) << shift;
+    const int64_t dense = four ? cache_bytes(kv->dtype, values) : values, unit = four ? 1 : value_bytes(kv->dtype);
     const int64_t stride = kv->page_stride ? kv->page_stride : dense;
     if (stride < dense) return fail(fn, RT_HIP_E_ARG, "page_stride below a page's values");
-    if (stride > 0xffffffffLL / value_bytes(kv->dtype)) return fail(fn, RT_HIP_E_SHAPE, "page_stride must be below 2^32 bytes");
-    if (!aligned(kv->k, 16) || !aligned(kv->v, 16) || stride * value_bytes(kv->dtype) % 16)
+    if (stride > 0xffffffffLL / unit) return fail(fn, RT_HIP_E_SHAPE, "page_stride must be below 2^32 bytes");
+    if (!aligned(kv->k, 16) || !aligned(kv->v, 16) || stride * unit % 16)
         return fail(fn, RT_HIP_E_ALIGN, "pages must be 16-byte aligned");
     out->k = kv->k;
     out->v = kv->v;
@@ -70,15 +80,13 @@ int cache_args(const char* fn, const rt_hip_paged_kv* kv, PagedKv* out) {
 }
 
 Range pages_of(const PagedKv& c, const void* p) {
-    const int64_t page = (static_cast<int64_t>(c.n_kv) * c.head_dim) << c.page_shift;
-    return {p, ((c.n_pages - 1) * c.page_stride + page) * value_bytes(c.dtype)};
+    return {p, (c.n_pages - 1) * stride_bytes(c) + page_bytes(c)};
 }
 
 // Whether a page of keys and one of values share memory (pages of the two may lie in turn).
 bool keys_over_values(const PagedKv& c) {
     const uintptr_t k = reinterpret_cast<uintptr_t>(c.k), v = reinterpret_cast<uintptr_t>(c.v), apart = k < v ? v - k : k - v;
-    const uintptr_t stride = c.page_stride * value_bytes(c.dtype);
-    const uintptr_t page = ((static_cast<uintptr_t>(c.n_kv) * c.head_dim) << c.page_shift) * value_bytes(c.dtype);
+    const uintptr_t stride = stride_bytes(c), page = page_bytes(c);
     if (apart >= (c.n_pages - 1) * stride + page) return false;
     // (a page's nearest of the other kind starts apart % stride before it, or what is left of a stride behind it)
     return apart % stride < page || stride - apart % stride < page;
@@ -149,6 +157,13 @@ int rt_hip_paged_plan(const int32_t* cached, const int32_t* fresh, const int32_t
     return launched(fn, launch_paged_plan(p, counters, s));
 }
 
+int64_t rt_hip_paged_page_bytes(int32_t dtype, int32_t page_size, int32_t n_kv_heads, int32_t head_dim) {
+    void* const some = reinterpret_cast<void*>(uintptr_t{16});  // (only the sizes are looked at)
+    const rt_hip_paged_kv kv = {some, some, dtype, 1, page_size, n_kv_heads, head_dim, 0};
+    PagedKv c;
+    return cache_args("rt_hip_paged_page_bytes", &kv, &c) ? -1 : page_bytes(c);
+}
+
 int rt_hip_paged_append(const rt_hip_paged_kv* kv, const void* k, const void* v, int32_t dtype, int64_t row_stride,
                         const int32_t* slots, int32_t n_tokens, rt_hip_stream stream) {
     const char* fn = "rt_hip_paged_append";
@@ -169,7 +184,39 @@ int rt_hip_paged_append(const rt_hip_paged_kv* kv, const void* k, const void* v,
     for (const void* src : {k, v})
         for (const void* dst : {static_cast<const void*>(c.k), static_cast<const void*>(c.v)})
             if (overlap({src, bytes}, pages_of(c, dst))) return fail(fn, RT_HIP_E_ARG, "k or v overlaps the cache");
-    return launched(fn, launch_paged_append(dtype, k, v, row_stride, c, slots, n_tokens, static_cast<hipStream_t>(stream)));
+    const auto launch = c.dtype == RT_HIP_Q4KV ? launch_paged4_append : launch_paged_append;
+    return launched(fn, launch(dtype, k, v, row_stride, c, slots, n_tokens, static_cast<hipStream_t>(stream)));
+}
+
+int rt_hip_paged_read(const rt_hip_paged_kv* kv, const int32_t* slots, int32_t n_tokens, void* k, void* v, int32_t dtype,
+                      int64_t row_stride, rt_hip_stream stream) {
+    const char* fn = "rt_hip_paged_read";
+    PagedKv c;
+    if (const int rc = cache_args(fn, kv, &c)) return rc;
+    if (n_tokens < 0) return fail(fn, RT_HIP_E_ARG, "n_tokens must be >= 0");
+    if (!value_bytes(dtype)) return fail(fn, RT_HIP_E_UNSUPPORTED, "k and v must be F32, F16 or BF16");
+    if (n_tokens == 0) return RT_HIP_OK;
+    if (!k || !v || !slots) return fail(fn, RT_HIP_E_ARG, "null pointer");
+    const int64_t row = static_cast<int64_t>(c.n_kv) * c.head_dim;
+    if (row_stride < row) return fail(fn, RT_HIP_E_ARG, "row_stride below a row's values");
+    if (row_stride > 0x7fffffffffffLL / n_tokens) return fail(fn, RT_HIP_E_SHAPE, "n_tokens * row_stride must be below 2^47");
+    if (!aligned(k, 16) || !aligned(v, 16) || row_stride * value_bytes(dtype) % 16)
+        return fail(fn, RT_HIP_E_ALIGN, "rows must be 16-byte aligned");
+    if (row / 8 * n_tokens > 0x7fffffffLL - 256)
+        return fail(fn, RT_HIP_E_SHAPE, "n_tokens * n_kv_heads * head_dim must be below 2^34");
+    const int64_t bytes = ((n_tokens - 1) * row_stride + row) * value_bytes(dtype);
+    const Range slot_range = {slots, 4 * static_cast<int64_t>(n_tokens)};
+    for (const void* dst : {k, v}) {
+        if (overlap({dst, bytes}, pages_of(c, c.k)) || overlap({dst, bytes}, pages_of(c, c.v)))
+            return fail(fn, RT_HIP_E_ARG, "k or v overlaps the cache");
+        if (overlap({dst, bytes}, slot_range)) return fail(fn, RT_HIP_E_ARG, "k or v overlaps slots");
+    }
+    // (rows of the two may lie in turn, as halves of one tensor)
+    const uintptr_t a = reinterpret_cast<uintptr_t>(k), b = reinterpret_cast<uintptr_t>(v);
+    const uintptr_t apart = a < b ? b - a : a - b, stride = row_stride * value_bytes(dtype), dense = row * value_bytes(dtype);
+    if (apart < static_cast<uintptr_t>(bytes) && (apart % stride < dense || stride - apart % stride < dense))
+        return fail(fn, RT_HIP_E_ARG, "k and v overlap");
+    return launched(fn, launch_paged_read(c, slots, n_tokens, dtype, k, v, row_stride, static_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"
@@ -179,8 +226,8 @@ namespace {
 int attention_args(const char* fn, const rt_hip_paged_kv* kv, int32_t dtype, int32_t n_q_heads, int32_t n_seq,
                    int32_t n_tokens, int32_t max_fresh, PagedAttn* p) {
     if (const int rc = cache_args(fn, kv, &p->kv)) return rc;
-    if (!value_bytes(dtype) || (dtype != RT_HIP_F32 && dtype != p->kv.dtype))
-        return fail(fn, RT_HIP_E_UNSUPPORTED, "q must be F32 or of the cache's type");
+    if (!value_bytes(dtype) || (dtype != RT_HIP_F32 && dtype != p->kv.dtype && p->kv.dtype != RT_HIP_Q4KV))
+        return fail(fn, RT_HIP_E_UNSUPPORTED, "q must be F32 or of the cache's type (any over Q4KV)");
     if (n_q_heads < p->kv.n_kv || n_q_heads % p->kv.n_kv || n_q_heads > 1024)
         return fail(fn, RT_HIP_E_SHAPE, "n_q_heads must be a multiple of n_kv_heads, at most 1024");
     if (n_seq < 0 || n_tokens < 0 || max_fresh < 0) return fail(fn, RT_HIP_E_ARG, "negative size");
@@ -237,9 +284,10 @@ int rt_hip_paged_attention(const void* q, int32_t dtype, int64_t q_stride, int32
     uint32_t* const counters = arrival_counters(s, &e);
     if (!counters) return launched(fn, e);
     void* part = nullptr;
-    if (const size_t need = paged_attention_workspace(p))
+    const bool four = p.kv.dtype == RT_HIP_Q4KV;
+    if (const size_t need = four ? paged4_attention_workspace(p) : paged_attention_workspace(p))
         if (!(part = workspace(need, s, &e))) return launched(fn, e);
-    return launched(fn, launch_paged_attention(p, part, counters, s));
+    return launched(fn, (four ? launch_paged4_attention : launch_paged_attention)(p, part, counters, s));
 }
 
 int64_t rt_hip_paged_attention_workspace_bytes(const rt_hip_paged_kv* kv, int32_t dtype, int32_t n_q_heads,
@@ -247,7 +295,8 @@ int64_t rt_hip_paged_attention_workspace_bytes(const rt_hip_paged_kv* kv, int32_
     PagedAttn p;
     if (attention_args("rt_hip_paged_attention_workspace_bytes", kv, dtype, n_q_heads, n_seq, n_tokens, max_fresh, &p))
         return -1;
-    return n_seq == 0 || n_tokens == 0 ? 0 : static_cast<int64_t>(paged_attention_workspace(p));
+    if (n_seq == 0 || n_tokens == 0) return 0;
+    return static_cast<int64_t>(p.kv.dtype == RT_HIP_Q4KV ? paged4_attention_workspace(p) : paged_attention_workspace(p));
 }
 
 }  // extern "C"

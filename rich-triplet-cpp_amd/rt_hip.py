@@ -19,7 +19,7 @@ ROOT = os.path.dirname(HERE)
 LIB_PATH = os.environ.get("RT_HIP_LIB_PATH", os.path.join(HERE, "lib", "librt_hip.so"))
 HEADER_PATH = os.path.join(ROOT, "include", "rt_hip.h")
 
-F32, BF16, Q4K, Q4_0, Q4MAT, Q6K, F16 = 0, 1, 2, 3, 4, 5, 6
+F32, BF16, Q4K, Q4_0, Q4MAT, Q6K, F16, Q4KV = range(8)
 GEMV_MAX_M = 8
 
 _vp, _i64, _i32 = C.c_void_p, C.c_int64, C.c_int32
@@ -84,6 +84,7 @@ _SIGNATURES = {
     "rt_hip_paged_plan": [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp,
                           _vp],
     "rt_hip_paged_append": [C.POINTER(PagedKvStruct), _vp, _vp, _i32, _i64, _vp, _i32, _vp],
+    "rt_hip_paged_read": [C.POINTER(PagedKvStruct), _vp, _i32, _vp, _vp, _i32, _i64, _vp],
     "rt_hip_paged_attention": [_vp, _i32, _i64, _i32, C.POINTER(PagedKvStruct), _vp, _i64, _vp, _vp, _i32, _i32, _i32,
                                C.c_float, _i32, _vp, _i64, _vp],
     "rt_hip_verify_drafts": [_vp, _i64, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp,
@@ -101,6 +102,7 @@ _SIZE_SIGNATURES = {
     "rt_hip_flux_attention_workspace_bytes": [_i64, _i32, _i32],
     "rt_hip_q4mat_bytes": [_i64, _i64],
     "rt_hip_q4mat_scales_offset": [_i64, _i64],
+    "rt_hip_paged_page_bytes": [_i32, _i32, _i32, _i32],
     "rt_hip_paged_attention_workspace_bytes": [C.POINTER(PagedKvStruct), _i32, _i32, _i32, _i32, _i32],
     "rt_hip_verify_drafts_workspace_bytes": [_i32, _i32, _i32, _i32, _i32],
 }
@@ -770,6 +772,38 @@ class PagedKV:
         self.ref = C.byref(self.struct)
 
 
+def paged_page_bytes(dtype: int, page_size: int, n_kv_heads: int, head_dim: int) -> int:
+    """Bytes of a dense page of keys, or of values; -1 for sizes that no cache has."""
+    _fits(dtype=dtype, page_size=page_size, n_kv_heads=n_kv_heads, head_dim=head_dim)
+    return int(library().lib.rt_hip_paged_page_bytes(dtype, page_size, n_kv_heads, head_dim))
+
+
+class PagedKV4(PagedKV):
+    """A KV cache in 4 bits (Q4KV): k and v [n_pages, paged_page_bytes(Q4KV, page_size,
+    n_kv_heads, head_dim)] of uint8, pages with any one stride between them.  The
+    calls that take a PagedKV take it; what they keep of values is in rt_hip.h."""
+
+    def __init__(self, k, v, page_size: int, n_kv_heads: int, head_dim: int):
+        if not (k.is_cuda and v.is_cuda and k.device == v.device):
+            raise ValueError("rt_hip: the cache must live on one GPU")
+        size = paged_page_bytes(Q4KV, page_size, n_kv_heads, head_dim)
+        if size < 0:
+            raise ValueError("rt_hip: no 4-bit cache has these sizes: " + library().lib.rt_hip_last_error().decode())
+        if k.dtype is not _torch().uint8 or v.dtype is not k.dtype or k.dim() != 2 or k.shape != v.shape or k.shape[1] != size:
+            raise ValueError(f"rt_hip: k and v must be uint8 [n_pages, {size}]")
+        n_pages = k.shape[0]
+        if k.stride(1) != 1 or v.stride(1) != 1:
+            raise ValueError("rt_hip: the pages of the cache must be dense")
+        stride = k.stride(0) if n_pages > 1 else size
+        if n_pages > 1 and v.stride(0) != stride:
+            raise ValueError("rt_hip: k and v must have one page stride")
+        if stride < size:  # (0 among them, which the call would take as dense)
+            raise ValueError("rt_hip: the pages of the cache overlap")
+        self.k, self.v, self.device = k, v, k.get_device()
+        self.struct = PagedKvStruct(k.data_ptr(), v.data_ptr(), Q4KV, n_pages, page_size, n_kv_heads, head_dim, stride)
+        self.ref = C.byref(self.struct)
+
+
 class PagedPlan:
     """What paged_plan writes (int32 tensors): q_start [n_seq + 1], kv_len
     [n_seq], slots and positions [tokens], and the state after the step, held
@@ -826,10 +860,34 @@ def paged_append(kv: PagedKV, k, v, slots, stream=None) -> None:
              slots.data_ptr(), n)
 
 
+def paged_read(kv: PagedKV, slots, dtype=None, out=None, stream=None):
+    """The cache's keys and values at slots [tokens], a pair [tokens, n_kv_heads,
+    head_dim] of dtype (the cache's; of a 4-bit one float16); zeros for a slot that
+    is none of the cache's.  out: a pair to write into, rows with any one stride."""
+    torch = _torch()
+    c, device = kv.struct, kv.device
+    n = slots.shape[0]
+    _want(device, (slots, "slots", torch.int32, (n,)))
+    if out is None:
+        dtype = dtype or (torch.float16 if c.dtype == Q4KV else kv.k.dtype)
+        with _made_on(stream):
+            out = torch.empty((2, n, c.n_kv_heads, c.head_dim), dtype=dtype, device=kv.k.device).unbind(0)
+    k, v = out
+    if (dtype is not None and k.dtype is not dtype) or v.dtype is not k.dtype or k.shape[0] != n or v.shape[0] != n:
+        raise ValueError("rt_hip: out must be a pair of slots' length and of dtype")
+    stride = _rows(device, k, "k", c.n_kv_heads, c.head_dim)
+    if _rows(device, v, "v", c.n_kv_heads, c.head_dim) != stride:
+        raise ValueError("rt_hip: k and v must have one stride")
+    _call_on(device, "rt_hip_paged_read", stream, kv.ref, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), _value_type(k),
+             stride)
+    return k, v
+
+
 def paged_attention(q, kv: PagedKV, table, q_start, kv_len, scale: float, window: int = 0, max_fresh: int = 0, out=None,
                     stream=None):
     """Attention of the step's rows q [tokens, n_q_heads, head_dim] over the
-    pages; the cache's dtype, or float32 over any cache.  max_fresh: the most
+    pages; the cache's dtype, or float32 over any cache, or any of the three
+    over a 4-bit one.  max_fresh: the most
     new tokens of one request, where known.  Rows of out outside every request
     are left as they were (a new out starts with zeros)."""
     torch = _torch()
