@@ -19,7 +19,7 @@
  * launch was accepted.  Calls on different streams may run concurrently,
  * except calls that use the per-device library workspace or its arrival
  * counters -- argmax, GEMM, decode, paged and FLUX attention, paged_plan,
- * verify_drafts, and GEMV with m > 1 (its K-slice partials and
+ * verify_drafts, lora_add, and GEMV with m > 1 (its K-slice partials and
  * arrival counters), of any format and size: those must not overlap on one
  * device (issue them on one stream, or order the streams).
  *
@@ -92,8 +92,8 @@ int rt_hip_init(int ordinal);
  * copies of f32 A and of a Q4_K weight shared by several M tiles, split-K
  * partials), the batched GEMV of every format (K-slice partials), decode
  * attention (split partials), FLUX and paged attention (the states of blocks cut
- * between workgroups), verify_drafts (the rows' sums) and argmax (8 bytes per
- * row).  It grows on demand (the reference likewise grows its Metal scratch on
+ * between workgroups), verify_drafts (the rows' sums), lora_add (sums over slices
+ * of k) and argmax (8 bytes per row).  It grows on demand (the reference likewise grows its Metal scratch on
  * demand, src/metal_ops.mm:378-423).  A
  * replaced buffer is kept until the process ends, because a hipGraph that
  * captured a call still writes the buffer that call used on every replay.
@@ -803,6 +803,48 @@ int rt_hip_verify_drafts(const void* logits, int64_t logit_stride, const void* d
 int64_t rt_hip_verify_drafts_workspace_bytes(int32_t vocab, int32_t n_seq, int32_t n_rows, int32_t max_draft,
                                              int32_t with_draft_logits);
 
+/* rt_hip_adjust_logits: logits [n_rows][vocab] (stride apart, F32 or BF16), in
+ * place, under what the requests' rules say, before rt_hip_verify_drafts or a draw.
+ * Rows and tokens are rt_hip_verify_drafts': row_start[s] .. row_start[s + 1] are
+ * request s's last accepted token and its drafts, row i of them predicting what
+ * follows its first i drafts.  With T the request's history, history[s][0 ..
+ * history_len[s]) of [n_seq][history_cols] (its last accepted token among it), and
+ * behind it tokens of its rows 1 .. i, a logit x of token v becomes, in f32 and
+ * in this order:
+ *   v in T:            x > 0 ? x / repetition[s] : x * repetition[s]
+ *   c > 0 times in T behind the history's first prompt_len[s] tokens (drafts always
+ *   are):              (x - frequency[s] * c) - presence[s]
+ *   v among bias_token[bias_start[s] .. bias_start[s + 1]):  x + the last such
+ *                      entry's bias
+ *   v's bit 0 in the row's mask:  -inf
+ * rounded once.  Rows of masks have bit v % 32 of word v / 32 for token v,
+ * mask_stride words from one to the next; row r has mask mask_row[r], none where that
+ * is no row of mask (-1), or mask r where mask_row is null.  Any pointer of the rules
+ * may be null: no history, no drafts (tokens), prompt 0, repetition 1, presence and
+ * frequency 0, no biases, no masks.  A repetition that is not above 0 counts as 1;
+ * tokens outside the vocabulary count for nothing.  What no rule changes is not
+ * written.  row_start must not decrease; a row that two requests claim is undefined.
+ * vocab <= 2^20, n_seq <= 4096, history_cols < 2^30. */
+typedef struct rt_hip_logit_rules {
+    const int32_t* history;
+    int64_t history_cols;
+    const int32_t* history_len;
+    const int32_t* prompt_len;
+    const float* repetition;
+    const float* presence;
+    const float* frequency;
+    const int32_t* bias_start;
+    const int32_t* bias_token;
+    const float* bias;
+    const uint32_t* mask;
+    int64_t mask_stride;
+    const int32_t* mask_row;
+    int32_t n_bias, n_masks;
+} rt_hip_logit_rules;
+int rt_hip_adjust_logits(void* logits, int64_t stride, int32_t dtype, int32_t vocab, const int32_t* row_start,
+                         int32_t n_seq, int32_t n_rows, const int32_t* tokens, const rt_hip_logit_rules* rules,
+                         rt_hip_stream stream);
+
 /* ---- linear dispatch ------------------------------------------------------
  * The QLinear / Linear2::fused_linear dispatch over whichever weight format
  * is loaded (src/qlinear.cpp:55-80, src/nn2.cpp:143-203: Q4Mat, Q4_K, BF16;
@@ -811,6 +853,33 @@ int64_t rt_hip_verify_drafts_workspace_bytes(int32_t vocab, int32_t n_seq, int32
  * added to every row (qlinear.cpp:42-53).  x is f32.  Every format at any M. */
 int rt_hip_linear_forward(int32_t format, const void* w, const float* bias, const float* x,
                           float* y, int64_t m, int64_t n, int64_t k, rt_hip_stream stream);
+
+/* ---- low-rank adapters beside a shared projection --------------------------
+ * No counterpart in the reference, whose weights are one model's.  Here the
+ * requests of a step share a projection (rt_hip_linear_forward, rt_hip_gemm ...)
+ * and each may have an adapter of its own: a [n_adapters][rank][k] and b
+ * [n_adapters][n][rank] of type dtype (RT_HIP_BF16 or RT_HIP_F16, 16-byte aligned),
+ * scale [n_adapters] f32, all in device memory.  (An adapter of a lower rank than
+ * the others' has zeros behind its own.)
+ * rt_hip_lora_add: rows row_start[s] .. row_start[s + 1] (as rt_hip_paged_plan's
+ * q_start) of y [n_rows][n] f32, what the projection has left, become
+ *   y += scale[i] * b[i] (a[i] x),   i = adapter[s],
+ * x [n_rows][k] of type x_dtype (F32, F16 or BF16).  Rows of requests whose adapter is
+ * none of them (-1), and rows outside every request, are left as they were.  Sums in
+ * f32, every factor with its 24 bits.  Deterministic.  rank is a multiple of 8 from 8 to
+ * 128, k a multiple of 8, k and n <= 2^20, n_rows <= 2^24, n_seq <= 4096; rows of x
+ * 16-byte aligned.  row_start must not decrease; a row that two requests claim is
+ * undefined.  Uses the library workspace (rt_hip_lora_workspace_bytes, to reserve
+ * before a graph capture; -1 for invalid sizes). */
+typedef struct rt_hip_lora {
+    const void* a;
+    const void* b;
+    const float* scale;
+    int32_t dtype, n_adapters, rank, k, n;
+} rt_hip_lora;
+int rt_hip_lora_add(float* y, int64_t y_stride, const void* x, int32_t x_dtype, int64_t x_stride, const rt_hip_lora* lora,
+                    const int32_t* row_start, const int32_t* adapter, int32_t n_seq, int32_t n_rows, rt_hip_stream stream);
+int64_t rt_hip_lora_workspace_bytes(const rt_hip_lora* lora, int32_t n_seq, int32_t n_rows);
 
 /* ---- launch-ceiling calibration --------------------------------------------
  * No counterpart in the reference: two kernels that do none of the path's

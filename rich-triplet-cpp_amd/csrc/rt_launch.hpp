@@ -334,6 +334,49 @@ hipError_t launch_paged_attention(const PagedAttn& p, void* part, uint32_t* coun
 // Over a cache of 4 bits (paged4_attention.hip).
 size_t paged4_attention_workspace(const PagedAttn& p);
 hipError_t launch_paged4_attention(const PagedAttn& p, void* part, uint32_t* counters, hipStream_t s);
+// Logits under penalties, biases and masks, in place (logits.hip).
+struct AdjustLogits {
+    void* logits = nullptr;  // rows of vocab values, stride apart
+    int64_t stride = 0;
+    int dtype = 0;           // RT_HIP_F32 or RT_HIP_BF16
+    int vocab = 0, n_seq = 0, n_rows = 0;
+    const int32_t* row_start = nullptr;    // [n_seq + 1]
+    const int32_t* tokens = nullptr;       // [n_rows] or null: no drafts
+    const int32_t* history = nullptr;      // [n_seq][history_cols] or null
+    int64_t history_cols = 0;
+    const int32_t* history_len = nullptr;  // [n_seq]
+    const int32_t* prompt_len = nullptr;   // [n_seq] or null: 0
+    const float* repetition = nullptr;     // [n_seq] or null: 1
+    const float* presence = nullptr;       // [n_seq] or null: 0
+    const float* frequency = nullptr;
+    const int32_t* bias_start = nullptr;   // [n_seq + 1]
+    const int32_t* bias_token = nullptr;   // [n_bias]
+    const float* bias = nullptr;           // [n_bias] or null: none
+    const uint32_t* mask = nullptr;        // [n_masks] rows of bits, mask_stride words apart, or null
+    int64_t mask_stride = 0;
+    const int32_t* mask_row = nullptr;     // [n_rows] or null: row r has mask r
+    int n_bias = 0, n_masks = 0;
+};
+hipError_t launch_adjust_logits(const AdjustLogits& p, hipStream_t s);
+// Adapters added to a projection's output (lora.hip); rank and k multiples of 8.
+struct LoraAdd {
+    float* y = nullptr;           // rows of n values, y_stride apart
+    const void* x = nullptr;      // rows of k values, x_stride apart
+    int64_t y_stride = 0, x_stride = 0;
+    int x_dtype = 0, w_dtype = 0;  // F32, F16 or BF16; F16 or BF16
+    const void* a = nullptr;      // [n_adapters][rank][k]
+    const void* b = nullptr;      // [n_adapters][n][rank]
+    const float* scale = nullptr; // [n_adapters]
+    int n_adapters = 0, rank = 0, k = 0, n = 0;
+    const int32_t* row_start = nullptr;  // [n_seq + 1]
+    const int32_t* adapter = nullptr;    // [n_seq]
+    int n_seq = 0, n_rows = 0;
+    float* part = nullptr;        // lora_workspace bytes
+    bool y_wide = false;          // four values of y from a multiple of four columns are 16-byte aligned, and n has whole fours
+    int slices = 0, k_slice = 0;  // (the launcher's)
+};
+size_t lora_workspace(int rank, int k, int n_seq, int n_rows);
+hipError_t launch_lora_add(LoraAdd p, hipStream_t s);
 // Drafted tokens against the target's distributions (verify.hip).
 struct VerifyDrafts {
     const void* logits = nullptr;        // rows of vocab values, logit_stride apart

@@ -382,3 +382,140 @@ int64_t rt_hip_verify_drafts_workspace_bytes(int32_t vocab, int32_t n_seq, int32
 }
 
 }  // extern "C"
+
+extern "C" {
+
+int rt_hip_adjust_logits(void* logits, int64_t stride, int32_t dtype, int32_t vocab, const int32_t* row_start,
+                         int32_t n_seq, int32_t n_rows, const int32_t* tokens, const rt_hip_logit_rules* rules,
+                         rt_hip_stream stream) {
+    const char* fn = "rt_hip_adjust_logits";
+    if (dtype != RT_HIP_F32 && dtype != RT_HIP_BF16) return fail(fn, RT_HIP_E_UNSUPPORTED, "logits must be F32 or BF16");
+    if (!rules) return fail(fn, RT_HIP_E_ARG, "null rules");
+    const rt_hip_logit_rules& u = *rules;
+    if (vocab < 1 || n_seq < 0 || n_rows < 0 || u.n_bias < 0 || u.n_masks < 0)
+        return fail(fn, RT_HIP_E_ARG, "negative size or no vocabulary");
+    if (vocab > kMaxVocab) return fail(fn, RT_HIP_E_SHAPE, "vocab must be at most 2^20");
+    if (n_seq > kPlanMaxSeq) return fail(fn, RT_HIP_E_SHAPE, "n_seq must be at most " + std::to_string(kPlanMaxSeq));
+    if (u.history && (!u.history_len || u.history_cols < 1)) return fail(fn, RT_HIP_E_ARG, "a history needs history_len and history_cols");
+    if (u.history && u.history_cols > 0x3fffffff) return fail(fn, RT_HIP_E_SHAPE, "history_cols must be below 2^30");
+    if (u.bias && (!u.bias_start || (u.n_bias > 0 && !u.bias_token))) return fail(fn, RT_HIP_E_ARG, "biases need bias_start and bias_token");
+    const int64_t words = (static_cast<int64_t>(vocab) + 31) / 32;
+    if (u.mask && u.mask_stride < words) return fail(fn, RT_HIP_E_ARG, "mask_stride below a row's words");
+    if (u.mask && !u.mask_row && u.n_masks < n_rows) return fail(fn, RT_HIP_E_ARG, "fewer masks than rows, and no mask_row");
+    if (n_seq == 0 || n_rows == 0) return RT_HIP_OK;
+    if (!logits || !row_start) return fail(fn, RT_HIP_E_ARG, "null pointer");
+    if (stride < vocab) return fail(fn, RT_HIP_E_ARG, "row stride below vocab");
+    const int64_t b = value_bytes(dtype), rows = n_rows, n = n_seq;
+    if (stride > 0x7fffffffffffLL / rows || (u.mask && u.n_masks > 0 && u.mask_stride > 0x7fffffffffffLL / u.n_masks))
+        return fail(fn, RT_HIP_E_SHAPE, "rows * stride must be below 2^47");
+    if (!aligned(logits, static_cast<uintptr_t>(b))) return fail(fn, RT_HIP_E_ALIGN, "logits must be aligned to their type");
+    const Range written = {logits, ((rows - 1) * stride + vocab) * b};
+    const Range read[] = {{row_start, 4 * (n + 1)}, {tokens, tokens ? 4 * rows : 0},
+                          {u.history, u.history ? 4 * n * u.history_cols : 0}, {u.history_len, u.history_len ? 4 * n : 0},
+                          {u.prompt_len, u.prompt_len ? 4 * n : 0}, {u.repetition, u.repetition ? 4 * n : 0},
+                          {u.presence, u.presence ? 4 * n : 0}, {u.frequency, u.frequency ? 4 * n : 0},
+                          {u.bias_start, u.bias ? 4 * (n + 1) : 0}, {u.bias_token, u.bias ? 4LL * u.n_bias : 0},
+                          {u.bias, u.bias ? 4LL * u.n_bias : 0},
+                          {u.mask, u.mask && u.n_masks > 0 ? 4 * ((u.n_masks - 1) * u.mask_stride + words) : 0},
+                          {u.mask_row, u.mask_row ? 4 * rows : 0}};
+    for (const Range& r : read)
+        if (overlap(written, r)) return fail(fn, RT_HIP_E_ARG, "logits overlap an input");
+    AdjustLogits p;
+    p.logits = logits;
+    p.stride = stride;
+    p.dtype = dtype;
+    p.vocab = vocab;
+    p.n_seq = n_seq;
+    p.n_rows = n_rows;
+    p.row_start = row_start;
+    p.tokens = tokens;
+    p.history = u.history;
+    p.history_cols = u.history_cols;
+    p.history_len = u.history_len;
+    p.prompt_len = u.prompt_len;
+    p.repetition = u.repetition;
+    p.presence = u.presence;
+    p.frequency = u.frequency;
+    p.bias_start = u.bias_start;
+    p.bias_token = u.bias_token;
+    p.bias = u.bias;
+    p.mask = u.mask;
+    p.mask_stride = u.mask_stride;
+    p.mask_row = u.mask_row;
+    p.n_bias = u.n_bias;
+    p.n_masks = u.n_masks;
+    return launched(fn, launch_adjust_logits(p, static_cast<hipStream_t>(stream)));
+}
+
+}  // extern "C"
+
+namespace {
+
+int lora_args(const char* fn, const rt_hip_lora* l, int32_t n_seq, int32_t n_rows) {
+    if (!l) return fail(fn, RT_HIP_E_ARG, "null adapters");
+    if (l->dtype != RT_HIP_BF16 && l->dtype != RT_HIP_F16) return fail(fn, RT_HIP_E_UNSUPPORTED, "adapters must be BF16 or F16");
+    if (l->n_adapters < 0 || n_seq < 0 || n_rows < 0) return fail(fn, RT_HIP_E_ARG, "negative size");
+    if (l->k < 1 || l->n < 1 || l->k > (1 << 20) || l->n > (1 << 20)) return fail(fn, RT_HIP_E_SHAPE, "k and n must be in [1, 2^20]");
+    if (l->rank < 8 || l->rank > 128) return fail(fn, RT_HIP_E_SHAPE, "rank must be in [8, 128]");
+    if (l->rank % 8 || l->k % 8) return fail(fn, RT_HIP_E_ALIGN, "rank and k must be multiples of 8");
+    if (n_seq > kPlanMaxSeq) return fail(fn, RT_HIP_E_SHAPE, "n_seq must be at most " + std::to_string(kPlanMaxSeq));
+    if (n_rows > (1 << 24)) return fail(fn, RT_HIP_E_SHAPE, "n_rows must be at most 2^24");
+    return RT_HIP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int rt_hip_lora_add(float* y, int64_t y_stride, const void* x, int32_t x_dtype, int64_t x_stride, const rt_hip_lora* lora,
+                    const int32_t* row_start, const int32_t* adapter, int32_t n_seq, int32_t n_rows, rt_hip_stream stream) {
+    const char* fn = "rt_hip_lora_add";
+    if (const int rc = lora_args(fn, lora, n_seq, n_rows)) return rc;
+    const rt_hip_lora& l = *lora;
+    if (!value_bytes(x_dtype)) return fail(fn, RT_HIP_E_UNSUPPORTED, "x must be F32, F16 or BF16");
+    if (n_seq == 0 || n_rows == 0 || l.n_adapters == 0) return RT_HIP_OK;
+    if (!y || !x || !row_start || !adapter || !l.a || !l.b || !l.scale) return fail(fn, RT_HIP_E_ARG, "null pointer");
+    if (y_stride < l.n || x_stride < l.k) return fail(fn, RT_HIP_E_ARG, "y_stride or x_stride below a row's values");
+    const int64_t rows = n_rows, xb = value_bytes(x_dtype), m = l.n_adapters;
+    if (y_stride > 0x7fffffffffffLL / rows || x_stride > 0x7fffffffffffLL / rows)
+        return fail(fn, RT_HIP_E_SHAPE, "n_rows * stride must be below 2^47");
+    if (!aligned(x, 16) || x_stride * xb % 16 || !aligned(l.a, 16) || !aligned(l.b, 16))
+        return fail(fn, RT_HIP_E_ALIGN, "rows of x, and a and b, must be 16-byte aligned");
+    if (!aligned(y, 4)) return fail(fn, RT_HIP_E_ALIGN, "y must be 4-byte aligned");
+    const Range written = {y, 4 * ((rows - 1) * y_stride + l.n)};
+    const Range read[] = {{x, ((rows - 1) * x_stride + l.k) * xb}, {l.a, 2 * m * l.rank * l.k}, {l.b, 2 * m * l.rank * l.n},
+                          {l.scale, 4 * m}, {row_start, 4 * (static_cast<int64_t>(n_seq) + 1)}, {adapter, 4 * static_cast<int64_t>(n_seq)}};
+    for (const Range& r : read)
+        if (overlap(written, r)) return fail(fn, RT_HIP_E_ARG, "y overlaps an input");
+    LoraAdd p;
+    p.y = y;
+    p.x = x;
+    p.y_stride = y_stride;
+    p.x_stride = x_stride;
+    p.x_dtype = x_dtype;
+    p.w_dtype = l.dtype;
+    p.a = l.a;
+    p.b = l.b;
+    p.scale = l.scale;
+    p.n_adapters = l.n_adapters;
+    p.rank = l.rank;
+    p.k = l.k;
+    p.n = l.n;
+    p.row_start = row_start;
+    p.adapter = adapter;
+    p.n_seq = n_seq;
+    p.n_rows = n_rows;
+    p.y_wide = aligned(y, 16) && y_stride % 4 == 0 && l.n % 4 == 0;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    hipError_t e;
+    p.part = static_cast<float*>(workspace(lora_workspace(l.rank, l.k, n_seq, n_rows), s, &e));
+    if (!p.part) return launched(fn, e);
+    return launched(fn, launch_lora_add(p, s));
+}
+
+int64_t rt_hip_lora_workspace_bytes(const rt_hip_lora* lora, int32_t n_seq, int32_t n_rows) {
+    if (lora_args("rt_hip_lora_workspace_bytes", lora, n_seq, n_rows)) return -1;
+    return n_seq == 0 || n_rows == 0 ? 0 : static_cast<int64_t>(lora_workspace(lora->rank, lora->k, n_seq, n_rows));
+}
+
+}  // extern "C"

@@ -31,6 +31,19 @@ class PagedKvStruct(C.Structure):
                 ("head_dim", _i32), ("page_stride", _i64)]
 
 
+class LogitRulesStruct(C.Structure):
+    """rt_hip_logit_rules (include/rt_hip.h)."""
+    _fields_ = [("history", _vp), ("history_cols", _i64), ("history_len", _vp), ("prompt_len", _vp), ("repetition", _vp),
+                ("presence", _vp), ("frequency", _vp), ("bias_start", _vp), ("bias_token", _vp), ("bias", _vp),
+                ("mask", _vp), ("mask_stride", _i64), ("mask_row", _vp), ("n_bias", _i32), ("n_masks", _i32)]
+
+
+class LoraStruct(C.Structure):
+    """rt_hip_lora (include/rt_hip.h)."""
+    _fields_ = [("a", _vp), ("b", _vp), ("scale", _vp), ("dtype", _i32), ("n_adapters", _i32), ("rank", _i32), ("k", _i32),
+                ("n", _i32)]
+
+
 # name -> argtypes (restype is int unless noted)
 _SIGNATURES = {
     "rt_hip_init": [C.c_int],
@@ -87,6 +100,8 @@ _SIGNATURES = {
     "rt_hip_paged_read": [C.POINTER(PagedKvStruct), _vp, _i32, _vp, _vp, _i32, _i64, _vp],
     "rt_hip_paged_attention": [_vp, _i32, _i64, _i32, C.POINTER(PagedKvStruct), _vp, _i64, _vp, _vp, _i32, _i32, _i32,
                                C.c_float, _i32, _vp, _i64, _vp],
+    "rt_hip_adjust_logits": [_vp, _i64, _i32, _i32, _vp, _i32, _i32, _vp, C.POINTER(LogitRulesStruct), _vp],
+    "rt_hip_lora_add": [_vp, _i64, _vp, _i32, _i64, C.POINTER(LoraStruct), _vp, _vp, _i32, _i32, _vp],
     "rt_hip_verify_drafts": [_vp, _i64, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp,
                              _vp],
 }
@@ -104,6 +119,7 @@ _SIZE_SIGNATURES = {
     "rt_hip_q4mat_scales_offset": [_i64, _i64],
     "rt_hip_paged_page_bytes": [_i32, _i32, _i32, _i32],
     "rt_hip_paged_attention_workspace_bytes": [C.POINTER(PagedKvStruct), _i32, _i32, _i32, _i32, _i32],
+    "rt_hip_lora_workspace_bytes": [C.POINTER(LoraStruct), _i32, _i32],
     "rt_hip_verify_drafts_workspace_bytes": [_i32, _i32, _i32, _i32, _i32],
 }
 
@@ -951,6 +967,150 @@ def verify_drafts(logits, tokens, row_start, accept_u, sample_u, max_draft: int,
              _value_type(logits), vocab, tokens.data_ptr(), row_start.data_ptr(), accept_u.data_ptr(),
              sample_u.data_ptr(), _ptr(temperature), n, rows, max_draft, out[0].data_ptr(), out[1].data_ptr())
     return out
+
+
+class LogitRules:
+    """What adjust_logits does to the requests' logits (tensors on one GPU, any of
+    them None): history [n_seq, cols] int32 with history_len [n_seq], prompt_len
+    [n_seq]; repetition, presence, frequency [n_seq] float32; bias [n] float32 with
+    bias_token [n] and bias_start [n_seq + 1]; mask [masks, words] int32, words at
+    least (vocab + 31) / 32, rows with any stride, and mask_row [rows], the row of
+    mask of each row of logits (-1: none).  The tensors are kept, and read when a call
+    runs: a program changes their contents from step to step."""
+
+    def __init__(self, history=None, history_len=None, prompt_len=None, repetition=None, presence=None, frequency=None,
+                 bias_start=None, bias_token=None, bias=None, mask=None, mask_row=None):
+        torch = _torch()
+        i32, f32 = torch.int32, torch.float32
+        if (history is None) != (history_len is None):
+            raise ValueError("rt_hip: a history needs history_len")
+        if len({x is None for x in (bias_start, bias_token, bias)}) > 1:
+            raise ValueError("rt_hip: biases need bias_start, bias_token and bias")
+        if mask_row is not None and mask is None:
+            raise ValueError("rt_hip: mask_row needs mask")
+        given = [t for t in (history, prompt_len, repetition, presence, frequency, bias, mask) if t is not None]
+        self.device = given[0].get_device() if given else None
+        self.n_seq = None
+        for t, name, dtype, shape in ((history, "history", i32, (None, None)), (history_len, "history_len", i32, (None,)),
+                                      (prompt_len, "prompt_len", i32, (None,)), (repetition, "repetition", f32, (None,)),
+                                      (presence, "presence", f32, (None,)), (frequency, "frequency", f32, (None,))):
+            if t is None:
+                continue
+            _want(self.device, (t, name, dtype, shape))
+            self._requests(t.shape[0])
+        if bias is not None:
+            _want(self.device, (bias_start, "bias_start", i32, (None,)), (bias, "bias", f32, (None,)),
+                  (bias_token, "bias_token", i32, tuple(bias.shape)))
+            self._requests(bias_start.shape[0] - 1)
+        self.words = self.rows = None
+        stride = masks = 0
+        if mask is not None:
+            if mask.dtype is not i32 or mask.dim() != 2 or (mask.shape[1] > 1 and mask.stride(1) != 1):
+                raise ValueError("rt_hip: mask must be dense rows of int32")
+            if self.device < 0 or mask.get_device() != self.device:
+                raise ValueError("rt_hip: mask must live on the GPU of the others")
+            masks, self.words = mask.shape
+            stride = mask.stride(0) if masks > 1 else self.words
+            if stride < self.words:
+                raise ValueError("rt_hip: the rows of mask overlap")
+            if mask_row is not None:
+                _want(self.device, (mask_row, "mask_row", i32, (None,)))
+                self.rows = mask_row.shape[0]
+        self.tensors = (history, history_len, prompt_len, repetition, presence, frequency, bias_start, bias_token, bias, mask,
+                        mask_row)
+        cols = 0 if history is None else history.shape[1]
+        self.struct = LogitRulesStruct(_ptr(history) if cols else None, cols, _ptr(history_len), _ptr(prompt_len),
+                                       _ptr(repetition), _ptr(presence), _ptr(frequency), _ptr(bias_start), _ptr(bias_token),
+                                       _ptr(bias), _ptr(mask), stride, _ptr(mask_row), 0 if bias is None else bias.shape[0],
+                                       masks)
+        self.ref = C.byref(self.struct)
+
+    def _requests(self, n: int) -> None:
+        if self.n_seq is None:
+            self.n_seq = n
+        if n != self.n_seq:
+            raise ValueError("rt_hip: the rules must be of one number of requests")
+
+
+def adjust_logits(logits, row_start, rules: LogitRules, tokens=None, stream=None):
+    """logits [rows, vocab], float32 or bfloat16, rows dense with any stride, in place
+    under the rules; tokens [rows]: the drafts, as verify_drafts takes them."""
+    i32 = _torch().int32
+    rows, vocab = logits.shape
+    n, device = row_start.shape[0] - 1, logits.get_device()
+    if device < 0:
+        raise ValueError("rt_hip: tensors must live on the GPU")
+    if rules.device is not None and rules.device != device:
+        raise ValueError("rt_hip: the rules must live on the GPU of logits")
+    if vocab > 1 and logits.stride(1) != 1:
+        raise ValueError("rt_hip: logits must be dense rows")
+    stride = logits.stride(0) if rows > 1 else vocab
+    _want(device, (row_start, "row_start", i32, (None,)))
+    if tokens is not None:
+        _want(device, (tokens, "tokens", i32, (rows,)))
+    if n < 0 or rules.n_seq not in (None, n):
+        raise ValueError(f"rt_hip: the rules are of {rules.n_seq} requests, row_start of {n}")
+    if rules.rows not in (None, rows):
+        raise ValueError("rt_hip: mask_row must have an entry for each row of logits")
+    if rules.words is not None and rules.words * 32 < vocab:
+        raise ValueError("rt_hip: the masks are shorter than the vocabulary")
+    _call_on(device, "rt_hip_adjust_logits", stream, logits.data_ptr(), stride, _value_type(logits), vocab,
+             row_start.data_ptr(), n, rows, _ptr(tokens), rules.ref)
+    return logits
+
+
+# ------------------------------------- adapters beside a shared projection --
+
+class Adapters:
+    """Low-rank adapters: a [n_adapters, rank, k] and b [n_adapters, n, rank], bfloat16
+    or float16, scale [n_adapters] float32."""
+
+    def __init__(self, a, b, scale):
+        torch = _torch()
+        if a.dim() != 3 or b.dim() != 3 or a.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError("rt_hip: adapters are a [n_adapters, rank, k] and b [n_adapters, n, rank], bfloat16 or float16")
+        m, rank, k = a.shape
+        self.device = a.get_device()
+        _want(self.device, (a, "a", a.dtype, (m, rank, k)), (b, "b", a.dtype, (m, None, rank)),
+              (scale, "scale", torch.float32, (m,)))
+        n = b.shape[1]
+        _fits(n_adapters=m, rank=rank, k=k, n=n)
+        self.a, self.b, self.scale = a, b, scale
+        self.struct = LoraStruct(a.data_ptr(), b.data_ptr(), scale.data_ptr(), _value_type(a), m, rank, k, n)
+        self.ref = C.byref(self.struct)
+
+
+def _dense_rows(device: int, t, name: str, cols: int) -> int:
+    """Stride in values between the rows of t [rows, cols], whose rows are dense."""
+    if t.dim() != 2 or t.shape[1] != cols:
+        raise ValueError(f"rt_hip: {name} must have shape (rows, {cols}), not {tuple(t.shape)}")
+    if device < 0 or t.get_device() != device:
+        raise ValueError(f"rt_hip: {name} must live on the GPU of the others" if t.is_cuda else
+                         "rt_hip: tensors must live on the GPU")
+    if cols > 1 and t.stride(1) != 1:
+        raise ValueError(f"rt_hip: the rows of {name} must be dense")
+    return t.stride(0) if t.shape[0] > 1 else cols
+
+
+def lora_add(y, x, adapters: Adapters, row_start, adapter, stream=None):
+    """y [rows, n] float32, a projection's output, in place: y += scale[i] * b[i] (a[i] x)
+    for the rows row_start[s] .. row_start[s + 1] of each request s, i = adapter[s] (-1:
+    none).  x [rows, k] float32, float16 or bfloat16; rows dense with any stride."""
+    torch = _torch()
+    c, device = adapters.struct, adapters.device
+    y_stride, x_stride = _dense_rows(device, y, "y", c.n), _dense_rows(device, x, "x", c.k)
+    rows, n_seq = y.shape[0], adapter.shape[0]
+    if y.dtype is not torch.float32 or x.shape[0] != rows:
+        raise ValueError("rt_hip: y must be float32 and have as many rows as x")
+    _want(device, (row_start, "row_start", torch.int32, (n_seq + 1,)), (adapter, "adapter", torch.int32, (n_seq,)))
+    _call_on(device, "rt_hip_lora_add", stream, y.data_ptr(), y_stride, x.data_ptr(), _value_type(x), x_stride, adapters.ref,
+             row_start.data_ptr(), adapter.data_ptr(), n_seq, rows)
+    return y
+
+
+def lora_workspace_bytes(adapters: Adapters, n_seq: int, rows: int) -> int:
+    _fits(n_seq=n_seq, rows=rows)
+    return int(library().lib.rt_hip_lora_workspace_bytes(adapters.ref, n_seq, rows))
 
 
 # ---------------------------------------------------------------- decoder --
