@@ -58,7 +58,7 @@ __global__ __launch_bounds__(256) void k_paged4_append(const S* __restrict__ k, 
     for (int e = 0; e < 8; ++e) {
         const float y = rintf((x[e] - bf) * steps) - 16.0f;
         const uint32_t code = static_cast<uint32_t>(fminf(fmaxf(y, 0.0f), 15.0f));
-        word |= code << (4 * (e >> 1) + 16 * (e & 1));
+        word |= code_at(code, e);
     }
     uint32_t ab = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, a)) | static_cast<uint32_t>(__builtin_bit_cast(uint16_t, b)) << 16;
     if (far != 0.0f) {
@@ -111,7 +111,7 @@ __global__ __launch_bounds__(256) void k_paged_read(PagedKv kv, const int32_t* _
                     base + P::value_numbers(in_page, kv.page_shift) + 8 * (w & ~3u) + 2 * (in_page & 7));
                 ab = num[0] | static_cast<uint32_t>(num[8]) << 16;
             }
-            const u32x4 y = values_of(word, ab);
+            const u32x4 y = Codes().word(word, ab);
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = f16_bits_to_f32(y[e >> 1] >> (16 * (e & 1)) & 0xffffu);
         } else {

@@ -82,9 +82,13 @@ struct Few {
     float m[RBLK], l[RBLK], c[RBLK];
     int last[RBLK], first[RBLK];
     int n, kg;
-    // the tile's codes and numbers, as they came from memory
-    uint32_t kc[2][SETS][WORDS], kn[2][SETS];
-    u32x4 vc[SETS][2], va[SETS], vb[SETS];
+    // A tile's codes and numbers, as they come from memory.
+    struct Tile {
+        uint32_t kc[2][SETS][WORDS], kn[2][SETS];
+        u32x4 vc[SETS][2], va[SETS], vb[SETS];
+        bool no_keys, no_values;  // this lane's group of 8 is on a page that is none
+    };
+    Codes codes;
 
     __device__ __forceinline__ void setup() {
         n = threadIdx.x & 15;
@@ -98,7 +102,20 @@ struct Few {
         else return t / 8 * 128 + 8 * (4 * kg + e) + 2 * (t & 3) + (t >> 2 & 1);
     }
 
-    __device__ __forceinline__ void load_q(int b, const Q* row, float c1) {
+    // A row of q as it is in memory, this lane's dims of it; zeros for null.
+    struct Row {
+        u32x4 x[STEPS][sizeof(Q) / 2];
+    };
+    __device__ __forceinline__ Row load_row(const Q* row) const {
+        Row r;
+#pragma unroll
+        for (int t = 0; t < STEPS; ++t)
+#pragma unroll
+            for (int i = 0; i < static_cast<int>(sizeof(Q)) / 2; ++i)
+                r.x[t][i] = row ? ld16(row + dim_q(t) + 4 * i) : u32x4{0, 0, 0, 0};
+        return r;
+    }
+    __device__ __forceinline__ void set_q(int b, const Row& row, float c1) {
         m[b] = -kInf;
         l[b] = 0.0f;
 #pragma unroll
@@ -106,18 +123,22 @@ struct Few {
         c[b] = c1;
         if constexpr (!kScaled) {
 #pragma unroll
-            for (int t = 0; t < STEPS; ++t) q[b][0][t] = row ? ld16(row + dim_q(t)) : u32x4{0, 0, 0, 0};
+            for (int t = 0; t < STEPS; ++t) q[b][0][t] = row.x[t][0];
         } else {
-            f32x4 x[STEPS][2];
+            auto two = [&](int t, int i) {
+                if constexpr (sizeof(Q) == 4) {
+                    const u32x4 w = row.x[t][i >> 1];
+                    return f32x2{__uint_as_float(w[2 * (i & 1)]), __uint_as_float(w[2 * (i & 1) + 1])};
+                } else {
+                    const uint32_t w = row.x[t][0][i];
+                    return f32x2{bf16_lo_to_f32(w), bf16_hi_to_f32(w)};
+                }
+            };
             float big = 0.0f;
 #pragma unroll
             for (int t = 0; t < STEPS; ++t)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    x[t][i] = row ? Limb::four(row + dim_q(t) + 4 * i) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) big = fmaxf(big, fabsf(x[t][i][e]));
-                }
+                for (int i = 0; i < 4; ++i) big = fmaxf(big, fmaxf(fabsf(two(t, i)[0]), fabsf(two(t, i)[1])));
             float up;
             c[b] = Limb::scaled(Limb::across_max(big), c1, &up);
 #pragma unroll
@@ -125,7 +146,7 @@ struct Few {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     uint32_t y[NL];
-                    Limb::limbs(x[t][i >> 1][2 * (i & 1)] * up, x[t][i >> 1][2 * (i & 1) + 1] * up, y);
+                    Limb::limbs(two(t, i)[0] * up, two(t, i)[1] * up, y);
 #pragma unroll
                     for (int k = 0; k < NL; ++k) q[b][k][t][i] = y[k];
                 }
@@ -133,55 +154,57 @@ struct Few {
     }
 
     // Loads of a tile's keys from key0 on; id: the page of this lane's group of
-    // 8, key0 + 8 (n / 4).  (Behind the last key that one again.)
-    __device__ __forceinline__ void load_keys(const Pages4& g, uint32_t key0, int id) {
-        const bool real = real_page(g, id);
-        const uint8_t* const page = g.k + static_cast<uint64_t>(static_cast<uint32_t>(id)) * g.page_bytes;
-        const uint8_t* const base = real ? page : reinterpret_cast<const uint8_t*>(kZeros);
-        const uint32_t group = key0 + 8u * (static_cast<uint32_t>(n) >> 2);
+    // 8, key0 + 8 (n / 4), behind the last key that one's.  (What is read there then
+    // is some of that page, and for a page that is none some of page 0.)
+    __device__ __forceinline__ void load_keys(Tile& x, const Pages4& g, uint32_t key0, int id) const {
+        x.no_keys = !real_page(g, id);
+        const uint8_t* const page = g.k + static_cast<uint64_t>(x.no_keys ? 0u : static_cast<uint32_t>(id)) * g.page_bytes;
+        const uint32_t slot = ((key0 + 8u * (static_cast<uint32_t>(n) >> 2)) & ((1u << g.shift) - 1)) + (static_cast<uint32_t>(n) & 3u);
+        const uint8_t* const at = page + (Page4<HD>::key_codes(slot) + kg * (W / 2));
+        const uint8_t* const num = page + (Page4<HD>::key_numbers(slot, g.shift) + (HD == 64 ? kg >> 1 : kg) * 4);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const uint32_t key = min(group + 4u * j + (static_cast<uint32_t>(n) & 3u), static_cast<uint32_t>(g.end));
-            const uint32_t slot = key & ((1u << g.shift) - 1);
-            const uint32_t codes = real ? Page4<HD>::key_codes(slot) + kg * (W / 2) : 0u;
-            const uint32_t numbers = real ? Page4<HD>::key_numbers(slot, g.shift) + (HD == 64 ? kg >> 1 : kg) * 4 : 0u;
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int u = 0; u < SETS; ++u) {
                 if constexpr (WORDS == 4) {
-                    const u32x4 x = *(const GLOBAL_AS u32x4*)(base + codes + 64 * u);
+                    const u32x4 y = *(const GLOBAL_AS u32x4*)(at + Page4<HD>::key_codes(4 * j) + 64 * u);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) kc[j][u][i] = x[i];
+                    for (int i = 0; i < 4; ++i) x.kc[j][u][i] = y[i];
                 } else {
-                    const u32x2 x = *(const GLOBAL_AS u32x2*)(base + codes);
+                    const u32x2 y = *(const GLOBAL_AS u32x2*)(at + Page4<HD>::key_codes(4 * j));
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) kc[j][u][i] = x[i];
+                    for (int i = 0; i < 2; ++i) x.kc[j][u][i] = y[i];
                 }
-                kn[j][u] = *(const GLOBAL_AS uint32_t*)(base + numbers + 16 * u);
+                x.kn[j][u] = *(const GLOBAL_AS uint32_t*)(num + 4 * j * (Page4<HD>::kGroups * 4) + 16 * u);
             }
-        }
     }
     // Loads of the values; id: the page of this lane's group of 8, key0 + 8 kg.
-    __device__ __forceinline__ void load_values(const Pages4& g, uint32_t key0, int id) {
-        const bool real = real_page(g, id);
-        const uint8_t* const page = g.v + static_cast<uint64_t>(static_cast<uint32_t>(id)) * g.page_bytes;
-        const uint8_t* const base = real ? page : reinterpret_cast<const uint8_t*>(kZeros);
-        const uint32_t slot = min(key0 + 8u * kg, static_cast<uint32_t>(g.end)) & ((1u << g.shift) - 1);
+    __device__ __forceinline__ void load_values(Tile& x, const Pages4& g, uint32_t key0, int id) const {
+        x.no_values = !real_page(g, id);
+        const uint8_t* const page = g.v + static_cast<uint64_t>(x.no_values ? 0u : static_cast<uint32_t>(id)) * g.page_bytes;
+        const uint32_t slot = (key0 + 8u * kg) & ((1u << g.shift) - 1);
         const int word = HD == 64 ? n >> 1 : n;
-        const uint32_t codes = real ? Page4<HD>::value_codes(slot) + 32 * word : 0u;
-        const uint32_t numbers = real ? Page4<HD>::value_numbers(slot, g.shift) + 32 * (word >> 2) : 0u;
+        const uint8_t* const at = page + (Page4<HD>::value_codes(slot) + 32 * word);
+        const uint8_t* const num = page + (Page4<HD>::value_numbers(slot, g.shift) + 32 * (word >> 2));
 #pragma unroll
         for (int u = 0; u < SETS; ++u) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) vc[u][i] = *(const GLOBAL_AS u32x4*)(base + codes + 512 * u + 16 * i);
-            va[u] = *(const GLOBAL_AS u32x4*)(base + numbers + 128 * u);
-            vb[u] = *(const GLOBAL_AS u32x4*)(base + numbers + 128 * u + 16);
+            for (int i = 0; i < 2; ++i) x.vc[u][i] = *(const GLOBAL_AS u32x4*)(at + 512 * u + 16 * i);
+            x.va[u] = *(const GLOBAL_AS u32x4*)(num + 128 * u);
+            x.vb[u] = *(const GLOBAL_AS u32x4*)(num + 128 * u + 16);
         }
     }
 
     __device__ __forceinline__ static f32x4 mma(u32x4 a, u32x4 b, f32x4 x) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), x, 0, 0, 0);
     }
-    __device__ __forceinline__ void scores() {
+    __device__ __forceinline__ void scores(Tile& x) {
+        if (__builtin_amdgcn_ballot_w64(x.no_keys) != 0) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int u = 0; u < SETS; ++u) x.kn[j][u] = x.no_keys ? 0u : x.kn[j][u];
+        }
 #pragma unroll
         for (int b = 0; b < RBLK; ++b)
 #pragma unroll
@@ -190,7 +213,7 @@ struct Few {
         for (int t = 0; t < STEPS; ++t)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const u32x4 a = values_of(kc[j][t / WORDS][t % WORDS], kn[j][t / WORDS]);
+                const u32x4 a = codes.word(x.kc[j][t / WORDS][t % WORDS], x.kn[j][t / WORDS]);
 #pragma unroll
                 for (int k = NL - 1; k >= 0; --k)
 #pragma unroll
@@ -245,7 +268,7 @@ struct Few {
     }
     // a and b made 0 for values that are no numbers and for keys behind `end`
     // (what is there was never written); whether some of the first were met.
-    __device__ __forceinline__ bool clean(int key, int end) {
+    __device__ __forceinline__ bool clean(Tile& x, int key, int end) const {
         bool any = false;
 #pragma unroll
         for (int u = 0; u < SETS; ++u)
@@ -253,43 +276,54 @@ struct Few {
             for (int i = 0; i < 8; ++i) {
                 const int sh = 16 * (i & 1);
                 const bool behind = key + 8 * kg + i > end;
-                const bool bad = no_number(va[u][i >> 1] >> sh, vb[u][i >> 1] >> sh);
+                const bool bad = no_number(x.va[u][i >> 1] >> sh, x.vb[u][i >> 1] >> sh);
                 any |= bad && !behind;
                 const uint32_t keep = bad || behind ? ~(0xffffu << sh) : ~0u;
-                va[u][i >> 1] &= keep;
-                vb[u][i >> 1] &= keep;
+                x.va[u][i >> 1] &= keep;
+                x.vb[u][i >> 1] &= keep;
             }
         return any;
     }
     // o += P V.  Two keys' words are exchanged by halves, so that each has the
     // same four values of both.
-    __device__ __forceinline__ void pv() {
+    __device__ __forceinline__ void pv(Tile& tile) {
+        if (__builtin_amdgcn_ballot_w64(tile.no_values) != 0) {
+#pragma unroll
+            for (int u = 0; u < SETS; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    tile.va[u][i] = tile.no_values ? 0u : tile.va[u][i];
+                    tile.vb[u][i] = tile.no_values ? 0u : tile.vb[u][i];
+                }
+        }
 #pragma unroll
         for (int u = 0; u < SETS; ++u)
 #pragma unroll
             for (int h = 0; h < (HD == 64 ? 1 : 2); ++h) {
+                const bool high = HD == 64 ? (n & 1) != 0 : h != 0;
+                const uint32_t sel = high ? 0x07060302u : 0x05040100u, swapped = high ? 0x06070203u : 0x04050001u;
                 uint32_t x[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t even = vc[u][i >> 1][2 * (i & 1)], odd = vc[u][i >> 1][2 * (i & 1) + 1];
-                    const uint32_t sel = HD == 64 ? (n & 1 ? 0x07060302u : 0x05040100u) : (h ? 0x07060302u : 0x05040100u);
-                    x[i] = __builtin_amdgcn_perm(odd, even, sel);
-                }
-                auto step = [&](int t, auto pair) {
-                    u32x4 a;
+                auto exchange = [&](uint32_t by) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        a[i] = pair(x[i], halves(va[u][i]), halves(vb[u][i]));
+                        x[i] = __builtin_amdgcn_perm(tile.vc[u][i >> 1][2 * (i & 1) + 1], tile.vc[u][i >> 1][2 * (i & 1)], by);
+                };
+                auto step = [&](int t, auto values) {
+                    u32x4 a;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) a[i] = values(x[i], halves(tile.va[u][i]), halves(tile.vb[u][i]));
 #pragma unroll
                     for (int k = NL - 1; k >= 0; --k)
 #pragma unroll
                         for (int b = 0; b < RBLK; ++b) o[b][t] = mma(a, w[b][k], o[b][t]);
                 };
                 const int t = u * 8 + h * 4;
-                step(t, [](uint32_t y, h2 a, h2 b) { return value_pair<0>(y, a, b); });
-                step(t + 1, [](uint32_t y, h2 a, h2 b) { return value_pair<1>(y, a, b); });
-                step(t + 2, [](uint32_t y, h2 a, h2 b) { return value_pair<2>(y, a, b); });
-                step(t + 3, [](uint32_t y, h2 a, h2 b) { return value_pair<3>(y, a, b); });
+                exchange(sel);
+                step(t, [&](uint32_t y, h2 a, h2 b) { return codes.template values<0>(y, a, b); });
+                step(t + 1, [&](uint32_t y, h2 a, h2 b) { return codes.template values<1>(y, a, b); });
+                step(t + 2, [&](uint32_t y, h2 a, h2 b) { return codes.template values<2>(y, a, b); });
+                exchange(swapped);
+                step(t + 3, [&](uint32_t y, h2 a, h2 b) { return codes.template values<3>(y, a, b); });
             }
     }
     // NaN to the rows that see `key` where its group of this lane's dims is no number.
@@ -307,17 +341,36 @@ struct Few {
     }
 };
 
-// LDS of it: the four waves' states, and at least the join's.
-constexpr int few_lds(int bm, int hd) {
-    return 4 * bm * hd * 4 > 256 * static_cast<int>(sizeof(State)) ? 4 * bm * hd * 4 : 256 * static_cast<int>(sizeof(State));
+// LDS of it: the waves' states, and at least the join's.
+constexpr int few_lds(int waves, int bm, int hd) {
+    const int join = waves * 64 * static_cast<int>(sizeof(State));
+    return waves * bm * hd * 4 > join ? waves * bm * hd * 4 : join;
 }
 
-// Workgroups of it that a CU holds: by the registers.
-constexpr int few_per_cu(int bm, int hd) { return bm == 16 && hd < 256 ? 3 : 2; }
+// A wave's priority goes down as its range is done, a step each quarter: a SIMD
+// serves its oldest wave first, and of as many ranges of one length some would end
+// at two thirds of the time and leave the others alone, with their latencies.
+struct Progress {
+    int quarter, until, level = 3;
+    __device__ __forceinline__ explicit Progress(int steps) : quarter(max(steps / 4, 1)), until(quarter) {
+        __builtin_amdgcn_s_setprio(3);
+    }
+    __device__ __forceinline__ void step() {
+        if (--until != 0) return;
+        until = quarter;
+        if (level == 3) __builtin_amdgcn_s_setprio(2);
+        else if (level == 2) __builtin_amdgcn_s_setprio(1);
+        else __builtin_amdgcn_s_setprio(0);
+        --level;
+    }
+};
 
-template <class Q, int HD, int RBLK>
-__global__ __launch_bounds__(256, few_per_cu(16 * RBLK, HD)) void k_paged4_narrow(PagedAttn p, Launch la) {
-    constexpr int NW = 4, DB = 16, BM = DB * RBLK, BK = 32, BN = NW * BK;
+// Workgroups of it that a CU holds: by the registers.
+constexpr int few_per_cu(int waves, int bm, int hd) { return waves > 4 ? 1 : bm == 16 && hd < 256 ? 3 : 2; }
+
+template <class Q, int HD, int RBLK, int NW>
+__global__ __launch_bounds__(NW * 64, few_per_cu(NW, 16 * RBLK, HD)) void k_paged4_narrow(PagedAttn p, Launch la) {
+    constexpr int DB = 16, BM = DB * RBLK, BK = 32, BN = NW * BK, NT = NW * 64;
     using C = Few<Q, HD, RBLK>;
     constexpr int kPart = part_floats(BM, HD);
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];  // the waves' states; a join's results
@@ -326,14 +379,18 @@ __global__ __launch_bounds__(256, few_per_cu(16 * RBLK, HD)) void k_paged4_narro
     __shared__ int flag;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int nw = gridDim.x, w = place_of(blockIdx.x, nw);
-    constexpr int EXTRA = 4;  // tiles that take as long as an item's start and end
+        // Tiles that take as long as an item's start and end.  (64 requests decoding, head_dim
+    // 128 in four waves, us: 64.9 with 0, 58.0 with 1, 56.8 with 2, 56.1 with 4; 128 shorter
+    // ones 34.8, 30.4, 30.3, 32.7.  16 requests of 5 tokens in eight waves 34.0, 30.0, 29.2, 27.0.)
+    constexpr int EXTRA = NW == 4 ? 2 : 3;
     Walk<BM, BN, EXTRA> walk(p, la);
     int64_t skip = 0, per = 0;
-    int64_t left = find_range<256>(walk, w, nw, &skip, &per);
+    int64_t left = find_range<NT>(walk, w, nw, &skip, &per);
     int64_t item_at = w * per - skip + EXTRA;  // of the item's first tile in the sequence
     const float c1 = p.scale * kLog2e;
     C core;
     core.setup();
+    Progress progress(static_cast<int>(min(left, int64_t{0x7fffffff})));
     while ((left = uniform(left)) > 0) {
         walk.pin();
         const int from = uniform(static_cast<int>(skip));
@@ -352,40 +409,51 @@ __global__ __launch_bounds__(256, few_per_cu(16 * RBLK, HD)) void k_paged4_narro
         int nt = b - a;
         if (static_cast<int64_t>(key0) + static_cast<int64_t>(nt - 1) * BN >= hi) --nt;  // (the last tile's keys may end before this wave's)
         const uint32_t my_k = 8u * (core.n >> 2), my_v = 8u * core.kg;
-        int id_k = 0, id_v = 0;
-        if (nt > 0) {
-            const int k = page4_at(pages, key0 + my_k), v = page4_at(pages, key0 + my_v);
-            id_k = page4_at(pages, key0 + BN + my_k);
-            id_v = page4_at(pages, key0 + BN + my_v);
-            core.load_keys(pages, key0, k);
-            core.load_values(pages, key0, v);
-        }
+        int id_k = 0, id_v = 0;  // pages of the tile that is loaded next
+        typename C::Tile tile;
+        auto find = [&](int i) {
+            id_k = page4_at(pages, key0 + i * BN + my_k);
+            id_v = page4_at(pages, key0 + i * BN + my_v);
+        };
+        if (nt > 0) find(0);
+        // (q is asked for before the first tile, so that it can be made limbs of while that is on its way)
+        typename C::Row row_q[RBLK];
 #pragma unroll
         for (int i = 0; i < RBLK; ++i) {
             const int r = i * DB + core.n, row = row_first + r;
             const bool real = r < rows;
             const int t = walk.token(row);
-            core.load_q(i, real ? static_cast<const Q*>(p.q) + (walk.row0 + t) * p.q_stride +
-                                      (walk.kvh * walk.group + walk.head(row, t)) * HD
-                                : nullptr, c1);
+            row_q[i] = core.load_row(real ? static_cast<const Q*>(p.q) + (walk.row0 + t) * p.q_stride +
+                                                (walk.kvh * walk.group + walk.head(row, t)) * HD
+                                          : nullptr);
             core.last[i] = real ? pos0 + t : -1;
             core.first[i] = walk.first_seen(core.last[i]);
         }
+        if (nt > 0) {
+            core.load_keys(tile, pages, key0, id_k);
+            core.load_values(tile, pages, key0, id_v);
+            find(1);
+        }
+#pragma unroll
+        for (int i = 0; i < RBLK; ++i) core.set_q(i, row_q[i], c1);
         auto is_edge = [&](int key) { return key + BK - 1 > low_pos || (p.window && hi - 1 - key >= p.window); };
         bool special = false;
+        // (The loads of a tile go into the registers that the products before it have
+        // left.  With a second set, sent a whole tile ahead, 64 requests decoding took as long.)
         for (int i = 0; i < nt; ++i) {
             const uint32_t at = key0 + i * BN;
             const int key = static_cast<int>(at);
-            const bool edge = is_edge(key);
-            core.scores();
-            // (behind the last tile its last keys once more, for no one)
-            core.load_keys(pages, at + BN, id_k);
-            id_k = page4_at(pages, at + 2 * BN + my_k);
+            const bool edge = is_edge(key), more = i + 1 < nt;
+            progress.step();
+            core.scores(tile);
+            if (more) core.load_keys(tile, pages, at + BN, id_k);
             core.softmax(key, edge);
-            if (edge) special |= __builtin_amdgcn_ballot_w64(core.clean(key, hi - 1)) != 0;
-            core.pv();
-            core.load_values(pages, at + BN, id_v);
-            id_v = page4_at(pages, at + 2 * BN + my_v);
+            if (edge) special |= __builtin_amdgcn_ballot_w64(core.clean(tile, key, hi - 1)) != 0;
+            core.pv(tile);
+            if (more) {
+                core.load_values(tile, pages, at + BN, id_v);
+                find(i + 2);
+            }
         }
         if (special) {
             for (int i = 0; i < nt; ++i)
@@ -424,7 +492,7 @@ __global__ __launch_bounds__(256, few_per_cu(16 * RBLK, HD)) void k_paged4_narro
         const int first_wg = static_cast<int>(item_at / per), last_wg = static_cast<int>((item_at + walk.tiles - 1) / per);
         const bool cut = first_wg != last_wg;
         float* const part = la.part + (static_cast<int64_t>(w) * 2 + (w == first_wg)) * kPart;
-        for (int i = tid; i < rows * (HD / 4); i += 256) {
+        for (int i = tid; i < rows * (HD / 4); i += NT) {
             const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
             float M = -kInf, L = 0.0f;
 #pragma unroll
@@ -451,7 +519,7 @@ __global__ __launch_bounds__(256, few_per_cu(16 * RBLK, HD)) void k_paged4_narro
         }
         if (cut) {
             if (arrive(la.counters + first_wg, last_wg - first_wg + 1, &flag))
-                join_parts<Q, BM, HD, 256>(walk, first_wg, last_wg, rows, reinterpret_cast<State*>(lds));
+                join_parts<Q, BM, HD, NT>(walk, first_wg, last_wg, rows, reinterpret_cast<State*>(lds));
         }
         __syncthreads();  // the states are read
         item_at += walk.tiles + EXTRA;
@@ -463,13 +531,18 @@ __global__ __launch_bounds__(256, few_per_cu(16 * RBLK, HD)) void k_paged4_narro
 // As paged_attention.hip's, but for how tiles reach LDS: a lane's word of codes
 // and its numbers are loaded a step ahead into registers, and become 16 bytes of
 // the tile among the products.  LDS holds two tiles of K and two of V.
+// Keys of its tiles.  (At head_dim 256 the words on their way to 64 do not fit the
+// registers beside the rest.)
+constexpr int wide4_keys(int hd) { return hd == 256 ? 32 : 64; }
+
 template <class Q, int HD, int NW>
 __global__ __launch_bounds__(NW * 64) void k_paged4_wide(PagedAttn p, Launch la) {
-    constexpr int DB = 32, BM = DB * NW, BK = 64, BN = BK, NT = NW * 64;
+    constexpr int DB = 32, BM = DB * NW, BK = wide4_keys(HD), BN = BK, NT = NW * 64;
     using C = Core<Q, _Float16, HD, DB, 1, BK>;
     constexpr int COPIES = BK / C::RPI / NW;  // pieces of a tile of K, or of V, by each wave: RPI keys
+    constexpr int GROUPS = (COPIES * C::RPI + 7) / 8;
     constexpr int kPart = wide_part_floats(BM, HD);
-    static_assert(COPIES >= 1 && COPIES * NW * C::RPI == BK, "every wave has as many pieces");
+    static_assert(COPIES >= 1 && COPIES * NW * C::RPI == BK && (COPIES * C::RPI) % 8 == 0, "every wave has as many pieces, of whole groups");
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];  // two tiles of K, two of V
     __shared__ int special;  // the last of this workgroup's items whose v held what was made 0
     __shared__ int flag;
@@ -484,6 +557,7 @@ __global__ __launch_bounds__(NW * 64) void k_paged4_wide(PagedAttn p, Launch la)
     const float c1 = p.scale * kLog2e;
     if (tid == 0) special = -1;
     int item = 0;
+    const Codes codes;
     C core;
     core.setup();
     while ((left = uniform(left)) > 0) {
@@ -510,65 +584,90 @@ __global__ __launch_bounds__(NW * 64) void k_paged4_wide(PagedAttn p, Launch la)
         const uint32_t key0 = static_cast<uint32_t>(walk.tile0 + a) * BN;
         const int nt = hi > 0 ? b - a : 0;
         auto is_edge = [&](int key) { return key + BK - 1 > low_pos || (p.window && hi - 1 - key >= p.window); };
-        // This lane's key of piece x of tile i, behind the last one that one.
-        auto row_of = [&](int x) { return (wave * COPIES + x) * C::RPI + lane / C::CPR; };
-        auto key_of = [&](int i, int x) {
-            return min(key0 + static_cast<uint32_t>(i * BN + row_of(x)), static_cast<uint32_t>(pages.end));
+        // A wave's pieces of a tile are of GROUPS groups of 8 keys.  Where a group is, from
+        // the pages' first bytes, for the keys that are loaded next and for the
+        // values, a tile behind them; behind the last key its group.
+        struct Place {
+            int64_t codes, numbers;  // the first slot's; below 0: on a page that is none
         };
         uint32_t kc[COPIES], kn[COPIES], vc[COPIES], va[COPIES], vb[COPIES];
-        int id_k[COPIES], id_v[COPIES];
-        auto find_pages = [&](int i, int x) { return page4_at(pages, key_of(i, x)); };
-        auto fetch_k = [&](int i, int x) {
-            const int id = id_k[x], c = (lane % C::CPR) ^ C::swz_k(row_of(x));
-            const bool there = real_page(pages, id);
-            const uint32_t slot = key_of(i, x) & ((1u << pages.shift) - 1);
-            const uint8_t* const base = there ? pages.k + static_cast<uint64_t>(static_cast<uint32_t>(id)) * pages.page_bytes
-                                              : reinterpret_cast<const uint8_t*>(kZeros);
-            kc[x] = *(const GLOBAL_AS uint32_t*)(base + (there ? Page4<HD>::key_codes(slot) + 4 * c : 0u));
-            kn[x] = *(const GLOBAL_AS uint32_t*)(base + (there ? Page4<HD>::key_numbers(slot, pages.shift) + (c & ~3) : 0u));
+        int id[GROUPS];  // pages of the groups a tile further on
+        Place at_k[GROUPS], at_v[GROUPS];
+        auto group_of = [&](int i, int x) {
+            return min(key0 + static_cast<uint32_t>(i * BN + wave * COPIES * C::RPI + 8 * x), static_cast<uint32_t>(pages.end)) & ~7u;
         };
-        auto fetch_v = [&](int i, int x) {
-            const int id = id_v[x], c = (lane % C::CPR) ^ C::swz_v(row_of(x));
-            const bool there = real_page(pages, id);
-            const uint32_t slot = key_of(i, x) & ((1u << pages.shift) - 1);
-            const uint8_t* const base = there ? pages.v + static_cast<uint64_t>(static_cast<uint32_t>(id)) * pages.page_bytes
-                                              : reinterpret_cast<const uint8_t*>(kZeros);
-            vc[x] = *(const GLOBAL_AS uint32_t*)(base + (there ? Page4<HD>::value_codes(slot) + 32 * c + 4 * (slot & 7) : 0u));
-            const uint8_t* const num = base + (there ? Page4<HD>::value_numbers(slot, pages.shift) + 8 * (c & ~3) + 2 * (slot & 7) : 0u);
-            va[x] = *(const GLOBAL_AS uint16_t*)num;
-            vb[x] = *(const GLOBAL_AS uint16_t*)(num + 16);
+        auto find_pages = [&](int i) {
+#pragma unroll
+            for (int x = 0; x < GROUPS; ++x) id[x] = pages.table[group_of(i, x) >> pages.shift];
+        };
+        auto find_places = [&](int i) {
+#pragma unroll
+            for (int x = 0; x < GROUPS; ++x) {
+                const int page = uniform(id[x]);
+                const uint32_t slot = static_cast<uint32_t>(uniform(static_cast<int>(group_of(i, x)))) & ((1u << pages.shift) - 1);
+                const int64_t first = static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(page)) * pages.page_bytes);
+                at_v[x] = at_k[x];
+                at_k[x].codes = real_page(pages, page) ? first + Page4<HD>::key_codes(slot) : -1;
+                at_k[x].numbers = first + Page4<HD>::key_numbers(slot, pages.shift);
+            }
+        };
+        // (of a group of 8 values the words and the numbers start where those of 8 keys do)
+        static_assert(Page4<HD>::value_codes(8) == Page4<HD>::key_codes(8) &&
+                      Page4<HD>::value_numbers(8, 3) == Page4<HD>::key_numbers(8, 3), "one place for both");
+        const uint8_t* const none = reinterpret_cast<const uint8_t*>(kZeros);
+        // This lane's slot of a piece's group, and its word: as tiles lie in LDS.
+        auto slot_of = [&](int x) { return static_cast<uint32_t>((wave * COPIES + x) * C::RPI & 7) + static_cast<uint32_t>(lane / C::CPR); };
+        auto word_of = [&](int x, bool v) {
+            const int row = (wave * COPIES + x) * C::RPI + lane / C::CPR;
+            return static_cast<uint32_t>((lane % C::CPR) ^ (v ? C::swz_v(row) : C::swz_k(row)));
+        };
+        auto fetch_k = [&](int x) {
+            const Place& g = at_k[x * C::RPI / 8];
+            const uint8_t* const codes_at = g.codes < 0 ? none : pages.k + g.codes;
+            const uint8_t* const numbers_at = g.codes < 0 ? none : pages.k + g.numbers;
+            const uint32_t c = word_of(x, false);
+            kc[x] = *(const GLOBAL_AS uint32_t*)(codes_at + (Page4<HD>::key_codes(slot_of(x)) + 4 * c));
+            kn[x] = *(const GLOBAL_AS uint32_t*)(numbers_at + (slot_of(x) * (Page4<HD>::kGroups * 4) + (c & ~3u)));
+        };
+        auto fetch_v = [&](int x) {
+            const Place& g = at_v[x * C::RPI / 8];
+            const uint8_t* const codes_at = g.codes < 0 ? none : pages.v + g.codes;
+            const uint8_t* const numbers_at = g.codes < 0 ? none : pages.v + g.numbers;
+            const uint32_t c = word_of(x, true);
+            vc[x] = *(const GLOBAL_AS uint32_t*)(codes_at + (4 * slot_of(x) + 32 * c));
+            va[x] = *(const GLOBAL_AS uint16_t*)(numbers_at + (2 * slot_of(x) + 8 * (c & ~3u)));
+            vb[x] = *(const GLOBAL_AS uint16_t*)(numbers_at + (2 * slot_of(x) + 8 * (c & ~3u)) + 16);
         };
         auto put = [&](uint32_t tile, int x, u32x4 y) {
             *(LDS_AS u32x4*)(static_cast<uintptr_t>(tile + (wave * COPIES + x) * 1024 + lane * 16)) = y;
         };
-        auto put_k = [&](int slot, int x) { put(lds_at + slot * C::TB, x, values_of(kc[x], kn[x])); };
-        auto put_v = [&](int slot, int x, bool edge) {
+        auto put_k = [&](int slot, int x) { put(lds_at + slot * C::TB, x, codes.word(kc[x], kn[x])); };
+        auto put_v = [&](int slot, int x, int key, bool edge) {
             uint32_t ab = va[x] | vb[x] << 16;
             if (edge) {
+                // (what is behind the last key was never written, and is no one's)
+                const bool behind = key + (wave * COPIES + x) * C::RPI + lane / C::CPR > pages.end;
                 const bool bad = no_number(ab, ab >> 16);
-                if (__builtin_amdgcn_ballot_w64(bad) != 0) special = item;
+                if (__builtin_amdgcn_ballot_w64(bad && !behind) != 0) special = item;
                 ab = bad ? 0u : ab;
             }
-            put(lds_at + (2 + slot) * C::TB, x, values_of(vc[x], ab));
+            put(lds_at + (2 + slot) * C::TB, x, codes.word(vc[x], ab));
         };
         lds_barrier();  // (every wave is done with the item before)
         if (nt > 0) {
+            find_pages(0);
+            find_places(0);
+            find_pages(1);
 #pragma unroll
-            for (int x = 0; x < COPIES; ++x) id_k[x] = find_pages(0, x);
+            for (int x = 0; x < COPIES; ++x) fetch_k(x);
 #pragma unroll
-            for (int x = 0; x < COPIES; ++x) {
-                fetch_k(0, x);
-                id_v[x] = id_k[x];
-                id_k[x] = find_pages(1, x);
-            }
+            for (int x = 0; x < COPIES; ++x) put_k(0, x);
+            find_places(1);
+            find_pages(2);
 #pragma unroll
-            for (int x = 0; x < COPIES; ++x) {
-                put_k(0, x);
-                fetch_v(0, x);
-                fetch_k(1, x);
-                id_v[x] = id_k[x];
-                id_k[x] = find_pages(2, x);
-            }
+            for (int x = 0; x < COPIES; ++x) fetch_v(x);
+#pragma unroll
+            for (int x = 0; x < COPIES; ++x) fetch_k(x);
         }
         core.load_q(0, real ? static_cast<const Q*>(p.q) + (walk.row0 + t) * p.q_stride + head : nullptr, c1);
         core.last[0] = real ? pos0 + t : -1;
@@ -595,15 +694,16 @@ __global__ __launch_bounds__(NW * 64) void k_paged4_wide(PagedAttn p, Launch la)
                 // after; scores of no tile are not used)
                 __builtin_amdgcn_s_setprio(1);
                 core.template products<2 * COPIES>(lds_at + now * C::TB, lds_at + (2 + (now ^ 1)) * C::TB, [&](int x) {
+                    if (x == 0) {
+                        find_places(i + 2);
+                        find_pages(i + 3);
+                    }
                     if (x < COPIES) {
-                        put_v(now, x, edge_v);
-                        fetch_v(i + 1, x);
+                        put_v(now, x, static_cast<int>(key0 + i * BN), edge_v);
+                        fetch_v(x);
                     } else {
-                        x -= COPIES;
-                        put_k(now ^ 1, x);
-                        fetch_k(i + 2, x);
-                        id_v[x] = id_k[x];
-                        id_k[x] = find_pages(i + 3, x);
+                        put_k(now ^ 1, x - COPIES);
+                        fetch_k(x - COPIES);
                     }
                 });
                 __builtin_amdgcn_s_setprio(0);
@@ -683,9 +783,21 @@ __global__ __launch_bounds__(NW * 64) void k_paged4_wide(PagedAttn p, Launch la)
 // Rows of a request up to which its keys are split over the waves.
 constexpr int kFewRows = 32;
 
-// Rows of a block of the few-row form; its workgroups, those the CUs hold at once.
+// Rows of a block of the few-row form; the waves of a workgroup; its workgroups,
+// those the CUs hold at once.  Where two waves to a SIMD are all that the
+// registers allow, they are one workgroup of eight or two of four: one has fewer
+// states to join across workgroups, two work on while one of them ends an item.
+// us, four and eight waves: blocks of 32 rows at head_dim 128, 16 requests of 5
+// tokens 34 and 27, 24 of 10 tokens 43 and 37.  head_dim 256: 64 and 128 items 21.5
+// and 17.6, 50 and 45; 512 items, 64 requests decoding, 62 and 72.
 int few_block(int64_t rows, int hd) { return rows <= 16 || hd == 256 ? 16 : 32; }
-int few_slots(int64_t rows, int hd) { return slots() * few_per_cu(few_block(rows, hd), hd); }
+int few_waves(const PagedAttn& p, int64_t rows) {
+    if (p.kv.head_dim < 256) return few_block(rows, p.kv.head_dim) == 16 ? 4 : 8;
+    return static_cast<int64_t>(p.n_seq) * p.kv.n_kv > slots() ? 4 : 8;
+}
+int few_slots(const PagedAttn& p, int64_t rows) {
+    return slots() * few_per_cu(few_waves(p, rows), few_block(rows, p.kv.head_dim), p.kv.head_dim);
+}
 
 // Whether blocks of 256 rows, eight waves, or of 128, four (as over 16-bit caches).
 bool eight_waves(const PagedAttn& p, int64_t rows) {
@@ -702,15 +814,24 @@ hipError_t run(const PagedAttn& p, float* part, uint32_t* counters, hipStream_t 
         la.min_rows = narrow ? kFewRows : 0;
         const bool eight = MOST == 8 && eight_waves(p, rows);
         hipLaunchKernelGGL((eight ? k_paged4_wide<Q, HD, MOST> : k_paged4_wide<Q, HD, 4>), dim3(static_cast<unsigned>(slots())),
-                           dim3(eight ? 512 : 256), 4 * 64 * HD * 2, s, p, la);
+                           dim3(eight ? 512 : 256), 4 * wide4_keys(HD) * HD * 2, s, p, la);
     }
     if (narrow) {
         la.min_rows = 0;
         la.max_rows = wide ? kFewRows : 0x7fffffff;
-        constexpr int MOST = HD == 256 ? 1 : 2;
-        const auto kernel = rows <= 16 ? k_paged4_narrow<Q, HD, 1> : k_paged4_narrow<Q, HD, MOST>;
-        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(few_slots(rows, HD))), dim3(256),
-                           few_lds(few_block(rows, HD), HD), s, p, la);
+        const unsigned grid = static_cast<unsigned>(few_slots(p, rows));
+        auto launch = [&](auto blocks, auto waves) {
+            constexpr int B = decltype(blocks)::value, NW = decltype(waves)::value;
+            hipLaunchKernelGGL((k_paged4_narrow<Q, HD, B, NW>), dim3(grid), dim3(NW * 64), few_lds(NW, 16 * B, HD), s, p, la);
+        };
+        using std::integral_constant;
+        if constexpr (HD < 256) {
+            if (few_block(rows, HD) == 16) launch(integral_constant<int, 1>(), integral_constant<int, 4>());
+            else launch(integral_constant<int, 2>(), integral_constant<int, 8>());
+        } else {
+            if (few_waves(p, rows) == 4) launch(integral_constant<int, 1>(), integral_constant<int, 4>());
+            else launch(integral_constant<int, 1>(), integral_constant<int, 8>());
+        }
     }
     return hipGetLastError();
 }
@@ -729,13 +850,13 @@ hipError_t run_hd(const PagedAttn& p, float* part, uint32_t* counters, hipStream
 size_t paged4_attention_workspace(const PagedAttn& p) {
     const int64_t rows = most_rows(p);
     const int hd = p.kv.head_dim, waves = hd < 256 ? 8 : 4;
-    const size_t narrow = static_cast<size_t>(few_slots(rows, hd)) * 2 * part_floats(few_block(rows, hd), hd);
+    const size_t narrow = static_cast<size_t>(few_slots(p, rows)) * 2 * part_floats(few_block(rows, hd), hd);
     const size_t wide = rows > kFewRows ? static_cast<size_t>(slots()) * 2 * wide_part_floats(waves * 32, hd) : 0;
     return (narrow > wide ? narrow : wide) * sizeof(float);
 }
 
 hipError_t launch_paged4_attention(const PagedAttn& p, void* part, uint32_t* counters, hipStream_t s) {
-    if (static_cast<size_t>(few_slots(1, 64)) > kArrivalCounters) return hipErrorInvalidValue;
+    if (static_cast<size_t>(few_slots(p, most_rows(p))) > kArrivalCounters) return hipErrorInvalidValue;
     float* const f = static_cast<float*>(part);
     if (p.dtype == RT_HIP_BF16) return run_hd<__bf16>(p, f, counters, s);
     if (p.dtype == RT_HIP_F16) return run_hd<_Float16>(p, f, counters, s);
