@@ -9,121 +9,180 @@
 // In place: only what changes is read and written, so a step without masks costs
 // its histories, and a masked row the store of its -inf.
 //
-// A workgroup has a request and kChunk tokens of the vocabulary: it counts the
+// A workgroup has a request and kChunk tokens of the vocabulary.  It counts the
 // whole history's tokens that fall into the chunk in LDS (integers: the order of
-// the additions does not matter), takes the last bias of each, and walks the
-// request's rows, a draft more counted for each.
+// the additions does not matter), takes the last bias of each, and lists the
+// tokens it met; then it goes through the request's rows with that list alone.  A
+// mask closes whole quads of tokens by one store and the rest one by one, so it
+// reads no logits, and list and mask never meet at a token.
 #include "rt_common.hpp"
 #include "rt_launch.hpp"
 
 namespace rt_hip {
 namespace {
 
-constexpr int kChunk = 4096, kThreads = 256;
-constexpr float kNone = -__builtin_inff();
+// (4032 tokens: four workgroups' counts, lists and entries fit a CU's LDS, with 4096
+// three; 64 requests, half of them masked: 17.2 and 20.3 us.  In workgroups of twice
+// the threads and tokens 22.4, of as many threads and half the tokens 19.4.)
+constexpr int kChunk = 4032, kThreads = 256;
+constexpr int kQuads = (kChunk / 4 + kThreads - 1) / kThreads;  // of a thread: four tokens each, kThreads * 4 apart
+constexpr uint32_t kListed = 1u << 31;
 
 __device__ __forceinline__ float load(const float* p) { return *p; }
-__device__ __forceinline__ float load(const __bf16* p) { return static_cast<float>(*p); }
+__device__ __forceinline__ float load(const __bf16* p) { return __uint_as_float(static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p)) << 16); }
 __device__ __forceinline__ void store(float* p, float x) { *p = x; }
-__device__ __forceinline__ void store(__bf16* p, float x) {
-    *reinterpret_cast<uint16_t*>(p) = f32_to_bf16_rne(x);
+__device__ __forceinline__ void store(__bf16* p, float x) { *reinterpret_cast<uint16_t*>(p) = f32_to_bf16_rne(x); }
+// -inf; four of them, at an address aligned to them.
+__device__ __forceinline__ void close(float* p) { *p = -__builtin_inff(); }
+__device__ __forceinline__ void close(__bf16* p) { *reinterpret_cast<uint16_t*>(p) = 0xff80u; }
+__device__ __forceinline__ void close4(float* p) {
+    *reinterpret_cast<u32x4*>(p) = u32x4{0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u};
 }
-// Four -inf, `p` aligned to them.
-__device__ __forceinline__ void close4(float* p) { *reinterpret_cast<f32x4*>(p) = f32x4{kNone, kNone, kNone, kNone}; }
 __device__ __forceinline__ void close4(__bf16* p) { *reinterpret_cast<u32x2*>(p) = u32x2{0xff80ff80u, 0xff80ff80u}; }
 
 template <class T>
 __global__ __launch_bounds__(kThreads) void k_adjust_logits(AdjustLogits p) {
-    __shared__ __attribute__((aligned(16))) uint32_t seen[kChunk];  // twice the count behind the prompt, 1: in the prompt
-    __shared__ __attribute__((aligned(16))) int entry[kChunk];      // 1 + the last bias entry, 0: none
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    // Per token of the chunk: kListed, twice the count behind the prompt, 1 if in the prompt ...
+    uint32_t* const seen = reinterpret_cast<uint32_t*>(lds);
+    uint16_t* const list = reinterpret_cast<uint16_t*>(seen + kChunk);   // the tokens met
+    uint32_t* const entry = reinterpret_cast<uint32_t*>(list + kChunk);  // ... 1 + the last bias entry (where there are biases)
+    __shared__ int listed, n_drafts;
+    __shared__ int draft_row[64], draft_at[64];  // the rows' drafts that fall into the chunk
     const int s = blockIdx.y, tid = threadIdx.x;
-    const int row0 = min(max(p.row_start[s], 0), p.n_rows);
-    const int rows = min(max(p.row_start[s + 1], row0), p.n_rows) - row0;
+    // (everything of the request at once: what is not there is read from row_start and not used)
+    const float* const some = reinterpret_cast<const float*>(p.row_start);
+    const int start = p.row_start[s], stop = p.row_start[s + 1];
+    const float rep0 = (p.repetition ? p.repetition : some)[s], pres0 = (p.presence ? p.presence : some)[s],
+                freq0 = (p.frequency ? p.frequency : some)[s];
+    const int32_t* const starts = p.bias ? p.bias_start : p.row_start;
+    const int bias0 = starts[s], bias1 = starts[s + 1];
+    const int len0 = (p.history ? p.history_len : p.row_start)[s], prompt0 = (p.prompt_len ? p.prompt_len : p.row_start)[s];
+    const int row0 = min(max(start, 0), p.n_rows);
+    const int rows = min(max(stop, row0), p.n_rows) - row0;
     if (rows == 0) return;
     const int base = static_cast<int>(blockIdx.x) * kChunk, here = min(kChunk, p.vocab - base);
-    float rep = p.repetition ? p.repetition[s] : 1.0f;
-    rep = rep > 0.0f ? rep : 1.0f;
-    const float pres = p.presence ? p.presence[s] : 0.0f, freq = p.frequency ? p.frequency[s] : 0.0f;
+    const float rep = p.repetition && rep0 > 0.0f ? rep0 : 1.0f;
+    const float pres = p.presence ? pres0 : 0.0f, freq = p.frequency ? freq0 : 0.0f;
+    const int len = p.history ? static_cast<int>(min(static_cast<int64_t>(max(len0, 0)), p.history_cols)) : 0;
+    const int prompt = p.prompt_len ? prompt0 : 0;
     const bool counts = rep != 1.0f || pres != 0.0f || freq != 0.0f;
-    int b0 = 0, b1 = 0;
-    if (p.bias) {
-        b0 = min(max(p.bias_start[s], 0), p.n_bias);
-        b1 = min(max(p.bias_start[s + 1], b0), p.n_bias);
-    }
+    const int b0 = p.bias ? min(max(bias0, 0), p.n_bias) : 0, b1 = p.bias ? min(max(bias1, b0), p.n_bias) : 0;
     const bool biased = b1 > b0;
+    T* const logits = static_cast<T*>(p.logits) + static_cast<int64_t>(row0) * p.stride + base;
+    auto mask_of = [&](int i) -> const uint32_t* {
+        const int m = !p.mask ? -1 : p.mask_row ? p.mask_row[row0 + i] : row0 + i;
+        return static_cast<uint32_t>(m) < static_cast<uint32_t>(p.n_masks) ? p.mask + m * p.mask_stride + base / 32 : nullptr;
+    };
+    const int32_t* const text = p.history + s * p.history_cols;
+    constexpr int kAhead = 8;  // loads in flight together
+    int x[kAhead];
+    auto ask = [&](int i) {
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) x[k] = i + k * kThreads < len ? text[i + k * kThreads] : -1;
+    };
+    int first_bias = -1, first_draft = -1;
     if (counts || biased) {
+        if (counts) ask(tid);
+        if (b0 + tid < b1) first_bias = p.bias_token[b0 + tid];
+        if (counts && p.tokens && 1 + tid < rows) first_draft = p.tokens[row0 + 1 + tid];
         for (int i = tid * 4; i < kChunk; i += kThreads * 4) {
             *reinterpret_cast<u32x4*>(seen + i) = u32x4{0, 0, 0, 0};
             if (biased) *reinterpret_cast<u32x4*>(entry + i) = u32x4{0, 0, 0, 0};
         }
-        __syncthreads();
-        if (counts && p.history) {
-            const int len = static_cast<int>(min(static_cast<int64_t>(max(p.history_len[s], 0)), p.history_cols));
-            const int prompt = p.prompt_len ? p.prompt_len[s] : 0;
-            const int32_t* const text = p.history + s * p.history_cols;
-            auto count = [&](int i, int token) {
-                const uint32_t at = static_cast<uint32_t>(token) - static_cast<uint32_t>(base);
-                if (at >= static_cast<uint32_t>(here)) return;  // (tokens below 0 too)
-                if (i < prompt) atomicOr(seen + at, 1u);
-                else atomicAdd(seen + at, 2u);
-            };
-            constexpr int kAhead = 8;  // loads in flight together
-            int i = tid;
-            for (; i + (kAhead - 1) * kThreads < len; i += kAhead * kThreads) {
-                int x[kAhead];
-#pragma unroll
-                for (int k = 0; k < kAhead; ++k) x[k] = text[i + k * kThreads];
-#pragma unroll
-                for (int k = 0; k < kAhead; ++k) count(i + k * kThreads, x[k]);
-            }
-            for (; i < len; i += kThreads) count(i, text[i]);
-        }
-        for (int i = b0 + tid; i < b1; i += kThreads) {
-            const uint32_t at = static_cast<uint32_t>(p.bias_token[i]) - static_cast<uint32_t>(base);
-            if (at < static_cast<uint32_t>(here)) atomicMax(entry + at, i - b0 + 1);
-        }
-        __syncthreads();
+        if (tid == 0) listed = n_drafts = 0;
     }
-    T* const logits = static_cast<T*>(p.logits) + base;
-    for (int r = row0; r < row0 + rows; ++r) {
-        if (r > row0 && counts && p.tokens) {
-            __syncthreads();  // (every thread is done with the row before)
-            const uint32_t at = static_cast<uint32_t>(p.tokens[r]) - static_cast<uint32_t>(base);
-            if (tid == 0 && at < static_cast<uint32_t>(here)) seen[at] += 2;
-            __syncthreads();
-        }
-        T* const row = logits + static_cast<int64_t>(r) * p.stride;
-        const uint32_t* mask = nullptr;
-        if (p.mask) {
-            const int m = p.mask_row ? p.mask_row[r] : r;
-            if (static_cast<uint32_t>(m) < static_cast<uint32_t>(p.n_masks)) mask = p.mask + m * p.mask_stride + base / 32;
-        }
-        if (!mask && !counts && !biased) continue;
-        const bool whole = (reinterpret_cast<uintptr_t>(row) & (4 * sizeof(T) - 1)) == 0;
-        for (int i = tid * 4; i < here; i += kThreads * 4) {
-            uint32_t open = mask ? mask[i / 32] >> (i % 32) & 15u : 15u;
-            const int n = min(4, here - i);
-            if (open == 0 && whole && n == 4) {
-                close4(row + i);
-                continue;
-            }
-            u32x4 t = {0, 0, 0, 0}, e = {0, 0, 0, 0};
-            if (counts) t = *reinterpret_cast<const u32x4*>(seen + i);
-            if (biased) e = *reinterpret_cast<const u32x4*>(entry + i);
+    // The masks, while the history is on its way.  (Four rows' words asked for
+    // together: one row 3.2 us instead of 2.4, drafts' rows no faster.)
+    if (p.mask) {
+        for (int i = 0; i < rows; ++i) {
+            const uint32_t* const mask = mask_of(i);
+            if (!mask) continue;
+            T* const row = logits + i * p.stride;
+            const bool aligned = (reinterpret_cast<uintptr_t>(row) & (4 * sizeof(T) - 1)) == 0;
+            uint32_t word[kQuads];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if (k >= n) break;
-                if (!(open >> k & 1)) {
-                    store(row + i + k, kNone);
-                } else if (t[k] | e[k]) {
-                    float x = load(row + i + k);
-                    if (t[k]) x = x > 0.0f ? x / rep : x * rep;
-                    if (t[k] > 1) x = (x - freq * static_cast<float>(t[k] >> 1)) - pres;
-                    if (e[k]) x += p.bias[b0 + static_cast<int>(e[k]) - 1];
-                    store(row + i + k, x);
+            for (int q = 0; q < kQuads; ++q) {
+                const int v = (q * kThreads + tid) * 4;
+                word[q] = v < here ? mask[v / 32] : ~0u;
+            }
+#pragma unroll
+            for (int q = 0; q < kQuads; ++q) {
+                const int v = (q * kThreads + tid) * 4;
+                const uint32_t open = word[q] >> (v % 32) & 15u;
+                if (open == 15u) continue;
+                if (open == 0 && aligned && v + 4 <= here) {
+                    close4(row + v);
+                } else {
+                    // (reading the quad and writing it back with its holes took 45 us where this takes 33)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (!(open >> k & 1) && v + k < here) close(row + v + k);
                 }
             }
         }
+    }
+    if (!counts && !biased) return;
+    __syncthreads();
+    // A token of the chunk is met: `as` says how (0: only to be listed).
+    auto meet = [&](uint32_t at, uint32_t as) {
+        if (!(atomicOr(seen + at, kListed | (as & 1u)) & kListed)) list[atomicAdd(&listed, 1)] = static_cast<uint16_t>(at);
+        if (as > 1) atomicAdd(seen + at, as);
+    };
+    auto in_chunk = [&](int token, uint32_t* at) {
+        *at = static_cast<uint32_t>(token) - static_cast<uint32_t>(base);  // (tokens below 0 too)
+        return *at < static_cast<uint32_t>(here);
+    };
+    uint32_t at;
+    if (counts) {
+        for (int i = tid; i < len; i += kAhead * kThreads) {
+            if (i != tid) ask(i);
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k)
+                if (in_chunk(x[k], &at)) meet(at, i + k * kThreads < prompt ? 1u : 2u);
+        }
+        if (p.tokens)
+            for (int i = 1 + tid; i < rows; i += kThreads)
+                if (in_chunk(i == 1 + tid ? first_draft : p.tokens[row0 + i], &at)) {
+                    meet(at, 0);
+                    const int d = atomicAdd(&n_drafts, 1);
+                    if (d < 64) draft_row[d] = i, draft_at[d] = static_cast<int>(at);
+                }
+    }
+    for (int i = b0 + tid; i < b1; i += kThreads)
+        if (in_chunk(i == b0 + tid ? first_bias : p.bias_token[i], &at)) {
+            meet(at, 0);
+            atomicMax(entry + at, static_cast<uint32_t>(i - b0 + 1));
+        }
+    __syncthreads();
+    const uint32_t n = static_cast<uint32_t>(listed);
+    const int drafts = n_drafts;
+    if (n == 0) return;
+    // A thread has a token of the list in a row; its mask and its logit are asked for together.
+    const uint32_t each = (n + 63) / 64 * 64;  // (a wave has one row)
+    for (uint64_t job = tid; job < static_cast<uint64_t>(each) * static_cast<uint32_t>(rows); job += kThreads) {
+        const int i = __builtin_amdgcn_readfirstlane(static_cast<int>(job / each));
+        const uint32_t at_list = static_cast<uint32_t>(job - static_cast<uint64_t>(i) * each);
+        if (at_list >= n) continue;
+        const uint32_t v = list[at_list];
+        T* const where = logits + i * p.stride + v;
+        const uint32_t* const mask = mask_of(i);
+        const uint32_t bits = mask ? mask[v / 32] : ~0u;
+        const float old = load(where);
+        const uint32_t e = biased ? entry[v] : 0u;
+        const float bias = e ? p.bias[b0 + static_cast<int>(e) - 1] : 0.0f;
+        uint32_t t = seen[v] & ~kListed;
+        if (drafts <= 64) {
+            for (int d = 0; d < drafts; ++d) t += draft_row[d] <= i && draft_at[d] == static_cast<int>(v) ? 2u : 0u;
+        } else {
+            for (int k = 1; k <= i; ++k) t += in_chunk(p.tokens[row0 + k], &at) && at == v ? 2u : 0u;
+        }
+        if (!(bits >> (v % 32) & 1) || (t | e) == 0) continue;
+        float y = old;
+        if (t) y = y > 0.0f ? y / rep : y * rep;
+        if (t > 1) y = (y - freq * static_cast<float>(t >> 1)) - pres;
+        if (e) y += bias;
+        store(where, y);
     }
 }
 
@@ -131,8 +190,9 @@ __global__ __launch_bounds__(kThreads) void k_adjust_logits(AdjustLogits p) {
 
 hipError_t launch_adjust_logits(const AdjustLogits& p, hipStream_t s) {
     const dim3 grid((static_cast<unsigned>(p.vocab) + kChunk - 1) / kChunk, static_cast<unsigned>(p.n_seq));
-    if (p.dtype == RT_HIP_F32) hipLaunchKernelGGL(k_adjust_logits<float>, grid, dim3(kThreads), 0, s, p);
-    else hipLaunchKernelGGL(k_adjust_logits<__bf16>, grid, dim3(kThreads), 0, s, p);
+    const size_t lds = kChunk * (sizeof(uint32_t) + sizeof(uint16_t) + (p.bias ? sizeof(uint32_t) : 0));
+    if (p.dtype == RT_HIP_F32) hipLaunchKernelGGL(k_adjust_logits<float>, grid, dim3(kThreads), lds, s, p);
+    else hipLaunchKernelGGL(k_adjust_logits<__bf16>, grid, dim3(kThreads), lds, s, p);
     return hipGetLastError();
 }
 
