@@ -20,8 +20,6 @@ namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kRows = 16;  // of a block
-
 __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
@@ -37,18 +35,29 @@ __device__ __forceinline__ Limbs limbs_of(f32x4 a, f32x4 b) {
     return {u32x4{h0[0], h0[1], h1[0], h1[1]}, u32x4{m0[0], m0[1], m1[0], m1[1]}, u32x4{l0[0], l0[1], l1[0], l1[1]}};
 }
 
-// c + w x for eight weights a lane, as they are in memory.
-template <class W>
-__device__ __forceinline__ f32x4 add_product(u32x4 w, const Limbs& x, f32x4 c) {
-    if constexpr (__is_same(W, __bf16)) {
+// Eight weights a lane: bf16 as they are in memory, f16 as two bf16 each.
+template <class W> struct Weights;
+template <> struct Weights<__bf16> {
+    u32x4 w;
+    __device__ __forceinline__ explicit Weights(u32x4 raw) : w(raw) {}
+    // c + w x, weights along the rows; along the columns.
+    __device__ __forceinline__ f32x4 times(const Limbs& x, f32x4 c) const {
         c = mma(w, x.l, c);
         c = mma(w, x.m, c);
         return mma(w, x.h, c);
-    } else {
-        u32x4 hi, lo;
+    }
+    __device__ __forceinline__ f32x4 under(const Limbs& x, f32x4 c) const {
+        c = mma(x.l, w, c);
+        c = mma(x.m, w, c);
+        return mma(x.h, w, c);
+    }
+};
+template <> struct Weights<_Float16> {
+    u32x4 hi, lo;
+    __device__ __forceinline__ explicit Weights(u32x4 raw) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t u = w[i];
+            const uint32_t u = raw[i];
             const float a = f16_bits_to_f32(u & 0xffffu), b = f16_bits_to_f32(u >> 16);
             const uint32_t top = bf16_pair(a, b);
             hi[i] = top;
@@ -57,38 +66,54 @@ __device__ __forceinline__ f32x4 add_product(u32x4 w, const Limbs& x, f32x4 c) {
             const float rb = fabsf(b) < 65520.0f ? b - bf16_hi_to_f32(top) : 0.0f;
             lo[i] = bf16_pair(ra, rb);
         }
+    }
+    __device__ __forceinline__ f32x4 times(const Limbs& x, f32x4 c) const {
         c = mma(hi, x.l, c);
         c = mma(lo, x.m, c);
         c = mma(hi, x.m, c);
         c = mma(lo, x.h, c);
         return mma(hi, x.h, c);
     }
+    __device__ __forceinline__ f32x4 under(const Limbs& x, f32x4 c) const {
+        c = mma(x.l, hi, c);
+        c = mma(x.m, lo, c);
+        c = mma(x.m, hi, c);
+        c = mma(x.h, lo, c);
+        return mma(x.h, hi, c);
+    }
+};
+
+// Eight values of x, as they are in memory, as limbs.
+template <class X>
+__device__ __forceinline__ Limbs limbs_at(const uint8_t* p) {
+    const u32x4 a = ld16(p);
+    if constexpr (sizeof(X) == 4) {
+        return limbs_of(__builtin_bit_cast(f32x4, a), *reinterpret_cast<const f32x4*>(p + 16));
+    } else if constexpr (__is_same(X, __bf16)) {
+        return {a, u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}};
+    } else {
+        f32x4 x, y;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t u = a[i], v = a[i + 2];
+            x[2 * i] = f16_bits_to_f32(u & 0xffffu);
+            x[2 * i + 1] = f16_bits_to_f32(u >> 16);
+            y[2 * i] = f16_bits_to_f32(v & 0xffffu);
+            y[2 * i + 1] = f16_bits_to_f32(v >> 16);
+        }
+        return limbs_of(x, y);
+    }
 }
 
-// Eight values of a row of x.
-__device__ __forceinline__ Limbs load_x(const float* p) {
-    return limbs_of(*reinterpret_cast<const f32x4*>(p), *reinterpret_cast<const f32x4*>(p + 4));
-}
-__device__ __forceinline__ Limbs load_x(const __bf16* p) {
-    return {ld16(p), u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}};
-}
-__device__ __forceinline__ Limbs load_x(const _Float16* p) {
-    const u32x4 u = ld16(p);
-    f32x4 a, b;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        a[2 * i] = f16_bits_to_f32(u[i] & 0xffffu);
-        a[2 * i + 1] = f16_bits_to_f32(u[i] >> 16);
-        b[2 * i] = f16_bits_to_f32(u[i + 2] & 0xffffu);
-        b[2 * i + 1] = f16_bits_to_f32(u[i + 2] >> 16);
-    }
-    return limbs_of(a, b);
-}
+// What a wave has stored to its part of LDS is there for all of its lanes (they
+// are served in order; this is for the compiler).
+__device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); }
 
 // Block `index` of the rows that have an adapter: its rows and that adapter.
 struct Block {
     int row, rows, adapter;
 };
+template <int kRows>
 __device__ __forceinline__ bool find_block(const LoraAdd& p, int index, Block* out) {
     const int lane = threadIdx.x & 63;
     int before = 0;
@@ -115,137 +140,276 @@ __device__ __forceinline__ bool find_block(const LoraAdd& p, int index, Block* o
     return false;
 }
 
-// t = A x of a block over a slice of k: RT tiles of 16 ranks.  The four waves
-// take 32 values of k in turn, and their sums are added in LDS.
-template <class X, class W, int RT>
+// Operands take one row to a lane, 16 lanes at 16 rows: loaded so, every lane's 16
+// bytes are an access of their own for the cache.  So waves load rows 64 bytes and
+// more at a time and turn them in LDS, each in a part of its own, its rows 16 bytes
+// apart for the banks.
+
+// t = A x of a block of 16 RB rows over a slice of k: RT tiles of 16 ranks.  The
+// four waves take 32 values of k in turn, and their sums are added in LDS.
+template <class X, class W, int RT, int RB>
 __global__ __launch_bounds__(256) void k_lora_shrink(LoraAdd p) {
-    __shared__ __attribute__((aligned(16))) f32x4 sums[3][RT][64];
+    constexpr int kAhead = RT * RB >= 8 ? 2 : 4;  // steps whose loads are in flight together
+    constexpr int XB = 32 * sizeof(X), XC = XB / 16, XL = 16 * RB * XC / 64;  // bytes of a row of x in a step, chunks, loads
+    constexpr int XS = XB + 16, WS = 64 + 16;  // bytes between rows in LDS
+    constexpr int kWave = 16 * RB * XS + 16 * RT * WS, kSums = 3 * RB * RT * 64 * 16;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kWave > kSums ? 4 * kWave : kSums];
     Block blk;
-    if (!find_block(p, blockIdx.x, &blk)) return;
+    if (!find_block<16 * RB>(p, blockIdx.x, &blk)) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, kg = lane >> 4;
     const int k0 = blockIdx.y * p.k_slice, k1 = min(p.k, k0 + p.k_slice);
-    const X* const x = static_cast<const X*>(p.x) + static_cast<int64_t>(blk.row + min(n, blk.rows - 1)) * p.x_stride;
-    const W* const a = static_cast<const W*>(p.a) + static_cast<int64_t>(blk.adapter) * p.rank * p.k;
-    f32x4 c[RT];
+    uint8_t* const xs = lds + wave * kWave;
+    uint8_t* const ws = xs + 16 * RB * XS;
+    // This lane's chunks: of row lane / XC (+ 64 / XC for each further load) of x, of rank lane / 4 (+ 16) of a.
+    const X* x[XL];
+    const W* a[RT];
+    bool there[XL];
 #pragma unroll
-    for (int t = 0; t < RT; ++t) c[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    // (rows past the block's repeat its last, ranks past the last repeat that: no one reads their sums)
-    for (int kk = k0 + wave * 32; kk < k1; kk += 128) {
-        const int at = kk + kg * 8;
-        const bool in = at < k1;
-        u32x4 w[RT];
-#pragma unroll
-        for (int t = 0; t < RT; ++t)
-            w[t] = in ? ld16(a + static_cast<int64_t>(min(t * 16 + n, p.rank - 1)) * p.k + at) : u32x4{0, 0, 0, 0};
-        const Limbs v = in ? load_x(x + at) : Limbs{u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}};
-#pragma unroll
-        for (int t = 0; t < RT; ++t) c[t] = add_product<W>(w[t], v, c[t]);
+    for (int i = 0; i < XL; ++i) {
+        const int row = i * (64 / XC) + lane / XC;
+        there[i] = row < blk.rows;
+        x[i] = static_cast<const X*>(p.x) + static_cast<int64_t>(blk.row + (there[i] ? row : 0)) * p.x_stride;
     }
-    if (wave > 0) {
+    // (ranks past the last repeat that: no one reads their sums)
 #pragma unroll
-        for (int t = 0; t < RT; ++t) sums[wave - 1][t][lane] = c[t];
+    for (int t = 0; t < RT; ++t)
+        a[t] = static_cast<const W*>(p.a) + (static_cast<int64_t>(blk.adapter) * p.rank + min(t * 16 + lane / 4, p.rank - 1)) * p.k;
+    f32x4 c[RB][RT];
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int t = 0; t < RT; ++t) c[b][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int kk = k0 + wave * 32; kk < k1; kk += 128 * kAhead) {
+        u32x4 w[kAhead][RT], v[kAhead][XL];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int at_x = kk + u * 128 + lane % XC * (16 / static_cast<int>(sizeof(X))), at_w = kk + u * 128 + lane % 4 * 8;
+#pragma unroll
+            for (int t = 0; t < RT; ++t) w[u][t] = at_w < k1 ? ld16(a[t] + at_w) : u32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < XL; ++i) v[u][i] = there[i] && at_x < k1 ? ld16(x[i] + at_x) : u32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            if (u > 0 && kk + u * 128 >= k1) break;
+            wave_fence();  // (the step before is read)
+#pragma unroll
+            for (int i = 0; i < XL; ++i)
+                *reinterpret_cast<u32x4*>(xs + (i * (64 / XC) + lane / XC) * XS + lane % XC * 16) = v[u][i];
+#pragma unroll
+            for (int t = 0; t < RT; ++t) *reinterpret_cast<u32x4*>(ws + (t * 16 + lane / 4) * WS + lane % 4 * 16) = w[u][t];
+            wave_fence();
+            Limbs l[RB];
+#pragma unroll
+            for (int b = 0; b < RB; ++b) l[b] = limbs_at<X>(xs + (b * 16 + n) * XS + kg * (8 * sizeof(X)));
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                const Weights<W> m(ld16(ws + (t * 16 + n) * WS + kg * 16));
+#pragma unroll
+                for (int b = 0; b < RB; ++b) c[b][t] = m.times(l[b], c[b][t]);
+            }
+        }
     }
     __syncthreads();
-    if (wave > 0 || n >= blk.rows) return;
-    float* const out = p.part + (static_cast<int64_t>(blockIdx.y) * p.n_rows + blk.row + n) * p.rank;
+    f32x4(*const sums)[RB][RT][64] = reinterpret_cast<f32x4(*)[RB][RT][64]>(lds);
+    if (wave > 0) {
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        const int r = t * 16 + kg * 4;  // (the rank is a multiple of 8)
-        if (r < p.rank) *reinterpret_cast<f32x4*>(out + r) = ((c[t] + sums[0][t][lane]) + sums[1][t][lane]) + sums[2][t][lane];
+        for (int b = 0; b < RB; ++b)
+#pragma unroll
+            for (int t = 0; t < RT; ++t) sums[wave - 1][b][t][lane] = c[b][t];
+    }
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        if (b * 16 + n >= blk.rows) continue;
+        float* const out = p.part + (static_cast<int64_t>(blockIdx.y) * p.n_rows + blk.row + b * 16 + n) * p.rank;
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            const int r = t * 16 + kg * 4;  // (the rank is a multiple of 8)
+            if (r < p.rank)
+                *reinterpret_cast<f32x4*>(out + r) = ((c[b][t] + sums[0][b][t][lane]) + sums[1][b][t][lane]) + sums[2][b][t][lane];
+        }
     }
 }
 
-// y += B t of a block over kCols columns: RS steps of 32 ranks.
-constexpr int kCols = 256;
-template <class W, int RS>
+// y += B t of a block over p.cols columns: RS steps of 32 ranks.  Rows of t along
+// the rows of the product, so that a lane has one column of four rows and 16
+// lanes 64 bytes of a row of y.
+template <class W, int RS, int RB>
 __global__ __launch_bounds__(256) void k_lora_expand(LoraAdd p) {
+    constexpr int kAhead = 2;  // tiles of 16 columns whose loads are in flight together
+    constexpr int TS = RS * 64 + 16, kT = 16 * RB * TS;  // bytes between rows of t, and of weights; of a limb of t
+    constexpr int kTile = 16 * TS, kWaves = 4 * kAhead * kTile;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[3 * kT > kWaves ? 3 * kT : kWaves];
     Block blk;
-    if (!find_block(p, blockIdx.x, &blk)) return;
+    if (!find_block<16 * RB>(p, blockIdx.x, &blk)) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, kg = lane >> 4;
-    const bool mine = n < blk.rows;
     const float scale = p.scale[blk.adapter];
-    Limbs t[RS];
-#pragma unroll
-    for (int q = 0; q < RS; ++q) {
-        const int r = q * 32 + kg * 8;
-        f32x4 lo = {0.0f, 0.0f, 0.0f, 0.0f}, hi = lo;
-        if (mine && r < p.rank)
-            for (int s = 0; s < p.slices; ++s) {
-                const float* const at = p.part + (static_cast<int64_t>(s) * p.n_rows + blk.row + n) * p.rank + r;
-                lo += *reinterpret_cast<const f32x4*>(at);
-                hi += *reinterpret_cast<const f32x4*>(at + 4);
-            }
-        t[q] = limbs_of(lo * scale, hi * scale);
+    // t of the block, the slices' sums added in order, as limbs in LDS; then in registers.
+    const int quads = p.rank / 4;
+    for (int i = threadIdx.x; i < 16 * RB * quads; i += 256) {
+        const int row = i / quads, r = (i - row * quads) * 4;
+        f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (row < blk.rows) {
+            const float* at = p.part + (static_cast<int64_t>(blk.row) + row) * p.rank + r;
+#pragma unroll 4
+            for (int s = 0; s < p.slices; ++s, at += static_cast<int64_t>(p.n_rows) * p.rank) sum += *reinterpret_cast<const f32x4*>(at);
+        }
+        u32x2 h, m, l;
+        bf16_limbs4(sum * scale, h, m, l);
+        uint8_t* const to = lds + row * TS + r * 2;
+        *reinterpret_cast<u32x2*>(to) = h;
+        *reinterpret_cast<u32x2*>(to + kT) = m;
+        *reinterpret_cast<u32x2*>(to + 2 * kT) = l;
     }
-    const W* const b = static_cast<const W*>(p.b) + static_cast<int64_t>(blk.adapter) * p.n * p.rank;
-    float* const y = p.y + static_cast<int64_t>(blk.row + (mine ? n : 0)) * p.y_stride;
-    const int c1 = min(p.n, (static_cast<int>(blockIdx.y) + 1) * kCols);
-    for (int c0 = blockIdx.y * kCols + wave * 16; c0 < c1; c0 += 64) {
-        f32x4 c = {0.0f, 0.0f, 0.0f, 0.0f};
+    __syncthreads();
+    Limbs t[RB][RS];
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
 #pragma unroll
         for (int q = 0; q < RS; ++q) {
-            const int r = q * 32 + kg * 8;
-            const u32x4 w = r < p.rank ? ld16(b + static_cast<int64_t>(min(c0 + n, p.n - 1)) * p.rank + r) : u32x4{0, 0, 0, 0};
-            c = add_product<W>(w, t[q], c);
+            const uint8_t* const at = lds + (b * 16 + n) * TS + q * 64 + kg * 16;
+            const bool in = q * 32 + kg * 8 < p.rank;
+            t[b][q].h = in ? ld16(at) : u32x4{0, 0, 0, 0};
+            t[b][q].m = in ? ld16(at + kT) : u32x4{0, 0, 0, 0};
+            t[b][q].l = in ? ld16(at + 2 * kT) : u32x4{0, 0, 0, 0};
         }
-        const int col = c0 + kg * 4;
-        if (!mine || col >= c1) continue;
-        if (p.y_wide) {
-            f32x4* const at = reinterpret_cast<f32x4*>(y + col);
-            *at += c;
-        } else {
+    __syncthreads();
+    // The weights of 16 columns are neighbours in memory: chunk i of them is column i / (rank / 8)'s.
+    const int chunks = p.rank / 8;
+    int col_of[RS], to_of[RS];  // of this lane's chunks: the column, the place in LDS
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (col + e < p.n) y[col + e] += c[e];
+    for (int q = 0; q < RS; ++q) {
+        const int i = q * 64 + lane;
+        col_of[q] = i / chunks;
+        to_of[q] = col_of[q] * TS + (i - col_of[q] * chunks) * 16;
+    }
+    uint8_t* const ws = lds + wave * (kAhead * kTile);
+    const W* const b0 = static_cast<const W*>(p.b) + static_cast<int64_t>(blk.adapter) * p.n * p.rank;
+    float* const y = p.y + static_cast<int64_t>(blk.row) * p.y_stride;
+    const int c1 = min(p.n, (static_cast<int>(blockIdx.y) + 1) * p.cols);
+    for (int c0 = blockIdx.y * p.cols + wave * (16 * kAhead); c0 < c1; c0 += 64 * kAhead) {
+        u32x4 w[kAhead][RS];
+        f32x4 old[kAhead][RB];
+        // Values of this lane in block b, tile u: rows 16 b + 4 kg + e.  (No row of the
+        // wave from the first past the block's on, as for single tokens 15 of 16.)
+        auto each = [&](auto f) {
+#pragma unroll
+            for (int b = 0; b < RB; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (b * 16 + e >= blk.rows) continue;
+                    const int row = b * 16 + 4 * kg + e;
+#pragma unroll
+                    for (int u = 0; u < kAhead; ++u)
+                        if (const int col = c0 + u * 16 + n; row < blk.rows && col < c1) f(u, b, e, y + row * p.y_stride + col);
+                }
+        };
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+            for (int q = 0; q < RS; ++q) {
+                const bool in = col_of[q] < 16 && c0 + u * 16 + col_of[q] < c1;
+                w[u][q] = in ? ld16(b0 + static_cast<int64_t>(c0 + u * 16) * p.rank + (q * 64 + lane) * 8) : u32x4{0, 0, 0, 0};
+            }
+        each([&](int u, int b, int e, const float* at) { old[u][b][e] = *at; });
+        wave_fence();  // (the tiles before are read)
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+            for (int q = 0; q < RS; ++q)
+                if (col_of[q] < 16) *reinterpret_cast<u32x4*>(ws + u * kTile + to_of[q]) = w[u][q];
+        wave_fence();
+        f32x4 c[kAhead][RB];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+#pragma unroll
+            for (int b = 0; b < RB; ++b) c[u][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int q = 0; q < RS; ++q) {
+                const bool in = q * 32 + kg * 8 < p.rank;
+                const Weights<W> m(in ? ld16(ws + u * kTile + n * TS + q * 64 + kg * 16) : u32x4{0, 0, 0, 0});
+#pragma unroll
+                for (int b = 0; b < RB; ++b) c[u][b] = m.under(t[b][q], c[u][b]);
+            }
         }
+        each([&](int u, int b, int e, float* at) { *at = old[u][b][e] + c[u][b][e]; });
     }
 }
 
-template <class X, class W>
-void shrink(const LoraAdd& p, dim3 grid, hipStream_t s) {
-    const auto kernel = p.rank <= 16 ? k_lora_shrink<X, W, 1> : p.rank <= 32 ? k_lora_shrink<X, W, 2>
-                        : p.rank <= 64 ? k_lora_shrink<X, W, 4> : k_lora_shrink<X, W, 8>;
-    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, p);
-}
-template <class W>
-void run(const LoraAdd& p, unsigned blocks, hipStream_t s) {
-    const dim3 slices(blocks, static_cast<unsigned>(p.slices));
-    switch (p.x_dtype) {
-        case RT_HIP_F32: shrink<float, W>(p, slices, s); break;
-        case RT_HIP_F16: shrink<_Float16, W>(p, slices, s); break;
-        default: shrink<__bf16, W>(p, slices, s);
-    }
-    const dim3 parts(blocks, (static_cast<unsigned>(p.n) + kCols - 1) / kCols);
-    const auto kernel = p.rank <= 32 ? k_lora_expand<W, 1> : p.rank <= 64 ? k_lora_expand<W, 2> : k_lora_expand<W, 4>;
-    hipLaunchKernelGGL(kernel, parts, dim3(256), 0, s, p);
-}
-
+// Blocks of 16 rows that a workgroup takes together, in each launch: two where
+// requests have as many rows on average, so that weights are read, and f16 ones
+// split, half as often.  (One in the first launch past rank 64, whose sums leave no
+// registers: 4000 rows at rank 128 61 us, with two 75.  Four in the second: 2700
+// rows at rank 64 62 us, with two 54.)
+int tall(int n_seq, int n_rows, int most) { return most == 2 && n_rows / n_seq >= 32 ? 2 : 1; }
+int tall_shrink(int rank, int n_seq, int n_rows) { return tall(n_seq, n_rows, rank > 64 ? 1 : 2); }
+int tall_expand(int n_seq, int n_rows) { return tall(n_seq, n_rows, 2); }
 // Blocks that there can be: every request's last may be partly empty.
-int64_t most_blocks(int n_seq, int n_rows) {
-    const int64_t b = (static_cast<int64_t>(n_rows) + kRows - 1) / kRows + n_seq - 1;
+int64_t most_blocks(int n_seq, int n_rows, int tall) {
+    const int64_t b = (static_cast<int64_t>(n_rows) + 16 * tall - 1) / (16 * tall) + n_seq - 1;
     return b < n_rows ? b : n_rows;
 }
-// Slices of k: as many workgroups as twice the CUs, of 512 values each at least.
-int slices_of(int n_seq, int n_rows, int k) {
-    const int64_t want = (2 * static_cast<int64_t>(device_info().cus) + most_blocks(n_seq, n_rows) - 1) / most_blocks(n_seq, n_rows);
-    const int64_t most = (static_cast<int64_t>(k) + 511) / 512;
+// Slices of k: so that there are two workgroups to a CU, of 512 values each at least.
+// (Every workgroup of the second launch reads all slices' sums of its rows: with
+// as many slices again 2048 rows at rank 16 are no faster, 4000 at rank 128 slower.)
+int slices_of(int rank, int n_seq, int n_rows, int k) {
+    const int64_t blocks = most_blocks(n_seq, n_rows, tall_shrink(rank, n_seq, n_rows));
+    const int64_t want = (2 * static_cast<int64_t>(device_info().cus) + blocks - 1) / blocks, most = (static_cast<int64_t>(k) + 511) / 512;
     return static_cast<int>(want < most ? want : most);
+}
+
+template <class X, class W, int RB>
+void shrink(const LoraAdd& p, dim3 grid, hipStream_t s) {
+    const auto kernel = p.rank <= 16 ? k_lora_shrink<X, W, 1, RB> : p.rank <= 32 ? k_lora_shrink<X, W, 2, RB>
+                        : p.rank <= 64 ? k_lora_shrink<X, W, 4, RB> : k_lora_shrink<X, W, 8, RB>;
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, p);
+}
+template <class X, class W>
+void shrink_rows(const LoraAdd& p, dim3 grid, hipStream_t s) {
+    if (tall_shrink(p.rank, p.n_seq, p.n_rows) == 2) shrink<X, W, 2>(p, grid, s);
+    else shrink<X, W, 1>(p, grid, s);
+}
+template <class W, int RB>
+void expand(const LoraAdd& p, dim3 grid, hipStream_t s) {
+    const auto kernel = p.rank <= 32 ? k_lora_expand<W, 1, RB> : p.rank <= 64 ? k_lora_expand<W, 2, RB> : k_lora_expand<W, 4, RB>;
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, p);
+}
+
+template <class W>
+void run(LoraAdd p, hipStream_t s) {
+    const dim3 slices(static_cast<unsigned>(most_blocks(p.n_seq, p.n_rows, tall_shrink(p.rank, p.n_seq, p.n_rows))), static_cast<unsigned>(p.slices));
+    switch (p.x_dtype) {
+        case RT_HIP_F32: shrink_rows<float, W>(p, slices, s); break;
+        case RT_HIP_F16: shrink_rows<_Float16, W>(p, slices, s); break;
+        default: shrink_rows<__bf16, W>(p, slices, s);
+    }
+    // Columns of a workgroup of the second launch: a multiple of its 128 of a step, so
+    // that there are at most four workgroups to a CU.  (With eight 2048 rows at rank 16
+    // take 27.4 us instead of 24.7, 64 decoding requests 15.8 instead of 15.3.)
+    const int rows = tall_expand(p.n_seq, p.n_rows);
+    const int64_t blocks = most_blocks(p.n_seq, p.n_rows, rows), steps = (static_cast<int64_t>(p.n) + 127) / 128;
+    const int64_t most = 4 * static_cast<int64_t>(device_info().cus), want = (blocks * steps + most - 1) / most;
+    p.cols = static_cast<int>(128 * (want < steps ? want : steps));
+    const dim3 parts(static_cast<unsigned>(blocks), (static_cast<unsigned>(p.n) + static_cast<unsigned>(p.cols) - 1) / static_cast<unsigned>(p.cols));
+    if (rows == 2) expand<W, 2>(p, parts, s);
+    else expand<W, 1>(p, parts, s);
 }
 
 }  // namespace
 
 size_t lora_workspace(int rank, int k, int n_seq, int n_rows) {
-    return static_cast<size_t>(slices_of(n_seq, n_rows, k)) * n_rows * rank * sizeof(float);
+    return static_cast<size_t>(slices_of(rank, n_seq, n_rows, k)) * n_rows * rank * sizeof(float);
 }
 
 hipError_t launch_lora_add(LoraAdd p, hipStream_t s) {
-    p.slices = slices_of(p.n_seq, p.n_rows, p.k);
+    p.slices = slices_of(p.rank, p.n_seq, p.n_rows, p.k);
     p.k_slice = ((p.k + p.slices - 1) / p.slices + 127) / 128 * 128;
-    const unsigned blocks = static_cast<unsigned>(most_blocks(p.n_seq, p.n_rows));
-    if (p.w_dtype == RT_HIP_BF16) run<__bf16>(p, blocks, s);
-    else run<_Float16>(p, blocks, s);
+    if (p.w_dtype == RT_HIP_BF16) run<__bf16>(p, s);
+    else run<_Float16>(p, s);
     return hipGetLastError();
 }
 

@@ -372,8 +372,7 @@ struct LoraAdd {
     const int32_t* adapter = nullptr;    // [n_seq]
     int n_seq = 0, n_rows = 0;
     float* part = nullptr;        // lora_workspace bytes
-    bool y_wide = false;          // four values of y from a multiple of four columns are 16-byte aligned, and n has whole fours
-    int slices = 0, k_slice = 0;  // (the launcher's)
+    int slices = 0, k_slice = 0, cols = 0;  // (the launcher's)
 };
 size_t lora_workspace(int rank, int k, int n_seq, int n_rows);
 hipError_t launch_lora_add(LoraAdd p, hipStream_t s);

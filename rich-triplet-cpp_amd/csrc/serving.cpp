@@ -505,7 +505,6 @@ int rt_hip_lora_add(float* y, int64_t y_stride, const void* x, int32_t x_dtype, 
     p.adapter = adapter;
     p.n_seq = n_seq;
     p.n_rows = n_rows;
-    p.y_wide = aligned(y, 16) && y_stride % 4 == 0 && l.n % 4 == 0;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     hipError_t e;
     p.part = static_cast<float*>(workspace(lora_workspace(l.rank, l.k, n_seq, n_rows), s, &e));
