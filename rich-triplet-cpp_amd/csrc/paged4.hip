@@ -69,13 +69,14 @@ __global__ __launch_bounds__(256) void k_paged4_append(const S* __restrict__ k, 
     uint8_t* const base = static_cast<uint8_t*>(blockIdx.y ? kv.v : kv.k) +
                           static_cast<uint64_t>(slot >> kv.page_shift) * static_cast<uint64_t>(kv.page_stride) +
                           (static_cast<uint32_t>(P::kSlotAll) << kv.page_shift) * head;
+    uint8_t* const codes = base + P::codes(in_page);
+    uint8_t* const numbers = base + P::numbers(in_page, kv.page_shift);
     if (blockIdx.y == 0) {
-        *reinterpret_cast<uint32_t*>(base + P::key_codes(in_page) + 4 * w) = word;
-        if (w % 4 == 0) *reinterpret_cast<uint32_t*>(base + P::key_numbers(in_page, kv.page_shift) + w) = ab;
+        *reinterpret_cast<uint32_t*>(codes + P::key_word(in_page & 7, w)) = word;
+        if (w % 4 == 0) *reinterpret_cast<uint32_t*>(numbers + P::key_number(in_page & 7, w / 4)) = ab;
     } else {
-        *reinterpret_cast<uint32_t*>(base + P::value_codes(in_page) + 32 * w + 4 * (in_page & 7)) = word;
-        uint16_t* const num = reinterpret_cast<uint16_t*>(base + P::value_numbers(in_page, kv.page_shift) + 8 * (w & ~3u) +
-                                                          2 * (in_page & 7));
+        *reinterpret_cast<uint32_t*>(codes + P::value_word(in_page & 7, w)) = word;
+        uint16_t* const num = reinterpret_cast<uint16_t*>(numbers + P::value_number(in_page & 7, w / 4));
         if (w % 4 == 0) num[0] = static_cast<uint16_t>(ab);
         if (w % 4 == 1) num[8] = static_cast<uint16_t>(ab >> 16);
     }
@@ -101,14 +102,15 @@ __global__ __launch_bounds__(256) void k_paged_read(PagedKv kv, const int32_t* _
             const uint32_t head = c / (HD / 8), w = c % (HD / 8);
             const uint8_t* const base = pages + static_cast<uint64_t>(slot >> kv.page_shift) * static_cast<uint64_t>(kv.page_stride) +
                                         (static_cast<uint32_t>(P::kSlotAll) << kv.page_shift) * head;
+            const uint8_t* const codes = base + P::codes(in_page);
+            const uint8_t* const numbers = base + P::numbers(in_page, kv.page_shift);
             uint32_t word, ab;
             if (blockIdx.y == 0) {
-                word = *reinterpret_cast<const uint32_t*>(base + P::key_codes(in_page) + 4 * w);
-                ab = *reinterpret_cast<const uint32_t*>(base + P::key_numbers(in_page, kv.page_shift) + (w & ~3u));
+                word = *reinterpret_cast<const uint32_t*>(codes + P::key_word(in_page & 7, w));
+                ab = *reinterpret_cast<const uint32_t*>(numbers + P::key_number(in_page & 7, w / 4));
             } else {
-                word = *reinterpret_cast<const uint32_t*>(base + P::value_codes(in_page) + 32 * w + 4 * (in_page & 7));
-                const uint16_t* const num = reinterpret_cast<const uint16_t*>(
-                    base + P::value_numbers(in_page, kv.page_shift) + 8 * (w & ~3u) + 2 * (in_page & 7));
+                word = *reinterpret_cast<const uint32_t*>(codes + P::value_word(in_page & 7, w));
+                const uint16_t* const num = reinterpret_cast<const uint16_t*>(numbers + P::value_number(in_page & 7, w / 4));
                 ab = num[0] | static_cast<uint32_t>(num[8]) << 16;
             }
             const u32x4 y = Codes().word(word, ab);

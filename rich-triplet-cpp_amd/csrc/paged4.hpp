@@ -9,16 +9,18 @@
 // less than half of the time that HBM takes to bring it.
 //
 // A page (page_size slots, n_kv heads) holds head after head; of a head first
-// the codes of its slots, then their groups' numbers:
-//   keys    codes [slot][hd / 8] words; numbers [slot][hd / 32] of a, b
-//   values  codes [slot / 8][hd / 8][slot % 8] words;
-//           numbers [slot / 8][hd / 32] of a [slot % 8], then b [slot % 8]
+// the codes of its slots, 8 slots after 8, then their groups' numbers.  Of 8 slots:
+//   keys    codes [hd / 32][slot % 8] of the group's four words; numbers
+//           [hd / 32][slot % 8] of a, b
+//   values  codes [slot / 4 % 2][hd / 8][slot % 4] words; numbers [hd / 32] of
+//           a [slot % 8], then b [slot % 8]
 // A word has eight neighbouring values' codes, 2 i in its low and 2 i + 1 in its
 // high half at bits 4 i + 2 (mod 16), so that of a half's four codes one is where
 // f16's top bits of mantissa are, two are a shift and one is an exchange of bytes away.
 // The matrix steps take keys along their dims and
-// values along 8 keys: either way a lane's operands are 16 and 32 neighbouring
-// bytes, and a token's codes are whole words, so that no two tokens share one.
+// values along 8 keys.  Either way four neighbouring lanes' operands are 64
+// neighbouring bytes (with a key's words together they were four accesses of the
+// cache), and a token's codes are whole words, so that no two tokens share one.
 #pragma once
 
 #include "rt_common.hpp"
@@ -33,16 +35,20 @@ struct Page4 {
     static constexpr int kSlot = HD / 2;                // bytes of a slot's codes
     static constexpr int kGroups = HD / 32;
     static constexpr int kSlotAll = HD / 2 + HD / 8;    // ... and of its numbers
-    // (bytes from the head's first)
-    __host__ __device__ __forceinline__ static constexpr uint32_t key_codes(uint32_t slot) { return slot * kSlot; }
-    __host__ __device__ __forceinline__ static constexpr uint32_t key_numbers(uint32_t slot, int page_shift) {
-        return (static_cast<uint32_t>(kSlot) << page_shift) + slot * (kGroups * 4);
-    }
-    // The 8 slots that `slot` is of: word w of slot i at 32 w + 4 i, numbers of group g at 32 g + 2 i (b: 16 on).
-    __host__ __device__ __forceinline__ static constexpr uint32_t value_codes(uint32_t slot) { return (slot >> 3) * (8 * kSlot); }
-    __host__ __device__ __forceinline__ static constexpr uint32_t value_numbers(uint32_t slot, int page_shift) {
+    // The codes, and the numbers, of the 8 slots that `slot` is of: bytes from the head's first.
+    __host__ __device__ __forceinline__ static constexpr uint32_t codes(uint32_t slot) { return (slot >> 3) * (8 * kSlot); }
+    __host__ __device__ __forceinline__ static constexpr uint32_t numbers(uint32_t slot, int page_shift) {
         return (static_cast<uint32_t>(kSlot) << page_shift) + (slot >> 3) * (kGroups * 32);
     }
+    // Word w and the numbers of group g of slot i of 8, from those; of a value a's (b: 16 on).
+    __host__ __device__ __forceinline__ static constexpr uint32_t key_word(uint32_t i, uint32_t w) {
+        return (w >> 2) * 128 + i * 16 + (w & 3) * 4;
+    }
+    __host__ __device__ __forceinline__ static constexpr uint32_t key_number(uint32_t i, uint32_t g) { return g * 32 + i * 4; }
+    __host__ __device__ __forceinline__ static constexpr uint32_t value_word(uint32_t i, uint32_t w) {
+        return (i >> 2) * (4 * kSlot) + w * 16 + (i & 3) * 4;
+    }
+    __host__ __device__ __forceinline__ static constexpr uint32_t value_number(uint32_t i, uint32_t g) { return g * 32 + i * 2; }
 };
 
 // (By value: the cast of a vector's element would read the vector's first.)

@@ -54,8 +54,8 @@ __device__ __forceinline__ uint32_t value_numbers_of(const Pages4& g, int key, i
     if (!real_page(g, id)) return 0;
     const uint32_t slot = key & ((1 << g.shift) - 1);
     const uint16_t* const at = reinterpret_cast<const uint16_t*>(
-        g.v + static_cast<uint64_t>(static_cast<uint32_t>(id)) * g.page_bytes + Page4<HD>::value_numbers(slot, g.shift) +
-        32 * grp + 2 * (slot & 7));
+        g.v + static_cast<uint64_t>(static_cast<uint32_t>(id)) * g.page_bytes + Page4<HD>::numbers(slot, g.shift) +
+        Page4<HD>::value_number(slot & 7, grp));
     return at[0] | static_cast<uint32_t>(at[8]) << 16;
 }
 
@@ -159,23 +159,25 @@ struct Few {
     __device__ __forceinline__ void load_keys(Tile& x, const Pages4& g, uint32_t key0, int id) const {
         x.no_keys = !real_page(g, id);
         const uint8_t* const page = g.k + static_cast<uint64_t>(x.no_keys ? 0u : static_cast<uint32_t>(id)) * g.page_bytes;
-        const uint32_t slot = ((key0 + 8u * (static_cast<uint32_t>(n) >> 2)) & ((1u << g.shift) - 1)) + (static_cast<uint32_t>(n) & 3u);
-        const uint8_t* const at = page + (Page4<HD>::key_codes(slot) + kg * (W / 2));
-        const uint8_t* const num = page + (Page4<HD>::key_numbers(slot, g.shift) + (HD == 64 ? kg >> 1 : kg) * 4);
+        const uint32_t slot = (key0 + 8u * (static_cast<uint32_t>(n) >> 2)) & ((1u << g.shift) - 1);
+        const uint32_t i0 = static_cast<uint32_t>(n) & 3u;  // the lane's slots of the eight: this and 4 on
+        const uint8_t* const at = page + (Page4<HD>::codes(slot) + Page4<HD>::key_word(i0, kg * WORDS));
+        const uint8_t* const num = page + (Page4<HD>::numbers(slot, g.shift) + Page4<HD>::key_number(i0, HD == 64 ? kg >> 1 : kg));
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int u = 0; u < SETS; ++u) {
+                const uint8_t* const codes_at = at + Page4<HD>::key_word(4 * j, 16 * u);
                 if constexpr (WORDS == 4) {
-                    const u32x4 y = *(const GLOBAL_AS u32x4*)(at + Page4<HD>::key_codes(4 * j) + 64 * u);
+                    const u32x4 y = *(const GLOBAL_AS u32x4*)codes_at;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) x.kc[j][u][i] = y[i];
                 } else {
-                    const u32x2 y = *(const GLOBAL_AS u32x2*)(at + Page4<HD>::key_codes(4 * j));
+                    const u32x2 y = *(const GLOBAL_AS u32x2*)codes_at;
 #pragma unroll
                     for (int i = 0; i < 2; ++i) x.kc[j][u][i] = y[i];
                 }
-                x.kn[j][u] = *(const GLOBAL_AS uint32_t*)(num + 4 * j * (Page4<HD>::kGroups * 4) + 16 * u);
+                x.kn[j][u] = *(const GLOBAL_AS uint32_t*)(num + Page4<HD>::key_number(4 * j, 4 * u));
             }
     }
     // Loads of the values; id: the page of this lane's group of 8, key0 + 8 kg.
@@ -184,14 +186,14 @@ struct Few {
         const uint8_t* const page = g.v + static_cast<uint64_t>(x.no_values ? 0u : static_cast<uint32_t>(id)) * g.page_bytes;
         const uint32_t slot = (key0 + 8u * kg) & ((1u << g.shift) - 1);
         const int word = HD == 64 ? n >> 1 : n;
-        const uint8_t* const at = page + (Page4<HD>::value_codes(slot) + 32 * word);
-        const uint8_t* const num = page + (Page4<HD>::value_numbers(slot, g.shift) + 32 * (word >> 2));
+        const uint8_t* const at = page + (Page4<HD>::codes(slot) + Page4<HD>::value_word(0, word));
+        const uint8_t* const num = page + (Page4<HD>::numbers(slot, g.shift) + Page4<HD>::value_number(0, word >> 2));
 #pragma unroll
         for (int u = 0; u < SETS; ++u) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) x.vc[u][i] = *(const GLOBAL_AS u32x4*)(at + 512 * u + 16 * i);
-            x.va[u] = *(const GLOBAL_AS u32x4*)(num + 128 * u);
-            x.vb[u] = *(const GLOBAL_AS u32x4*)(num + 128 * u + 16);
+            for (int i = 0; i < 2; ++i) x.vc[u][i] = *(const GLOBAL_AS u32x4*)(at + Page4<HD>::value_word(4 * i, 16 * u));
+            x.va[u] = *(const GLOBAL_AS u32x4*)(num + Page4<HD>::value_number(0, 4 * u));
+            x.vb[u] = *(const GLOBAL_AS u32x4*)(num + Page4<HD>::value_number(0, 4 * u) + 16);
         }
     }
 
@@ -607,13 +609,10 @@ __global__ __launch_bounds__(NW * 64) void k_paged4_wide(PagedAttn p, Launch la)
                 const uint32_t slot = static_cast<uint32_t>(uniform(static_cast<int>(group_of(i, x)))) & ((1u << pages.shift) - 1);
                 const int64_t first = static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(page)) * pages.page_bytes);
                 at_v[x] = at_k[x];
-                at_k[x].codes = real_page(pages, page) ? first + Page4<HD>::key_codes(slot) : -1;
-                at_k[x].numbers = first + Page4<HD>::key_numbers(slot, pages.shift);
+                at_k[x].codes = real_page(pages, page) ? first + Page4<HD>::codes(slot) : -1;
+                at_k[x].numbers = first + Page4<HD>::numbers(slot, pages.shift);
             }
         };
-        // (of a group of 8 values the words and the numbers start where those of 8 keys do)
-        static_assert(Page4<HD>::value_codes(8) == Page4<HD>::key_codes(8) &&
-                      Page4<HD>::value_numbers(8, 3) == Page4<HD>::key_numbers(8, 3), "one place for both");
         const uint8_t* const none = reinterpret_cast<const uint8_t*>(kZeros);
         // This lane's slot of a piece's group, and its word: as tiles lie in LDS.
         auto slot_of = [&](int x) { return static_cast<uint32_t>((wave * COPIES + x) * C::RPI & 7) + static_cast<uint32_t>(lane / C::CPR); };
@@ -626,17 +625,18 @@ __global__ __launch_bounds__(NW * 64) void k_paged4_wide(PagedAttn p, Launch la)
             const uint8_t* const codes_at = g.codes < 0 ? none : pages.k + g.codes;
             const uint8_t* const numbers_at = g.codes < 0 ? none : pages.k + g.numbers;
             const uint32_t c = word_of(x, false);
-            kc[x] = *(const GLOBAL_AS uint32_t*)(codes_at + (Page4<HD>::key_codes(slot_of(x)) + 4 * c));
-            kn[x] = *(const GLOBAL_AS uint32_t*)(numbers_at + (slot_of(x) * (Page4<HD>::kGroups * 4) + (c & ~3u)));
+            kc[x] = *(const GLOBAL_AS uint32_t*)(codes_at + Page4<HD>::key_word(slot_of(x), c));
+            kn[x] = *(const GLOBAL_AS uint32_t*)(numbers_at + Page4<HD>::key_number(slot_of(x), c >> 2));
         };
         auto fetch_v = [&](int x) {
             const Place& g = at_v[x * C::RPI / 8];
             const uint8_t* const codes_at = g.codes < 0 ? none : pages.v + g.codes;
             const uint8_t* const numbers_at = g.codes < 0 ? none : pages.v + g.numbers;
             const uint32_t c = word_of(x, true);
-            vc[x] = *(const GLOBAL_AS uint32_t*)(codes_at + (4 * slot_of(x) + 32 * c));
-            va[x] = *(const GLOBAL_AS uint16_t*)(numbers_at + (2 * slot_of(x) + 8 * (c & ~3u)));
-            vb[x] = *(const GLOBAL_AS uint16_t*)(numbers_at + (2 * slot_of(x) + 8 * (c & ~3u)) + 16);
+            vc[x] = *(const GLOBAL_AS uint32_t*)(codes_at + Page4<HD>::value_word(slot_of(x), c));
+            const uint32_t number = Page4<HD>::value_number(slot_of(x), c >> 2);
+            va[x] = *(const GLOBAL_AS uint16_t*)(numbers_at + number);
+            vb[x] = *(const GLOBAL_AS uint16_t*)(numbers_at + number + 16);
         };
         auto put = [&](uint32_t tile, int x, u32x4 y) {
             *(LDS_AS u32x4*)(static_cast<uintptr_t>(tile + (wave * COPIES + x) * 1024 + lane * 16)) = y;
