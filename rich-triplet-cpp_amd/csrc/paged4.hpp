@@ -80,11 +80,8 @@ struct Codes {
         return u32x4{values<0>(w, a, b), values<1>(w, a, b), values<2>(w, a, b), values<3>(swapped(w), a, b)};
     }
 };
-// Where code e of eight is in a word: at these bits, of a half that is turned by them.
-__device__ __forceinline__ uint32_t code_at(uint32_t code, int e) {
-    const uint32_t half = code << (4 * (e >> 1)) << 2;  // (18 bits: the top two go round)
-    return ((half | half >> 16) & 0xffffu) << (16 * (e & 1));
-}
+// A word of eight codes from its halves' plain ones (code e at bits 4 (e / 2) of half e % 2): each half turned by two bits.
+__device__ __forceinline__ uint32_t turned_codes(uint32_t w) { return (w << 2 & 0xfffcfffcu) | (w >> 14 & 0x00030003u); }
 // Whether a or b (16 bits each) is an infinity or a NaN.
 __device__ __forceinline__ bool no_number(uint32_t a, uint32_t b) {
     return (a & 0x7c00u) == 0x7c00u || (b & 0x7c00u) == 0x7c00u;

@@ -147,3 +147,58 @@ def test_captured(rt):
         graph.replay()
         torch.cuda.synchronize()
         assert same(out[0], kept(x)) and same(out[1], kept(x)), i
+
+
+def many_slots(order, tokens, n_slots):
+    """Slots of many tokens: from the first on, from an odd one on, in pieces of every length, in any order."""
+    g = torch.Generator(device="cuda").manual_seed(tokens)
+    n = torch.arange(tokens, device="cuda")
+    if order == "first":
+        slots = n
+    elif order == "odd":
+        slots = n + 1
+    elif order == "pieces":  # (-1 now and then, then a hole)
+        slots = n + n // 7
+        slots[::61] = -1
+    else:
+        slots = torch.randperm(n_slots, generator=g, device="cuda")[:tokens]
+    slots = slots.to(torch.int32)
+    if order != "any":
+        slots[tokens // 2 // 4 * 4 + 3] = n_slots  # (one of four in a row is none)
+    return slots
+
+
+@pytest.mark.parametrize("order", ["first", "odd", "pieces", "any"])
+@pytest.mark.parametrize("src, dim, heads, page, tokens", [("bf16", 256, 8, 32, 2051), ("f32", 128, 8, 8, 4099),
+                                                           ("f16", 64, 24, 512, 2742)])
+def test_many_tokens(rt, src, dim, heads, page, tokens, order):
+    say("many", src, dim, heads, page, tokens, order)
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    n_pages = -(-(tokens + tokens // 7 + 2) // page)
+    n_slots = n_pages * page
+    kv = filled(rt, n_pages, page, heads, dim)
+    rows = (torch.randn((tokens, 2 * heads, dim), generator=g, device="cuda") * 3).to(DT[src])
+    k, v = rows[:, :heads], rows[:, heads:]
+    slots = many_slots(order, tokens, n_slots)
+    rt.paged_append(kv, k, v, slots)
+    ok = (slots >= 0) & (slots < n_slots)
+    got = rt.paged_read(kv, slots)
+    one = [rt.paged_read(kv, part) for part in slots.split(500)]  # (few at a time)
+    for i, x in enumerate((k, v)):
+        assert same(got[i], torch.where(ok[:, None, None], kept(x), 0.0))
+        assert same(got[i], torch.cat([o[i] for o in one]))
+    other = torch.ones(n_slots, dtype=torch.bool, device="cuda")
+    other[slots[ok].long()] = False
+    for x in rt.paged_read(kv, torch.nonzero(other)[:, 0].to(torch.int32)):
+        assert torch.isnan(x).all()
+
+
+@pytest.mark.parametrize("cache", list(DT))
+def test_many_tokens_of_other_caches(rt, cache):
+    raw = torch.randn((2, 300, 16, 8, 128), device="cuda").to(DT[cache])
+    kv = rt.PagedKV(raw[0], raw[1])
+    slots = torch.randint(-3, 4810, (4101,), device="cuda", dtype=torch.int32)
+    ok = (slots >= 0) & (slots < 4800)
+    for i, got in enumerate(rt.paged_read(kv, slots)):
+        want = raw[i].reshape(4800, 8, 128)[torch.where(ok, slots, 0).long()]
+        assert torch.equal(got, torch.where(ok[:, None, None], want, 0.0))
