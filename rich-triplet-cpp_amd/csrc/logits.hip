@@ -11,22 +11,26 @@
 //
 // A workgroup has a request and kChunk tokens of the vocabulary.  It counts the
 // whole history's tokens that fall into the chunk in LDS (integers: the order of
-// the additions does not matter), takes the last bias of each, and lists the
-// tokens it met; then it goes through the request's rows with that list alone.  A
-// mask closes whole quads of tokens by one store and the rest one by one, so it
-// reads no logits, and list and mask never meet at a token.
+// the additions does not matter), collects its biases, and lists the tokens it
+// met; then it goes through the request's rows with that list alone.  A mask
+// closes whole quads of tokens by one store and the rest one by one, so it reads
+// no logits, and list and mask never meet at a token.
+// 64 requests under penalties and biases take 13 us, of which 3 are the start and
+// the rest one after another a request's numbers, its history, LDS and the logits
+// met; masks of 160 bf16 rows of 262144 tokens 23 us, bound by the lines written.
 #include "rt_common.hpp"
 #include "rt_launch.hpp"
 
 namespace rt_hip {
 namespace {
 
-// (4032 tokens: four workgroups' counts, lists and entries fit a CU's LDS, with 4096
-// three; 64 requests, half of them masked: 17.2 and 20.3 us.  In workgroups of twice
-// the threads and tokens 22.4, of as many threads and half the tokens 19.4.)
+// (Eight workgroups' counts and lists fit a CU's LDS: 64 requests, half of them
+// masked, 15.4 us; with a list as long as the chunk and an array for the biases, four
+// to a CU, 17.2, and with three to a CU 20.3.)
 constexpr int kChunk = 4032, kThreads = 256;
 constexpr int kQuads = (kChunk / 4 + kThreads - 1) / kThreads;  // of a thread: four tokens each, kThreads * 4 apart
 constexpr uint32_t kListed = 1u << 31;
+constexpr int kListedMost = 1792, kFew = 32;  // tokens of a list; drafts, and biases, of one
 
 __device__ __forceinline__ float load(const float* p) { return *p; }
 __device__ __forceinline__ float load(const __bf16* p) { return __uint_as_float(static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p)) << 16); }
@@ -41,14 +45,14 @@ __device__ __forceinline__ void close4(float* p) {
 __device__ __forceinline__ void close4(__bf16* p) { *reinterpret_cast<u32x2*>(p) = u32x2{0xff80ff80u, 0xff80ff80u}; }
 
 template <class T>
-__global__ __launch_bounds__(kThreads) void k_adjust_logits(AdjustLogits p) {
+__global__ __launch_bounds__(kThreads, 7) void k_adjust_logits(AdjustLogits p) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     // Per token of the chunk: kListed, twice the count behind the prompt, 1 if in the prompt ...
     uint32_t* const seen = reinterpret_cast<uint32_t*>(lds);
     uint16_t* const list = reinterpret_cast<uint16_t*>(seen + kChunk);   // the tokens met
-    uint32_t* const entry = reinterpret_cast<uint32_t*>(list + kChunk);  // ... 1 + the last bias entry (where there are biases)
-    __shared__ int listed, n_drafts;
-    __shared__ int draft_row[64], draft_at[64];  // the rows' drafts that fall into the chunk
+    __shared__ int listed, n_drafts, n_entries;
+    __shared__ int draft_row[kFew], draft_at[kFew];  // the rows' drafts that fall into the chunk
+    __shared__ int entry_of[kFew], entry_at[kFew];   // the request's biases that do
     const int s = blockIdx.y, tid = threadIdx.x;
     // (everything of the request at once: what is not there is read from row_start and not used)
     const float* const some = reinterpret_cast<const float*>(p.row_start);
@@ -81,16 +85,16 @@ __global__ __launch_bounds__(kThreads) void k_adjust_logits(AdjustLogits p) {
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) x[k] = i + k * kThreads < len ? text[i + k * kThreads] : -1;
     };
+    auto clear = [&] {
+        for (int i = tid * 4; i < kChunk; i += kThreads * 4) *reinterpret_cast<u32x4*>(seen + i) = u32x4{0, 0, 0, 0};
+        if (tid == 0) listed = n_drafts = n_entries = 0;
+    };
     int first_bias = -1, first_draft = -1;
     if (counts || biased) {
         if (counts) ask(tid);
         if (b0 + tid < b1) first_bias = p.bias_token[b0 + tid];
         if (counts && p.tokens && 1 + tid < rows) first_draft = p.tokens[row0 + 1 + tid];
-        for (int i = tid * 4; i < kChunk; i += kThreads * 4) {
-            *reinterpret_cast<u32x4*>(seen + i) = u32x4{0, 0, 0, 0};
-            if (biased) *reinterpret_cast<u32x4*>(entry + i) = u32x4{0, 0, 0, 0};
-        }
-        if (tid == 0) listed = n_drafts = 0;
+        clear();
     }
     // The masks, while the history is on its way.  (Four rows' words asked for
     // together: one row 3.2 us instead of 2.4, drafts' rows no faster.)
@@ -124,65 +128,97 @@ __global__ __launch_bounds__(kThreads) void k_adjust_logits(AdjustLogits p) {
     }
     if (!counts && !biased) return;
     __syncthreads();
-    // A token of the chunk is met: `as` says how (0: only to be listed).
+    // The chunk's tokens from `from` on, `size` of them: all, or where more biases meet
+    // them than are collected one half and then the other, whose last entries take the
+    // place of the other's counts.
+    uint32_t* const last = seen + kChunk / 2;  // 1 + a token's last entry
+    bool halves = false;
+    int from = 0, size = here;
+    auto in_part = [&](int token, uint32_t* at) {
+        *at = static_cast<uint32_t>(token) - static_cast<uint32_t>(base + from);  // (tokens below 0 too)
+        return *at < static_cast<uint32_t>(size);
+    };
+    // A token is met: `as` says how (0: only to be listed).
     auto meet = [&](uint32_t at, uint32_t as) {
-        if (!(atomicOr(seen + at, kListed | (as & 1u)) & kListed)) list[atomicAdd(&listed, 1)] = static_cast<uint16_t>(at);
+        if (!(atomicOr(seen + at, kListed | (as & 1u)) & kListed)) {
+            const int i = atomicAdd(&listed, 1);
+            if (i < kListedMost) list[i] = static_cast<uint16_t>(at);
+        }
         if (as > 1) atomicAdd(seen + at, as);
     };
-    auto in_chunk = [&](int token, uint32_t* at) {
-        *at = static_cast<uint32_t>(token) - static_cast<uint32_t>(base);  // (tokens below 0 too)
-        return *at < static_cast<uint32_t>(here);
-    };
-    uint32_t at;
-    if (counts) {
-        for (int i = tid; i < len; i += kAhead * kThreads) {
-            if (i != tid) ask(i);
+    for (bool again = false;;) {
+        uint32_t at;
+        if (counts) {
+            for (int i = tid; i < len; i += kAhead * kThreads) {
+                if (i != tid || again) ask(i);
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k)
-                if (in_chunk(x[k], &at)) meet(at, i + k * kThreads < prompt ? 1u : 2u);
+                for (int k = 0; k < kAhead; ++k)
+                    if (in_part(x[k], &at)) meet(at, i + k * kThreads < prompt ? 1u : 2u);
+            }
+            if (p.tokens)
+                for (int i = 1 + tid; i < rows; i += kThreads)
+                    if (in_part(i == 1 + tid ? first_draft : p.tokens[row0 + i], &at)) {
+                        meet(at, 0);
+                        const int d = atomicAdd(&n_drafts, 1);
+                        if (d < kFew) draft_row[d] = i, draft_at[d] = static_cast<int>(at);
+                    }
         }
-        if (p.tokens)
-            for (int i = 1 + tid; i < rows; i += kThreads)
-                if (in_chunk(i == 1 + tid ? first_draft : p.tokens[row0 + i], &at)) {
-                    meet(at, 0);
-                    const int d = atomicAdd(&n_drafts, 1);
-                    if (d < 64) draft_row[d] = i, draft_at[d] = static_cast<int>(at);
+        for (int i = b0 + tid; i < b1; i += kThreads)
+            if (in_part(i == b0 + tid ? first_bias : p.bias_token[i], &at)) {
+                meet(at, 0);
+                if (halves) {
+                    atomicMax(last + at, static_cast<uint32_t>(i - b0 + 1));
+                } else if (const int e = atomicAdd(&n_entries, 1); e < kFew) {
+                    entry_of[e] = i, entry_at[e] = static_cast<int>(at);
                 }
-    }
-    for (int i = b0 + tid; i < b1; i += kThreads)
-        if (in_chunk(i == b0 + tid ? first_bias : p.bias_token[i], &at)) {
-            meet(at, 0);
-            atomicMax(entry + at, static_cast<uint32_t>(i - b0 + 1));
+            }
+        __syncthreads();
+        // (more tokens than the list holds: every token of the part)
+        const bool all = listed > kListedMost;
+        const uint32_t n = static_cast<uint32_t>(all ? size : listed);
+        const int drafts = n_drafts, entries = n_entries;
+        if (entries <= kFew) {
+            // A thread has a token of the list in a row; its mask and its logit are asked for together.
+            const uint32_t each = (n + 63) / 64 * 64;  // (a wave has one row)
+            for (uint64_t job = tid; job < static_cast<uint64_t>(each) * static_cast<uint32_t>(rows); job += kThreads) {
+                const int i = __builtin_amdgcn_readfirstlane(static_cast<int>(job / each));
+                const uint32_t at_list = static_cast<uint32_t>(job - static_cast<uint64_t>(i) * each);
+                if (at_list >= n) continue;
+                const uint32_t mine = all ? at_list : list[at_list], v = static_cast<uint32_t>(from) + mine;
+                T* const where = logits + i * p.stride + v;
+                const uint32_t* const mask = mask_of(i);
+                const uint32_t bits = mask ? mask[v / 32] : ~0u;
+                const float old = load(where);
+                int e = -1;  // the token's last entry
+                if (halves) {
+                    e = b0 - 1 + static_cast<int>(last[mine]);
+                    if (e < b0) e = -1;
+                } else {
+                    for (int k = 0; k < entries; ++k) e = entry_at[k] == static_cast<int>(mine) ? max(e, entry_of[k]) : e;
+                }
+                const float bias = e >= 0 ? p.bias[e] : 0.0f;
+                uint32_t t = seen[mine] & ~kListed;
+                if (drafts <= kFew) {
+                    for (int d = 0; d < drafts; ++d) t += draft_row[d] <= i && draft_at[d] == static_cast<int>(mine) ? 2u : 0u;
+                } else {
+                    for (int k = 1; k <= i; ++k) t += in_part(p.tokens[row0 + k], &at) && at == mine ? 2u : 0u;
+                }
+                if (!(bits >> (v % 32) & 1) || (t == 0 && e < 0)) continue;
+                float y = old;
+                if (t) y = y > 0.0f ? y / rep : y * rep;
+                if (t > 1) y = (y - freq * static_cast<float>(t >> 1)) - pres;
+                if (e >= 0) y += bias;
+                store(where, y);
+            }
+            from += size;
+            if (from >= here) break;
         }
-    __syncthreads();
-    const uint32_t n = static_cast<uint32_t>(listed);
-    const int drafts = n_drafts;
-    if (n == 0) return;
-    // A thread has a token of the list in a row; its mask and its logit are asked for together.
-    const uint32_t each = (n + 63) / 64 * 64;  // (a wave has one row)
-    for (uint64_t job = tid; job < static_cast<uint64_t>(each) * static_cast<uint32_t>(rows); job += kThreads) {
-        const int i = __builtin_amdgcn_readfirstlane(static_cast<int>(job / each));
-        const uint32_t at_list = static_cast<uint32_t>(job - static_cast<uint64_t>(i) * each);
-        if (at_list >= n) continue;
-        const uint32_t v = list[at_list];
-        T* const where = logits + i * p.stride + v;
-        const uint32_t* const mask = mask_of(i);
-        const uint32_t bits = mask ? mask[v / 32] : ~0u;
-        const float old = load(where);
-        const uint32_t e = biased ? entry[v] : 0u;
-        const float bias = e ? p.bias[b0 + static_cast<int>(e) - 1] : 0.0f;
-        uint32_t t = seen[v] & ~kListed;
-        if (drafts <= 64) {
-            for (int d = 0; d < drafts; ++d) t += draft_row[d] <= i && draft_at[d] == static_cast<int>(v) ? 2u : 0u;
-        } else {
-            for (int k = 1; k <= i; ++k) t += in_chunk(p.tokens[row0 + k], &at) && at == v ? 2u : 0u;
-        }
-        if (!(bits >> (v % 32) & 1) || (t | e) == 0) continue;
-        float y = old;
-        if (t) y = y > 0.0f ? y / rep : y * rep;
-        if (t > 1) y = (y - freq * static_cast<float>(t >> 1)) - pres;
-        if (e) y += bias;
-        store(where, y);
+        halves = true;
+        size = min(kChunk / 2, here - from);
+        again = true;
+        __syncthreads();  // (the part's numbers are read)
+        clear();
+        __syncthreads();
     }
 }
 
@@ -190,7 +226,7 @@ __global__ __launch_bounds__(kThreads) void k_adjust_logits(AdjustLogits p) {
 
 hipError_t launch_adjust_logits(const AdjustLogits& p, hipStream_t s) {
     const dim3 grid((static_cast<unsigned>(p.vocab) + kChunk - 1) / kChunk, static_cast<unsigned>(p.n_seq));
-    const size_t lds = kChunk * (sizeof(uint32_t) + sizeof(uint16_t) + (p.bias ? sizeof(uint32_t) : 0));
+    const size_t lds = kChunk * sizeof(uint32_t) + kListedMost * sizeof(uint16_t);
     if (p.dtype == RT_HIP_F32) hipLaunchKernelGGL(k_adjust_logits<float>, grid, dim3(kThreads), lds, s, p);
     else hipLaunchKernelGGL(k_adjust_logits<__bf16>, grid, dim3(kThreads), lds, s, p);
     return hipGetLastError();

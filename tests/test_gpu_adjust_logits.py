@@ -157,6 +157,41 @@ def test_long_histories(rt, dtype):
     Case(9000, [1, 3, 2], dtype, history=7001, seed=6, spread=3).check(rt)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows, bias", [([1, 90, 3], 6), ([40, 1], 300), ([2, 200], 33)])
+def test_many_in_a_place(rt, dtype, rows, bias):
+    """More drafts, and more biases, of one request in one part of the vocabulary than are kept in a list."""
+    Case(9000, rows, dtype, history=300, seed=14, bias=bias, spread=200).check(rt)
+    Case(4100, [2, 1], dtype, history=9000, seed=15, bias=bias, spread=4100).check(rt)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_other_stream(rt, dtype):
+    """On a stream that has work before it; rows that start anywhere."""
+    c = Case(5000, [3, 1, 2], dtype, seed=16)
+    stream = torch.cuda.Stream()
+    for first in (1, 2, 3):
+        c.store = torch.randn((8, 5011), device="cuda").to(dtype)
+        c.logits = c.store[:6, :5000]
+        shifted = torch.randn((7, 5003), device="cuda").to(dtype)[:6, first:first + 5000]
+        rules, starts, tokens = c.rules(rt), i32(c.starts), i32(c.tokens)
+        want = shifted.clone()
+        rt.adjust_logits(want, starts, rules, tokens=tokens)
+        later = torch.zeros_like(shifted)
+        keep = torch.full((6, 5003), 7.0, device="cuda", dtype=dtype)
+        odd = keep[:, first:first + 5000]
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                later.add_(shifted)
+                later.sub_(shifted)
+            odd.copy_(shifted)
+            rt.adjust_logits(odd, starts, rules, tokens=tokens)
+        stream.synchronize()
+        assert torch.equal(odd, want)
+        assert (keep[:, :first] == 7).all() and (keep[:, first + 5000:] == 7).all()
+
+
 def test_numbers_out_of_range(rt):
     """Lengths, starts, tokens and masks that are none: nothing outside is read or written."""
     c = Case(600, [2, 3, 1], seed=7, spread=600)
