@@ -381,7 +381,7 @@ __global__ __launch_bounds__(NW * 64, few_per_cu(NW, 16 * RBLK, HD)) void k_page
     __shared__ int flag;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int nw = gridDim.x, w = place_of(blockIdx.x, nw);
-        // Tiles that take as long as an item's start and end.  (64 requests decoding, head_dim
+    // Tiles that take as long as an item's start and end.  (64 requests decoding, head_dim
     // 128 in four waves, us: 64.9 with 0, 58.0 with 1, 56.8 with 2, 56.1 with 4; 128 shorter
     // ones 34.8, 30.4, 30.3, 32.7.  16 requests of 5 tokens in eight waves 34.0, 30.0, 29.2, 27.0.)
     constexpr int EXTRA = NW == 4 ? 2 : 3;
