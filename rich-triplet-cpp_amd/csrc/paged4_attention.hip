@@ -673,18 +673,16 @@ __global__ __launch_bounds__(NW * 64) void k_paged4_wide(PagedAttn p, Launch la)
         core.last[0] = real ? pos0 + t : -1;
         core.first[0] = walk.first_seen(core.last[0]);
         lds_barrier();
-        // Step i in two halves: the products, O += P V of tile i - 1 and the
-        // scores of tile i, and the weighing of tile i.  With eight waves, w and
-        // w + 4 share a SIMD: the second four run a half behind the first, so
-        // that one wave of a SIMD has the matrix cores while the other has the
-        // VALU, a barrier between the halves.
+        // Step i: the products, O += P V of tile i - 1 and the scores of tile i, and
+        // the weighing of tile i; a wave among its products goes before one that weighs.
+        // (2048 tokens over 8048 keys, us, f16 and bf16 rows: 267 and 273.  The second
+        // four waves a half step behind the first, with a barrier between the halves:
+        // 275 and 274, there without priorities 283 and 284; on a slower card 293 and
+        // 293 where this takes 286 and 288.)
         // Among its products a wave puts V of tile i and K of tile i + 1 where V of
         // tile i - 2 and K of tile i - 1 were, whose products every wave has behind
         // it, and sends the loads of the tiles behind them.
-        constexpr bool kTwo = NW == 8;
-        const bool second = kTwo && wave >= 4;
         if (nt > 0) {
-            if (second) lds_barrier();
             for (int i = 0; i <= nt; ++i) {
                 const int now = i & 1;
                 const bool edge_v = is_edge(static_cast<int>(key0 + i * BN));
@@ -708,13 +706,11 @@ __global__ __launch_bounds__(NW * 64) void k_paged4_wide(PagedAttn p, Launch la)
                 });
                 __builtin_amdgcn_s_setprio(0);
                 if (i == 0) core.no_values();
-                if (kTwo) lds_barrier();
                 // (behind the last tile: from hi on, keys that no row sees, which change nothing)
                 const int key = i < nt ? static_cast<int>(key0) + i * BN : hi;
                 core.softmax(key, i == nt || key + BK - 1 > wave_low || (p.window && wave_hi - key >= p.window));
                 lds_barrier();
             }
-            if (kTwo && !second) lds_barrier();
         }
         if (uniform(special) == item) {
             for (int i = 0; i < nt; ++i)
