@@ -177,3 +177,59 @@ def test_a_server_with_adapters_and_rules(rt, captured):
     guess = lambda s, t: [int(x) if rng.random() < 0.8 else int(rng.integers(VOCAB)) for x in want[s][len(t):len(t) + WIDTH]]  # noqa: E731
     assert serve(guess) == want
     assert all(len(set(t[-steps:])) > 5 for t in want)
+
+
+def test_two_graphs_share_the_workspace(rt):
+    """A graph of single tokens and one of chunks, replayed in turn with eager calls between: each as the eager call."""
+    g = torch.Generator(device="cuda").manual_seed(21)
+    randn = lambda *shape: torch.randn(shape, generator=g, device="cuda")  # noqa: E731
+    pages, page = 40, 16
+    size = rt.paged_page_bytes(rt.Q4KV, page, KV_HEADS, DIM)
+    raw = torch.full((2, pages, size), 255, dtype=torch.uint8, device="cuda")
+    kv = rt.PagedKV4(raw[0], raw[1], page, KV_HEADS, DIM)
+    rt.paged_append(kv, randn(pages * page, KV_HEADS, DIM), randn(pages * page, KV_HEADS, DIM),
+                    torch.arange(pages * page, dtype=torch.int32, device="cuda"))
+    adapters = rt.Adapters(randn(3, RANK, HIDDEN).to(torch.bfloat16), randn(3, HIDDEN, RANK).to(torch.bfloat16), randn(3))
+
+    class Calls:
+        def __init__(self, rows, lens):
+            self.starts, self.lens = i32(np.cumsum([0] + rows)), i32(lens)
+            self.adapter = i32(np.arange(len(rows)) % 4 - 1)
+            self.table = torch.randperm(pages, generator=g, device="cuda").to(torch.int32).repeat(len(rows), 1)
+            self.x, self.q, self.y = (randn(sum(rows), HIDDEN) for _ in range(3))
+            self.out = torch.zeros((sum(rows), HEADS, DIM), device="cuda")
+
+        def run(self):
+            self.y.copy_(self.q)
+            rt.lora_add(self.y, self.x, adapters, self.starts, self.adapter)
+            rt.paged_attention(self.y.view(-1, HEADS, DIM), kv, self.table, self.starts, self.lens, 1 / math.sqrt(DIM), out=self.out)
+
+        def want(self):
+            self.run()
+            torch.cuda.synchronize()
+            return self.out.clone()
+
+    few, many, other = Calls([1] * 9, [600, 1, 33, 640, 17, 16, 15, 500, 64]), Calls([70, 1, 130], [70, 300, 640]), Calls([5] * 6, [400] * 6)
+    rt.reserve_workspace(max(rt.paged_attention_workspace_bytes(kv, rt.F32, HEADS, 9, 201), rt.lora_workspace_bytes(adapters, 9, 201)))
+    graphs = []
+    for c in (few, many):
+        c.want()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            c.run()
+        graphs.append(graph)
+    for i in range(3):
+        for c in (few, many):
+            c.x.copy_(randn(*c.x.shape)), c.q.copy_(randn(*c.q.shape))
+        want = [c.want() for c in (few, many)]
+        for c in (few, many):
+            c.out.fill_(9.0)
+        torch.cuda.synchronize()
+        graphs[0].replay()
+        graphs[1].replay()
+        if i:
+            other.run()
+        graphs[0].replay()
+        torch.cuda.synchronize()
+        for c, w in zip((few, many), want):
+            assert torch.equal(c.out, w), i
