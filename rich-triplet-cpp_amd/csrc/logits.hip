@@ -118,7 +118,8 @@ __global__ __launch_bounds__(kThreads, 7) void k_adjust_logits(AdjustLogits p) {
                 if (open == 0 && aligned && v + 4 <= here) {
                     close4(row + v);
                 } else {
-                    // (reading the quad and writing it back with its holes took 45 us where this takes 33)
+                    // (Masks of 160 bf16 rows: 22.2 us.  Where many of a wave's quads have holes,
+                    // quads read and written back whole 23.9, tokens stored 64 after 64 23.7.)
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         if (!(open >> k & 1) && v + k < here) close(row + v + k);
