@@ -887,13 +887,15 @@ def paged_read(kv: PagedKV, slots, dtype=None, out=None, stream=None):
     if out is None:
         dtype = dtype or (torch.float16 if c.dtype == Q4KV else kv.k.dtype)
         with _made_on(stream):
-            out = torch.empty((2, n, c.n_kv_heads, c.head_dim), dtype=dtype, device=kv.k.device).unbind(0)
-    k, v = out
-    if (dtype is not None and k.dtype is not dtype) or v.dtype is not k.dtype or k.shape[0] != n or v.shape[0] != n:
-        raise ValueError("rt_hip: out must be a pair of slots' length and of dtype")
-    stride = _rows(device, k, "k", c.n_kv_heads, c.head_dim)
-    if _rows(device, v, "v", c.n_kv_heads, c.head_dim) != stride:
-        raise ValueError("rt_hip: k and v must have one stride")
+            k, v = torch.empty((2, n, c.n_kv_heads, c.head_dim), dtype=dtype, device=kv.k.device).unbind(0)
+        stride = c.n_kv_heads * c.head_dim
+    else:
+        k, v = out
+        if (dtype is not None and k.dtype is not dtype) or v.dtype is not k.dtype or k.shape[0] != n or v.shape[0] != n:
+            raise ValueError("rt_hip: out must be a pair of slots' length and of dtype")
+        stride = _rows(device, k, "k", c.n_kv_heads, c.head_dim)
+        if _rows(device, v, "v", c.n_kv_heads, c.head_dim) != stride:
+            raise ValueError("rt_hip: k and v must have one stride")
     _call_on(device, "rt_hip_paged_read", stream, kv.ref, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), _value_type(k),
              stride)
     return k, v
