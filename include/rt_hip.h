@@ -824,7 +824,7 @@ int64_t rt_hip_verify_drafts_workspace_bytes(int32_t vocab, int32_t n_seq, int32
  * frequency 0, no biases, no masks.  A repetition that is not above 0 counts as 1;
  * tokens outside the vocabulary count for nothing.  What no rule changes keeps its
  * bits.  row_start must not decrease; a row that two requests claim is undefined.
- * vocab <= 2^20, n_seq <= 4096, history_cols < 2^30. */
+ * vocab <= 2^20, n_seq <= 4096, history_cols < 2^28. */
 typedef struct rt_hip_logit_rules {
     const int32_t* history;
     int64_t history_cols;

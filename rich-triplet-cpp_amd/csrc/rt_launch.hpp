@@ -356,8 +356,9 @@ struct AdjustLogits {
     int64_t mask_stride = 0;
     const int32_t* mask_row = nullptr;     // [n_rows] or null: row r has mask r
     int n_bias = 0, n_masks = 0;
+    int chunk;  // tokens of a workgroup, a multiple of 32 (the launch's)
 };
-hipError_t launch_adjust_logits(const AdjustLogits& p, hipStream_t s);
+hipError_t launch_adjust_logits(AdjustLogits p, hipStream_t s);
 // Adapters added to a projection's output (lora.hip); rank and k multiples of 8.
 struct LoraAdd {
     float* y = nullptr;           // rows of n values, y_stride apart

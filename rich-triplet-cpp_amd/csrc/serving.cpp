@@ -397,7 +397,7 @@ int rt_hip_adjust_logits(void* logits, int64_t stride, int32_t dtype, int32_t vo
     if (vocab > kMaxVocab) return fail(fn, RT_HIP_E_SHAPE, "vocab must be at most 2^20");
     if (n_seq > kPlanMaxSeq) return fail(fn, RT_HIP_E_SHAPE, "n_seq must be at most " + std::to_string(kPlanMaxSeq));
     if (u.history && (!u.history_len || u.history_cols < 1)) return fail(fn, RT_HIP_E_ARG, "a history needs history_len and history_cols");
-    if (u.history && u.history_cols > 0x3fffffff) return fail(fn, RT_HIP_E_SHAPE, "history_cols must be below 2^30");
+    if (u.history && u.history_cols > 0x0fffffff) return fail(fn, RT_HIP_E_SHAPE, "history_cols must be below 2^28");
     if (u.bias && (!u.bias_start || (u.n_bias > 0 && !u.bias_token))) return fail(fn, RT_HIP_E_ARG, "biases need bias_start and bias_token");
     const int64_t words = (static_cast<int64_t>(vocab) + 31) / 32;
     if (u.mask && u.mask_stride < words) return fail(fn, RT_HIP_E_ARG, "mask_stride below a row's words");

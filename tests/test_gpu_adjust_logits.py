@@ -166,6 +166,35 @@ def test_many_in_a_place(rt, dtype, rows, bias):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bias", [94, 97])
+def test_many_biases_in_a_place(rt, dtype, bias):
+    """As many different biases in one part as its table takes, and more."""
+    c = Case(4100, [2, 1, 3], dtype, seed=17, bias=bias)
+    c.bias_start = np.array([0, bias, bias, 2 * bias])
+    c.bias_token = np.concatenate([np.arange(bias), 100 - np.arange(bias)])
+    c.bias = np.random.default_rng(0).normal(size=2 * bias)
+    c.check(rt)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_requests(rt, dtype):
+    """More parts than the card takes at once; among the requests some with long histories, many biases, many drafts."""
+    rows = [1, 2, 1] * 66 + [40, 1, 2]
+    c = Case(12100, rows, dtype, history=9000, seed=18, bias=4, spread=8000)
+    long = c.history_len.copy()
+    c.history_len = np.minimum(c.history_len, 40)
+    c.history_len[[3, 150]] = long[[3, 150]] = 9000
+    c.prompt_len = (c.history_len * 0.3).astype(int)
+    c.tokens[c.starts[198]:c.starts[199]] = np.arange(40) % 36 + 4000
+    start = c.bias_start[7]
+    more = np.random.default_rng(1).integers(0, 300, 150)
+    c.bias_token = np.concatenate([c.bias_token[:start], more, c.bias_token[start:]])
+    c.bias = np.concatenate([c.bias[:start], np.random.default_rng(2).normal(size=150), c.bias[start:]])
+    c.bias_start[8:] += 150
+    c.check(rt)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_other_stream(rt, dtype):
     """On a stream that has work before it; rows that start anywhere."""
     c = Case(5000, [3, 1, 2], dtype, seed=16)
