@@ -246,7 +246,7 @@ hipError_t launch_adjust_logits(AdjustLogits p, hipStream_t s) {
     // waves where a CU has two at most (3 requests' 2 rows of 4042 tokens, histories of
     // 3000: 7 us, with kChunk tokens and 256 threads 27; one row of 128256 after 400 tokens
     // 4.5 and 5.1; 52 requests' 5 rows of 9309 tokens 20 and 40, with 1024 threads 16, but
-    // there 45 requests' rows of 3026 after 94 tokens 6.5 instead of 5.7).
+    // there 44 requests' rows of 3026 after 94 tokens 6.5 instead of 5.7).
     const int64_t cus = device_info().cus, parts = cus > p.n_seq ? cus / p.n_seq : 1, even = (p.vocab + parts - 1) / parts;
     p.chunk = static_cast<int>(even < 128 ? 128 : even < kChunk ? (even + 31) / 32 * 32 : kChunk);
     const dim3 grid((static_cast<unsigned>(p.vocab) + p.chunk - 1) / p.chunk, static_cast<unsigned>(p.n_seq));
