@@ -13,6 +13,9 @@
 // with such pairs the group's a and b are made 0, and NaN is added at the end to
 // the rows that see it.  In the other tiles every row sees every key, and a NaN
 // times any weight is the NaN that the row is to have.
+// Keys behind the last one may never have been written.  Their a and b are made 0
+// whatever they are: finite ones may still stand for infinities (a = b = 61280,
+// say), which a weight of 0 makes NaN.
 #include "paged4.hpp"
 #include "paged_core.hpp"
 
@@ -645,11 +648,10 @@ __global__ __launch_bounds__(NW * 64) void k_paged4_wide(PagedAttn p, Launch la)
         auto put_v = [&](int slot, int x, int key, bool edge) {
             uint32_t ab = va[x] | vb[x] << 16;
             if (edge) {
-                // (what is behind the last key was never written, and is no one's)
                 const bool behind = key + (wave * COPIES + x) * C::RPI + lane / C::CPR > pages.end;
                 const bool bad = no_number(ab, ab >> 16);
                 if (__builtin_amdgcn_ballot_w64(bad && !behind) != 0) special = item;
-                ab = bad ? 0u : ab;
+                ab = bad || behind ? 0u : ab;
             }
             put(lds_at + (2 + slot) * C::TB, x, codes.word(vc[x], ab));
         };
