@@ -13,9 +13,9 @@
 // with such pairs the group's a and b are made 0, and NaN is added at the end to
 // the rows that see it.  In the other tiles every row sees every key, and a NaN
 // times any weight is the NaN that the row is to have.
-// Keys behind the last one may never have been written.  Their a and b are made 0
-// whatever they are: finite ones may still stand for infinities (a = b = 61280,
-// say), which a weight of 0 makes NaN.
+// Keys that no row sees, behind the last one and in front of the first, may never
+// have been written.  Their a and b are made 0 whatever they are: finite ones may
+// still stand for infinities (a = b = 61280, say), which a weight of 0 makes NaN.
 #include "paged4.hpp"
 #include "paged_core.hpp"
 
@@ -271,19 +271,20 @@ struct Few {
             l[b] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         }
     }
-    // a and b made 0 for values that are no numbers and for keys behind `end`
-    // (what is there was never written); whether some of the first were met.
-    __device__ __forceinline__ bool clean(Tile& x, int key, int end) const {
+    // a and b made 0 for values that are no numbers and for keys before `begin` and
+    // behind `end` (no row sees those); whether some of the first were met.
+    __device__ __forceinline__ bool clean(Tile& x, int key, int begin, int end) const {
         bool any = false;
 #pragma unroll
         for (int u = 0; u < SETS; ++u)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int sh = 16 * (i & 1);
-                const bool behind = key + 8 * kg + i > end;
+                const int at = key + 8 * kg + i;
+                const bool unseen = at < begin || at > end;
                 const bool bad = no_number(x.va[u][i >> 1] >> sh, x.vb[u][i >> 1] >> sh);
-                any |= bad && !behind;
-                const uint32_t keep = bad || behind ? ~(0xffffu << sh) : ~0u;
+                any |= bad && !unseen;
+                const uint32_t keep = bad || unseen ? ~(0xffffu << sh) : ~0u;
                 x.va[u][i >> 1] &= keep;
                 x.vb[u][i >> 1] &= keep;
             }
@@ -453,7 +454,7 @@ __global__ __launch_bounds__(NW * 64, few_per_cu(NW, 16 * RBLK, HD)) void k_page
             core.scores(tile);
             if (more) core.load_keys(tile, pages, at + BN, id_k);
             core.softmax(key, edge);
-            if (edge) special |= __builtin_amdgcn_ballot_w64(core.clean(tile, key, hi - 1)) != 0;
+            if (edge) special |= __builtin_amdgcn_ballot_w64(core.clean(tile, key, lo, hi - 1)) != 0;
             core.pv(tile);
             if (more) {
                 core.load_values(tile, pages, at + BN, id_v);
@@ -648,10 +649,10 @@ __global__ __launch_bounds__(NW * 64) void k_paged4_wide(PagedAttn p, Launch la)
         auto put_v = [&](int slot, int x, int key, bool edge) {
             uint32_t ab = va[x] | vb[x] << 16;
             if (edge) {
-                const bool behind = key + (wave * COPIES + x) * C::RPI + lane / C::CPR > pages.end;
-                const bool bad = no_number(ab, ab >> 16);
-                if (__builtin_amdgcn_ballot_w64(bad && !behind) != 0) special = item;
-                ab = bad || behind ? 0u : ab;
+                const int at = key + (wave * COPIES + x) * C::RPI + lane / C::CPR;
+                const bool unseen = at < lo || at > pages.end, bad = no_number(ab, ab >> 16);
+                if (__builtin_amdgcn_ballot_w64(bad && !unseen) != 0) special = item;
+                ab = bad || unseen ? 0u : ab;
             }
             put(lds_at + (2 + slot) * C::TB, x, codes.word(vc[x], ab));
         };

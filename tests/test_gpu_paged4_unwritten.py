@@ -21,7 +21,8 @@ def poison(raw, byte, seed):
 
 
 class Unwritten(Step):
-    """A step over pages that held `byte` ("any": bits at random) before."""
+    """A step over pages that held `byte` ("any": bits at random) before, whose pages in front of
+    the first key that a request's rows see hold it again."""
 
     def __init__(self, rt, byte, *args, **kw):
         def before(step, k, v):
@@ -29,6 +30,13 @@ class Unwritten(Step):
                 poison(raw, byte, 10 + i)
 
         super().__init__(rt, *args, spoil=before, **kw)
+        self.stale = 0
+        for s, (n, length) in enumerate(self.lens):
+            first = length - n - self.window + 1 if self.window else 0
+            for c in range(max(0, first) // self.page):
+                for i, raw in enumerate((self.kv.k, self.kv.v)):
+                    poison(raw[int(self.table[s, c])], byte, 20 + i)
+                self.stale += 1
 
 
 BYTES = [0x7B, 0xFB, "any"]
@@ -44,6 +52,20 @@ def test_behind_the_last_key(rt, q, dim, byte):
     Unwritten(rt, byte, q, 6, 2, dim, 16, MIXED, seed=dim).check(rt)
     Unwritten(rt, byte, q, 2, 2, dim, 64, [(200, 459)], seed=dim + 1).check(rt)
     Unwritten(rt, byte, q, 8, 1, dim, 8, [(1, 700), (1, 9)], seed=dim + 2, joint=True).check(rt)
+
+
+@pytest.mark.parametrize("q", TYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("byte", BYTES)
+@pytest.mark.parametrize("page, window", [(8, 10), (16, 100), (8, 1)])
+def test_in_front_of_the_window(rt, q, dim, byte, page, window):
+    say("unwritten4 window", q, dim, byte, page, window)
+    step = Unwritten(rt, byte, q, 6, 2, dim, page, MIXED, seed=dim, window=window)
+    assert step.stale > 20
+    step.check(rt)
+    # keys that end with a tile: only those in front of the window were not written
+    for lens in ([(70, 448)], [(1, 256), (5, 640), (3, 1024), (2, 128)]):
+        Unwritten(rt, byte, q, 4, 2, dim, page, lens, seed=dim + 1, window=window).check(rt)
 
 
 def test_few_and_many_rows_alike(rt):
