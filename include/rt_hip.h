@@ -866,7 +866,8 @@ int rt_hip_linear_forward(int32_t format, const void* w, const float* bias, cons
  *   y += scale[i] * b[i] (a[i] x),   i = adapter[s],
  * x [n_rows][k] of type x_dtype (F32, F16 or BF16).  Rows of requests whose adapter is
  * none of them (-1), and rows outside every request, are left as they were.  Sums in
- * f32, every factor with its 24 bits.  Deterministic.  rank is a multiple of 8 from 8 to
+ * f32, every factor with its 24 bits; what is infinite or NaN as the formula has it.
+ * Deterministic.  rank is a multiple of 8 from 8 to
  * 128, k a multiple of 8, k and n <= 2^20, n_rows <= 2^24, n_seq <= 4096; rows of x
  * 16-byte aligned.  row_start must not decrease; a row that two requests claim is
  * undefined.  Uses the library workspace (rt_hip_lora_workspace_bytes, to reserve

@@ -13,6 +13,10 @@
 // Products on the bf16 matrix cores with f32's accuracy: x and t as three bf16
 // values that add up to the f32 one, bf16 weights as they are, f16 ones as two
 // (the product of the two last is below 2^-24 of the whole and left out).
+// An infinity has zeros for its other parts, whose products with one are NaN, and
+// what f32 holds past bf16's largest number becomes one: a sum that is no number is
+// computed again from the factors themselves.
+#include "paged_rows.hpp"
 #include "rt_common.hpp"
 #include "rt_launch.hpp"
 #include "wave_scan.hpp"
@@ -107,6 +111,14 @@ __device__ __forceinline__ Limbs limbs_at(const uint8_t* p) {
     }
 }
 
+// Whether some of four values is an infinity or a NaN.
+__device__ __forceinline__ bool no_numbers(f32x4 v) {
+    float any = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) any = __builtin_fmaf(v[e], 0.0f, any);
+    return any != any;
+}
+
 // What a wave has stored to its part of LDS is there for all of its lanes (they
 // are served in order; this is for the compiler).
 __device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); }
@@ -149,8 +161,11 @@ __device__ __forceinline__ bool find_block(const LoraAdd& p, int index, Block* o
 
 // t = A x of a block of 16 RB rows over a slice of k: RT tiles of 16 ranks.  The
 // four waves take 32 values of k in turn, and their sums are added in LDS.
+// (Waves to a SIMD: as many as the products' registers leave, which the code for
+// sums that are no numbers would otherwise lower by one.  The same in the second
+// launch: 2700 rows in both 38 us, without the bounds 44.)
 template <class X, class W, int RT, int RB>
-__global__ __launch_bounds__(256) void k_lora_shrink(LoraAdd p) {
+__global__ __launch_bounds__(256, RT < 4 ? 1 : sizeof(X) == 4 && RT * RB >= 8 ? 2 : 3) void k_lora_shrink(LoraAdd p) {
     constexpr int kAhead = RT * RB >= 8 ? 2 : 4;  // steps whose loads are in flight together
     constexpr int XB = 32 * sizeof(X), XC = XB / 16, XL = 16 * RB * XC / 64;  // bytes of a row of x in a step, chunks, loads
     constexpr int XS = XB + 16, WS = 64 + 16;  // bytes between rows in LDS
@@ -223,16 +238,40 @@ __global__ __launch_bounds__(256) void k_lora_shrink(LoraAdd p) {
     }
     __syncthreads();
     if (wave > 0) return;
+    float* const out = p.part + (static_cast<int64_t>(blockIdx.y) * p.n_rows + blk.row) * p.rank;
+    uint32_t again = 0;  // tiles of this lane's with sums that are no numbers
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
         if (b * 16 + n >= blk.rows) continue;
-        float* const out = p.part + (static_cast<int64_t>(blockIdx.y) * p.n_rows + blk.row + b * 16 + n) * p.rank;
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
             const int r = t * 16 + kg * 4;  // (the rank is a multiple of 8)
-            if (r < p.rank)
-                *reinterpret_cast<f32x4*>(out + r) = ((c[b][t] + sums[0][b][t][lane]) + sums[1][b][t][lane]) + sums[2][b][t][lane];
+            if (r >= p.rank) continue;
+            const f32x4 sum = ((c[b][t] + sums[0][b][t][lane]) + sums[1][b][t][lane]) + sums[2][b][t][lane];
+            *reinterpret_cast<f32x4*>(out + (b * 16 + n) * p.rank + r) = sum;
+            if (no_numbers(sum)) again |= 1u << (b * RT + t);
+            if (t % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (not all tiles' sums in registers at once)
         }
+    }
+#pragma unroll 1
+    for (; again != 0; again &= again - 1) {
+        const int i = __builtin_ctz(again), row = i / RT * 16 + n, r = i % RT * 16 + kg * 4;
+        const X* const xr = static_cast<const X*>(p.x) + static_cast<int64_t>(blk.row + row) * p.x_stride;
+        const W* const ar = static_cast<const W*>(p.a) + (static_cast<int64_t>(blk.adapter) * p.rank + r) * p.k;
+        f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+        for (int kk = k0; kk < k1; kk += 8) {
+            float xv[8], av[8];
+            load8(xr + kk, xv);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                load8(ar + q * p.k + kk, av);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum[q] = __builtin_fmaf(xv[e], av[e], sum[q]);
+            }
+            if (sum[0] != sum[0] && sum[1] != sum[1] && sum[2] != sum[2] && sum[3] != sum[3]) break;  // (NaN they stay)
+        }
+        *reinterpret_cast<f32x4*>(out + row * p.rank + r) = sum;
     }
 }
 
@@ -240,11 +279,12 @@ __global__ __launch_bounds__(256) void k_lora_shrink(LoraAdd p) {
 // the rows of the product, so that a lane has one column of four rows and 16
 // lanes 64 bytes of a row of y.
 template <class W, int RS, int RB>
-__global__ __launch_bounds__(256) void k_lora_expand(LoraAdd p) {
+__global__ __launch_bounds__(256, RS * RB == 8 ? 2 : RS * RB == 4 ? 4 : RS * RB == 2 ? 5 : 8) void k_lora_expand(LoraAdd p) {
     constexpr int kAhead = 2;  // tiles of 16 columns whose loads are in flight together
     constexpr int TS = RS * 64 + 16, kT = 16 * RB * TS;  // bytes between rows of t, and of weights; of a limb of t
     constexpr int kTile = 16 * TS, kWaves = 4 * kAhead * kTile;
     __shared__ __attribute__((aligned(16))) uint8_t lds[3 * kT > kWaves ? 3 * kT : kWaves];
+    __shared__ __attribute__((aligned(16))) float whole[16 * RB][RS * 32];  // t as it is
     Block blk;
     if (!find_block<16 * RB>(p, blockIdx.x, &blk)) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -260,8 +300,10 @@ __global__ __launch_bounds__(256) void k_lora_expand(LoraAdd p) {
 #pragma unroll 4
             for (int s = 0; s < p.slices; ++s, at += static_cast<int64_t>(p.n_rows) * p.rank) sum += *reinterpret_cast<const f32x4*>(at);
         }
+        sum *= scale;
+        *reinterpret_cast<f32x4*>(&whole[row][r]) = sum;
         u32x2 h, m, l;
-        bf16_limbs4(sum * scale, h, m, l);
+        bf16_limbs4(sum, h, m, l);
         uint8_t* const to = lds + row * TS + r * 2;
         *reinterpret_cast<u32x2*>(to) = h;
         *reinterpret_cast<u32x2*>(to + kT) = m;
@@ -293,7 +335,8 @@ __global__ __launch_bounds__(256) void k_lora_expand(LoraAdd p) {
     const W* const b0 = static_cast<const W*>(p.b) + static_cast<int64_t>(blk.adapter) * p.n * p.rank;
     float* const y = p.y + static_cast<int64_t>(blk.row) * p.y_stride;
     const int c1 = min(p.n, (static_cast<int>(blockIdx.y) + 1) * p.cols);
-    for (int c0 = blockIdx.y * p.cols + wave * (16 * kAhead); c0 < c1; c0 += 64 * kAhead) {
+    int c0 = blockIdx.y * p.cols + wave * (16 * kAhead);
+    for (; c0 < c1; c0 += 64 * kAhead) {
         u32x4 w[kAhead][RS];
         f32x4 old[kAhead][RB];
         // Values of this lane in block b, tile u: rows 16 b + 4 kg + e.  (No row of the
@@ -338,8 +381,55 @@ __global__ __launch_bounds__(256) void k_lora_expand(LoraAdd p) {
                 for (int b = 0; b < RB; ++b) c[u][b] = m.under(t[b][q], c[u][b]);
             }
         }
+        bool again = false;  // some sum of this lane's is no number
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+            for (int b = 0; b < RB; ++b) again |= no_numbers(c[u][b]);
+        if (__builtin_amdgcn_ballot_w64(again) != 0) break;
         each([&](int u, int b, int e, float* at) { *at = old[u][b][e] + c[u][b][e]; });
     }
+    // From the first such sum on: the same products tile by tile, where they are numbers.
+#pragma unroll 1
+    for (; c0 < c1; c0 += 64 * kAhead)
+#pragma unroll 1
+        for (int u = 0; u < kAhead; ++u) {
+            const int col = c0 + u * 16 + n;
+            const W* const w = b0 + static_cast<int64_t>(col) * p.rank;
+            f32x4 c[RB];
+#pragma unroll
+            for (int b = 0; b < RB; ++b) c[b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int q = 0; q < RS; ++q) {
+                const bool in = col < c1 && q * 32 + kg * 8 < p.rank;
+                const Weights<W> m(in ? ld16(w + q * 32 + kg * 8) : u32x4{0, 0, 0, 0});
+#pragma unroll
+                for (int b = 0; b < RB; ++b) c[b] = m.under(t[b][q], c[b]);
+            }
+            uint32_t which = 0;
+#pragma unroll
+            for (int b = 0; b < RB; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int row = b * 16 + 4 * kg + e;
+                    if (row >= blk.rows || col >= c1) continue;
+                    if (fabsf(c[b][e]) < __builtin_inff()) y[row * p.y_stride + col] += c[b][e];
+                    else which |= 1u << (b * 4 + e);
+                }
+#pragma unroll 1
+            for (; which != 0; which &= which - 1) {
+                const int i = __builtin_ctz(which), row = i / 4 * 16 + 4 * kg + i % 4;
+                float sum = 0.0f;
+#pragma unroll 1
+                for (int r = 0; r < p.rank && sum == sum; r += 8) {
+                    float wv[8];
+                    load8(w + r, wv);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) sum = __builtin_fmaf(whole[row][r + e], wv[e], sum);
+                }
+                y[row * p.y_stride + col] += sum;
+            }
+        }
 }
 
 // Blocks of 16 rows that a workgroup takes together, in each launch: two where
