@@ -871,7 +871,8 @@ int rt_hip_linear_forward(int32_t format, const void* w, const float* bias, cons
  * 128, k a multiple of 8, k and n <= 2^20, n_rows <= 2^24, n_seq <= 4096; rows of x
  * 16-byte aligned.  row_start must not decrease; a row that two requests claim is
  * undefined.  Uses the library workspace (rt_hip_lora_workspace_bytes, to reserve
- * before a graph capture; -1 for invalid sizes). */
+ * before a graph capture: enough for fewer requests and rows too; -1 for invalid
+ * sizes). */
 typedef struct rt_hip_lora {
     const void* a;
     const void* b;

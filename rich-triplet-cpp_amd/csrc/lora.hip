@@ -493,8 +493,12 @@ void run(LoraAdd p, hipStream_t s) {
 
 }  // namespace
 
-size_t lora_workspace(int rank, int k, int n_seq, int n_rows) {
-    return static_cast<size_t>(slices_of(rank, n_seq, n_rows, k)) * n_rows * rank * sizeof(float);
+// Enough for as many rows and fewer, of however many requests, though fewer blocks take
+// more slices: b blocks of at most 16 t rows take below 2 CUs / b + 1.
+size_t lora_workspace(int rank, int k, int n_rows) {
+    const int64_t rows = n_rows, most = (static_cast<int64_t>(k) + 511) / 512 * rows;
+    const int64_t some = 2 * static_cast<int64_t>(device_info().cus) * 16 * (rank > 64 ? 1 : 2) + rows;
+    return static_cast<size_t>(most < some ? most : some) * rank * sizeof(float);
 }
 
 hipError_t launch_lora_add(LoraAdd p, hipStream_t s) {

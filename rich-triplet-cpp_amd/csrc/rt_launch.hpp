@@ -375,7 +375,7 @@ struct LoraAdd {
     float* part = nullptr;        // lora_workspace bytes
     int slices = 0, k_slice = 0, cols = 0;  // (the launcher's)
 };
-size_t lora_workspace(int rank, int k, int n_seq, int n_rows);
+size_t lora_workspace(int rank, int k, int n_rows);
 hipError_t launch_lora_add(LoraAdd p, hipStream_t s);
 // Drafted tokens against the target's distributions (verify.hip).
 struct VerifyDrafts {

@@ -507,14 +507,14 @@ int rt_hip_lora_add(float* y, int64_t y_stride, const void* x, int32_t x_dtype, 
     p.n_rows = n_rows;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     hipError_t e;
-    p.part = static_cast<float*>(workspace(lora_workspace(l.rank, l.k, n_seq, n_rows), s, &e));
+    p.part = static_cast<float*>(workspace(lora_workspace(l.rank, l.k, n_rows), s, &e));
     if (!p.part) return launched(fn, e);
     return launched(fn, launch_lora_add(p, s));
 }
 
 int64_t rt_hip_lora_workspace_bytes(const rt_hip_lora* lora, int32_t n_seq, int32_t n_rows) {
     if (lora_args("rt_hip_lora_workspace_bytes", lora, n_seq, n_rows)) return -1;
-    return n_seq == 0 || n_rows == 0 ? 0 : static_cast<int64_t>(lora_workspace(lora->rank, lora->k, n_seq, n_rows));
+    return n_seq == 0 || n_rows == 0 ? 0 : static_cast<int64_t>(lora_workspace(lora->rank, lora->k, n_rows));
 }
 
 }  // extern "C"
