@@ -766,7 +766,8 @@ int rt_hip_paged_read(const rt_hip_paged_kv* kv, const int32_t* slots, int32_t n
  * max_fresh is a hint, the most rows a request of this step may have (0: not
  * known); the result does not depend on it beyond rounding.
  * Uses the library workspace (rt_hip_paged_attention_workspace_bytes, to
- * reserve before a graph capture; -1 for invalid sizes). */
+ * reserve before a graph capture: enough for fewer requests and rows too; -1 for
+ * invalid sizes). */
 int rt_hip_paged_attention(const void* q, int32_t dtype, int64_t q_stride, int32_t n_q_heads, const rt_hip_paged_kv* kv,
                            const int32_t* table, int64_t table_cols, const int32_t* q_start, const int32_t* kv_len,
                            int32_t n_seq, int32_t n_tokens, int32_t max_fresh, float scale, int32_t window, void* out,

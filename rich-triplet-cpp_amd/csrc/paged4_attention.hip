@@ -849,7 +849,9 @@ hipError_t run_hd(const PagedAttn& p, float* part, uint32_t* counters, hipStream
 size_t paged4_attention_workspace(const PagedAttn& p) {
     const int64_t rows = most_rows(p);
     const int hd = p.kv.head_dim, waves = hd < 256 ? 8 : 4;
-    const size_t narrow = static_cast<size_t>(few_slots(p, rows)) * 2 * part_floats(few_block(rows, hd), hd);
+    const auto few = [&](int64_t rows) { return static_cast<size_t>(few_slots(p, rows)) * 2 * part_floats(few_block(rows, hd), hd); };
+    // (enough for steps of fewer rows too: blocks of 16 take more than ones of 32)
+    const size_t narrow = few(1) > few(rows) ? few(1) : few(rows);
     const size_t wide = rows > kFewRows ? static_cast<size_t>(slots()) * 2 * wide_part_floats(waves * 32, hd) : 0;
     return (narrow > wide ? narrow : wide) * sizeof(float);
 }
