@@ -1056,6 +1056,8 @@ def adjust_logits(logits, row_start, rules: LogitRules, tokens=None, stream=None
         raise ValueError("rt_hip: mask_row must have an entry for each row of logits")
     if rules.words is not None and rules.words * 32 < vocab:
         raise ValueError("rt_hip: the masks are shorter than the vocabulary")
+    if rules.words is not None and rules.rows is None and rules.struct.n_masks < rows:
+        raise ValueError("rt_hip: fewer masks than rows, and no mask_row")
     _call_on(device, "rt_hip_adjust_logits", stream, logits.data_ptr(), stride, _value_type(logits), vocab,
              row_start.data_ptr(), n, rows, _ptr(tokens), rules.ref)
     return logits
