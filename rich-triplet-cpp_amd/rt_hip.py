@@ -731,6 +731,8 @@ def _rows(device: int, t, name: str, heads: int, dim: int) -> int:
     stride = t.stride()
     if stride[2] != 1 or (heads > 1 and stride[1] != dim):
         raise ValueError(f"rt_hip: the rows of {name} must be dense")
+    if have[0] >> 31:
+        _fits(rows=have[0])
     return stride[0] if have[0] > 1 else heads * dim
 
 
@@ -884,6 +886,8 @@ def paged_read(kv: PagedKV, slots, dtype=None, out=None, stream=None):
     c, device = kv.struct, kv.device
     n = slots.shape[0]
     _want(device, (slots, "slots", torch.int32, (n,)))
+    if n >> 31:
+        _fits(tokens=n)
     if out is None:
         dtype = dtype or (torch.float16 if c.dtype == Q4KV else kv.k.dtype)
         with _made_on(stream):
@@ -1020,11 +1024,11 @@ class LogitRules:
                 self.rows = mask_row.shape[0]
         self.tensors = (history, history_len, prompt_len, repetition, presence, frequency, bias_start, bias_token, bias, mask,
                         mask_row)
-        cols = 0 if history is None else history.shape[1]
+        cols, biases = 0 if history is None else history.shape[1], 0 if bias is None else bias.shape[0]
+        _fits(biases=biases, masks=masks)
         self.struct = LogitRulesStruct(_ptr(history) if cols else None, cols, _ptr(history_len), _ptr(prompt_len),
                                        _ptr(repetition), _ptr(presence), _ptr(frequency), _ptr(bias_start), _ptr(bias_token),
-                                       _ptr(bias), _ptr(mask), stride, _ptr(mask_row), 0 if bias is None else bias.shape[0],
-                                       masks)
+                                       _ptr(bias), _ptr(mask), stride, _ptr(mask_row), biases, masks)
         self.ref = C.byref(self.struct)
 
     def _requests(self, n: int) -> None:
@@ -1040,6 +1044,8 @@ def adjust_logits(logits, row_start, rules: LogitRules, tokens=None, stream=None
     i32 = _torch().int32
     rows, vocab = logits.shape
     n, device = row_start.shape[0] - 1, logits.get_device()
+    if (rows | vocab | n) >> 31:
+        _fits(rows=rows, vocab=vocab, n_seq=n)
     if device < 0:
         raise ValueError("rt_hip: tensors must live on the GPU")
     if rules.device is not None and rules.device != device:
@@ -1093,6 +1099,8 @@ def _dense_rows(device: int, t, name: str, cols: int) -> int:
                          "rt_hip: tensors must live on the GPU")
     if cols > 1 and t.stride(1) != 1:
         raise ValueError(f"rt_hip: the rows of {name} must be dense")
+    if t.shape[0] >> 31:
+        _fits(rows=t.shape[0])
     return t.stride(0) if t.shape[0] > 1 else cols
 
 
@@ -1104,6 +1112,8 @@ def lora_add(y, x, adapters: Adapters, row_start, adapter, stream=None):
     c, device = adapters.struct, adapters.device
     y_stride, x_stride = _dense_rows(device, y, "y", c.n), _dense_rows(device, x, "x", c.k)
     rows, n_seq = y.shape[0], adapter.shape[0]
+    if n_seq >> 31:
+        _fits(n_seq=n_seq)
     if y.dtype is not torch.float32 or x.shape[0] != rows:
         raise ValueError("rt_hip: y must be float32 and have as many rows as x")
     _want(device, (row_start, "row_start", torch.int32, (n_seq + 1,)), (adapter, "adapter", torch.int32, (n_seq,)))
