@@ -456,8 +456,9 @@ int slices_of(int rank, int n_seq, int n_rows, int k) {
 
 template <class X, class W, int RB>
 void shrink(const LoraAdd& p, dim3 grid, hipStream_t s) {
-    const auto kernel = p.rank <= 16 ? k_lora_shrink<X, W, 1, RB> : p.rank <= 32 ? k_lora_shrink<X, W, 2, RB>
-                        : p.rank <= 64 ? k_lora_shrink<X, W, 4, RB> : k_lora_shrink<X, W, 8, RB>;
+    auto kernel = p.rank <= 16 ? k_lora_shrink<X, W, 1, RB> : p.rank <= 32 ? k_lora_shrink<X, W, 2, RB> : k_lora_shrink<X, W, 4, RB>;
+    if constexpr (RB == 1)  // (two blocks go up to rank 64)
+        if (p.rank > 64) kernel = k_lora_shrink<X, W, 8, RB>;
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, p);
 }
 template <class X, class W>
