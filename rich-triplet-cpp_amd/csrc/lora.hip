@@ -6,9 +6,9 @@
 // are on the device: a launch has a workgroup for every block that there could
 // be, and each finds its own among the requests.  Slices of k leave their sums in
 // the workspace and the second launch adds them in order, so results do not
-// depend on who was first.  (In one launch, each workgroup of the second computing
-// t for itself: one token 8.2 us where the two take 7.4, 64 decoding requests 18.1
-// and 15.7, 32 of 5 rows 12.9 and 10.6.)
+// depend on who was first.  (One call behind another one token takes 7.1 us, 64
+// decoding requests 16.0.  In one launch, each workgroup of the second computing t for
+// itself, 8.2 and 18.1 where the two took 7.4 and 15.7, 32 of 5 rows 12.9 and 10.6.)
 //
 // Products on the bf16 matrix cores with f32's accuracy: x and t as three bf16
 // values that add up to the f32 one, bf16 weights as they are, f16 ones as two

@@ -374,6 +374,10 @@ struct Progress {
 // Workgroups of it that a CU holds: by the registers.
 constexpr int few_per_cu(int waves, int bm, int hd) { return waves > 4 ? 1 : bm == 16 && hd < 256 ? 3 : 2; }
 
+// (f32 rows' second limbs do not all fit the registers: 16 bytes of a lane go to memory
+// in blocks of 32 rows at head_dim 128, 20 at 256.  64 requests decoding, whose form has
+// none there, 56.5 us, bf16 rows 53.4; 16 requests of 5 tokens 28.3 and 24.3; a window
+// of 1024 at head_dim 256 19.8, f16 rows 16.5.)
 template <class Q, int HD, int RBLK, int NW>
 __global__ __launch_bounds__(NW * 64, few_per_cu(NW, 16 * RBLK, HD)) void k_paged4_narrow(PagedAttn p, Launch la) {
     constexpr int DB = 16, BM = DB * RBLK, BK = 32, BN = NW * BK, NT = NW * 64;
@@ -385,9 +389,10 @@ __global__ __launch_bounds__(NW * 64, few_per_cu(NW, 16 * RBLK, HD)) void k_page
     __shared__ int flag;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int nw = gridDim.x, w = place_of(blockIdx.x, nw);
-    // Tiles that take as long as an item's start and end.  (64 requests decoding, head_dim
-    // 128 in four waves, us: 64.9 with 0, 58.0 with 1, 56.8 with 2, 56.1 with 4; 128 shorter
-    // ones 34.8, 30.4, 30.3, 32.7.  16 requests of 5 tokens in eight waves 34.0, 30.0, 29.2, 27.0.)
+    // Tiles that take as long as an item's start and end.  (us with 0, 1, 2, 3, 4, head_dim
+    // 128: 64 requests decoding in four waves 77.7, 54.3, 54.3, 55.0, 55.2, 128 of up to 3000
+    // keys 53.4, 40.7, 39.7, 42.0, 42.4; 16 requests of 5 tokens in eight waves 33.7, 27.5,
+    // 26.4, 24.3, 24.5, 24 of 9 tokens 47.0, 31.9, 28.3, 28.1, 27.5.)
     constexpr int EXTRA = NW == 4 ? 2 : 3;
     Walk<BM, BN, EXTRA> walk(p, la);
     int64_t skip = 0, per = 0;
@@ -538,7 +543,9 @@ __global__ __launch_bounds__(NW * 64, few_per_cu(NW, 16 * RBLK, HD)) void k_page
 // and its numbers are loaded a step ahead into registers, and become 16 bytes of
 // the tile among the products.  LDS holds two tiles of K and two of V.
 // Keys of its tiles.  (At head_dim 256 the words on their way to 64 do not fit the
-// registers beside the rest.)
+// registers beside the rest.  Nor do all of f32 rows' limbs: 56 bytes of a lane go to
+// memory in eight waves at head_dim 128, 100 at 256.  2048 tokens over 8048 keys 431 us,
+// bf16 rows 271, of half as many products; 512 over 4512 at head_dim 256 109 and 93.)
 constexpr int wide4_keys(int hd) { return hd == 256 ? 32 : 64; }
 
 template <class Q, int HD, int NW>
@@ -787,8 +794,8 @@ constexpr int kFewRows = 32;
 // registers allow, they are one workgroup of eight or two of four: one has fewer
 // states to join across workgroups, two work on while one of them ends an item.
 // us, four and eight waves: blocks of 32 rows at head_dim 128, 16 requests of 5
-// tokens 34 and 27, 24 of 10 tokens 43 and 37.  head_dim 256: 64 and 128 items 21.5
-// and 17.6, 50 and 45; 512 items, 64 requests decoding, 62 and 72.
+// tokens 35.5 and 24.3, 24 of 9 tokens 35.7 and 28.2.  head_dim 256: 64 and 128 items
+// 21.1 and 16.8, 34.3 and 27.0; 512 items, 64 requests decoding, 52.3 and 56.5.
 int few_block(int64_t rows, int hd) { return rows <= 16 || hd == 256 ? 16 : 32; }
 int few_waves(const PagedAttn& p, int64_t rows) {
     if (p.kv.head_dim < 256) return few_block(rows, p.kv.head_dim) == 16 ? 4 : 8;

@@ -27,7 +27,8 @@ constexpr float kInf = __builtin_inff();
 #define CONST_AS __attribute__((address_space(4)))
 
 // A page of the cache that is none: its keys and values (at most one row of
-// 256 f32 is read, every row from the same place).
+// 256 f32 is read, every row from the same place; of a 4-bit page 8 slots' codes or
+// numbers, 1024 bytes too).
 __device__ const __attribute__((aligned(16))) float kZeros[256] = {};
 
 template <class T> struct KindOf;
